@@ -125,6 +125,102 @@ const pg_tensor *pg_amd_linear16_dz(const pg_node *n);
  * the activation pass reading dx); on by default. */
 void pg_amd_linear16_narrow(bool on);
 
+/* ---- gated feed-forward layer ----
+ * h = act(x Wg + bg) * (x Wu + bu), elementwise, for x [M, K], both weights
+ * side by side in W = [Wg | Wu] [K, 2F], and b = [bg | bu] [2F] or NULL; act
+ * one of PG_ACT_* (with the two below: GLU with SIGMOID, ReGLU, GEGLU, SwiGLU
+ * with SILU, bilinear with NONE).  Backward, with z = x W + b = [g | u]:
+ *   dg = dh u act'(g), du = dh act(g), dx = [dg | du] W^T,
+ *   dW = x^T [dg | du], db = column sums of [dg | du].
+ * The products run on the MFMA units with f32 accumulation; z, act, act' and
+ * the column sums are f32; [dg | du] is rounded to the 16-bit type for the
+ * two products.  The reference's layers (nn.c:46-125) have no gated form. */
+#define PG_ACT_SILU 3
+#define PG_ACT_SIGMOID 4
+/* On tensors that the caller holds: x and w of one 16-bit dtype, b f32, h [M,
+ * F] of x's dtype or f32.  z (f32 [M, 2F]) receives the pre-activations that
+ * the backward needs; NULL when there is none (serving).  Inputs may be
+ * strided; outputs are contiguous, written whole and overlap no input.
+ * Enqueued on the library stream.  false and pg_autograd_last_error() on bad
+ * arguments or a device error. */
+bool pg_amd_gated(const pg_tensor *x, const pg_tensor *w, const pg_tensor *b, int act, pg_tensor *h, pg_tensor *z);
+/* The grads for dh [M, F] (x's dtype or f32), with the z that pg_amd_gated
+ * kept: dx [M, K] and dw [K, 2F], of x's dtype or f32, db [2F] f32; each may be
+ * NULL. */
+bool pg_amd_gated_backward(const pg_tensor *x, const pg_tensor *w, const pg_tensor *z, const pg_tensor *dh, int act,
+                           pg_tensor *dx, pg_tensor *dw, pg_tensor *db);
+/* As a node of f32 operands, rounded to `dtype` as pg_amd_ag_linear16 rounds
+ * its own (kept 16-bit copies included); h is f32, with its 16-bit copy for
+ * the next layer.  NULL (pg_autograd_last_error) for bad shapes, dtype or
+ * act. */
+pg_node *pg_amd_ag_gated16(pg_node *x, pg_node *w, pg_node *b, int act, pg_dtype dtype);
+
+/* ---- products with matrices held in 4 bits ----
+ * A matrix rounded to the values 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives
+ * (e2m1) times one power of two for each block of 32 along the dimension that
+ * a product sums over (OCP microscaling, MXFP4: 17 bits per 4 values).  With m
+ * the largest magnitude of a block its power is 2^(floor(log2 m) - 2), at
+ * least 2^-127; values round to nearest, ties to the even code, and magnitudes
+ * past 6 powers to 6.  A block that holds a NaN or an infinity stands
+ * for NaN.  The reference has no form below 16 bits. */
+typedef struct pg_amd_mx4 pg_amd_mx4;
+/* t [rows, cols] of any dtype in 4 bits, the blocks along dimension `axis`
+ * (0 or 1); for the weights [K, N] of a product x W that is 0.  t is read,
+ * not kept.  NULL and pg_autograd_last_error() on bad arguments or a device
+ * error.  Freed with pg_amd_mx4_free. */
+pg_amd_mx4 *pg_amd_mx4_quantize(const pg_tensor *t, int axis);
+void pg_amd_mx4_free(pg_amd_mx4 *q);
+/* The device bytes q holds. */
+size_t pg_amd_mx4_bytes(const pg_amd_mx4 *q);
+/* out (the shape of q's source, any dtype; rounded to it) = the values that q
+ * stands for.  false and pg_autograd_last_error() on failure. */
+bool pg_amd_mx4_dequantize(const pg_amd_mx4 *q, pg_tensor *out);
+/* y [M, N] = Q(x) W for x [M, K] of any dtype, rounded to 4 bits along K in the
+ * call as above, and W [K, N] held in 4 bits (axis 0); the products of the
+ * 4-bit values are exact and accumulated in f32 on the MFMA units, and y (any
+ * dtype) is rounded once.  x may be strided; y is contiguous, written whole
+ * and does not overlap x.  Forward only: for frozen layers.  Enqueued on the
+ * library stream.  false and pg_autograd_last_error() on failure. */
+bool pg_amd_mx4_matmul(const pg_tensor *x, const pg_amd_mx4 *w, pg_tensor *y);
+
+/* ---- distillation from a teacher's top logits ----
+ * Per row s of the student's logits [N, V], with the teacher's logits t_k at
+ * the indices i_k of its top entries and a label:
+ *   p = softmax(t / T) over the entries, q = softmax(s / T), r = softmax(s)
+ *   loss = scale (alpha T^2 sum_k p_k (log p_k - log q_{i_k})
+ *                 + (1 - alpha) (-log r_label))
+ *   ds_j = scale (alpha T (q_j - sum_{k: i_k = j} p_k)
+ *                 + (1 - alpha) (r_j - [j = label]))
+ * An entry with an index outside [0, V) (-1, say) is padding, a label outside
+ * it no label.  A row without entries (none, or all at -inf) has no first
+ * part, one without a label no second; with neither, its loss and grad are 0
+ * whatever its logits hold.  An index that occurs twice counts twice.  A
+ * row of which every logit is -inf, or one is NaN or +inf, has no softmax: its
+ * loss and grad are NaN.  The reference's cross entropy
+ * (pg_ag_cross_entropy) is the case alpha = 0. */
+typedef struct pg_amd_distill_cfg {
+    float temperature; /* T > 0 */
+    float alpha;       /* 0 .. 1 */
+    float scale;       /* 1 / N for a mean over the rows */
+} pg_amd_distill_cfg;
+/* logits [N, V] of any dtype, V <= 2^24; top [N, k] of any dtype and top_idx
+ * [N, k] f32 (whole numbers, as the reference's embedding takes its indices),
+ * 1 <= k <= 256; labels [N] f32 or NULL; loss [N] f32, a value per row;
+ * dlogits [N, V], of logits' dtype or f32, or NULL for the loss alone.  dlogits
+ * may be logits itself: the grad then replaces them.  Otherwise the outputs
+ * must not overlap the inputs.  Both are written whole, in one pass over the
+ * logits.  Enqueued on the library stream.  false and
+ * pg_autograd_last_error() on bad arguments or a device error. */
+bool pg_amd_distill(const pg_tensor *logits, const pg_tensor *top, const pg_tensor *top_idx, const pg_tensor *labels,
+                    const pg_amd_distill_cfg *cfg, pg_tensor *loss, pg_tensor *dlogits);
+/* The loss as a node [1], the sum of the rows': its backward adds the grad to
+ * the logits node's.  logits is an f32 node [N, V]; top, top_idx and
+ * labels are read again by the backward, so they are kept (retained) and must
+ * not change until it has run.  NULL (pg_autograd_last_error) on bad
+ * arguments. */
+pg_node *pg_amd_ag_distill(pg_node *logits, const pg_tensor *top, const pg_tensor *top_idx, const pg_tensor *labels,
+                           const pg_amd_distill_cfg *cfg);
+
 /* The 16-bit operand copies of matmul16 (pg_amd_ag_matmul16) written by the
  * fused elementwise kernels beside their f32 outputs, in place of a cast
  * pass over them: a deferred forward run whose output a matmul16 takes as

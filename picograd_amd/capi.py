@@ -62,6 +62,10 @@ class AdamCfg(C.Structure):
                 ("weight_decay", C.c_float), ("amsgrad", C.c_bool), ("decoupled_wd", C.c_bool)]
 
 
+class DistillCfg(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("alpha", C.c_float), ("scale", C.c_float)]
+
+
 vp, sz, fl, bo, ip = C.c_void_p, C.c_size_t, C.c_float, C.c_bool, C.c_int
 SZP = C.POINTER(C.c_size_t)
 
@@ -187,6 +191,16 @@ _AMD_PROTOS = {
     "pg_amd_tensor_refresh16": (bo, [vp]),
     "pg_amd_tensor_to_dtype": (vp, [vp, ip]),
     "pg_amd_gemm_ex_noalloc": (ip, [ip, sz, sz, sz, vp, sz, vp, sz, vp, sz]),
+    "pg_amd_gated": (bo, [vp, vp, vp, ip, vp, vp]),
+    "pg_amd_gated_backward": (bo, [vp, vp, vp, vp, ip, vp, vp, vp]),
+    "pg_amd_ag_gated16": (vp, [vp, vp, vp, ip, ip]),
+    "pg_amd_mx4_quantize": (vp, [vp, ip]),
+    "pg_amd_mx4_free": (None, [vp]),
+    "pg_amd_mx4_bytes": (sz, [vp]),
+    "pg_amd_mx4_dequantize": (bo, [vp, vp]),
+    "pg_amd_mx4_matmul": (bo, [vp, vp, vp]),
+    "pg_amd_distill": (bo, [vp, vp, vp, vp, C.POINTER(DistillCfg), vp, vp]),
+    "pg_amd_ag_distill": (vp, [vp, vp, vp, vp, C.POINTER(DistillCfg)]),
     "pg_amd_sgd_buffer": (vp, [vp, sz]),
     "pg_tensor_clone": (vp, [vp]),
     "pg_tensor_view": (vp, [vp]),

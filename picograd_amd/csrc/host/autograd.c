@@ -163,6 +163,10 @@ void pg_node_free(pg_node *n)
         pg_tensor_free(t->grad);
         if (t->backward == pgm_linear16_backward)
             pgm_linear16_free_ctx(t->ctx);
+        else if (t->backward == pgo_gated_backward)
+            pgo_gated_free_ctx(t->ctx);
+        else if (t->backward == pgo_distill_backward)
+            pgo_distill_free_ctx(t->ctx);
         else
             free(t->ctx);
         if (sp + t->nparents > cap) {

@@ -116,7 +116,7 @@ static bool gemm16p(const gemm_place *pl, int dt, int ta, int tb, size_t m, size
     return pgd_check(rc, what);
 }
 
-static bool gemm16x(int dt, int ta, int tb, size_t m, size_t n, size_t k, const uint16_t *a, size_t lda, size_t sa,
+bool pgm_gemm16x(int dt, int ta, int tb, size_t m, size_t n, size_t k, const uint16_t *a, size_t lda, size_t sa,
                     size_t aext, const uint16_t *b, size_t ldb, size_t sb, size_t bext, float *c, size_t ldc,
                     size_t sc, size_t batch, int beta, const pgk_epi *epi, const char *what)
 {
@@ -128,7 +128,7 @@ static bool gemm16(int dt, int ta, int tb, size_t m, size_t n, size_t k, const u
                    size_t aext, const uint16_t *b, size_t ldb, size_t sb, size_t bext, float *c, size_t ldc,
                    size_t sc, size_t batch, int beta, const char *what)
 {
-    return gemm16x(dt, ta, tb, m, n, k, a, lda, sa, aext, b, ldb, sb, bext, c, ldc, sc, batch, beta, NULL, what);
+    return pgm_gemm16x(dt, ta, tb, m, n, k, a, lda, sa, aext, b, ldb, sb, bext, c, ldc, sc, batch, beta, NULL, what);
 }
 
 /* A matmul's dgrad and wgrad as ONE launch on the whole chip (the paired
@@ -137,7 +137,7 @@ static bool gemm16(int dt, int ta, int tb, size_t m, size_t n, size_t k, const u
  * first blocks start on the CUs the first leaves free while its last tiles
  * drain.  Measured 434 against 438 us for config 3's pair and 212 against
  * 215 us for a 4096^3 pair.  False (nothing launched) otherwise. */
-static bool pair_full(int dt, const pgk_gemm_desc *dd, const pgk_gemm_desc *dw, const char *what)
+bool pgm_pair_full(int dt, const pgk_gemm_desc *dd, const pgk_gemm_desc *dw, const char *what)
 {
     int sd = 0, sw = 0;
     if (!dd->m || !dd->n || !dd->k || !dd->batch || !dw->m || !dw->n || !dw->k || !dw->batch)
@@ -156,7 +156,7 @@ static bool pair_full(int dt, const pgk_gemm_desc *dd, const pgk_gemm_desc *dw, 
 /* The pair in one launch on a split-over-waves tile when both are small
  * enough to run at once: one launch instead of two, or of split-K's four.
  * False (nothing launched) otherwise. */
-static bool pair_ks(int dt, const pgk_gemm_desc *dd, const pgk_gemm_desc *dw, const char *what)
+bool pgm_pair_ks(int dt, const pgk_gemm_desc *dd, const pgk_gemm_desc *dw, const char *what)
 {
     if (!pgk_gemm16_ks_pair_tile(dd, dw))
         return false;
@@ -193,7 +193,7 @@ int pgm_grad_split(size_t M, size_t K, size_t N, size_t N8, size_t B, size_t Mw,
 
 /* 16-bit copy of `rows x cols` (leading dim lds, `batch` matrices `sstride`
  * apart) padded with zeros to rows_pad x cols_pad; src_dtype 0 casts f32 */
-static uint16_t *stage16(int dt, int src_dtype, const void *src, size_t rows, size_t cols, size_t lds,
+uint16_t *pgm_stage16(int dt, int src_dtype, const void *src, size_t rows, size_t cols, size_t lds,
                          size_t rows_pad, size_t cols_pad, size_t batch, size_t sstride, size_t *bytes)
 {
     *bytes = batch * rows_pad * cols_pad * 2;
@@ -261,12 +261,12 @@ pg_tensor *pgm_matmul_forward(const pg_tensor *a, const pg_tensor *b)
     size_t abytes = 0, bbytes = 0;
     bool ok = true;
     if (K8 != K) {
-        apad = stage16(dt, dt, a->dev, M, K, K, M, K8, ab, M * K, &abytes);
+        apad = pgm_stage16(dt, dt, a->dev, M, K, K, M, K8, ab, M * K, &abytes);
         ok = apad != NULL;
         ap = apad;
     }
     if (ok && (K8 != K || N8 != N)) {
-        bpad = stage16(dt, dt, b->dev, K, N, N, K8, N8, bb, K * N, &bbytes);
+        bpad = pgm_stage16(dt, dt, b->dev, K, N, N, K8, N8, bb, K * N, &bbytes);
         ok = bpad != NULL;
         bp = bpad;
     }
@@ -361,7 +361,7 @@ void pgm_matmul_backward(pg_node *n)
     /* dC rounded once to the operand dtype, [B*M, N8] (zero columns past N) */
     size_t N8 = up8(N) < 8 ? 8 : up8(N), K8 = up8(K) < 8 ? 8 : up8(K);
     size_t gbytes;
-    uint16_t *g16 = stage16(dt, 0, g->dev, B * M, N, N, B * M, N8, 1, 0, &gbytes);
+    uint16_t *g16 = pgm_stage16(dt, 0, g->dev, B * M, N, N, B * M, N8, 1, 0, &gbytes);
     if (!g16)
         return;
     /* dgrad operands: dA[M, K] (+)= dC[M, N] . W[K, N]^T, both contiguous
@@ -370,7 +370,7 @@ void pgm_matmul_backward(pg_node *n)
     uint16_t *wpad = NULL;
     size_t wbytes = 0, wb = s.bbat ? B : 1;
     if (ga && N8 != N)
-        wp = wpad = stage16(dt, dt, b->dev, K, N, N, K, N8, wb, K * N, &wbytes);
+        wp = wpad = pgm_stage16(dt, dt, b->dev, K, N, N, K, N8, wb, K * N, &wbytes);
     /* wgrad operands: dW[K, N] (+)= A[M, K]^T . dC[M, N], reduction over M
      * with K and N contiguous; A padded to K8 zero columns when needed.
      * When only A is batched the batch folds into the reduction (M_eff =
@@ -382,7 +382,7 @@ void pgm_matmul_backward(pg_node *n)
     uint16_t *apad = NULL;
     size_t abytes = 0;
     if (gb && K8 != K)
-        ap = apad = stage16(dt, dt, a->dev, a_rows, K, K, a_rows, K8, 1, 0, &abytes);
+        ap = apad = pgm_stage16(dt, dt, a->dev, a_rows, K, K, a_rows, K8, 1, 0, &abytes);
     size_t lda_w = K8 != K ? K8 : K, sa_w = (s.abat && !fold) ? M * K8 : 0;
     bool d_one = ga && wp && (s.abat || B == 1), w_one = gb && ap && (s.bbat || Bw == 1);
     /* x.x (one node on both sides) has ONE grad: dgrad writes it with the
@@ -402,7 +402,7 @@ void pgm_matmul_backward(pg_node *n)
                               B, ba};
     const pgk_gemm_desc dw = {K, N, Mw, ap, lda_w, sa_w, lda_w, g16, N8, Mw * N8, N8, gb ? gb->dev : NULL, N,
                               s.bbat ? K * N : 0, Bw, bbeta};
-    if (d_one && w_one && !alias && pair_ks(dt, &dd, &dw, "dgrad + wgrad")) {
+    if (d_one && w_one && !alias && pgm_pair_ks(dt, &dd, &dw, "dgrad + wgrad")) {
         if (wpad)
             pgd_free(wpad, wbytes);
         if (apad)
@@ -441,7 +441,7 @@ void pgm_matmul_backward(pg_node *n)
                 pw = (gemm_place){side, 5, 256 - best_cus, false};
             }
         } else {
-            if (pair_full(dt, &dd, &dw, "dgrad + wgrad")) {
+            if (pgm_pair_full(dt, &dd, &dw, "dgrad + wgrad")) {
                 if (wpad)
                     pgd_free(wpad, wbytes);
                 if (apad)
@@ -514,8 +514,8 @@ void pg_gemm_ex(pg_dtype dtype, size_t m, size_t n, size_t k, const void *a, siz
         return;
     }
     size_t K8 = up8(k), N8 = up8(n) < 8 ? 8 : up8(n), ab, bbytes;
-    uint16_t *ap = stage16(dt, dt, a, m, k, lda, m, K8, 1, 0, &ab);
-    uint16_t *bp = ap ? stage16(dt, dt, b, k, n, ldb, K8, N8, 1, 0, &bbytes) : NULL;
+    uint16_t *ap = pgm_stage16(dt, dt, a, m, k, lda, m, K8, 1, 0, &ab);
+    uint16_t *bp = ap ? pgm_stage16(dt, dt, b, k, n, ldb, K8, N8, 1, 0, &bbytes) : NULL;
     if (ap && bp)
         gemm16(dt, 0, 1, m, n, K8, ap, K8, 0, m, bp, N8, 0, N8, c, ldc, 0, 1, 0, "pg_gemm_ex");
     if (ap)
@@ -655,7 +655,7 @@ static bool mm16_dims(const pg_tensor *a, const pg_tensor *b, size_t *M, size_t 
  * shadow when only the rows are padded (cols_pad: whole 16-byte pieces)
  * and t is its whole storage -- kept, and rewritten by the optimisers like
  * the plain one -- else a padded copy returned in *owned (*bytes long) */
-static const uint16_t *operand16(pg_tensor *t, int dt, size_t rows, size_t cols, size_t rows_pad, size_t cols_pad,
+const uint16_t *pgm_operand16(pg_tensor *t, int dt, size_t rows, size_t cols, size_t rows_pad, size_t cols_pad,
                                  uint16_t **owned, size_t *bytes)
 {
     *owned = NULL;
@@ -667,7 +667,7 @@ static const uint16_t *operand16(pg_tensor *t, int dt, size_t rows, size_t cols,
         pgt_is_contiguous(t))
         return pgt_shadow16_rows(t, (pg_dtype)dt, cols, cols_pad);
     pgt_materialize(t); /* the copy reads the f32 elements */
-    *owned = stage16(dt, 0, t->dev, rows, cols, cols, rows_pad, cols_pad, 1, 0, bytes);
+    *owned = pgm_stage16(dt, 0, t->dev, rows, cols, cols, rows_pad, cols_pad, 1, 0, bytes);
     return *owned;
 }
 
@@ -685,7 +685,7 @@ static void mm16_backward(pg_node *n)
     /* the grad's 16-bit copy when the fused backward region wrote it beside
      * the grad (kept with the grad's storage), else a staged copy */
     const uint16_t *gk = N == N8 ? pgt_shadow16_fresh(g, (pg_dtype)dt) : NULL;
-    uint16_t *g16 = gk ? (uint16_t *)gk : stage16(dt, 0, g->dev, M, N, N, M, N8, 1, 0, &gbytes);
+    uint16_t *g16 = gk ? (uint16_t *)gk : pgm_stage16(dt, 0, g->dev, M, N, N, M, N8, 1, 0, &gbytes);
     if (!g16)
         return;
     /* each grad taken for writing once, then both GEMMs as one whole-chip
@@ -699,16 +699,16 @@ static void mm16_backward(pg_node *n)
     const bool alias = a->data_ref == b->data_ref || (ga && gb && (ga == gb || ga->data_ref == gb->data_ref));
     uint16_t *ownb = NULL, *owna = NULL;
     size_t obb = 0, oba = 0;
-    const uint16_t *qb = ga ? operand16(b, dt, K, N, K, N8, &ownb, &obb) : NULL;
-    const uint16_t *qa = gb && !alias ? operand16(a, dt, M, K, M, K8, &owna, &oba) : NULL;
+    const uint16_t *qb = ga ? pgm_operand16(b, dt, K, N, K, N8, &ownb, &obb) : NULL;
+    const uint16_t *qa = gb && !alias ? pgm_operand16(a, dt, M, K, M, K8, &owna, &oba) : NULL;
     const pgk_gemm_desc dd = {M, K, N8, g16, N8, 0, M, qb, N8, 0, K, ga ? ga->dev : NULL, K, 0, 1, ba};
     const pgk_gemm_desc dw = {K, N, M, qa, K8, 0, K8, g16, N8, 0, N8, gb ? gb->dev : NULL, N, 0, 1, bb};
     if (!(qb && qa &&
-          (pair_ks(dt, &dd, &dw, "matmul16 dgrad + wgrad") || pair_full(dt, &dd, &dw, "matmul16 dgrad + wgrad")))) {
+          (pgm_pair_ks(dt, &dd, &dw, "matmul16 dgrad + wgrad") || pgm_pair_full(dt, &dd, &dw, "matmul16 dgrad + wgrad")))) {
         if (qb)
             gemm16(dt, 0, 0, M, K, N8, g16, N8, 0, M, qb, N8, 0, K, ga->dev, K, 0, 1, ba, "matmul16 dgrad");
         if (gb && alias)
-            qa = operand16(a, dt, M, K, M, K8, &owna, &oba);
+            qa = pgm_operand16(a, dt, M, K, M, K8, &owna, &oba);
         if (qa)
             gemm16(dt, 1, 1, K, N, M, qa, K8, 0, K8, g16, N8, 0, N8, gb->dev, N, 0, 1, bb, "matmul16 wgrad");
     }
@@ -771,8 +771,8 @@ pg_node *pg_amd_ag_matmul16(pg_node *a, pg_node *b, pg_dtype dtype)
         size_t K8 = up8(K), N8 = up8(N);
         uint16_t *oa = NULL, *ob = NULL;
         size_t oab = 0, obb = 0;
-        const uint16_t *qa = operand16(av, dt, M, K, M, K8, &oa, &oab);
-        const uint16_t *qb = qa ? operand16(bv, dt, K, N, K8, N8, &ob, &obb) : NULL;
+        const uint16_t *qa = pgm_operand16(av, dt, M, K, M, K8, &oa, &oab);
+        const uint16_t *qb = qa ? pgm_operand16(bv, dt, K, N, K8, N8, &ob, &obb) : NULL;
         ok = qa && qb && gemm16(dt, 0, 1, M, N, K8, qa, K8, 0, M, qb, N8, 0, N8, c->dev, N, 0, 1, 0, "matmul16");
         if (oa)
             pgd_free(oa, oab);
@@ -1007,8 +1007,8 @@ void pgm_linear16_backward(pg_node *n)
      * is queued) and the GEMMs run one after the other, dgrad first (it
      * holds the grad's first beta) */
     const bool alias = x->data_ref == w->data_ref || (gx && gw && (gx == gw || gx->data_ref == gw->data_ref));
-    const uint16_t *qw = gx ? operand16(w, dt, K, N, K, N8, &ow, &obw) : NULL;
-    const uint16_t *qx = gw && !alias ? operand16(x, dt, M, K, M, K8, &ox, &obx) : NULL;
+    const uint16_t *qw = gx ? pgm_operand16(w, dt, K, N, K, N8, &ow, &obw) : NULL;
+    const uint16_t *qx = gw && !alias ? pgm_operand16(x, dt, M, K, M, K8, &ox, &obx) : NULL;
     const pgk_gemm_desc dd = {M, K, N8, dz16, N8, 0, M, qw, N8, 0, K, gx ? gx->dev : NULL, K, 0, 1, bx};
     const pgk_gemm_desc dw = {K, N, M, qx, K8, 0, K8, dz16, N8, 0, N8, gw ? gw->dev : NULL, N, 0, 1, bw};
     void *dz_owned = keep ? NULL : dz16;
@@ -1017,11 +1017,11 @@ void pgm_linear16_backward(pg_node *n)
         qw = NULL; /* formed, or pending on gx */
     }
     if (!(qw && qx &&
-          (pair_ks(dt, &dd, &dw, "linear16 dgrad + wgrad") || pair_full(dt, &dd, &dw, "linear16 dgrad + wgrad")))) {
+          (pgm_pair_ks(dt, &dd, &dw, "linear16 dgrad + wgrad") || pgm_pair_full(dt, &dd, &dw, "linear16 dgrad + wgrad")))) {
         if (qw)
             gemm16(dt, 0, 0, M, K, N8, dz16, N8, 0, M, qw, N8, 0, K, gx->dev, K, 0, 1, bx, "linear16 dgrad");
         if (gw && alias)
-            qx = operand16(x, dt, M, K, M, K8, &ox, &obx);
+            qx = pgm_operand16(x, dt, M, K, M, K8, &ox, &obx);
         if (qx)
             gemm16(dt, 1, 1, K, N, M, qx, K8, 0, K8, dz16, N8, 0, N8, gw->dev, N, 0, 1, bw, "linear16 wgrad");
     }
@@ -1098,16 +1098,16 @@ pg_node *pg_amd_ag_linear16(pg_node *x, pg_node *w, pg_node *b, int act, pg_dtyp
         pgk_epi epi = {bv ? (const float *)bv->dev : NULL, act, z ? (float *)z->dev : NULL,
                        out->data_ref->shadow, dt, lazy_out ? 1 : 0};
         if (!K) {
-            ok = gemm16x(dt, 0, 1, M, N, 0, NULL, 8, 0, M, NULL, 8, 0, up8(N), out->dev, N, 0, 1, 0, &epi,
+            ok = pgm_gemm16x(dt, 0, 1, M, N, 0, NULL, 8, 0, M, NULL, 8, 0, up8(N), out->dev, N, 0, 1, 0, &epi,
                          "linear16");
         } else {
             size_t K8 = up8(K), N8 = up8(N);
             uint16_t *oa = NULL, *ob = NULL;
             size_t oab = 0, obb = 0;
-            const uint16_t *qx = operand16(xv, dt, M, K, M, K8, &oa, &oab);
-            const uint16_t *qw = qx ? operand16(wv, dt, K, N, K8, N8, &ob, &obb) : NULL;
+            const uint16_t *qx = pgm_operand16(xv, dt, M, K, M, K8, &oa, &oab);
+            const uint16_t *qw = qx ? pgm_operand16(wv, dt, K, N, K8, N8, &ob, &obb) : NULL;
             ok = qx && qw &&
-                 gemm16x(dt, 0, 1, M, N, K8, qx, K8, 0, M, qw, N8, 0, N8, out->dev, N, 0, 1, 0, &epi, "linear16");
+                 pgm_gemm16x(dt, 0, 1, M, N, K8, qx, K8, 0, M, qw, N8, 0, N8, out->dev, N, 0, 1, 0, &epi, "linear16");
             if (oa)
                 pgd_free(oa, oab);
             if (ob)

@@ -186,6 +186,21 @@ pg_tensor *pgm_matmul_forward(const pg_tensor *a, const pg_tensor *b);
  * storage replaces its staging pass), else 0 */
 int pgm_mm16_grad16(const pg_node *n);
 void pgm_matmul_backward(pg_node *n);
+/* one MFMA GEMM (pgk_gemm16 semantics, optional epilogue) on the library
+ * stream and scratch; a matmul's dgrad and wgrad in one launch (false, nothing
+ * launched, where they do not pair) */
+bool pgm_gemm16x(int dt, int ta, int tb, size_t m, size_t n, size_t k, const uint16_t *a, size_t lda, size_t sa,
+                 size_t aext, const uint16_t *b, size_t ldb, size_t sb, size_t bext, float *c, size_t ldc, size_t sc,
+                 size_t batch, int beta, const pgk_epi *epi, const char *what);
+bool pgm_pair_ks(int dt, const pgk_gemm_desc *dd, const pgk_gemm_desc *dw, const char *what);
+bool pgm_pair_full(int dt, const pgk_gemm_desc *dd, const pgk_gemm_desc *dw, const char *what);
+/* a 16-bit copy of a matrix padded with zeros (freed with pgd_free, *bytes
+ * long); a tensor's 16-bit form as a GEMM operand: a kept copy, or one
+ * returned in *owned */
+uint16_t *pgm_stage16(int dt, int src_dtype, const void *src, size_t rows, size_t cols, size_t lds, size_t rows_pad,
+                      size_t cols_pad, size_t batch, size_t sstride, size_t *bytes);
+const uint16_t *pgm_operand16(pg_tensor *t, int dt, size_t rows, size_t cols, size_t rows_pad, size_t cols_pad,
+                              uint16_t **owned, size_t *bytes);
 int pgm_grad_split(size_t M, size_t K, size_t N, size_t N8, size_t B, size_t Mw, size_t Bw, bool *streams);
 /* a linear16 bias grad whose last step (the sum of its row-block partials)
  * the next activation pass was to run: run it now (the walk's end), or now
@@ -196,6 +211,24 @@ void pgm_colsum_flush_for(const pg_tensor *t);
  * (the kept pre-activation), called by pg_node_free */
 void pgm_linear16_backward(pg_node *n);
 void pgm_linear16_free_ctx(void *ctx);
+
+/* pg_amd_ag_gated16's backward and the destructor of its node context, called
+ * by pg_node_free; pg_amd_ag_distill's */
+void pgo_gated_backward(pg_node *n);
+void pgo_gated_free_ctx(void *ctx);
+void pgo_distill_backward(pg_node *n);
+void pgo_distill_free_ctx(void *ctx);
+
+/* ---- operands of the calls that write to tensors of the caller ----
+ * t as an input: its elements current and in row-major order (*owned a copy
+ * to free with pg_tensor_free when it was strided).  NULL (autograd error
+ * set) otherwise. */
+const pg_tensor *pgo_input(const char *what, const pg_tensor *t, pg_tensor **owned);
+/* t as an output written whole: contiguous and non-overlapping with the
+ * inputs in[0 .. nin) (NULL entries are skipped); false with the autograd error set */
+bool pgo_output_ok(const char *what, const pg_tensor *t, const pg_tensor *const *in, size_t nin);
+/* right before the launch that writes t whole */
+void pgo_output(pg_tensor *t);
 
 /* ---- JIT internals used by the walker (jit.c) ---- */
 typedef struct pgj_region pgj_region;

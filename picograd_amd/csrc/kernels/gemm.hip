@@ -1086,9 +1086,16 @@ extern "C" int pgk_gemm16_cu(int dtype, int ta, int tb, size_t m, size_t n, size
         const int rc = launch_ks_any(f16, ta, tb, g, fused ? *epi : pgk_epi{}, fused, st);
         if (rc || fused || (!ktail && !has_epi))
             return rc;
-    } else if (has_epi && !sp && !ktail && !ta && tb) {
+    } else if (has_epi && !sp && !ktail && (tb || !ta)) {
+        // a forward product's epilogue, or a grad's rounded to 16 bits
         gemm_args g = {a, lda, stride_a, (int)a_extent, b, ldb, stride_b, (int)b_extent, c, ldc, stride_c,
                        (int)m, (int)n, (int)kmain, 0, 1u, pl.tile};
+        if (!tb)
+            return f16 ? launch_layout<false, false, true, true>(g, st, *epi)
+                       : launch_layout<false, false, false, true>(g, st, *epi);
+        if (ta)
+            return f16 ? launch_layout<true, true, true, true>(g, st, *epi)
+                       : launch_layout<true, true, false, true>(g, st, *epi);
         return f16 ? launch_layout<false, true, true, true>(g, st, *epi)
                    : launch_layout<false, true, false, true>(g, st, *epi);
     }

@@ -262,6 +262,65 @@ int pgk_act_bwd16n(int act, const uint16_t *dn, const uint16_t *wn, int kw, int 
                    const float *z, size_t m, size_t n, uint16_t *d16, size_t ldd, int dtype, float *db, int db_beta,
                    void *ws, const pgk_colsum_job *fold, pgk_colsum_job *defer, pgk_stream s);
 
+/* Gated feed-forward layer (gated.hip), z = x W + b = [g | u] [m, 2 f] f32:
+ * h = act(g) u, acts PGK_ACT_* and the two below.
+ * _act: h [m, f] from z, in f32 (h32) and / or 16 bits (h16, RNE; rows of f).
+ * _bwd: dg = dh u act'(g), du = dh act(g) from dh [m, f] (dh_dtype 0 = f32,
+ * else 16-bit of that dtype), RNE into dz16 [m, 2 f8] (dg at column 0, du at
+ * f8 = f rounded up to 8, zeros between) and, when db is given, their column
+ * sums db [2 f] (beta ? += : =) in a fixed order (ws: pgk_gated_bwd_workspace
+ * bytes). */
+enum { PGK_ACT_SILU = 3, PGK_ACT_SIGMOID = 4 };
+int pgk_gated_act(int act, const float *z, size_t m, size_t f, float *h32, uint16_t *h16, int dtype, pgk_stream s);
+size_t pgk_gated_bwd_workspace(size_t m, size_t f);
+int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float *z, size_t m, size_t f, uint16_t *dz16, int dtype,
+                  float *db, int db_beta, void *ws, pgk_stream s);
+
+/* 4-bit matrices with a power of two per 32 values along the reduction
+ * (mx4.hip).  codes: [rows] rows of `pitch` bytes (16 per block of 32 values,
+ * value 2 i in the low half of byte i), zeros past cols.  scales: exponents
+ * biased by 127 (255: the block is NaN) as [ceil(blocks / 8)][rows_p][8], rows_p
+ * = rows rounded up to 16; those past the last row or block are unset. */
+typedef struct {
+    size_t rows, cols; /* cols: along the reduction */
+    size_t pitch, rows_p;
+    uint8_t *codes, *scales;
+} pgk_mx4;
+/* sets rows, cols, pitch and rows_p; the byte sizes of codes and scales */
+void pgk_mx4_shape(pgk_mx4 *q, size_t rows, size_t cols, size_t *code_bytes, size_t *scale_bytes);
+/* q = src, dense of dtype 0 = f32, 1 = f16, 2 = bf16: [rows, cols], or with
+ * `trans` [cols, rows] */
+int pgk_mx4_quantize(const pgk_mx4 *q, const void *src, int dtype, int trans, pgk_stream s);
+/* dst (dense, as src above) = the values q stands for */
+int pgk_mx4_dequantize(const pgk_mx4 *q, void *dst, int dtype, int trans, pgk_stream s);
+/* y [x->rows, w->rows] of y_dtype = x w^T over their shared cols, f32
+ * accumulation */
+int pgk_mx4_matmul(const pgk_mx4 *x, const pgk_mx4 *w, void *y, int y_dtype, pgk_stream s);
+
+/* Distillation from a teacher's top logits (distill.hip): per-row losses
+ * and, when ds is given, the grad of the logits s [n, v] (dense rows).  t and
+ * idx [n, top], label [n] or NULL; indices are whole numbers held as f32, one
+ * outside [0, v) is no entry.  dtypes: 0 = f32, 1 = f16, 2 = bf16; ds_dtype is
+ * dtype or 0.  up: a device scalar the grad is scaled by, or NULL.  beta (f32
+ * ds): added to ds.  ds may be s itself (one dtype).  loss may be NULL. */
+#define PGK_DISTILL_TOP 256             /* entries per row at most */
+#define PGK_DISTILL_MAX_V ((size_t)1 << 24) /* whole numbers that f32 holds */
+typedef struct {
+    const void *s;
+    int dtype;
+    size_t n, v;
+    const void *t;
+    int top_dtype;
+    const float *idx, *label;
+    int top;
+    float temperature, alpha, scale;
+    const float *up;
+    float *loss;
+    void *ds;
+    int ds_dtype, beta;
+} pgk_distill_args;
+int pgk_distill(const pgk_distill_args *a, pgk_stream s);
+
 /* multi-tensor SGD */
 typedef struct {
     float *p;

@@ -1,0 +1,280 @@
+"""The gated layer (pg_amd_gated, pg_amd_gated_backward, pg_amd_ag_gated16)
+against the formula in 64 bits on the same 16-bit operands, and its grads
+against differences.
+
+Bounds: a dot product of n terms in f32 is off by at most (n + 4) 2^-24 times
+the sum of its terms' magnitudes; act and act' are within 2^-20 of their
+argument's scale (a few units of f32 over an exponential); every rounding to
+16 bits adds half a unit in the last place of what it rounds.
+"""
+import numpy as np
+import pytest
+import torch
+
+from op_tools import NAMES, TINY, UNIT, Bench, rounded, within
+from picograd_amd.capi import BF16, F16, F32, shape_arg
+
+pytestmark = pytest.mark.gpu
+
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
+F = 2.0 ** -24
+MATH = 2.0 ** -20
+
+
+@pytest.fixture()
+def bench(lib):
+    b = Bench(lib)
+    yield b
+    b.close()
+
+
+def act64(g, act):
+    g = torch.as_tensor(g).clone().requires_grad_()
+    a = {"none": lambda v: v * 1.0, "relu": torch.relu, "sigmoid": torch.sigmoid, "silu": lambda v: v * torch.sigmoid(v),
+         "gelu": lambda v: v * torch.special.ndtr(v)}[act](g)
+    a.sum().backward()
+    return a.detach().numpy(), g.grad.numpy()
+
+
+def data(m, k, f, dtype, bias, seed=0):
+    r = np.random.default_rng(seed)
+    x = rounded(r.standard_normal((m, k)), dtype)
+    w = rounded(r.uniform(-1, 1, (k, 2 * f)) * max(k, 1) ** -0.5, dtype)
+    b = rounded(r.standard_normal(2 * f) * 0.1, F32) if bias else None
+    dh = rounded(r.standard_normal((m, f)) * 0.5, dtype)
+    return x, w, b, dh
+
+
+def model(x, w, b, dh, act, dtype):
+    """Values and bounds: name -> (value, f32 bound)."""
+    f = w.shape[1] // 2
+    z = x @ w + (0 if b is None else b)
+    ez = (x.shape[1] + 4) * F * (np.abs(x) @ np.abs(w) + (0 if b is None else np.abs(b))) + TINY[F32]
+    g, u, eg, eu = z[:, :f], z[:, f:], ez[:, :f], ez[:, f:]
+    a, da = act64(g, act)
+    ea = 1.2 * eg + MATH * (np.abs(a) + np.abs(g) * 2.0 ** -2)
+    eda = 1.2 * eg + MATH * (1 + np.abs(g) * 2.0 ** -2)
+    if act == "relu":
+        eda = np.where(np.abs(g) <= eg, 1.0, 0.0)
+    out = {"z": (z, ez), "h": (a * u, np.abs(a) * eu + np.abs(u) * ea + ea * eu + 2 * F * np.abs(a * u))}
+    if dh is None:
+        return out
+    dz = np.concatenate([dh * u * da, dh * a], 1)
+    e32 = np.concatenate([np.abs(dh) * (np.abs(u) * eda + np.abs(da) * eu + eda * eu), np.abs(dh) * ea], 1)
+    e32 = e32 + 3 * F * np.abs(dz) + TINY[F32]
+    e16 = e32 + UNIT[dtype] * (np.abs(dz) + e32) + TINY[dtype]
+    m = x.shape[0]
+    out["db"] = (dz.sum(0), e32.sum(0) + (m + 4) * F * np.abs(dz).sum(0))
+    out["dx"] = (dz @ w.T, e16 @ np.abs(w).T + (2 * f + 4) * F * ((np.abs(dz) + e16) @ np.abs(w).T))
+    out["dw"] = (x.T @ dz, np.abs(x).T @ e16 + (m + 4) * F * (np.abs(x).T @ (np.abs(dz) + e16)))
+    return out
+
+
+def check(got, pair, dtype, what):
+    want, bound = pair
+    within(got, want, bound + (0 if dtype == F32 else UNIT[dtype] * (np.abs(want) + bound) + TINY[dtype]), what)
+
+
+SHAPES = [(1, 8, 8), (1, 1024, 512), (1, 7, 3), (2, 64, 32), (5, 33, 40), (16, 256, 136), (17, 100, 64), (33, 1000, 9),
+          (64, 64, 64), (100, 72, 200), (130, 520, 129), (257, 40, 264), (300, 136, 1000)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("m,k,f", SHAPES)
+def test_forward_and_backward(bench, dtype, m, k, f):
+    L = bench.L
+    act = sorted(ACTS)[(m + k + f) % 5]
+    x, w, b, dh = data(m, k, f, dtype, bias=(m + f) % 2 == 0)
+    ref = model(x, w, b, dh, act, dtype)
+    tx, tw, tb, th = bench.tensor(x, dtype), bench.tensor(w, dtype), None if b is None else bench.tensor(b), bench.tensor(dh, dtype)
+    for hd in (dtype, F32):
+        h, z = bench.unset((m, f), hd), bench.unset((m, 2 * f))
+        bench.ok(L.pg_amd_gated(tx, tw, tb, ACTS[act], h, z))
+        check(bench.read(h), ref["h"], hd, "h")
+        check(bench.read(z), ref["z"], F32, "z")
+        alone = bench.unset((m, f), hd)  # without z: the same values
+        bench.ok(L.pg_amd_gated(tx, tw, tb, ACTS[act], alone, None))
+        check(bench.read(alone), ref["h"], hd, "h alone")
+    for gd in (dtype, F32):
+        dx, dw, db = bench.unset((m, k), gd), bench.unset((k, 2 * f), gd), bench.unset((2 * f,))
+        bench.ok(L.pg_amd_gated_backward(tx, tw, z, th, ACTS[act], dx, dw, db))
+        check(bench.read(dx), ref["dx"], gd, "dx")
+        check(bench.read(dw), ref["dw"], gd, "dw")
+        check(bench.read(db), ref["db"], F32, "db")
+
+
+@pytest.mark.parametrize("act", sorted(ACTS))
+@pytest.mark.parametrize("m,f", [(3, 24), (40, 24), (200, 130)])
+def test_every_activation(bench, act, m, f):
+    L, dtype, k = bench.L, BF16, 48
+    x, w, b, dh = data(m, k, f, dtype, True, seed=3)
+    w = rounded(w * 6, dtype)  # gates into their flat ends
+    ref = model(x, w, b, dh, act, dtype)
+    t = [bench.tensor(x, dtype), bench.tensor(w, dtype), bench.tensor(b)]
+    h, z = bench.unset((m, f), F32), bench.unset((m, 2 * f))
+    bench.ok(L.pg_amd_gated(*t, ACTS[act], h, z))
+    check(bench.read(h), ref["h"], F32, "h")
+    dx, dw = bench.unset((m, k), F32), bench.unset((k, 2 * f), F32)
+    dh32 = bench.tensor(dh)  # an f32 upstream grad
+    bench.ok(L.pg_amd_gated_backward(t[0], t[1], z, dh32, ACTS[act], dx, dw, None))
+    check(bench.read(dx), ref["dx"], F32, "dx")
+    check(bench.read(dw), ref["dw"], F32, "dw")
+
+
+def test_each_grad_alone_and_strided_inputs(bench):
+    L, dtype, m, k, f = bench.L, F16, 37, 56, 48
+    x, w, b, dh = data(m, k, f, dtype, True, seed=5)
+    ref = model(x, w, b, dh, "silu", dtype)
+    tx, tw, th = (bench.transposed(v, dtype) for v in (x, w, dh))
+    h, z = bench.unset((m, f), dtype), bench.unset((m, 2 * f))
+    bench.ok(L.pg_amd_gated(tx, tw, bench.tensor(b), 3, h, z))
+    check(bench.read(h), ref["h"], dtype, "h")
+    for name, shape, gd in (("dx", (m, k), dtype), ("dw", (k, 2 * f), F32), ("db", (2 * f,), F32)):
+        g = bench.unset(shape, gd)
+        args = {"dx": None, "dw": None, "db": None, name: g}
+        bench.ok(L.pg_amd_gated_backward(tx, tw, z, th, 3, args["dx"], args["dw"], args["db"]))
+        check(bench.read(g), ref[name], gd, name)
+
+
+def test_a_nan_stays_in_its_row(bench):
+    L, m, k, f = bench.L, 20, 40, 16
+    x, w, b, dh = data(m, k, f, BF16, False)
+    x[7, 3] = np.nan
+    x[9, 0] = np.inf
+    h = bench.unset((m, f), F32)
+    bench.ok(L.pg_amd_gated(bench.tensor(x, BF16), bench.tensor(w, BF16), None, 3, h, None))
+    got = bench.read(h)
+    assert np.isnan(got[7]).all()
+    rows = [i for i in range(m) if i not in (7, 9)]
+    assert np.isfinite(got[rows]).all()
+
+
+def test_empty_batches(bench):
+    L, k, f = bench.L, 16, 24
+    w = bench.tensor(np.ones((k, 2 * f)), BF16)
+    nd, sh = shape_arg((0, k))
+    x0 = L.pg_tensor_empty_dtype(BF16, nd, sh)
+    h0 = L.pg_tensor_empty_dtype(BF16, 2, shape_arg((0, f))[1])
+    z0 = L.pg_tensor_empty_dtype(F32, 2, shape_arg((0, 2 * f))[1])
+    if not (x0 and h0 and z0):
+        pytest.skip("no tensors without elements")
+    bench.ok(L.pg_amd_gated(x0, w, None, 3, h0, z0))
+    dw = bench.unset((k, 2 * f), F32)
+    bench.ok(L.pg_amd_gated_backward(x0, w, z0, h0, 3, None, dw, None))
+    assert (bench.read(dw) == 0).all()
+    for t in (x0, h0, z0):
+        L.pg_tensor_free(t)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("m,k,f,bias", [(4, 16, 8, True), (64, 128, 256, False), (33, 50, 21, True), (128, 64, 72, True)])
+def test_node(bench, dtype, m, k, f, bias):
+    """f32 nodes, rounded to the 16-bit type; the grads add up over two nodes."""
+    L = bench.L
+    r = np.random.default_rng(11)
+    x, w = r.standard_normal((m, k)).astype(np.float32), (r.uniform(-1, 1, (k, 2 * f)) * k ** -0.5).astype(np.float32)
+    b = (r.standard_normal(2 * f) * 0.1).astype(np.float32) if bias else None
+    dh = (r.standard_normal((m, f)) * 0.5).astype(np.float32)
+    nx, nw, nb = bench.var(x), bench.var(w), bench.var(b) if bias else None
+    ref = model(rounded(x, dtype), rounded(w, dtype), None if b is None else b.astype(np.float64), dh.astype(np.float64),
+                "silu", dtype)
+    seed = bench.tensor(dh)
+    for times in (1, 2):
+        h = bench.node(L.pg_amd_ag_gated16(nx, nw, nb, 3, dtype))
+        check(L.value(h).astype(np.float64), ref["h"], F32, "h")
+        if times == 2:  # two nodes over the same leaves
+            h = bench.node(L.pg_ag_add(h, bench.node(L.pg_amd_ag_gated16(nx, nw, nb, 3, dtype))))
+        L.pg_amd_backward_from(h, seed)
+        for n, name in ((nx, "dx"), (nw, "dw")) + (((nb, "db"),) if bias else ()):
+            want, bound = ref[name]
+            within(L.grad(n), times * want, times * bound + 2 * F * np.abs(want), name)
+
+
+def test_node_feeds_a_linear_layer(bench):
+    """gated16 then linear16, their grads against differences of the f32 formula."""
+    L, m, k, f, n = bench.L, 24, 32, 40, 16
+    r = np.random.default_rng(2)
+    x, wg, wd = r.standard_normal((m, k)), r.standard_normal((k, 2 * f)) * 0.3, r.standard_normal((f, n)) * 0.3
+    x, wg, wd = (rounded(v, F16) for v in (x, wg, wd))  # nothing lost by the operands' rounding
+
+    def loss(x, wg, wd):
+        z = x @ wg
+        g, u = z[:, :f], z[:, f:]
+        return ((g / (1 + np.exp(-g)) * u) @ wd).sum()
+
+    nodes = [bench.var(v) for v in (x, wg, wd)]
+    h = bench.node(L.pg_amd_ag_gated16(nodes[0], nodes[1], None, 3, F16))
+    y = bench.node(L.pg_amd_ag_linear16(h, nodes[2], None, 0, F16))
+    total = bench.node(L.pg_ag_sum_all(y))
+    L.pg_backward(total)
+    for which, v in enumerate((x, wg, wd)):
+        got = L.grad(nodes[which]).astype(np.float64)
+        scale = np.abs(got).max()
+        for _ in range(12):
+            at = tuple(r.integers(0, s) for s in v.shape)
+            args = [[a.copy() for a in (x, wg, wd)] for _ in range(2)]
+            args[0][which][at] += 1e-5
+            args[1][which][at] -= 1e-5
+            slope = (loss(*args[0]) - loss(*args[1])) / 2e-5
+            # three roundings to f16 (h, dz, the upstream grad) of values under the largest grad's scale
+            assert abs(got[at] - slope) <= 8 * UNIT[F16] * scale, (which, at)
+
+
+def test_node_without_grads_keeps_nothing(bench):
+    L = bench.L
+    x, w = bench.var(np.ones((4, 8)), False), bench.var(np.ones((8, 16)), False)
+    n = bench.node(L.pg_amd_ag_gated16(x, w, None, 3, BF16))
+    assert not L.node(n).ctx and not L.node(n).requires_grad
+
+
+def test_one_tensor_as_both_operands(bench):
+    """x and W in one storage: each of their grads lands in it."""
+    L, k = bench.L, 32
+    r = np.random.default_rng(4)
+    v = rounded(r.standard_normal((k, k)) * 0.2, F16)
+    dh = rounded(r.standard_normal((k, k // 2)), F16)
+    n = bench.var(v)
+    h = bench.node(L.pg_amd_ag_gated16(n, n, None, 3, F16))
+    ref = model(v, v, None, dh, "silu", F16)
+    check(L.value(h), ref["h"], F32, "h")
+    L.pg_amd_backward_from(h, bench.tensor(dh))
+    within(L.grad(n), ref["dx"][0] + ref["dw"][0], ref["dx"][1] + ref["dw"][1] + 2 * F * np.abs(ref["dx"][0] + ref["dw"][0]),
+           "grad")
+
+
+def test_refusals(bench):
+    L = bench.L
+    x, w, b = bench.tensor(np.ones((4, 8)), BF16), bench.tensor(np.ones((8, 12)), BF16), bench.tensor(np.ones(12))
+    h, z = bench.unset((4, 6), BF16), bench.unset((4, 12))
+    good = (x, w, b, 3, h, z)
+    bench.ok(L.pg_amd_gated(*good))
+    bench.refused(L.pg_amd_gated(None, *good[1:]), "null")
+    bench.refused(L.pg_amd_gated(x, w, b, 5, h, z), "act")
+    bench.refused(L.pg_amd_gated(x, w, b, -1, h, z), "act")
+    bench.refused(L.pg_amd_gated(bench.tensor(np.ones((4, 8)), F16), *good[1:]), "dtype")
+    bench.refused(L.pg_amd_gated(bench.tensor(np.ones((4, 8))), *good[1:]), "dtype")
+    bench.refused(L.pg_amd_gated(bench.tensor(np.ones((4, 7)), BF16), *good[1:]), "x [M, K]")
+    bench.refused(L.pg_amd_gated(x, bench.tensor(np.ones((8, 11)), BF16), None, 3, h, z), "x [M, K]")
+    bench.refused(L.pg_amd_gated(x, w, bench.tensor(np.ones(6)), 3, h, z), "x [M, K]")
+    bench.refused(L.pg_amd_gated(x, w, b, 3, bench.unset((4, 12), BF16), z), "h must be")
+    bench.refused(L.pg_amd_gated(x, w, b, 3, bench.unset((4, 6), F16), z), "h must be")
+    bench.refused(L.pg_amd_gated(x, w, b, 3, None, z), "h must be")
+    bench.refused(L.pg_amd_gated(x, w, b, 3, h, bench.unset((4, 6))), "h must be")
+    square = bench.tensor(np.ones((8, 16)), BF16)
+    xs = bench.tensor(np.ones((8, 8)), BF16)
+    bench.refused(L.pg_amd_gated(xs, square, None, 3, xs, None), "overlaps")
+    dh, dx, dw, db = (bench.unset(s, BF16) for s in ((4, 6), (4, 8), (8, 12), (12,)))
+    db = bench.unset((12,))
+    bench.ok(L.pg_amd_gated_backward(x, w, z, dh, 3, dx, dw, db))
+    bench.refused(L.pg_amd_gated_backward(x, w, None, dh, 3, dx, dw, db), "z f32")
+    bench.refused(L.pg_amd_gated_backward(x, w, z, None, 3, dx, dw, db), "dh")
+    bench.refused(L.pg_amd_gated_backward(x, w, z, bench.unset((4, 6), F16), 3, dx, dw, db), "dh")
+    bench.refused(L.pg_amd_gated_backward(x, w, z, dh, 3, bench.unset((4, 6), BF16), dw, db), "dx must be")
+    bench.refused(L.pg_amd_gated_backward(x, w, z, dh, 3, dx, bench.unset((8, 12), F16), db), "dx must be")
+    bench.refused(L.pg_amd_gated_backward(x, w, z, dh, 3, dx, dw, bench.unset((6,))), "dx must be")
+    bench.refused(L.pg_amd_gated_backward(x, w, z, dh, 3, x, dw, db), "overlaps")
+    nx, nw = bench.var(np.ones((4, 8))), bench.var(np.ones((8, 12)))
+    for bad, word in (((None, nw, None, 3, BF16), "null"), ((nx, nw, None, 3, F32), "dtype"),
+                      ((nx, nw, None, 9, BF16), "act"), ((nx, nx, None, 3, BF16), "x [M, K]")):
+        assert not L.pg_amd_ag_gated16(*bad)
+        assert word in L.pg_autograd_last_error().decode()
