@@ -4,20 +4,40 @@ from __future__ import annotations
 import ctypes as C
 
 import numpy as np
-import torch
 
 from picograd_amd.capi import BF16, F16, F32, shape_arg
 
-TORCH = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}
 # half a unit in the last place, relative
 UNIT = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
 TINY = {F32: 2.0 ** -150, F16: 2.0 ** -25, BF16: 2.0 ** -134}  # half the smallest subnormal
 NAMES = {F32: "f32", F16: "f16", BF16: "bf16"}
 
 
+def to_bits(a, dtype) -> np.ndarray:
+    """a as f32, or as the bits of a 16-bit dtype (rounded to nearest even)."""
+    a = np.asarray(a, np.float32)
+    if dtype == F32:
+        return a
+    if dtype == F16:
+        with np.errstate(over="ignore"):
+            return a.astype(np.float16).view(np.uint16)
+    u = np.atleast_1d(a).view(np.uint32)
+    near = ((u + np.uint32(0x7FFF) + ((u >> 16) & np.uint32(1))) >> 16).astype(np.uint16)
+    return np.where(np.isnan(a), np.uint16(0x7FC0), near.reshape(a.shape))
+
+
+def from_bits(bits, dtype) -> np.ndarray:
+    """The values in 64 bits."""
+    if dtype == F32:
+        return np.asarray(bits, np.float32).astype(np.float64)
+    if dtype == F16:
+        return np.asarray(bits).view(np.float16).astype(np.float64)
+    return (np.asarray(bits).astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+
+
 def rounded(a, dtype) -> np.ndarray:
     """a's values rounded to dtype, in 64 bits."""
-    return torch.as_tensor(np.asarray(a, np.float32)).to(TORCH[dtype]).double().numpy()
+    return from_bits(to_bits(a, dtype), dtype)
 
 
 class Bench:
@@ -33,9 +53,7 @@ class Bench:
             setattr(self, name, fn)
 
     def tensor(self, a, dtype=F32) -> int:
-        a = np.asarray(a, np.float32)
-        bits = a if dtype == F32 else torch.as_tensor(a).to(TORCH[dtype]).view(torch.int16).numpy().view(np.uint16)
-        t = self.L.tensor(bits, dtype)
+        t = self.L.tensor(to_bits(a, dtype), dtype)
         self.frees.append((self.L.pg_tensor_free, t))
         return t
 
@@ -66,13 +84,7 @@ class Bench:
         return n
 
     def read(self, t) -> np.ndarray:
-        return self.values(self.L.read(t), self.L.tinfo(t).dtype)
-
-    @staticmethod
-    def values(bits, dtype) -> np.ndarray:
-        if dtype == F32:
-            return bits.astype(np.float64)
-        return torch.as_tensor(bits.view(np.int16).copy()).view(TORCH[dtype]).double().numpy()
+        return from_bits(self.L.read(t), self.L.tinfo(t).dtype)
 
     def ok(self, done):
         assert done, self.L.pg_autograd_last_error().decode() or self.L.pg_amd_last_error().decode()
