@@ -55,7 +55,12 @@ static bool launch(const pg_tensor *logits, const pg_tensor *top, const pg_tenso
                           .label = labels ? labels->dev : NULL, .top = (int)top->shape[1],
                           .temperature = cfg->temperature, .alpha = cfg->alpha, .scale = cfg->scale, .up = up,
                           .loss = loss, .ds = ds, .ds_dtype = (int)ds_dtype, .beta = beta};
-    if (pgd_check(pgk_distill(&a, pgd_stream()), WHAT))
+    const size_t wb = pgk_distill_workspace(&a);
+    void *ws = wb ? pgd_malloc(wb) : NULL; /* freed in stream order */
+    const bool ok = (ws || !wb) && pgd_check(pgk_distill(&a, ws, pgd_stream()), WHAT);
+    if (ws)
+        pgd_free(ws, wb);
+    if (ok)
         return true;
     pga_set_err("%s", pg_amd_last_error());
     return false;

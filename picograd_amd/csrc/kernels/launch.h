@@ -302,7 +302,8 @@ int pgk_mx4_matmul(const pgk_mx4 *x, const pgk_mx4 *w, void *y, int y_dtype, pgk
  * idx [n, top], label [n] or NULL; indices are whole numbers held as f32, one
  * outside [0, v) is no entry.  dtypes: 0 = f32, 1 = f16, 2 = bf16; ds_dtype is
  * dtype or 0.  up: a device scalar the grad is scaled by, or NULL.  beta (f32
- * ds): added to ds.  ds may be s itself (one dtype).  loss may be NULL. */
+ * ds): added to ds.  ds may be s itself (one dtype).  loss may be NULL.
+ * ws: pgk_distill_workspace bytes. */
 #define PGK_DISTILL_TOP 256             /* entries per row at most */
 #define PGK_DISTILL_MAX_V ((size_t)1 << 24) /* whole numbers that f32 holds */
 typedef struct {
@@ -319,7 +320,8 @@ typedef struct {
     void *ds;
     int ds_dtype, beta;
 } pgk_distill_args;
-int pgk_distill(const pgk_distill_args *a, pgk_stream s);
+size_t pgk_distill_workspace(const pgk_distill_args *a);
+int pgk_distill(const pgk_distill_args *a, void *ws, pgk_stream s);
 
 /* multi-tensor SGD */
 typedef struct {

@@ -77,7 +77,7 @@ def data(n, v, top, dtype, labels, seed=0):
     r = np.random.default_rng(seed)
     s = rounded(r.standard_normal((n, v)) * 2, dtype)
     t = rounded(r.standard_normal((n, top)) * 2 + 4, F32)
-    idx = np.stack([r.permutation(v)[:top] if top <= v else r.integers(0, v, top) for _ in range(n)]).astype(np.float64)
+    idx = np.stack([r.choice(v, top, replace=top > v) for _ in range(n)]).astype(np.float64)
     idx[r.random((n, top)) < 0.15] = -1
     lab = r.integers(0, v, n).astype(np.float64) if labels else None
     if labels:
@@ -141,6 +141,24 @@ def test_long_rows(bench, dtype, n, v):
     if n > 2:
         idx[2, :3] = [0, v - 1, v // 2]
     check(bench, s, t, idx, lab, 2.0, 0.5, 1.0, dtype)
+
+
+@pytest.mark.parametrize("dtype,n,v", [(BF16, 300, 66001), (F32, 300, 33001), (F16, 600, 33003), (F32, 600, 16500),
+                                       (BF16, 1100, 8300), (F32, 1100, 4200), (F16, 1700, 2100), (F32, 1900, 300)])
+def test_many_rows(bench, dtype, n, v):
+    """Blocks that take several rows each, rows of every alignment among them."""
+    s, t, idx, lab = data(n, v, 5, dtype, True)
+    check(bench, s, t, idx, lab, 1.7, 0.5, 1.0 / n if dtype != F16 else 1.0, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("n,v", [(200, 600), (700, 64), (50, 256), (33, 65), (9, 257)])
+def test_short_rows(bench, dtype, n, v):
+    for top in (1, 16, 17, 64, 65):
+        if top <= v:
+            s, t, idx, lab = data(n, v, top, dtype, True, seed=top)
+            check(bench, s, t, idx, lab, 2.0, 0.5, 1.0, dtype)
+            check(bench, s, t, idx, None, 1.0, 1.0, 1.0, dtype, out=F32)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
