@@ -8,7 +8,7 @@
 
 struct pg_amd_mx4 {
     pgk_mx4 q;
-    size_t code_bytes, scale_bytes;
+    size_t code_bytes, power_bytes;
     int axis; /* the source's dimension that the blocks run along */
 };
 
@@ -16,30 +16,30 @@ static void release(pg_amd_mx4 *m)
 {
     if (m->q.codes)
         pgd_free(m->q.codes, m->code_bytes);
-    if (m->q.scales)
-        pgd_free(m->q.scales, m->scale_bytes);
-    m->q.codes = m->q.scales = NULL;
+    if (m->q.powers)
+        pgd_free(m->q.powers, m->power_bytes);
+    m->q.codes = m->q.powers = NULL;
 }
 
 static bool reserve(pg_amd_mx4 *m, size_t rows, size_t cols)
 {
-    pgk_mx4_shape(&m->q, rows, cols, &m->code_bytes, &m->scale_bytes);
+    pgk_mx4_shape(&m->q, rows, cols, &m->code_bytes, &m->power_bytes);
     m->q.codes = pgd_malloc(m->code_bytes);
-    m->q.scales = pgd_malloc(m->scale_bytes);
-    if (m->q.codes && m->q.scales)
+    m->q.powers = pgd_malloc(m->power_bytes);
+    if (m->q.codes && m->q.powers)
         return true;
     release(m);
     return false;
 }
 
 /* sizes that the kernels' 32-bit indices hold */
-static bool fits(size_t rows, size_t cols) { return rows && cols && rows <= 0x3fffffff && cols <= 0x3fffffff; }
+static bool fits(size_t rows, size_t cols) { return rows && cols && rows <= 0x3fffffff && cols <= (size_t)1 << 24; }
 
 pg_amd_mx4 *pg_amd_mx4_quantize(const pg_tensor *t, int axis)
 {
     static const char *const what = "pg_amd_mx4_quantize";
-    if (!t || t->ndim != 2 || (axis != 0 && axis != 1) || !fits(t->shape[0], t->shape[1])) {
-        pga_set_err("%s: needs a matrix that is not empty and axis 0 or 1", what);
+    if (!t || t->ndim != 2 || (axis != 0 && axis != 1) || !fits(t->shape[1 - axis], t->shape[axis])) {
+        pga_set_err("%s: needs a matrix that is not empty, of up to 2^24 along axis 0 or 1", what);
         return NULL;
     }
     if (!pgd_ok()) {
@@ -70,7 +70,7 @@ void pg_amd_mx4_free(pg_amd_mx4 *q)
     free(q);
 }
 
-size_t pg_amd_mx4_bytes(const pg_amd_mx4 *q) { return q ? q->code_bytes + q->scale_bytes : 0; }
+size_t pg_amd_mx4_bytes(const pg_amd_mx4 *q) { return q ? q->code_bytes + q->power_bytes : 0; }
 
 bool pg_amd_mx4_dequantize(const pg_amd_mx4 *q, pg_tensor *out)
 {
@@ -109,9 +109,15 @@ bool pg_amd_mx4_matmul(const pg_tensor *x, const pg_amd_mx4 *w, pg_tensor *y)
         return false;
     pgo_output(y);
     pg_amd_mx4 t = {0}; /* x in 4 bits, freed in stream order */
-    const bool ok = reserve(&t, x->shape[0], x->shape[1]) &&
-                    pgd_check(pgk_mx4_quantize(&t.q, c->dev, (int)c->dtype, 0, pgd_stream()), what) &&
-                    pgd_check(pgk_mx4_matmul(&t.q, &w->q, y->dev, (int)y->dtype, pgd_stream()), what);
+    bool ok;
+    if (pgk_mx4_few_rows(x->shape[0]))
+        ok = pgd_check(pgk_mx4_matmul_few(c->dev, (int)c->dtype, x->shape[0], &w->q, y->dev, (int)y->dtype,
+                                          pgd_stream()),
+                       what);
+    else
+        ok = reserve(&t, x->shape[0], x->shape[1]) &&
+             pgd_check(pgk_mx4_quantize(&t.q, c->dev, (int)c->dtype, 0, pgd_stream()), what) &&
+             pgd_check(pgk_mx4_matmul(&t.q, &w->q, y->dev, (int)y->dtype, pgd_stream()), what);
     release(&t);
     pg_tensor_free(own);
     if (!ok)

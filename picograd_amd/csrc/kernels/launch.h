@@ -277,24 +277,32 @@ int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float *z, size_t 
                   float *db, int db_beta, void *ws, pgk_stream s);
 
 /* 4-bit matrices with a power of two per 32 values along the reduction
- * (mx4.hip).  codes: [rows] rows of `pitch` bytes (16 per block of 32 values,
- * value 2 i in the low half of byte i), zeros past cols.  scales: exponents
- * biased by 127 (255: the block is NaN) as [ceil(blocks / 8)][rows_p][8], rows_p
- * = rows rounded up to 16; those past the last row or block are unset. */
+ * (mx4.hip), in the order in which the 16 x 16 x 128 matrix instruction takes
+ * its operands.  Rows come in tiles of 16, the reduction in steps of 128 (four
+ * blocks of 32), an even number of them:
+ *   codes  [tiles][steps][64][16 bytes]: entry l of a step is block l / 16 of row
+ *          l % 16, value 2 i in the low half of byte i
+ *   powers [tiles][steps / 2][64][2]: the exponents, biased by 127 (255: the
+ *          block is NaN), of entry l in the two steps
+ * Codes past the last column are 0 (a power there is any but 255); past the
+ * last row both are unset. */
 typedef struct {
     size_t rows, cols; /* cols: along the reduction */
-    size_t pitch, rows_p;
-    uint8_t *codes, *scales;
+    size_t tiles, steps;
+    uint8_t *codes, *powers;
 } pgk_mx4;
-/* sets rows, cols, pitch and rows_p; the byte sizes of codes and scales */
-void pgk_mx4_shape(pgk_mx4 *q, size_t rows, size_t cols, size_t *code_bytes, size_t *scale_bytes);
+/* sets rows, cols, tiles and steps; the byte sizes of codes and powers */
+void pgk_mx4_shape(pgk_mx4 *q, size_t rows, size_t cols, size_t *code_bytes, size_t *power_bytes);
 /* q = src, dense of dtype 0 = f32, 1 = f16, 2 = bf16: [rows, cols], or with
  * `trans` [cols, rows] */
 int pgk_mx4_quantize(const pgk_mx4 *q, const void *src, int dtype, int trans, pgk_stream s);
 /* dst (dense, as src above) = the values q stands for */
 int pgk_mx4_dequantize(const pgk_mx4 *q, void *dst, int dtype, int trans, pgk_stream s);
 /* y [x->rows, w->rows] of y_dtype = x w^T over their shared cols, f32
- * accumulation */
+ * accumulation; _few: x [m, w->cols] dense of dtype, rounded in the launch, for
+ * the m that pgk_mx4_few_rows takes */
+int pgk_mx4_few_rows(size_t m);
+int pgk_mx4_matmul_few(const void *x, int dtype, size_t m, const pgk_mx4 *w, void *y, int y_dtype, pgk_stream s);
 int pgk_mx4_matmul(const pgk_mx4 *x, const pgk_mx4 *w, void *y, int y_dtype, pgk_stream s);
 
 /* Distillation from a teacher's top logits (distill.hip): per-row losses

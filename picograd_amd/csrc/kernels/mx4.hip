@@ -1,40 +1,56 @@
 // Matrices in 4 bits: e2m1 values (0, .5, 1, 1.5, 2, 3, 4, 6 and their
 // negatives) with one power of two for each 32 along the reduction, and their
-// product on the block-scaled matrix instructions.
+// product on the block-scaled matrix instruction
+// (v_mfma_scale_f32_16x16x128_f8f6f4, four times the rate of the 16-bit ones).
+//
+// The block's power is 2^(floor(log2 max |v|) - 2), so the largest magnitude
+// lies in [4, 8) units; what is past 6 becomes 6, the rest is rounded to
+// nearest, ties to the even code.  y = Q(x) Q(W)^T over both operands' rows: the
+// products of two 4-bit values are exact, their sums f32, y is rounded once.
+//
+// Both operands are held in the instruction's own order (pgk_mx4), so a wave
+// loads a 16-row operand of 128 values as 1 KiB in a row, to registers or to LDS,
+// with no padding, swizzle or bounds check along the reduction.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include "convert16.h"
+#include <math.h>
+
+#include <type_traits>
+
+#include "gemm_tile.h"
 #include "launch.h"
 
 namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+#define INLINE __attribute__((always_inline)) // of a lambda
 
 constexpr int kBlock = 32; // values under one power of two
 
-__device__ __forceinline__ float ld_any(int dtype, const void *p, size_t i)
+// the bytes of step s of tile t, and of its powers (of the pair of steps s / 2)
+__device__ __forceinline__ uint8_t *codes_at(const pgk_mx4 &q, size_t t, size_t s)
 {
-    return dtype == 0 ? ((const float *)p)[i] : dtype == 1 ? (float)((const _Float16 *)p)[i] : (float)((const __bf16 *)p)[i];
+    return q.codes + (t * q.steps + s) * 1024;
 }
-__device__ __forceinline__ void st_any(int dtype, void *p, size_t i, float v)
+__device__ __forceinline__ uint16_t *powers_at(const pgk_mx4 &q, size_t t, size_t s)
 {
-    if (dtype == 0)
-        ((float *)p)[i] = v;
-    else
-        ((uint16_t *)p)[i] = to16(dtype, v);
+    return (uint16_t *)(q.powers + (t * (q.steps / 2) + s / 2) * 128);
 }
+
+// ---------------------------------------------------------------- rounding
 
 // The block's exponent byte for its largest magnitude, given as the bits of
 // |v| (whose order is that of the magnitudes, infinities and NaN last):
 // floor(log2) - 2 with the bias, 0 at least; 255 for a block with either.
-__device__ __forceinline__ uint32_t scale_byte(uint32_t top)
+__device__ __forceinline__ uint32_t power_byte(uint32_t top)
 {
     const uint32_t e = top >> 23;
     return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
 }
-__device__ __forceinline__ float scale_of(uint32_t byte)
+__device__ __forceinline__ float power_of(uint32_t byte)
 {
     return byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u); // 2^-127 is subnormal
 }
@@ -50,123 +66,660 @@ __device__ __forceinline__ uint32_t pack8(const float *v, float scale)
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], scale, 3);
     return r;
 }
-
-__device__ __forceinline__ uint8_t *scale_at(const pgk_mx4 &q, size_t row, size_t blk)
+// a block of 32 values in 4 bits, and its exponent byte
+__device__ __forceinline__ uint4 round_block(const float *v, uint32_t &byte)
 {
-    return q.scales + ((blk >> 3) * q.rows_p + row) * 8 + (blk & 7);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kBlock; ++i) {
+        const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+        top = a > top ? a : top;
+    }
+    byte = power_byte(top);
+    if (byte == 255)
+        return make_uint4(0, 0, 0, 0);
+    const float s = power_of(byte);
+    return make_uint4(pack8(v, s), pack8(v + 8, s), pack8(v + 16, s), pack8(v + 24, s));
 }
 
-// One thread per block of 32 values.
-__global__ void __launch_bounds__(256) k_mx4_quantize(pgk_mx4 q, const void *__restrict__ src, int dtype, int trans)
+// a block of a row as f32: 16-byte loads (VEC: p is aligned) or one by one;
+// values at and past `left` are 0
+template <class T, bool VEC>
+__device__ __forceinline__ void load_block(const T *p, int left, float *v)
 {
-    const size_t nb = q.pitch / 16, n = nb * q.rows;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        // along the source's contiguous dimension
-        const size_t row = trans ? i % q.rows : i / nb, blk = trans ? i / q.rows : i % nb;
+    if (VEC && left >= kBlock) {
+        constexpr int E = 16 / sizeof(T);
+        typedef T tv __attribute__((ext_vector_type(E)));
+#pragma unroll
+        for (int i = 0; i < kBlock / E; ++i) {
+            const tv q = ((const tv *)p)[i];
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                v[i * E + j] = (float)q[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i)
+            v[i] = i < left ? (float)p[i] : 0.0f;
+    }
+}
+
+// Blocks along the source's rows: a wave makes two steps of one tile, lane l
+// the blocks that are entry l of each, so a lane rounds a block by itself and
+// the codes leave as whole kilobytes.  Bound by the stream of the source.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) k_mx4_rows(pgk_mx4 q, const T *__restrict__ src)
+{
+    const int lane = (int)threadIdx.x & 63;
+    const size_t pairs = q.steps / 2, n = q.tiles * pairs;
+    for (size_t i = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (size_t)gridDim.x * 4) {
+        const size_t t = i / pairs, s = (i - t * pairs) * 2, row = t * 16 + (lane & 15);
+        uint32_t both = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const size_t c = (s + h) * 128 + (size_t)(lane >> 4) * kBlock;
+            float v[kBlock];
+            const bool in = row < q.rows && c < q.cols;
+            load_block<T, VEC>(src + (in ? row * q.cols + c : 0), in ? (int)(q.cols - c < kBlock ? q.cols - c : kBlock) : 0, v);
+            uint32_t byte;
+            ((uint4 *)codes_at(q, t, s + h))[lane] = round_block(v, byte);
+            both |= byte << (8 * h);
+        }
+        powers_at(q, t, s)[lane] = (uint16_t)both;
+    }
+}
+
+// Blocks down the source's columns ([cols, rows]): a thread takes block `wave`
+// of two steps of one column, so that a wave reads whole row pieces of 64
+// columns (four tiles).  Bound by the stream of the source.
+template <class T>
+__global__ void __launch_bounds__(256) k_mx4_columns(pgk_mx4 q, const T *__restrict__ src)
+{
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const size_t row = (size_t)blockIdx.x * 64 + lane, s = (size_t)blockIdx.y * 2, t = row >> 4;
+    if (t >= q.tiles)
+        return;
+    const int entry = wave * 16 + (lane & 15);
+    uint32_t both = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const size_t c0 = (s + h) * 128 + (size_t)wave * kBlock;
         float v[kBlock];
-        uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < kBlock; ++j) {
-            const size_t c = blk * kBlock + j;
-            v[j] = c < q.cols ? ld_any(dtype, src, trans ? c * q.rows + row : row * q.cols + c) : 0.0f;
-            const uint32_t a = __float_as_uint(v[j]) & 0x7fffffffu;
-            top = a > top ? a : top;
-        }
-        const uint32_t b = scale_byte(top);
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (b != 255) {
-            const float s = scale_of(b);
-            w = make_uint4(pack8(v, s), pack8(v + 8, s), pack8(v + 16, s), pack8(v + 24, s));
-        }
-        *(uint4 *)(q.codes + row * q.pitch + blk * 16) = w;
-        *scale_at(q, row, blk) = (uint8_t)b;
+        for (int j = 0; j < kBlock; ++j)
+            v[j] = row < q.rows && c0 + j < q.cols ? (float)src[(c0 + j) * q.rows + row] : 0.0f;
+        uint32_t byte;
+        ((uint4 *)codes_at(q, t, s + h))[entry] = round_block(v, byte);
+        both |= byte << (8 * h);
     }
+    powers_at(q, t, s)[entry] = (uint16_t)both;
 }
 
-__device__ __forceinline__ float value_of(uint32_t code, uint32_t byte)
+// ---------------------------------------------------------------- reading back
+
+// the eight values of a dword of codes
+__device__ __forceinline__ void unpack8(uint32_t w, uint32_t byte, float *v)
 {
-    const uint32_t m = code & 7;
-    // e2m1: 0, .5, then (1 + m0 / 2) 2^(e - 1)
-    const float a = m < 2 ? 0.5f * (float)m : (float)(2 + (m & 1)) * (float)(1 << (m >> 1)) * 0.25f;
-    const float s = byte == 255 ? __uint_as_float(0x7fc00000u) : scale_of(byte);
-    return (code & 8 ? -a : a) * s;
+    const float s = power_of(byte), bad = __uint_as_float(0x7fc00000u);
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+    const float q[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = byte == 255 ? bad : q[i];
 }
 
-__global__ void __launch_bounds__(256) k_mx4_dequantize(pgk_mx4 q, void *__restrict__ dst, int dtype, int trans)
+// Rows back: four lanes per block, eight values each, along the row.
+template <class O>
+__global__ void __launch_bounds__(256) k_mx4_back_rows(pgk_mx4 q, O *__restrict__ dst)
 {
-    const size_t n = q.rows * q.cols;
+    const size_t per = (q.cols + 7) / 8, n = per * q.rows;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const size_t row = trans ? i % q.rows : i / q.cols, c = trans ? i / q.rows : i % q.cols;
-        const uint32_t code = q.codes[row * q.pitch + c / 2] >> (4 * (c & 1));
-        st_any(dtype, dst, i, value_of(code & 15, *scale_at(q, row, c / kBlock)));
+        const size_t row = i / per, part = i - row * per, c = part * 8, s = c / 128;
+        const int entry = (int)(c / kBlock & 3) * 16 + (int)(row & 15);
+        float v[8];
+        unpack8(((const uint32_t *)codes_at(q, row >> 4, s))[entry * 4 + (part & 3)],
+                powers_at(q, row >> 4, s)[entry] >> (8 * (s & 1)) & 255, v);
+        O *p = dst + row * q.cols + c;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (c + j < q.cols)
+                p[j] = (O)v[j];
     }
 }
 
-// One wave per 32 x 32 tile of y, the operands straight from memory: lane l
-// gives row l % 32 and the block l / 32 of each pair of blocks.
-__global__ void __launch_bounds__(64) k_mx4_tile32(pgk_mx4 x, pgk_mx4 w, void *__restrict__ y, int y_dtype)
+// Columns back, as k_mx4_columns reads them.
+template <class O>
+__global__ void __launch_bounds__(256) k_mx4_back_columns(pgk_mx4 q, O *__restrict__ dst)
 {
-    const int lane = (int)threadIdx.x, lr = lane & 31, lk = lane >> 5;
-    const size_t m0 = (size_t)blockIdx.y * 32, n0 = (size_t)blockIdx.x * 32;
-    const size_t rx = m0 + lr < x.rows ? m0 + lr : x.rows - 1, rw = n0 + lr < w.rows ? n0 + lr : w.rows - 1;
-    const size_t nb = x.pitch / 16;
-    f32x16 acc = {};
-    for (size_t b0 = 0; b0 < nb; b0 += 2) {
-        const size_t b = b0 + lk;
-        uint4 a = make_uint4(0, 0, 0, 0), c = a;
-        int sa = 127, sc = 127;
-        if (b < nb) {
-            a = *(const uint4 *)(x.codes + rx * x.pitch + b * 16);
-            c = *(const uint4 *)(w.codes + rw * w.pitch + b * 16);
-            sa = *scale_at(x, rx, b);
-            sc = *scale_at(w, rw, b);
-        }
-        const v8i va = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-        const v8i vc = {(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0};
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vc, acc, 4, 4, 0, sa, 0, sc);
-    }
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const size_t row = (size_t)blockIdx.x * 64 + lane, s = (size_t)blockIdx.y * 2, t = row >> 4;
+    if (row >= q.rows)
+        return;
+    const int entry = wave * 16 + (lane & 15);
+    const uint32_t both = powers_at(q, t, s)[entry];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const size_t m = m0 + (e >> 2) * 8 + lk * 4 + (e & 3), n = n0 + lr;
-        if (m < x.rows && n < w.rows)
-            st_any(y_dtype, y, m * w.rows + n, acc[e]);
+    for (int h = 0; h < 2; ++h) {
+        const uint4 w = ((const uint4 *)codes_at(q, t, s + h))[entry];
+        const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+        const size_t c0 = (s + h) * 128 + (size_t)wave * kBlock;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float v[8];
+            unpack8(d[j], both >> (8 * h) & 255, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c0 + j * 8 + e < q.cols)
+                    dst[(c0 + j * 8 + e) * q.rows + row] = (O)v[e];
+        }
     }
 }
+
+// ---------------------------------------------------------------- products
+
+// 16 x 16 over a step of 128: the powers of the lanes' entries in byte H of sa
+// and sb; lane l gets column l % 16 of rows 4 (l / 16) .. + 3
+template <int H>
+__device__ __forceinline__ f32x4 mfma4(const uint4 &a, const uint4 &b, const f32x4 &c, uint32_t sa, uint32_t sb)
+{
+    const v8i va = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+    const v8i vb = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, H, (int)sa, H, (int)sb);
+}
+
+// `n` neighbours of a row of y, at most four; v4: whole rows keep the alignment
+// of four
+template <class O>
+__device__ __forceinline__ void store4(O *p, const f32x4 &v, int n, bool v4)
+{
+    typedef O o4 __attribute__((ext_vector_type(4)));
+    if (v4 && n >= 4) {
+        *(o4 *)p = __builtin_convertvector(v, o4);
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (q < n)
+            p[q] = (O)v[q];
+}
+template <class O>
+__device__ __forceinline__ bool rows_keep_four(const O *y, size_t n)
+{
+    return (n & 3) == 0 && (((uintptr_t)y) & (4 * sizeof(O) - 1)) == 0;
+}
+
+// Up to 16 rows of x: a thread block owns 16 columns of y and its waves split
+// the reduction, so the weights stream past once.  A lane rounds its own blocks of x
+// on the way (entry l of a step is one block of one row): no other launch.  The
+// waves' partial tiles are added through LDS in wave order.  Bound by the loads'
+// latency and the launch at 4096 x 4096.
+constexpr int kFewWaves = 8;
+
+template <class T, class O, bool VEC>
+__global__ void __launch_bounds__(kFewWaves * 64, 1) k_mx4_few(const T *__restrict__ x, int m, pgk_mx4 w, O *__restrict__ y)
+{
+    constexpr int U = 4; // steps in flight
+    __shared__ float part[kFewWaves][16][17];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    const int t = xcd_tile((int)blockIdx.x, (int)gridDim.x), steps = (int)w.steps, k = (int)w.cols;
+    // runs of U neighbouring steps, dealt to the waves in turn
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = wave * U; s0 < steps; s0 += kFewWaves * U) {
+        uint4 b[U];
+        uint32_t sb[U / 2];
+#pragma unroll
+        for (int u = 0; u < U; u += 2) {
+            const int s = s0 + u < steps ? s0 + u : s0; // an even number of steps
+            b[u] = ((const uint4 *)codes_at(w, t, s))[lane];
+            b[u + 1] = ((const uint4 *)codes_at(w, t, s + 1))[lane];
+            sb[u / 2] = powers_at(w, t, s)[lane];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = (s0 + u) * 128 + g * kBlock;
+            uint4 a = make_uint4(0, 0, 0, 0);
+            uint32_t sa = 127;
+            if (r < m && c < k) { // (steps past the end have no column)
+                float v[kBlock];
+                load_block<T, VEC>(x + (size_t)r * k + c, k - c, v);
+                a = round_block(v, sa);
+            }
+            // a step past the end repeats one of the weights, whose powers may be NaN
+            if (s0 + u < steps)
+                acc = u & 1 ? mfma4<1>(a, b[u], acc, sa << 8, sb[u / 2]) : mfma4<0>(a, b[u], acc, sa, sb[u / 2]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        part[wave][4 * g + e][r] = acc[e];
+    __syncthreads();
+    const int row = tid >> 4, col = tid & 15;
+    const size_t n = (size_t)t * 16 + col;
+    if (row < m && row < 16 && n < w.rows) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kFewWaves; ++i)
+            v += part[i][row][col];
+        y[(size_t)row * w.rows + n] = (O)v;
+    }
+}
+
+// Products that the tiles below would not spread over the chip: a thread block
+// owns FM x FN tiles of 16 and its KG waves split the reduction, wave v taking the
+// pairs of steps v, v + KG, ... straight from memory into registers, the next
+// pair's loads in flight.  LDS only for the sum of the partial tiles: the upper
+// half of the waves leaves its own, the lower half adds them and leaves the
+// sums, which are added in wave order.  Bound by the loads' latency.
+template <int FM, int FN>
+struct pair_of_steps {
+    uint4 a[2][FM], b[2][FN];
+    uint32_t sa[FM], sb[FN];
+    __device__ __forceinline__ void load(const pgk_mx4 &x, const pgk_mx4 &w, const size_t (&tx)[FM], const size_t (&tw)[FN],
+                                         int s, int lane)
+    {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const uint4 *p = (const uint4 *)codes_at(x, tx[i], s);
+            a[0][i] = p[lane];
+            a[1][i] = p[64 + lane];
+            sa[i] = powers_at(x, tx[i], s)[lane];
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const uint4 *p = (const uint4 *)codes_at(w, tw[j], s);
+            b[0][j] = p[lane];
+            b[1][j] = p[64 + lane];
+            sb[j] = powers_at(w, tw[j], s)[lane];
+        }
+    }
+    __device__ __forceinline__ void multiply(f32x4 (&acc)[FM][FN]) const
+    {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = mfma4<0>(a[0][i], b[0][j], acc[i][j], sa[i], sb[j]);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = mfma4<1>(a[1][i], b[1][j], acc[i][j], sa[i], sb[j]);
+    }
+};
+
+template <int FM, int FN, int KG, class O>
+__global__ void __launch_bounds__(KG * 64, 1) k_mx4_split(pgk_mx4 x, pgk_mx4 w, O *__restrict__ y)
+{
+    constexpr int TM = 16 * FM, TN = 16 * FN, RS = TN + 4;
+    __shared__ float part[KG / 2][TM * RS];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lr = lane & 15, lg = lane >> 4;
+    const int tiles_n = (int)((w.tiles + FN - 1) / FN);
+    const int pid = xcd_tile((int)blockIdx.x, (int)gridDim.x);
+    const size_t m0 = (size_t)(pid / tiles_n) * FM, n0 = (size_t)(pid % tiles_n) * FN; // in tiles of 16
+    const int steps = (int)x.steps;
+    size_t tx[FM], tw[FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+        tx[i] = m0 + i < x.tiles ? m0 + i : x.tiles - 1;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+        tw[j] = n0 + j < w.tiles ? n0 + j : w.tiles - 1;
+    f32x4 acc[FM][FN] = {};
+    pair_of_steps<FM, FN> cur, next;
+    int s = wave * 2;
+    if (s < steps)
+        cur.load(x, w, tx, tw, s, lane);
+    for (; s < steps; s += 2 * KG) {
+        const int ahead = s + 2 * KG;
+        if (ahead < steps)
+            next.load(x, w, tx, tw, ahead, lane);
+        cur.multiply(acc);
+        cur = next;
+    }
+    auto at = [&](int slot, int i, int j, int e) -> float & {
+        return part[slot][(i * 16 + 4 * lg + e) * RS + j * 16 + lr];
+    };
+    if (wave >= KG / 2)
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    at(wave - KG / 2, i, j, e) = acc[i][j][e];
+    __syncthreads();
+    if (wave < KG / 2) // each in its own slot
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    at(wave, i, j, e) += acc[i][j][e];
+    __syncthreads();
+    const size_t M = x.rows, N = w.rows;
+    const bool v4 = rows_keep_four(y, N);
+#pragma unroll 1
+    for (int i = tid; i < TM * TN / 4; i += KG * 64) {
+        const int row = i / (TN / 4), c4 = i % (TN / 4) * 4;
+        const size_t gm = m0 * 16 + row, gn = n0 * 16 + c4;
+        if (gm >= M || gn >= N)
+            continue;
+        f32x4 v = *(const f32x4 *)&part[0][row * RS + c4];
+#pragma unroll
+        for (int p = 1; p < KG / 2; ++p)
+            v += *(const f32x4 *)&part[p][row * RS + c4];
+        store4(y + gm * N + gn, v, N - gn < 4 ? (int)(N - gn) : 4, v4);
+    }
+}
+
+// Large products: BM x BN tiles of y on WGM x WGN waves, the operands staged through
+// LDS by direct loads in two stages of two steps (256 values), their powers
+// beside them.  Within a step a wave's operand of x is read for the next
+// step as soon as its products are issued, w's into a second set, so the
+// reads spread over the step and each has a step to land; a stage is refilled
+// during its last step, behind the stage's one barrier, by which every wave has
+// read all of it.
+template <int BM, int BN, int WGM, int WGN, class O>
+__global__ void __launch_bounds__(64 * WGM *WGN, 1) k_mx4_tiles(pgk_mx4 x, pgk_mx4 w, O *__restrict__ y)
+{
+    constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
+    // a stage: A's tiles [BM / 16][2][64], B's, then their powers ([tile][64][2
+    // bytes], a kilobyte per eight tiles), one kilobyte per wave
+    constexpr int PA = BM / 8, PB = BN / 8, QA = PA / NW, QB = PB / NW; // kilobytes, and per wave
+    constexpr int SA = PA * 64, SB = PB * 64, STAGE = SA + SB + NW * 64;
+    static_assert(PA % NW == 0 && PB % NW == 0 && NW >= PA / 16 + PB / 16, "whole loads per wave");
+    __shared__ uint4 smem[2 * STAGE];
+    LDS uint4 *const lds = (LDS uint4 *)smem;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+    const int tiles_m = (int)((x.rows + BM - 1) / BM), tiles_n = (int)((w.rows + BN - 1) / BN);
+    const int pid = xcd_tile((int)blockIdx.x, (int)gridDim.x);
+    const int per_group = 8 * tiles_n, group = pid / per_group, first = group * 8;
+    const int gsz = tiles_m - first < 8 ? tiles_m - first : 8, in = pid - group * per_group;
+    const int m0 = (first + in % gsz) * BM, n0 = in / gsz * BN;
+    const int steps = (int)x.steps, KT = steps / 2, tx = (int)x.tiles, tw = (int)w.tiles;
+
+    // this wave's loads of a stage: kilobytes wave Q + q of A and of B, as byte
+    // offsets from the block's first tile; the base advances by two steps a stage
+    const uint8_t *const baseA = codes_at(x, m0 / 16, 0), *const baseB = codes_at(w, n0 / 16, 0);
+    uint32_t off[QA + QB];
+#pragma unroll
+    for (int q = 0; q < QA + QB; ++q) {
+        const bool of_a = q < QA;
+        const int p = of_a ? wave * QA + q : wave * QB + q - QA;
+        const int last = (of_a ? tx - m0 / 16 : tw - n0 / 16) - 1, t = p / 2 < last ? p / 2 : last;
+        off[q] = (uint32_t)((t * steps + (p & 1)) * 1024 + lane * 16);
+    }
+    // its kilobyte of powers: eight tiles, eight lanes each; waves past those
+    // that there are repeat A's first
+    constexpr int WPA = PA / 16, WPB = PB / 16;
+    const bool of_b = wave >= WPA && wave < WPA + WPB;
+    int pt = (of_b ? n0 / 16 + (wave - WPA) * 8 : m0 / 16 + (wave < WPA ? wave * 8 : 0)) + (lane >> 3);
+    pt = pt < (of_b ? tw : tx) ? pt : (of_b ? tw : tx) - 1;
+    const uint8_t *psrc = (const uint8_t *)powers_at(of_b ? w : x, pt, 0) + (lane & 7) * 16;
+    constexpr int LPT = QA + QB + 1;
+    auto dma = [&](int q, int t, int st) INLINE {
+        // (stages past the end are read by none)
+        const int tt = t < KT ? t : KT - 1;
+        LDS uint4 *base = lds + st * STAGE;
+        if (q < QA)
+            dma16s(off[q], baseA + (size_t)tt * 2048, base + (wave * QA + q) * 64);
+        else if (q < QA + QB)
+            dma16s(off[q], baseB + (size_t)tt * 2048, base + SA + (wave * QB + q - QA) * 64);
+        else
+            dma16(psrc + (size_t)tt * 128, base + SA + SB + wave * 64);
+    };
+    auto sync_stage = [&](auto newer) INLINE {
+        __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(decltype(newer)::value * LPT));
+        __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __asm__ volatile("" ::: "memory");
+    };
+    auto frag_a = [&](int st, int i, int h) INLINE {
+        return __builtin_bit_cast(uint4, ((const LDS u32x4 *)(lds + st * STAGE))[((wm * FM + i) * 2 + h) * 64 + lane]);
+    };
+    auto frag_b = [&](int st, int j, int h) INLINE {
+        return __builtin_bit_cast(uint4, ((const LDS u32x4 *)(lds + st * STAGE + SA))[((wn * FN + j) * 2 + h) * 64 + lane]);
+    };
+    auto power = [&](int st, int tile) INLINE { // of A's tiles, then B's
+        return (uint32_t)((const LDS uint16_t *)(lds + st * STAGE + SA + SB))[tile * 64 + lane];
+    };
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    uint4 fa[FM], fb[2][FN];
+    uint32_t pa[FM], pb[2][FN]; // B's of this stage and the next
+    // step h of stage u; `next`: the operands of the step behind it meanwhile;
+    // the second step refills the stage with tile `reload`
+    auto step = [&](auto hh, int u, bool next, int reload) INLINE {
+        constexpr int h = decltype(hh)::value;
+        const int nst = h ? u ^ 1 : u;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                acc[i][j] = mfma4<h>(fa[i], fb[h][j], acc[i][j], pa[i], pb[u][j]);
+                const int g = i * FN + j;
+                if (next) {
+                    if (j == FN - 1) {
+                        fa[i] = frag_a(nst, i, h ^ 1);
+                        if (h)
+                            pa[i] = power(nst, wm * FM + i);
+                    }
+                    if (g < FN) { // w's are needed first
+                        fb[h ^ 1][g] = frag_b(nst, g, h ^ 1);
+                        if (h)
+                            pb[u ^ 1][g] = power(nst, BM / 16 + wn * FN + g);
+                    }
+                }
+                if (h && next)
+#pragma unroll
+                    for (int q = g * LPT / (FM * FN); q < (g + 1) * LPT / (FM * FN); ++q)
+                        dma(q, reload, u);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    using first_step = std::integral_constant<int, 0>;
+    using second_step = std::integral_constant<int, 1>;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int q = 0; q < LPT; ++q)
+            dma(q, t, t);
+    sync_stage(std::integral_constant<int, 1>{});
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        fa[i] = frag_a(0, i, 0);
+        pa[i] = power(0, wm * FM + i);
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        fb[0][j] = frag_b(0, j, 0);
+        pb[0][j] = power(0, BM / 16 + wn * FN + j);
+    }
+    // the first step of the first stage, then links of a stage's second step and
+    // the next one's first, a barrier before each
+    step(first_step{}, 0, true, 0);
+    int t = 0;
+    auto link = [&](int u) INLINE {
+        sync_stage(std::integral_constant<int, 0>{}); // the next stage has landed, this one is read
+        step(second_step{}, u, true, t + 2);
+        step(first_step{}, u ^ 1, true, 0);
+        ++t;
+    };
+    while (t + 2 < KT) {
+        link(0);
+        link(1);
+    }
+    if (t + 1 < KT) {
+        link(0);
+        step(second_step{}, 1, false, 0);
+    } else {
+        step(second_step{}, 0, false, 0);
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(0)); // the loads past the end land before the LDS is used anew
+
+    // 32 rows of the wave's tile at a time through LDS, four columns a lane
+    constexpr int RS = WN + 4;
+    static_assert(WN == 64, "16 lanes of four columns per row");
+    static_assert(NW * 32 * RS * 4 <= 2 * STAGE * 16, "the regions fit the stages");
+    LDS float *reg = (LDS float *)lds + wave * 32 * RS;
+    const int c4 = (lane & 15) * 4, lg = lane >> 4, M = (int)x.rows, N = (int)w.rows;
+    const int col = n0 + wn * WN + c4;
+    const bool v4 = rows_keep_four(y, w.rows);
+#pragma unroll
+    for (int i = 0; i < FM; i += 2) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    reg[(k * 16 + 4 * lg + e) * RS + j * 16 + (lane & 15)] = acc[i + k][j][e];
+        __syncthreads();
+#pragma unroll 1
+        for (int p = 0; p < 8; ++p) {
+            const int row = (lane >> 4) + 4 * p, grow = m0 + wm * WM + i * 16 + row;
+            if (grow < M && col < N)
+                store4(y + (size_t)grow * N + col, f32x4(*(const LDS f32x4 *)(reg + row * RS + c4)), N - col, v4);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- launches
 
 unsigned blocks_for(size_t n) { return (unsigned)((n + 255) / 256 < 8192 ? (n + 255) / 256 : 8192); }
 
+template <class T>
+bool vector_rows(const T *p, size_t cols)
+{
+    return ((uintptr_t)p & 15) == 0 && cols * sizeof(T) % 16 == 0;
+}
+
+template <class T>
+int quantize(const pgk_mx4 &q, const T *src, int trans, hipStream_t st)
+{
+    if (trans) {
+        if (q.steps / 2 > 65535)
+            return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL(k_mx4_columns<T>, dim3((unsigned)((q.tiles + 3) / 4), (unsigned)(q.steps / 2)), dim3(256), 0, st,
+                           q, src);
+        return (int)hipGetLastError();
+    }
+    const dim3 grid(blocks_for(q.tiles * q.steps / 2 * 64));
+    if (vector_rows(src, q.cols))
+        hipLaunchKernelGGL((k_mx4_rows<T, true>), grid, dim3(256), 0, st, q, src);
+    else
+        hipLaunchKernelGGL((k_mx4_rows<T, false>), grid, dim3(256), 0, st, q, src);
+    return (int)hipGetLastError();
+}
+
+template <class O>
+int dequantize(const pgk_mx4 &q, O *dst, int trans, hipStream_t st)
+{
+    if (!trans)
+        hipLaunchKernelGGL(k_mx4_back_rows<O>, dim3(blocks_for(q.rows * ((q.cols + 7) / 8))), dim3(256), 0, st, q, dst);
+    else if (q.steps / 2 > 65535)
+        return (int)hipErrorInvalidValue;
+    else
+        hipLaunchKernelGGL(k_mx4_back_columns<O>, dim3((unsigned)((q.tiles + 3) / 4), (unsigned)(q.steps / 2)), dim3(256), 0,
+                           st, q, dst);
+    return (int)hipGetLastError();
+}
+
+template <class T, class O>
+int few(const T *x, size_t m, const pgk_mx4 &w, O *y, hipStream_t st)
+{
+    const dim3 grid((unsigned)w.tiles), block(kFewWaves * 64);
+    if (vector_rows(x, w.cols))
+        hipLaunchKernelGGL((k_mx4_few<T, O, true>), grid, block, 0, st, x, (int)m, w, y);
+    else
+        hipLaunchKernelGGL((k_mx4_few<T, O, false>), grid, block, 0, st, x, (int)m, w, y);
+    return (int)hipGetLastError();
+}
+
+template <int FM, int FN, int KG, class O>
+void split(const pgk_mx4 &x, const pgk_mx4 &w, O *y, hipStream_t st)
+{
+    const size_t blocks = (x.tiles + FM - 1) / FM * ((w.tiles + FN - 1) / FN);
+    hipLaunchKernelGGL((k_mx4_split<FM, FN, KG, O>), dim3((unsigned)blocks), dim3(KG * 64), 0, st, x, w, y);
+}
+
+template <class O>
+int product(const pgk_mx4 &x, const pgk_mx4 &w, O *y, hipStream_t st)
+{
+    auto tiles = [&](size_t bm, size_t bn) { return (x.rows + bm - 1) / bm * ((w.rows + bn - 1) / bn); };
+    if (tiles(128, 128) > 0x7fffffff)
+        return (int)hipErrorInvalidValue;
+    if (tiles(32, 32) <= 256)
+        split<2, 2, 8>(x, w, y, st);
+    else if (tiles(64, 32) <= 256)
+        split<4, 2, 8>(x, w, y, st);
+    else if (tiles(64, 64) <= 256)
+        split<4, 4, 8>(x, w, y, st);
+    else if (tiles(64, 64) <= 512)
+        split<4, 4, 4>(x, w, y, st);
+    else if (tiles(256, 256) < 200)
+        hipLaunchKernelGGL((k_mx4_tiles<128, 128, 2, 2, O>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, x, w, y);
+    else
+        hipLaunchKernelGGL((k_mx4_tiles<256, 256, 2, 4, O>), dim3((unsigned)tiles(256, 256)), dim3(512), 0, st, x, w, y);
+    return (int)hipGetLastError();
+}
+
+// fn with a null pointer of the type that a dtype code names
+template <class FN>
+int by_type(int dtype, FN fn)
+{
+    return dtype == 0 ? fn((float *)nullptr) : dtype == 1 ? fn((_Float16 *)nullptr) : fn((__bf16 *)nullptr);
+}
+
 } // namespace
 
-extern "C" void pgk_mx4_shape(pgk_mx4 *q, size_t rows, size_t cols, size_t *code_bytes, size_t *scale_bytes)
+extern "C" void pgk_mx4_shape(pgk_mx4 *q, size_t rows, size_t cols, size_t *code_bytes, size_t *power_bytes)
 {
-    const size_t nb = (cols + kBlock - 1) / kBlock;
     q->rows = rows;
     q->cols = cols;
-    q->pitch = nb * 16;
-    q->rows_p = (rows + 15) & ~(size_t)15;
-    *code_bytes = rows * q->pitch;
-    *scale_bytes = (nb + 7) / 8 * q->rows_p * 8;
+    q->tiles = (rows + 15) / 16;
+    q->steps = (cols + 255) / 256 * 2;
+    *code_bytes = q->tiles * q->steps * 1024;
+    *power_bytes = q->tiles * q->steps * 64;
 }
 
 extern "C" int pgk_mx4_quantize(const pgk_mx4 *q, const void *src, int dtype, int trans, pgk_stream s)
 {
-    hipLaunchKernelGGL(k_mx4_quantize, dim3(blocks_for(q->rows * (q->pitch / 16))), dim3(256), 0, (hipStream_t)s, *q,
-                       src, dtype, trans);
-    return (int)hipGetLastError();
+    return by_type(dtype, [&](auto t) { return quantize(*q, (decltype(t))src, trans, (hipStream_t)s); });
 }
 
 extern "C" int pgk_mx4_dequantize(const pgk_mx4 *q, void *dst, int dtype, int trans, pgk_stream s)
 {
-    hipLaunchKernelGGL(k_mx4_dequantize, dim3(blocks_for(q->rows * q->cols)), dim3(256), 0, (hipStream_t)s, *q, dst,
-                       dtype, trans);
-    return (int)hipGetLastError();
+    return by_type(dtype, [&](auto t) { return dequantize(*q, (decltype(t))dst, trans, (hipStream_t)s); });
+}
+
+extern "C" int pgk_mx4_few_rows(size_t m) { return m <= 16; }
+
+extern "C" int pgk_mx4_matmul_few(const void *x, int dtype, size_t m, const pgk_mx4 *w, void *y, int y_dtype, pgk_stream s)
+{
+    if (!pgk_mx4_few_rows(m) || w->rows > 0x3fffffff || w->cols > (size_t)1 << 24)
+        return (int)hipErrorInvalidValue;
+    return by_type(dtype, [&](auto t) {
+        return by_type(y_dtype, [&](auto o) {
+            return few((const std::remove_pointer_t<decltype(t)> *)x, m, *w, (decltype(o))y, (hipStream_t)s);
+        });
+    });
 }
 
 extern "C" int pgk_mx4_matmul(const pgk_mx4 *x, const pgk_mx4 *w, void *y, int y_dtype, pgk_stream s)
 {
-    if (x->cols != w->cols || x->rows > 65535 * (size_t)32)
+    // (the offsets within a block's 16 tiles fit 32 bits)
+    if (x->cols != w->cols || x->rows > 0x3fffffff || w->rows > 0x3fffffff || x->cols > (size_t)1 << 24)
         return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_mx4_tile32, dim3((unsigned)((w->rows + 31) / 32), (unsigned)((x->rows + 31) / 32)), dim3(64), 0,
-                       (hipStream_t)s, *x, *w, y, y_dtype);
-    return (int)hipGetLastError();
+    return by_type(y_dtype, [&](auto o) { return product(*x, *w, (decltype(o))y, (hipStream_t)s); });
 }
