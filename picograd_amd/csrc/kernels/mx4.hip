@@ -415,22 +415,25 @@ __global__ void __launch_bounds__(KG * 64, 1) k_mx4_split(pgk_mx4 x, pgk_mx4 w, 
 }
 
 // Large products: BM x BN tiles of y on WGM x WGN waves, the operands staged through
-// LDS by direct loads in two stages of two steps (256 values), their powers
-// beside them.  Within a step a wave's operand of x is read for the next
-// step as soon as its products are issued, w's into a second set, so the
-// reads spread over the step and each has a step to land; a stage is refilled
-// during its last step, behind the stage's one barrier, by which every wave has
-// read all of it.
+// LDS by direct loads in four stages of one step (128 values), their powers
+// beside them.  A step's operands are read during the step before: x's each as
+// soon as the products with the one it replaces are issued, w's into a second
+// set.  A stage is refilled during the step that follows its last read, behind
+// the step's one barrier, so its loads have three steps to land.  Tiles of
+// 128 x 128 on four waves, two blocks to a CU, of which one computes while the
+// other waits at its barrier.  8192 x 4096 x 4096 takes 92 us, 3.0 PFLOP/s where the matrix
+// units alone reach 6.0 on random codes; two stages of two steps take 109 and
+// 256 x 256 tiles, whose eight waves run out of registers, 90 to 111.
 template <int BM, int BN, int WGM, int WGN, class O>
 __global__ void __launch_bounds__(64 * WGM *WGN, 1) k_mx4_tiles(pgk_mx4 x, pgk_mx4 w, O *__restrict__ y)
 {
-    constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
-    // a stage: A's tiles [BM / 16][2][64], B's, then their powers ([tile][64][2
-    // bytes], a kilobyte per eight tiles), one kilobyte per wave
-    constexpr int PA = BM / 8, PB = BN / 8, QA = PA / NW, QB = PB / NW; // kilobytes, and per wave
-    constexpr int SA = PA * 64, SB = PB * 64, STAGE = SA + SB + NW * 64;
-    static_assert(PA % NW == 0 && PB % NW == 0 && NW >= PA / 16 + PB / 16, "whole loads per wave");
-    __shared__ uint4 smem[2 * STAGE];
+    constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16, S = 4;
+    // a stage: A's tiles [BM / 16][64], B's, then their powers ([tile][64][two
+    // steps], a kilobyte per eight tiles)
+    constexpr int TA = BM / 16, TB = BN / 16, QA = TA / NW, QB = TB / NW; // kilobytes, and per wave
+    constexpr int WPA = TA / 8, WPB = TB / 8, STAGE = (TA + TB + WPA + WPB) * 64;
+    static_assert(TA % NW == 0 && TB % NW == 0 && NW % (WPA + WPB) == 0, "whole loads per wave");
+    __shared__ uint4 smem[S * STAGE];
     LDS uint4 *const lds = (LDS uint4 *)smem;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
@@ -439,52 +442,48 @@ __global__ void __launch_bounds__(64 * WGM *WGN, 1) k_mx4_tiles(pgk_mx4 x, pgk_m
     const int per_group = 8 * tiles_n, group = pid / per_group, first = group * 8;
     const int gsz = tiles_m - first < 8 ? tiles_m - first : 8, in = pid - group * per_group;
     const int m0 = (first + in % gsz) * BM, n0 = in / gsz * BN;
-    const int steps = (int)x.steps, KT = steps / 2, tx = (int)x.tiles, tw = (int)w.tiles;
+    const int steps = (int)x.steps, tx = (int)x.tiles, tw = (int)w.tiles;
 
     // this wave's loads of a stage: kilobytes wave Q + q of A and of B, as byte
-    // offsets from the block's first tile; the base advances by two steps a stage
+    // offsets from the block's first tile; the base advances by a step a stage
     const uint8_t *const baseA = codes_at(x, m0 / 16, 0), *const baseB = codes_at(w, n0 / 16, 0);
     uint32_t off[QA + QB];
 #pragma unroll
     for (int q = 0; q < QA + QB; ++q) {
-        const bool of_a = q < QA;
-        const int p = of_a ? wave * QA + q : wave * QB + q - QA;
-        const int last = (of_a ? tx - m0 / 16 : tw - n0 / 16) - 1, t = p / 2 < last ? p / 2 : last;
-        off[q] = (uint32_t)((t * steps + (p & 1)) * 1024 + lane * 16);
+        const int p = q < QA ? wave * QA + q : wave * QB + q - QA;
+        const int last = (q < QA ? tx - m0 / 16 : tw - n0 / 16) - 1, t = p < last ? p : last;
+        off[q] = (uint32_t)(t * steps * 1024 + lane * 16);
     }
-    // its kilobyte of powers: eight tiles, eight lanes each; waves past those
-    // that there are repeat A's first
-    constexpr int WPA = PA / 16, WPB = PB / 16;
-    const bool of_b = wave >= WPA && wave < WPA + WPB;
-    int pt = (of_b ? n0 / 16 + (wave - WPA) * 8 : m0 / 16 + (wave < WPA ? wave * 8 : 0)) + (lane >> 3);
+    // a kilobyte of powers: eight tiles, eight lanes each; waves past those that
+    // there are bring the same ones again, to the same place
+    const int pw = wave % (WPA + WPB);
+    const bool of_b = pw >= WPA;
+    int pt = (of_b ? n0 / 16 + (pw - WPA) * 8 : m0 / 16 + pw * 8) + (lane >> 3);
     pt = pt < (of_b ? tw : tx) ? pt : (of_b ? tw : tx) - 1;
     const uint8_t *psrc = (const uint8_t *)powers_at(of_b ? w : x, pt, 0) + (lane & 7) * 16;
     constexpr int LPT = QA + QB + 1;
+    static_assert((S - 1) * LPT < 64, "the loads in flight fit the vmcnt counter");
     auto dma = [&](int q, int t, int st) INLINE {
-        // (stages past the end are read by none)
-        const int tt = t < KT ? t : KT - 1;
+        const int tt = t < steps ? t : steps - 1; // stages past the end are read by none
         LDS uint4 *base = lds + st * STAGE;
         if (q < QA)
-            dma16s(off[q], baseA + (size_t)tt * 2048, base + (wave * QA + q) * 64);
+            dma16s(off[q], baseA + (size_t)tt * 1024, base + (wave * QA + q) * 64);
         else if (q < QA + QB)
-            dma16s(off[q], baseB + (size_t)tt * 2048, base + SA + (wave * QB + q - QA) * 64);
+            dma16s(off[q], baseB + (size_t)tt * 1024, base + (TA + wave * QB + q - QA) * 64);
         else
-            dma16(psrc + (size_t)tt * 128, base + SA + SB + wave * 64);
+            dma16(psrc + (size_t)(tt >> 1) * 128, base + (TA + TB + pw) * 64);
     };
-    auto sync_stage = [&](auto newer) INLINE {
+    auto sync_stage = [&](auto newer) INLINE { // all but the newest stages' loads have landed
         __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(decltype(newer)::value * LPT));
         __asm__ volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
     };
-    auto frag_a = [&](int st, int i, int h) INLINE {
-        return __builtin_bit_cast(uint4, ((const LDS u32x4 *)(lds + st * STAGE))[((wm * FM + i) * 2 + h) * 64 + lane]);
+    auto frag = [&](int st, int tile) INLINE { // of A's tiles, then B's
+        return __builtin_bit_cast(uint4, ((const LDS u32x4 *)(lds + st * STAGE))[tile * 64 + lane]);
     };
-    auto frag_b = [&](int st, int j, int h) INLINE {
-        return __builtin_bit_cast(uint4, ((const LDS u32x4 *)(lds + st * STAGE + SA))[((wn * FN + j) * 2 + h) * 64 + lane]);
-    };
-    auto power = [&](int st, int tile) INLINE { // of A's tiles, then B's
-        return (uint32_t)((const LDS uint16_t *)(lds + st * STAGE + SA + SB))[tile * 64 + lane];
+    auto power = [&](int st, int tile) INLINE {
+        return (uint32_t)((const LDS uint16_t *)(lds + st * STAGE + (TA + TB) * 64))[tile * 64 + lane];
     };
     f32x4 acc[FM][FN];
 #pragma unroll
@@ -493,85 +492,87 @@ __global__ void __launch_bounds__(64 * WGM *WGN, 1) k_mx4_tiles(pgk_mx4 x, pgk_m
         for (int j = 0; j < FN; ++j)
             acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     uint4 fa[FM], fb[2][FN];
-    uint32_t pa[FM], pb[2][FN]; // B's of this stage and the next
-    // step h of stage u; `next`: the operands of the step behind it meanwhile;
-    // the second step refills the stage with tile `reload`
-    auto step = [&](auto hh, int u, bool next, int reload) INLINE {
-        constexpr int h = decltype(hh)::value;
-        const int nst = h ? u ^ 1 : u;
+    uint32_t pa[FM], pb[2][FN]; // powers of a pair of steps; w's of the next pair too
+    // the step in stage u; `next`: the operands of the step behind it are read and
+    // the stage takes step `reload`
+    auto step = [&](auto uu, bool next, int reload) INLINE {
+        constexpr int u = decltype(uu)::value, h = u & 1, nu = (u + 1) % S, pair = u >> 1 & 1;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                acc[i][j] = mfma4<h>(fa[i], fb[h][j], acc[i][j], pa[i], pb[u][j]);
+                acc[i][j] = mfma4<h>(fa[i], fb[h][j], acc[i][j], pa[i], pb[pair][j]);
                 const int g = i * FN + j;
                 if (next) {
+                    if (i == 0) { // w's are needed first
+                        fb[h ^ 1][j] = frag(nu, TA + wn * FN + j);
+                        if (h)
+                            pb[pair ^ 1][j] = power(nu, TA + wn * FN + j);
+                    }
                     if (j == FN - 1) {
-                        fa[i] = frag_a(nst, i, h ^ 1);
+                        fa[i] = frag(nu, wm * FM + i);
                         if (h)
-                            pa[i] = power(nst, wm * FM + i);
+                            pa[i] = power(nu, wm * FM + i);
                     }
-                    if (g < FN) { // w's are needed first
-                        fb[h ^ 1][g] = frag_b(nst, g, h ^ 1);
-                        if (h)
-                            pb[u ^ 1][g] = power(nst, BM / 16 + wn * FN + g);
-                    }
-                }
-                if (h && next)
 #pragma unroll
                     for (int q = g * LPT / (FM * FN); q < (g + 1) * LPT / (FM * FN); ++q)
                         dma(q, reload, u);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
     };
-    using first_step = std::integral_constant<int, 0>;
-    using second_step = std::integral_constant<int, 1>;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < S; ++t)
 #pragma unroll
         for (int q = 0; q < LPT; ++q)
             dma(q, t, t);
-    sync_stage(std::integral_constant<int, 1>{});
+    sync_stage(std::integral_constant<int, S - 1>{});
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        fa[i] = frag_a(0, i, 0);
+        fa[i] = frag(0, wm * FM + i);
         pa[i] = power(0, wm * FM + i);
     }
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-        fb[0][j] = frag_b(0, j, 0);
-        pb[0][j] = power(0, BM / 16 + wn * FN + j);
+        fb[0][j] = frag(0, TA + wn * FN + j);
+        pb[0][j] = power(0, TA + wn * FN + j);
     }
-    // the first step of the first stage, then links of a stage's second step and
-    // the next one's first, a barrier before each
-    step(first_step{}, 0, true, 0);
+    // each step but the last behind a barrier: the next stage has landed (two
+    // newer ones may be in flight) and every wave has read this one
     int t = 0;
-    auto link = [&](int u) INLINE {
-        sync_stage(std::integral_constant<int, 0>{}); // the next stage has landed, this one is read
-        step(second_step{}, u, true, t + 2);
-        step(first_step{}, u ^ 1, true, 0);
+    auto link = [&](auto u) INLINE {
+        sync_stage(std::integral_constant<int, S - 2>{});
+        step(u, true, t + S);
         ++t;
     };
-    while (t + 2 < KT) {
-        link(0);
-        link(1);
+    using U0 = std::integral_constant<int, 0>;
+    using U1 = std::integral_constant<int, 1>;
+    using U2 = std::integral_constant<int, 2>;
+    using U3 = std::integral_constant<int, 3>;
+    while (t + S < steps) {
+        link(U0{});
+        link(U1{});
+        link(U2{});
+        link(U3{});
     }
-    if (t + 1 < KT) {
-        link(0);
-        step(second_step{}, 1, false, 0);
+    link(U0{}); // two or four steps are left
+    if (t + 1 < steps) {
+        link(U1{});
+        link(U2{});
+        step(U3{}, false, 0);
     } else {
-        step(second_step{}, 0, false, 0);
+        step(U1{}, false, 0);
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(0)); // the loads past the end land before the LDS is used anew
 
     // 32 rows of the wave's tile at a time through LDS, four columns a lane
-    constexpr int RS = WN + 4;
-    static_assert(WN == 64, "16 lanes of four columns per row");
-    static_assert(NW * 32 * RS * 4 <= 2 * STAGE * 16, "the regions fit the stages");
+    constexpr int RS = WN + 4, CL = WN / 4; // lanes of a row
+    static_assert(CL == 16 || CL == 32, "whole rows per pass");
+    static_assert(NW * 32 * RS * 4 <= S * STAGE * 16, "the regions fit the stages");
     LDS float *reg = (LDS float *)lds + wave * 32 * RS;
-    const int c4 = (lane & 15) * 4, lg = lane >> 4, M = (int)x.rows, N = (int)w.rows;
+    const int c4 = (lane & (CL - 1)) * 4, lg = lane >> 4, M = (int)x.rows, N = (int)w.rows;
     const int col = n0 + wn * WN + c4;
     const bool v4 = rows_keep_four(y, w.rows);
 #pragma unroll
@@ -586,8 +587,8 @@ __global__ void __launch_bounds__(64 * WGM *WGN, 1) k_mx4_tiles(pgk_mx4 x, pgk_m
                     reg[(k * 16 + 4 * lg + e) * RS + j * 16 + (lane & 15)] = acc[i + k][j][e];
         __syncthreads();
 #pragma unroll 1
-        for (int p = 0; p < 8; ++p) {
-            const int row = (lane >> 4) + 4 * p, grow = m0 + wm * WM + i * 16 + row;
+        for (int row = lane / CL; row < 32; row += 64 / CL) {
+            const int grow = m0 + wm * WM + i * 16 + row;
             if (grow < M && col < N)
                 store4(y + (size_t)grow * N + col, f32x4(*(const LDS f32x4 *)(reg + row * RS + c4)), N - col, v4);
         }
@@ -667,10 +668,8 @@ int product(const pgk_mx4 &x, const pgk_mx4 &w, O *y, hipStream_t st)
         split<4, 4, 8>(x, w, y, st);
     else if (tiles(64, 64) <= 512)
         split<4, 4, 4>(x, w, y, st);
-    else if (tiles(256, 256) < 200)
-        hipLaunchKernelGGL((k_mx4_tiles<128, 128, 2, 2, O>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, x, w, y);
     else
-        hipLaunchKernelGGL((k_mx4_tiles<256, 256, 2, 4, O>), dim3((unsigned)tiles(256, 256)), dim3(512), 0, st, x, w, y);
+        hipLaunchKernelGGL((k_mx4_tiles<128, 128, 2, 2, O>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, x, w, y);
     return (int)hipGetLastError();
 }
 
