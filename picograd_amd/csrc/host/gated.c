@@ -32,23 +32,10 @@ static bool dims_ok(const pg_tensor *x, const pg_tensor *w, const pg_tensor *b, 
 static bool forward(const char *what, int dt, const gated_dims *d, int act, const uint16_t *x16, const uint16_t *w16,
                     const float *bias, float *z, float *h32, uint16_t *h16)
 {
-    const size_t zb = d->M * 2 * d->F * sizeof(float);
-    float *zz = z ? z : pgd_malloc(zb);
-    if (!zz)
-        return false;
-    bool ok = true;
-    /* both halves in one product where they lie at their place in z */
-    const int parts = d->F == d->F8 ? 1 : 2;
-    for (int p = 0; ok && p < parts; p++) {
-        const size_t n = parts == 1 ? 2 * d->F : d->F, n8 = parts == 1 ? 2 * d->F8 : d->F8;
-        const pgk_epi epi = {.bias = bias ? bias + p * d->F : NULL, .act = PGK_ACT_NONE, .dtype16 = dt};
-        ok = pgm_gemm16x(dt, 0, 1, d->M, n, d->K8, x16, d->K8 ? d->K8 : 8, 0, d->M, w16 + p * d->F8, 2 * d->F8, 0, n8,
-                         zz + p * d->F, 2 * d->F, 0, 1, 0, &epi, what);
-    }
-    ok = ok && pgd_check(pgk_gated_act(act, zz, d->M, d->F, h32, h16, dt, pgd_stream()), what);
-    if (!z)
-        pgd_free(zz, zb);
-    return ok;
+    int tk = pgd_tbegin(PGD_T_GEMM16);
+    const int rc = pgk_gated_forward(dt, act, d->M, d->F, d->K8, x16, d->K8, w16, d->F8, bias, z, h32, h16, pgd_stream());
+    pgd_tend(tk);
+    return pgd_check(rc, what);
 }
 
 /* an output of a product: f32 (beta: added to) or 16 bits, at p with leading

@@ -3,6 +3,8 @@
 #ifndef PGK_GATE_ACT_H
 #define PGK_GATE_ACT_H
 
+#include <type_traits>
+
 #include "launch.h"
 #include "pgmath.h"
 

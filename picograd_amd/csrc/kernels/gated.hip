@@ -1,5 +1,6 @@
-// Gated feed-forward layer: h = act(g) u over z = x W + b = [g | u], and the
-// backward of that product.
+// Gated feed-forward layer: h = act(g) u over z = x W + b = [g | u] in one launch,
+// and the backward of the gate (the two products of the layer's backward are
+// ordinary GEMMs over [dg | du]).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -7,108 +8,345 @@
 
 #include "convert16.h"
 #include "gate_act.h"
+#include "gemm_tile.h"
 #include "launch.h"
 
 namespace {
 
-__global__ void __launch_bounds__(256) k_gated_act(int act, const float *__restrict__ z, size_t m, size_t f, float *h32,
-                                                   uint16_t *h16, int dtype)
+// ---------------------------------------------------------------- forward
+
+// A tile of the product holds columns of Wg beside the same columns of Wu
+// (TileGate), so its epilogue has g and u of each output and z need not be
+// read back; z itself is written only for a backward.  Tiles and k-loops are
+// the 16-bit GEMM's.
+template <class CF>
+__global__ void __launch_bounds__(CF::NT, 1) k_gated(gemm_kargs g)
 {
-    const size_t n = m * f;
-    gate_switch(act, [&](auto code) {
-        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-            const size_t r = i / f, c = i - r * f;
-            const float h = gate_f<decltype(code)::value>(z[r * 2 * f + c]) * z[r * 2 * f + f + c];
-            if (h32)
-                h32[i] = h;
-            if (h16)
-                h16[i] = to16(dtype, h);
-        }
-    });
+    __shared__ uint4 smem[CF::LDS_U4];
+    gemm16_block<CF>(g, (int)blockIdx.x, (int)gridDim.x, true, 0, (LDS uint4 *)smem);
+}
+template <class CF>
+__global__ void __launch_bounds__(CF::NT, CF::KG == 4 ? 2 : 1) k_gated_ks(gemm_kargs g)
+{
+    __shared__ uint4 smem[CF::LDS_U4];
+    ks_block<CF>(g, 1, (int)blockIdx.x, (int)gridDim.x, true, 0, (LDS uint4 *)smem);
 }
 
-// dz over a strip of 64 columns of f and a run of rows per block; its four
-// waves take every fourth row each and keep the strip's column sums, joined
-// through LDS in wave order into the block's row of part
-__global__ void __launch_bounds__(256)
-    k_gated_bwd(int act, const void *__restrict__ dh, int dh_dtype, const float *__restrict__ z, size_t m, size_t f,
-                size_t f8, uint16_t *__restrict__ dz, int dtype, float *__restrict__ part, int rows)
+// Up to 16 rows: a block owns 16 outputs, whose 32 columns of W it streams past
+// once, its eight waves splitting the reduction, each with a ring of three
+// 64-deep chunks of its own and no block barrier until the waves' partial tiles
+// (16 x 16, one of g and one of u) are added through LDS in wave order.
+typedef float f32x4m __attribute__((ext_vector_type(4)));
+template <bool F16>
+__device__ __forceinline__ f32x4m mfma16(const uint4 &a, const uint4 &b, const f32x4m &c)
 {
-    __shared__ float sums[4][2][64];
-    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const size_t c = (size_t)blockIdx.x * 64 + lane;
-    const size_t r0 = (size_t)blockIdx.y * rows, r1 = r0 + rows < m ? r0 + rows : m;
-    float sg = 0.0f, su = 0.0f;
-    gate_switch(act, [&](auto code) {
-        for (size_t r = r0 + wave; r < r1; r += 4) {
-            float dg = 0.0f, du = 0.0f;
-            if (c < f) {
-                const float d = dh_dtype == 0 ? ((const float *)dh)[r * f + c]
-                                              : from16(dh_dtype, ((const uint16_t *)dh)[r * f + c]);
-                float da;
-                const float a = gate_fd<decltype(code)::value>(z[r * 2 * f + c], da);
-                dg = d * z[r * 2 * f + f + c] * da;
-                du = d * a;
-                sg += dg;
-                su += du;
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+}
+constexpr int kFewWaves = 8, kFewStages = 3, kFewK = 64;
+constexpr int kFewA = 16 * kFewK / 8, kFewB = kFewK * 32 / 8; // uint4 of one A and one B stage
+
+template <bool F16>
+__global__ void __launch_bounds__(kFewWaves * 64, 1) k_gated_few(gemm_kargs g)
+{
+    __shared__ uint4 smem[kFewWaves * kFewStages * (kFewA + kFewB)];
+    const int lane = (int)threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    // neighbouring blocks share each 128-byte line of a row: on one XCD
+    const int n0 = xcd_tile((int)blockIdx.x, (int)gridDim.x) * 16;
+    LDS uint4 *const ring = (LDS uint4 *)smem + wave * kFewStages * (kFewA + kFewB);
+    using TK = TileK<16, 64, kFewK>;
+    static_assert(TK::NQ == 2 && kFewB == 256, "two loads of A and four of B per stage");
+    constexpr int LPT = 6;
+    const int nct = (g.K + kFewK - 1) / kFewK, nc = nct > wave ? (nct - wave + kFewWaves - 1) / kFewWaves : 0;
+    // this wave's chunk c (chunk c * waves + wave of the reduction) into stage
+    // st; k at or past K reads the zero page
+    auto load = [&](int c, int st) {
+        const int ch = c * kFewWaves + wave, k0 = ch < nct ? ch * kFewK : g.K;
+        LDS uint4 *sa = ring + st * (kFewA + kFewB), *sb = sa + kFewA;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { // [64 k][16 of g, 16 of u]: four 16-byte chunks per k row
+            const int slot = q * 64 + lane, k = slot >> 2, half = slot >> 1 & 1;
+            int col = n0 + (slot & 1) * 8;
+            col = (col < g.b_extent ? col : g.b_extent - 8) + half * g.b_extent;
+            const void *src = k0 + k < g.K ? (const void *)(g.B + (size_t)(k0 + k) * g.ldb + col) : (const void *)&g_zero16;
+            dma16(src, sb + q * 64);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            TK::load_q(q, g.A, g.lda, 0, g.a_extent, k0, g.K, sa, lane);
+    };
+    const int grp = lane >> 4, q16 = lane & 15;
+    f32x4m acc[2] = {};
+    if (nc > 0) {
+#pragma unroll
+        for (int s = 0; s < kFewStages; ++s)
+            load(s, s);
+        int st = 0;
+        for (int c = 0; c < nc; ++c) {
+            const LDS uint4 *sa = ring + st * (kFewA + kFewB), *sb = sa + kFewA;
+            // chunk c landed (the newest kFewStages - 1 chunks may be in flight)
+            __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm((kFewStages - 1) * LPT));
+            __asm__ volatile("" ::: "memory");
+            // 16-lane group grp holds k = 32 s + 8 grp .. + 7 of row (A) or
+            // column (B) lane % 16; B from two transposing reads
+            uint4 fa[2], fb[2][2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const u32x4 v = ((const LDS u32x4 *)sa)[q16 * TK::CH + TK::swz(4 * s + grp, q16)];
+                fa[s] = __builtin_bit_cast(uint4, v);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    uint2 h2[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int k = 32 * s + 8 * grp + 4 * h + (q16 >> 2);
+                        h2[h] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                              (LDS v4s *)((const LDS char *)sb + k * 64 + t * 32 + (q16 & 3) * 8)));
+                    }
+                    fb[s][t] = make_uint4(h2[0].x, h2[0].y, h2[1].x, h2[1].y);
+                }
             }
-            if (c < f8) {
-                dz[r * 2 * f8 + c] = to16(dtype, dg);
-                dz[r * 2 * f8 + f8 + c] = to16(dtype, du);
+            // the stage's reads are done before its refill
+            __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(63));
+            __asm__ volatile("" ::: "memory");
+            load(c + kFewStages, st);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    acc[t] = mfma16<F16>(fa[s], fb[s][t], acc[t]);
+            st = st + 1 == kFewStages ? 0 : st + 1;
+        }
+        __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(0));
+    }
+    __syncthreads(); // the rings are done: the waves' partials through LDS, added in wave order
+    constexpr int RP = 36;
+    LDS float *part = (LDS float *)smem;
+    static_assert(kFewWaves * 16 * RP * 4 <= (int)sizeof(smem), "partials fit the rings");
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) // lane holds column lane % 16 of rows 4 (lane / 16) + e
+            part[(wave * 16 + 4 * grp + e) * RP + t * 16 + q16] = acc[t][e];
+    __syncthreads();
+    const int row = (int)threadIdx.x >> 2, c4 = ((int)threadIdx.x & 3) * 4;
+    if (row < 16 && row < g.M && n0 + c4 < g.N) {
+        f32x4 gv = {0.0f, 0.0f, 0.0f, 0.0f}, uv = gv;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w) {
+            gv += *(const LDS f32x4 *)(part + (w * 16 + row) * RP + c4);
+            uv += *(const LDS f32x4 *)(part + (w * 16 + row) * RP + 16 + c4);
+        }
+        gate_store(g.epi, g.C, g.N, row, n0 + c4, gv, uv);
+    }
+}
+
+template <class CF>
+int launch_tiles(gemm_kargs g, hipStream_t s)
+{
+    g.tiles_m = (g.M + CF::BM - 1) / CF::BM, g.tiles_n = (g.N + CF::BN / 2 - 1) / (CF::BN / 2);
+    hipLaunchKernelGGL(k_gated<CF>, dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(CF::NT), 0, s, g);
+    return (int)hipGetLastError();
+}
+template <class CF>
+int launch_split(gemm_kargs g, hipStream_t s)
+{
+    g.tiles_m = (g.M + CF::TM - 1) / CF::TM, g.tiles_n = (g.N + CF::TN / 2 - 1) / (CF::TN / 2);
+    hipLaunchKernelGGL(k_gated_ks<CF>, dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(CF::NT), 0, s, g);
+    return (int)hipGetLastError();
+}
+
+template <bool F16>
+int launch_forward(int tile, const gemm_kargs &g, hipStream_t s)
+{
+    if (g.M <= 16) {
+        hipLaunchKernelGGL(k_gated_few<F16>, dim3((unsigned)((g.N + 15) / 16)), dim3(kFewWaves * 64), 0, s, g);
+        return (int)hipGetLastError();
+    }
+    switch (tile) {
+    case 1: return launch_tiles<gcfg<128, 128, 2, 2, false, true, F16, true, 64, 2, true>>(g, s);
+    case 2: return launch_tiles<gcfg<256, 256, 2, 4, false, true, F16, true, 32, 4, true>>(g, s);
+    case 3: return launch_tiles<gcfg<128, 256, 2, 4, false, true, F16, true, 32, 4, true>>(g, s);
+    case 5: return launch_split<kscfg<32, 32, 8, 64, 2, false, true, F16, true>>(g, s);
+    case 6: return launch_split<kscfg<32, 64, 8, 32, 3, false, true, F16, true>>(g, s);
+    case 7: return launch_split<kscfg<64, 64, 4, 32, 2, false, true, F16, true>>(g, s);
+    default: return launch_split<kscfg<64, 64, 8, 32, 2, false, true, F16, true>>(g, s);
+    }
+}
+
+// ---------------------------------------------------------------- backward
+
+// The gate's backward over a strip of 64 V columns of f and a run of rows per block:
+// its four waves take every fourth row each, V neighbouring columns a lane (4
+// where every row keeps that alignment, else 1), and keep the strip's column
+// sums, joined through LDS in wave order into the block's row of part.  Bound by
+// the stream of z and dh in and dz out (4096 x 8192: 470 MB).
+template <int V, class T>
+__device__ __forceinline__ void load_as(const T *p, float *v)
+{
+    typedef T tv __attribute__((ext_vector_type(V)));
+    const tv q = __builtin_nontemporal_load((const tv *)p); // read once
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        v[i] = (float)q[i];
+}
+
+template <int V, int ACT, class D>
+__global__ void __launch_bounds__(256)
+    k_gated_bwd(const D *__restrict__ dh, const float *__restrict__ z, size_t m, size_t f, size_t f8,
+                uint16_t *__restrict__ dz, int dtype, float *__restrict__ part, int rows)
+{
+    __shared__ float sums[4][2][64 * V];
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const size_t c = ((size_t)blockIdx.x * 64 + lane) * V;
+    const size_t r0 = (size_t)blockIdx.y * rows, r1 = r0 + rows < m ? r0 + rows : m;
+    float sg[V] = {}, su[V] = {};
+    if (c < f8)
+#pragma unroll 2
+        for (size_t r = r0 + wave; r < r1; r += 4) {
+            float dg[V] = {}, du[V] = {};
+            if (c < f) {
+                float d[V], g[V], u[V];
+                load_as<V>(dh + r * f + c, d);
+                load_as<V>(z + r * 2 * f + c, g);
+                load_as<V>(z + r * 2 * f + f + c, u);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float da;
+                    const float a = gate_fd<ACT>(g[i], da);
+                    dg[i] = d[i] * u[i] * da;
+                    du[i] = d[i] * a;
+                    sg[i] += dg[i];
+                    su[i] += du[i];
+                }
+            }
+            uint16_t *p = dz + r * 2 * f8 + c;
+            if constexpr (V == 4) {
+                *(uint2 *)p = make_uint2(to16x2(dtype, dg[0], dg[1]), to16x2(dtype, dg[2], dg[3]));
+                *(uint2 *)(p + f8) = make_uint2(to16x2(dtype, du[0], du[1]), to16x2(dtype, du[2], du[3]));
+            } else {
+                p[0] = to16(dtype, dg[0]);
+                p[f8] = to16(dtype, du[0]);
             }
         }
-    });
     if (!part)
         return;
-    sums[wave][0][lane] = sg;
-    sums[wave][1][lane] = su;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        sums[wave][0][lane * V + i] = sg[i];
+        sums[wave][1][lane * V + i] = su[i];
+    }
     __syncthreads();
-    if (wave < 2 && c < f)
-        part[(size_t)blockIdx.y * 2 * f + wave * f + c] =
-            sums[0][wave][lane] + sums[1][wave][lane] + sums[2][wave][lane] + sums[3][wave][lane];
+    for (int i = (int)threadIdx.x; i < 2 * 64 * V; i += 256) {
+        const int half = i / (64 * V), j = i % (64 * V);
+        const size_t col = (size_t)blockIdx.x * 64 * V + j;
+        if (col < f)
+            part[(size_t)blockIdx.y * 2 * f + half * f + col] =
+                sums[0][half][j] + sums[1][half][j] + sums[2][half][j] + sums[3][half][j];
+    }
 }
 
-// rows per block: about 2048 blocks, at most 256 of them along the rows (the
-// partial column sums)
+// The blocks of rows: enough to fill the chip, at most 32 where they leave
+// partial column sums, which one more launch adds one after the other.
 struct bwd_plan {
+    int v;
     unsigned gx, gy;
     int rows;
 };
-bwd_plan plan_bwd(size_t m, size_t f)
+bwd_plan plan_bwd(size_t m, size_t f, bool v4, bool sums)
 {
-    const size_t gx = (f + 63) / 64;
-    size_t gy = 2048 / gx ? 2048 / gx : 1;
-    gy = gy > 256 ? 256 : gy;
+    const int v = v4 ? 4 : 1;
+    const size_t gx = (f + 64 * v - 1) / (64 * v);
+    size_t gy = (sums ? 1024 : 4096) / gx;
+    gy = gy < 1 ? 1 : sums && gy > 32 ? 32 : gy > 16384 ? 16384 : gy;
     size_t rows = (m + gy - 1) / gy;
     rows = (rows + 3) / 4 * 4;
-    return {(unsigned)gx, (unsigned)((m + rows - 1) / rows), (int)rows};
+    return {v, (unsigned)gx, (unsigned)((m + rows - 1) / rows), (int)rows};
+}
+
+struct bwd_args {
+    const void *dh;
+    const float *z;
+    size_t m, f;
+    uint16_t *dz;
+    int dtype;
+    float *part;
+};
+template <int V, int ACT, class D>
+void launch_bwd(const bwd_args &a, const bwd_plan &p, hipStream_t s)
+{
+    hipLaunchKernelGGL((k_gated_bwd<V, ACT, D>), dim3(p.gx, p.gy), dim3(256), 0, s, (const D *)a.dh, a.z, a.m, a.f,
+                       (a.f + 7) & ~(size_t)7, a.dz, a.dtype, a.part, p.rows);
+}
+template <int ACT>
+void launch_bwd(const bwd_args &a, int dh_dtype, const bwd_plan &p, hipStream_t s)
+{
+    if (p.v == 4)
+        dh_dtype == 0 ? launch_bwd<4, ACT, float>(a, p, s)
+                      : dh_dtype == 1 ? launch_bwd<4, ACT, _Float16>(a, p, s) : launch_bwd<4, ACT, __bf16>(a, p, s);
+    else
+        dh_dtype == 0 ? launch_bwd<1, ACT, float>(a, p, s)
+                      : dh_dtype == 1 ? launch_bwd<1, ACT, _Float16>(a, p, s) : launch_bwd<1, ACT, __bf16>(a, p, s);
+}
+
+// whether rows of dh and z keep pieces of four values aligned
+bool rows_of_four(const void *dh, int dh_dtype, const float *z, size_t f)
+{
+    return f % 4 == 0 && ((uintptr_t)z & 15) == 0 && ((uintptr_t)dh & (dh_dtype == 0 ? 15 : 7)) == 0;
 }
 
 } // namespace
 
-extern "C" int pgk_gated_act(int act, const float *z, size_t m, size_t f, float *h32, uint16_t *h16, int dtype,
-                             pgk_stream s)
+extern "C" int pgk_gated_forward(int dtype, int act, size_t m, size_t f, size_t k8, const uint16_t *x, size_t ldx,
+                                 const uint16_t *w, size_t f8, const float *bias, float *z, float *h32, uint16_t *h16,
+                                 pgk_stream s)
 {
-    const size_t n = m * f;
-    if (!n)
+    if (!m || !f)
         return 0;
-    const unsigned g = (unsigned)((n + 255) / 256 < 4096 ? (n + 255) / 256 : 4096);
-    hipLaunchKernelGGL(k_gated_act, dim3(g), dim3(256), 0, (hipStream_t)s, act, z, m, f, h32, h16, dtype);
-    return (int)hipGetLastError();
+    if (m > 0x7fffffff || f > 0x1fffffff || k8 > 0x7fff0000 || (k8 & 7) || (ldx & 7) || (f8 & 7) || f8 < f || ldx < k8 ||
+        ((((uintptr_t)x) | (uintptr_t)w) & 15) || (dtype != 1 && dtype != 2))
+        return (int)hipErrorInvalidValue;
+    gemm_kargs g = {};
+    g.A = x, g.lda = ldx, g.a_extent = (int)m;
+    g.B = w, g.ldb = 2 * f8, g.b_extent = (int)f8;
+    g.C = h32, g.ldc = f;
+    g.M = (int)m, g.N = (int)f, g.K = g.k_total = (int)k8;
+    g.epi.bias = bias, g.epi.act = act, g.epi.z = z, g.epi.c16 = h16, g.epi.dtype16 = dtype, g.epi.skip_out = !h32;
+    g.fast_ok = ldx < kFastLd && 2 * f8 < kFastLd;
+    const int tile = pgk_gemm16_whole_tile(m, 2 * f, k8);
+    return dtype == 1 ? launch_forward<true>(tile, g, (hipStream_t)s) : launch_forward<false>(tile, g, (hipStream_t)s);
 }
 
-extern "C" size_t pgk_gated_bwd_workspace(size_t m, size_t f) { return m && f ? plan_bwd(m, f).gy * 2 * f * sizeof(float) : 0; }
+extern "C" size_t pgk_gated_bwd_workspace(size_t m, size_t f)
+{
+    if (!m || !f)
+        return 0;
+    const size_t a = plan_bwd(m, f, true, true).gy, b = plan_bwd(m, f, false, true).gy;
+    return (a > b ? a : b) * 2 * f * sizeof(float);
+}
 
 extern "C" int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float *z, size_t m, size_t f, uint16_t *dz16,
                              int dtype, float *db, int db_beta, void *ws, pgk_stream s)
 {
     if (!m || !f)
         return 0;
-    if (m > 0x7fffffff || f > 0x3fffffff || (db && !ws))
+    if (m > 0x7fffffff || f > 0x1fffffff || (db && !ws) || ((uintptr_t)dz16 & 15) || act < 0 || act > PGK_ACT_SIGMOID)
         return (int)hipErrorInvalidValue;
-    const bwd_plan p = plan_bwd(m, f);
-    hipLaunchKernelGGL(k_gated_bwd, dim3(p.gx, p.gy), dim3(256), 0, (hipStream_t)s, act, dh, dh_dtype, z, m, f,
-                       (f + 7) & ~(size_t)7, dz16, dtype, db ? (float *)ws : nullptr, p.rows);
+    const bwd_plan p = plan_bwd(m, f, rows_of_four(dh, dh_dtype, z, f), db != nullptr);
+    const bwd_args a = {dh, z, m, f, dz16, dtype, db ? (float *)ws : nullptr};
+    hipStream_t st = (hipStream_t)s;
+    switch (act) {
+    case PGK_ACT_RELU: launch_bwd<PGK_ACT_RELU>(a, dh_dtype, p, st); break;
+    case PGK_ACT_GELU: launch_bwd<PGK_ACT_GELU>(a, dh_dtype, p, st); break;
+    case PGK_ACT_SILU: launch_bwd<PGK_ACT_SILU>(a, dh_dtype, p, st); break;
+    case PGK_ACT_SIGMOID: launch_bwd<PGK_ACT_SIGMOID>(a, dh_dtype, p, st); break;
+    default: launch_bwd<PGK_ACT_NONE>(a, dh_dtype, p, st); break;
+    }
     const int rc = (int)hipGetLastError();
     if (rc || !db)
         return rc;

@@ -868,7 +868,7 @@ static double ks_time(int tile, size_t m, size_t n, size_t k, size_t batch)
 // still win by 8 % over the best plan without one: its partials also cost
 // HBM capacity.
 static gemm_plan plan_gemm(int ta, int tb, size_t m, size_t n, size_t kin, size_t batch, int cu_budget = 0,
-                           double *time = nullptr)
+                           double *time = nullptr, bool whole_k = false)
 {
     const bool whole = !(cu_budget > 0 && cu_budget < kCUs);
     const double cus = whole ? (double)kCUs : (double)cu_budget;
@@ -889,7 +889,7 @@ static gemm_plan plan_gemm(int ta, int tb, size_t m, size_t n, size_t kin, size_
     double best_t = 1e300;
     for (const shape &sh : shapes) {
         const size_t tiles = ((m + sh.bm - 1) / sh.bm) * ((n + sh.bn - 1) / sh.bn) * batch;
-        const int max_sp = batch == 1 && kin >= 1024 ? 8 : 1;
+        const int max_sp = batch == 1 && kin >= 1024 && !whole_k ? 8 : 1;
         for (int sp = 1; sp <= max_sp; ++sp) {
             const size_t ks = ((kin + sp - 1) / sp + BK - 1) / BK * BK;
             if (sp > 1 && ks * (size_t)(sp - 1) >= kin)
@@ -989,6 +989,11 @@ extern "C" int pgk_gemm16_plan(int ta, int tb, size_t m, size_t n, size_t k, siz
     if (splits)
         *splits = pl.sp;
     return pl.tile;
+}
+
+extern "C" int pgk_gemm16_whole_tile(size_t m, size_t n, size_t k)
+{
+    return plan_gemm(0, 1, m, n, k, 1, 0, nullptr, true).tile;
 }
 
 extern "C" double pgk_gemm16_time(int ta, int tb, size_t m, size_t n, size_t k, size_t batch, int cu_budget)

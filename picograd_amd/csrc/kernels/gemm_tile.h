@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "convert16.h"
+#include "gate_act.h"
 #include "launch.h"
 #include "pgmath.h"
 
@@ -248,6 +249,47 @@ struct TileMN {
     }
 };
 
+// MN-contiguous tile of a gated layer's W = [Wg | Wu] [K, 2, extent]: groups of G
+// columns of Wg, each beside the same G columns of Wu, so that a block
+// holds g and u of the same outputs.  Fragments are TileMN's; column row0 counts
+// within either half.
+template <int ROWS, int NT, int KB, int G>
+struct TileGate : TileMN<ROWS, NT, KB> {
+    using Base = TileMN<ROWS, NT, KB>;
+    static_assert(G % 8 == 0 && ROWS % (2 * G) == 0, "whole chunks, whole pairs of groups");
+    // the column of W that tile column c (a multiple of 8) is; columns past
+    // `extent` of a half are clamped to its last 8 (never stored)
+    __device__ __forceinline__ static int column(int c, int row0, int extent)
+    {
+        const int f = row0 + c / (2 * G) * G + c % G;
+        return (c / G & 1) * extent + (f < extent ? f : extent - 8);
+    }
+    __device__ __forceinline__ static void load_q(int q, const uint16_t *__restrict__ p, size_t ld, int row0,
+                                                  int extent, int k0, int kend, LDS uint4 *dst, int tid)
+    {
+        const int lane = tid & 63, wave = tid >> 6;
+        const int base = (wave * Base::NQ + q) * 64;
+        const int slot = base + lane, k = slot / Base::CPR, logical = (slot % Base::CPR) ^ Base::fk(k);
+        const int mn = column(logical * 8, row0, extent);
+        const void *src = k0 + k < kend ? (const void *)(p + (size_t)(k0 + k) * ld + mn) : (const void *)&g_zero16;
+        dma16(src, dst + base);
+    }
+    using Fast = typename Base::Fast;
+    // the offset is from column 0 of the k-row, within a row of W for leading
+    // dims under kFastLd
+    __device__ __forceinline__ static Fast fast_q(int q, size_t ld, int row0, int extent, int wave, int lane)
+    {
+        const int base = (wave * Base::NQ + q) * 64, kq = base / Base::CPR;
+        const int slot = base + lane, k = slot / Base::CPR, logical = (slot % Base::CPR) ^ Base::fk(k);
+        return {(uint32_t)(((size_t)(k - kq) * ld + (size_t)column(logical * 8, row0, extent)) * 2), kq};
+    }
+    __device__ __forceinline__ static void load_fast(int q, const Fast &f, const uint16_t *__restrict__ p, size_t ld,
+                                                     int /*row0*/, int k0, LDS uint4 *dst, int wave)
+    {
+        dma16s(f.voff, p + (size_t)(k0 + f.srow) * ld, dst + (wave * Base::NQ + q) * 64);
+    }
+};
+
 // A GEMM launch's arguments (one problem; a paired launch takes two).
 struct gemm_kargs {
     const uint16_t *A;
@@ -265,13 +307,61 @@ struct gemm_kargs {
 
 // one kernel configuration: block tile BM x BN on WGM x WGN waves, operand
 // layouts TA / TB, f16 or bf16, fused epilogue, k-tile depth KB, S stages
-template <int BM_, int BN_, int WGM_, int WGN_, bool TA_, bool TB_, bool F16_, bool EPI_, int KB_, int S_>
+// GATE: the forward of a gated layer (TB, EPI; N, b_extent and n0 count the
+// columns of one half of W, a tile holds BN / 2 of them; epi.z [M, 2 N])
+template <int BM_, int BN_, int WGM_, int WGN_, bool TA_, bool TB_, bool F16_, bool EPI_, int KB_, int S_, bool GATE_ = false>
 struct gcfg {
+    static constexpr bool GATE = GATE_;
     static constexpr int BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, KB = KB_, S = S_;
     static constexpr bool TA = TA_, TB = TB_, F16 = F16_, EPI = EPI_;
     static constexpr int NT = 64 * WGM * WGN;
     static constexpr int LDS_U4 = S * (BM * KB / 8 + BN * KB / 8); // uint4 of LDS
 };
+
+// Four outputs of a gated layer, row `row`, columns col .. col + 3 of the n: z = [g | u]
+// and h = act(g) u, in f32 (c) unless skip_out and in 16 bits.  The stores are
+// whole pieces where the rows keep their alignment.
+__device__ __forceinline__ void gate_store(const pgk_epi &epi, float *c, int n, int row, int col, f32x4 gv, f32x4 uv)
+{
+    const size_t h = (size_t)row * n + col, zg = (size_t)row * 2 * n + col, zu = zg + n;
+    const bool v4 = (n & 3) == 0 && ((((uintptr_t)c) | (uintptr_t)epi.z) & 15) == 0 && (((uintptr_t)epi.c16) & 7) == 0;
+    f32x4 o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (epi.bias && col + q < n) {
+            gv[q] += epi.bias[col + q];
+            uv[q] += epi.bias[n + col + q];
+        }
+    gate_switch(epi.act, [&](auto code) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            o[q] = gate_f<decltype(code)::value>(gv[q]) * uv[q];
+    });
+    if (v4) {
+        if (epi.z) { // read again only by the backward, much later
+            __builtin_nontemporal_store(gv, (f32x4 *)(epi.z + zg));
+            __builtin_nontemporal_store(uv, (f32x4 *)(epi.z + zu));
+        }
+        if (!epi.skip_out)
+            *(f32x4 *)(c + h) = o;
+        if (epi.c16)
+            *(uint2 *)(epi.c16 + h) = make_uint2(to16x2(epi.dtype16, o[0], o[1]), to16x2(epi.dtype16, o[2], o[3]));
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (col + q >= n)
+            break;
+        if (epi.z) {
+            epi.z[zg + q] = gv[q];
+            epi.z[zu + q] = uv[q];
+        }
+        if (!epi.skip_out)
+            c[h + q] = o[q];
+        if (epi.c16)
+            epi.c16[h + q] = to16(epi.dtype16, o[q]);
+    }
+}
 
 // One block tile of problem g: tile pid of the nb tiles of batch entry (or
 // split-K slice) z, with the LDS ring at lds.  remap: block ids were dealt
@@ -294,7 +384,10 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
     constexpr int WM = BM / WGM, WN = BN / WGN;
     constexpr int FM = WM / 32, FN = WN / 32;
     using OA = typename std::conditional<TA, TileMN<BM, NT, KB>, TileK<BM, NT, KB>>::type;
-    using OB = typename std::conditional<TB, TileMN<BN, NT, KB>, TileK<BN, NT, KB>>::type;
+    constexpr bool GATE = CF::GATE;
+    using OB = typename std::conditional<
+        GATE, TileGate<BN, NT, KB, 32>,
+        typename std::conditional<TB, TileMN<BN, NT, KB>, TileK<BN, NT, KB>>::type>::type;
     // S-stage ring of A and B tiles in one LDS block; the k-loop below is
     // unrolled by S, so every stage index is a compile-time constant
     constexpr int SA = BM * KB / 8, SB = BN * KB / 8; // uint4 per stage
@@ -311,7 +404,7 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
     const int first_m = group * GM;
     const int gsz = tiles_m - first_m < GM ? tiles_m - first_m : GM;
     const int in_group = pid - group * per_group;
-    const int m0 = (first_m + in_group % gsz) * BM, n0 = (in_group / gsz) * BN;
+    const int m0 = (first_m + in_group % gsz) * BM, n0 = (in_group / gsz) * (GATE ? BN / 2 : BN);
 
     const uint16_t *Ab = A + (size_t)z * sA;
     const uint16_t *Bb = B + (size_t)z * sB;
@@ -492,7 +585,31 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
 
     // epilogue: lane holds column lane % 32 of rows (e/4)*8 + (lane/32)*4 + e%4
     const int lrow = lane & 31, lk = lane >> 5;
-    if constexpr (EPI) {
+    if constexpr (GATE) {
+        // through LDS as below: the wave's first 32 columns are g, the others u of
+        // the same 32 outputs, four outputs a lane
+        static_assert(WN == 64 && EPI && TB && !TA, "one group of g and one of u per wave");
+        constexpr int RS = WN + 8;
+        LDS float *reg = (LDS float *)((LDS char *)lds + wave * (32 * RS * 4));
+        const int c4 = (lane & 7) * 4, col = n0 + wn * 32 + c4;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    reg[((e >> 2) * 8 + lk * 4 + (e & 3)) * RS + j * 32 + lrow] = acc[i][j][e];
+            __syncthreads();
+#pragma unroll 1
+            for (int row = lane >> 3; row < 32; row += 8) {
+                const int grow = m0 + wm * WM + i * 32 + row;
+                if (grow < M && col < N)
+                    gate_store(epi, g.C, N, grow, col, *(const LDS f32x4 *)(reg + row * RS + c4),
+                               *(const LDS f32x4 *)(reg + row * RS + 32 + c4));
+            }
+        }
+    } else if constexpr (EPI) {
         // Through LDS, 32 rows of the wave's WM x WN tile at a time: the
         // accumulators land row-major in a per-wave [32][WN + 8] f32 region
         // (in the operand stages, free after the k-loop) and come back as
@@ -612,8 +729,10 @@ __device__ __forceinline__ void epi_store(const pgk_epi &epi, float *c, size_t o
 // back to back against the 128-tile plans (split-K where they split):
 // 512 x 1024 x 4096 dgrad 20.0 -> 14.4 us, 1024^3 20.1 -> 8.4 us, a
 // 512 x 4096 x 1024 gelu layer 22.8 -> 17.1 us, 256 x 256 x 512 9.5 -> 4.5 us.
-template <int TM_, int TN_, int KG_, int KB_, int S_, bool TA_, bool TB_, bool F16_>
+// GATE: as gcfg's
+template <int TM_, int TN_, int KG_, int KB_, int S_, bool TA_, bool TB_, bool F16_, bool GATE_ = false>
 struct kscfg {
+    static constexpr bool GATE = GATE_;
     static constexpr int TM = TM_, TN = TN_, KG = KG_, KB = KB_, S = S_;
     static constexpr bool TA = TA_, TB = TB_, F16 = F16_;
     static constexpr int NT = 64 * KG, RS = TN + 4; // floats of a partial tile's row
@@ -638,7 +757,9 @@ __device__ __forceinline__ void ks_block(const gemm_kargs &g, int has_epi, int p
     constexpr int TM = CF::TM, TN = CF::TN, KG = CF::KG, KB = CF::KB, S = CF::S, FM = TM / 32, FN = TN / 32;
     constexpr bool F16 = CF::F16;
     using OA = typename std::conditional<CF::TA, TileMN<TM, 64, KB>, TileK<TM, 64, KB>>::type;
-    using OB = typename std::conditional<CF::TB, TileMN<TN, 64, KB>, TileK<TN, 64, KB>>::type;
+    using OB = typename std::conditional<
+        CF::GATE, TileGate<TN, 64, KB, TN / 2>,
+        typename std::conditional<CF::TB, TileMN<TN, 64, KB>, TileK<TN, 64, KB>>::type>::type;
     constexpr int LPT = OA::NQ + OB::NQ, SA = TM * KB / 8, KS = KB / 16;
     static_assert((S - 1) * LPT < 64, "the loads in flight fit the vmcnt counter");
     const int lane = threadIdx.x & 63;
@@ -652,7 +773,7 @@ __device__ __forceinline__ void ks_block(const gemm_kargs &g, int has_epi, int p
         pid = xcd_tile(pid, nb);
     const int group = pid / (8 * g.tiles_n), first = group * 8;
     const int gsz = g.tiles_m - first < 8 ? g.tiles_m - first : 8, in = pid - group * 8 * g.tiles_n;
-    const int m0 = (first + in % gsz) * TM, n0 = in / gsz * TN;
+    const int m0 = (first + in % gsz) * TM, n0 = in / gsz * (CF::GATE ? TN / 2 : TN);
     const uint16_t *A = g.A + (size_t)z * g.sA, *B = g.B + (size_t)z * g.sB;
     LDS uint4 *const ring = lds + wave * S * CF::STAGE;
     const int nct = (g.K + KB - 1) / KB, nc = nct > wave ? (nct - wave + KG - 1) / KG : 0;
@@ -761,6 +882,22 @@ __device__ __forceinline__ void ks_block(const gemm_kargs &g, int has_epi, int p
             for (int e = 0; e < 16; ++e)
                 part[(wave * TM + i * 32 + (e >> 2) * 8 + lk * 4 + (e & 3)) * CF::RS + j * 32 + lrow] = acc[0][i][j][e];
     __syncthreads();
+    if constexpr (CF::GATE) {
+#pragma unroll 1
+        for (int i = (int)threadIdx.x; i < TM * TN / 8; i += CF::NT) {
+            const int row = i / (TN / 8), c4 = i % (TN / 8) * 4, gr = m0 + row, gc = n0 + c4;
+            if (gr >= g.M || gc >= g.N)
+                continue;
+            f32x4 gv = {0.0f, 0.0f, 0.0f, 0.0f}, uv = gv;
+#pragma unroll
+            for (int w = 0; w < KG; ++w) {
+                gv += *(const LDS f32x4 *)(part + (w * TM + row) * CF::RS + c4);
+                uv += *(const LDS f32x4 *)(part + (w * TM + row) * CF::RS + TN / 2 + c4);
+            }
+            gate_store(g.epi, g.C, g.N, gr, gc, gv, uv);
+        }
+        return;
+    }
     float *C = g.C + (size_t)z * g.sC;
     const pgk_epi &epi = g.epi;
     const bool v4 = (g.ldc & 3) == 0 && (((uintptr_t)C | (uintptr_t)epi.z) & 15) == 0 && (((uintptr_t)epi.c16) & 7) == 0;

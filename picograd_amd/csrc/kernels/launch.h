@@ -178,6 +178,9 @@ int pgk_gemm16_lean(int dtype, int ta, int tb, size_t m, size_t n, size_t k, con
 /* the tile (1: 128 x 128, 2: 256 x 256, 3: 128 x 256) and split-K factor
  * (*splits) pgk_gemm16_cu's main launch takes for these sizes */
 int pgk_gemm16_plan(int ta, int tb, size_t m, size_t n, size_t k, size_t batch, int cu_budget, int *splits);
+/* the tile (those, or the split-over-waves 5 to 8) of a forward product that
+ * one launch finishes, without split-K */
+int pgk_gemm16_whole_tile(size_t m, size_t n, size_t k);
 /* One GEMM problem of pgk_gemm16's parameters */
 typedef struct {
     size_t m, n, k;
@@ -262,16 +265,19 @@ int pgk_act_bwd16n(int act, const uint16_t *dn, const uint16_t *wn, int kw, int 
                    const float *z, size_t m, size_t n, uint16_t *d16, size_t ldd, int dtype, float *db, int db_beta,
                    void *ws, const pgk_colsum_job *fold, pgk_colsum_job *defer, pgk_stream s);
 
-/* Gated feed-forward layer (gated.hip), z = x W + b = [g | u] [m, 2 f] f32:
- * h = act(g) u, acts PGK_ACT_* and the two below.
- * _act: h [m, f] from z, in f32 (h32) and / or 16 bits (h16, RNE; rows of f).
+/* Gated feed-forward layer (gated.hip), z = x W + bias = [g | u] [m, 2 f] f32:
+ * h = act(g) u [m, f], acts PGK_ACT_* and the two below.
+ * _forward: from x [m, k8] (ldx) and W [k8, 2, f8] 16-bit of dtype, k8 and f8
+ * multiples of 8 (zeros past the layer's own sizes), one launch: h in f32 (h32)
+ * and / or 16 bits (h16, RNE), and z unless NULL.
  * _bwd: dg = dh u act'(g), du = dh act(g) from dh [m, f] (dh_dtype 0 = f32,
  * else 16-bit of that dtype), RNE into dz16 [m, 2 f8] (dg at column 0, du at
  * f8 = f rounded up to 8, zeros between) and, when db is given, their column
  * sums db [2 f] (beta ? += : =) in a fixed order (ws: pgk_gated_bwd_workspace
  * bytes). */
 enum { PGK_ACT_SILU = 3, PGK_ACT_SIGMOID = 4 };
-int pgk_gated_act(int act, const float *z, size_t m, size_t f, float *h32, uint16_t *h16, int dtype, pgk_stream s);
+int pgk_gated_forward(int dtype, int act, size_t m, size_t f, size_t k8, const uint16_t *x, size_t ldx, const uint16_t *w,
+                      size_t f8, const float *bias, float *z, float *h32, uint16_t *h16, pgk_stream s);
 size_t pgk_gated_bwd_workspace(size_t m, size_t f);
 int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float *z, size_t m, size_t f, uint16_t *dz16, int dtype,
                   float *db, int db_beta, void *ws, pgk_stream s);
