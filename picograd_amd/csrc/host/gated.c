@@ -47,12 +47,11 @@ typedef struct {
 } gated_out;
 
 static bool product(const char *what, int dt, int t, size_t m, size_t n, size_t k, const uint16_t *a, size_t lda,
-                    size_t aext, const uint16_t *b, size_t ldb, size_t bext, const gated_out *o, size_t off, size_t ldc)
+                    size_t aext, const uint16_t *b, size_t ldb, size_t bext, const gated_out *o, size_t ldc)
 {
     if (!o->is16)
-        return pgm_gemm16x(dt, t, t, m, n, k, a, lda, 0, aext, b, ldb, 0, bext, (float *)o->p + off, ldc, 0, 1, o->beta,
-                           NULL, what);
-    const pgk_epi epi = {.act = PGK_ACT_NONE, .c16 = (uint16_t *)o->p + off, .dtype16 = dt, .skip_out = 1};
+        return pgm_gemm16x(dt, t, t, m, n, k, a, lda, 0, aext, b, ldb, 0, bext, o->p, ldc, 0, 1, o->beta, NULL, what);
+    const pgk_epi epi = {.act = PGK_ACT_NONE, .c16 = o->p, .dtype16 = dt, .skip_out = 1};
     return pgm_gemm16x(dt, t, t, m, n, k, a, lda, 0, aext, b, ldb, 0, bext, NULL, ldc, 0, 1, 0, &epi, what);
 }
 
@@ -69,12 +68,13 @@ static bool grads(const char *what, int dt, const gated_dims *d, const uint16_t 
     }
     bool ok = true;
     if (dx->p)
-        ok = product(what, dt, 0, d->M, d->K, N8, dz16, N8, d->M, w16, N8, d->K, dx, 0, d->K);
+        ok = product(what, dt, 0, d->M, d->K, N8, dz16, N8, d->M, w16, N8, d->K, dx, d->K);
     if (dw->p && N == N8) {
-        ok = ok && product(what, dt, 1, d->K, N, d->M, x16, d->K8, d->K8, dz16, N8, N8, dw, 0, N);
-    } else if (dw->p) {
-        for (int p = 0; ok && p < 2; p++)
-            ok = product(what, dt, 1, d->K, d->F, d->M, x16, d->K8, d->K8, dz16 + p * d->F8, N8, d->F8, dw, p * d->F, N);
+        ok = ok && product(what, dt, 1, d->K, N, d->M, x16, d->K8, d->K8, dz16, N8, N8, dw, N);
+    } else if (ok && dw->p) { /* the halves of dW as a batch of two, F apart in its rows */
+        const pgk_epi epi = {.act = PGK_ACT_NONE, .c16 = dw->p, .dtype16 = dt, .skip_out = 1};
+        ok = pgm_gemm16x(dt, 1, 1, d->K, d->F, d->M, x16, d->K8, 0, d->K8, dz16, N8, d->F8, d->F8,
+                         dw->is16 ? NULL : dw->p, N, d->F, 2, dw->is16 ? 0 : dw->beta, dw->is16 ? &epi : NULL, what);
     }
     return ok;
 }
@@ -108,22 +108,25 @@ typedef struct {
     size_t bx, bw;
 } gated_ops;
 
-static bool stage(const gated_dims *d, int dt, const pg_tensor *x, const pg_tensor *w, gated_ops *o)
+static bool stage(const gated_dims *d, const pg_tensor *x, const pg_tensor *w, gated_ops *o)
 {
     *o = (gated_ops){x->dev, w->dev, NULL, NULL, 0, 0};
     if (!d->K)
         return true;
     if (d->K != d->K8 || !aligned16(x->dev)) {
-        o->x = o->ox = pgm_stage16(dt, dt, x->dev, d->M, d->K, d->K, d->M, d->K8, 1, 0, &o->bx);
+        o->bx = d->M * d->K8 * 2;
+        o->x = o->ox = pgd_malloc(o->bx);
         if (!o->x)
             return false;
     }
     if (d->K != d->K8 || d->F != d->F8 || !aligned16(w->dev)) {
-        o->w = o->ow = pgm_stage16(dt, dt, w->dev, 2 * d->K, d->F, d->F, 2 * d->K8, d->F8, 1, 0, &o->bw);
+        o->bw = d->K8 * 2 * d->F8 * 2;
+        o->w = o->ow = pgd_malloc(o->bw);
         if (!o->w)
             return false;
     }
-    return true;
+    return !(o->ox || o->ow) ||
+           pgd_check(pgk_gated_pad(x->dev, d->M, d->K, o->ox, w->dev, d->F, o->ow, pgd_stream()), "gated operands");
 }
 
 static void unstage(const gated_ops *o)
@@ -199,7 +202,7 @@ bool pg_amd_gated(const pg_tensor *x, const pg_tensor *w, const pg_tensor *b, in
         pgo_output(h);
         if (z)
             pgo_output(z);
-        ok = done(what, stage(&d, (int)x->dtype, xc, wc, &o) &&
+        ok = done(what, stage(&d, xc, wc, &o) &&
                             forward(what, (int)x->dtype, &d, act, o.x, o.w, bc ? bc->dev : NULL, z ? z->dev : NULL,
                                     h->dtype == PG_DTYPE_F32 ? h->dev : NULL,
                                     h->dtype == PG_DTYPE_F32 ? NULL : h->dev));
@@ -252,7 +255,7 @@ bool pg_amd_gated_backward(const pg_tensor *x, const pg_tensor *w, const pg_tens
         uint16_t *dz = make_dz(what, dt, &d, act, hc, zc->dev, db ? db->dev : NULL, 0);
         const gated_out ox = {dx && d.K ? dx->dev : NULL, dx && dx->dtype != PG_DTYPE_F32, 0};
         const gated_out ow = {dw && d.K ? dw->dev : NULL, dw && dw->dtype != PG_DTYPE_F32, 0};
-        ok = done(what, dz && stage(&d, dt, xc, wc, &o) && grads(what, dt, &d, o.x, o.w, dz, &ox, &ow));
+        ok = done(what, dz && stage(&d, xc, wc, &o) && grads(what, dt, &d, o.x, o.w, dz, &ox, &ow));
         unstage(&o);
         if (dz)
             pgd_free(dz, d.M * 2 * d.F8 * 2);

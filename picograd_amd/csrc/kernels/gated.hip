@@ -13,6 +13,32 @@
 
 namespace {
 
+// ---------------------------------------------------------------- operands
+
+// Two matrices of 16-bit values with their rows padded by zeros to whole 16-byte
+// pieces, in one launch: eight values a thread, read one by one (the rows'
+// own alignment is any).
+struct pad_job {
+    const uint16_t *src;
+    uint16_t *dst;
+    size_t rows, cols, rows_pad, cols8; // cols8: pieces of a padded row
+};
+__global__ void __launch_bounds__(256) k_gated_pad(pad_job a, pad_job b, size_t na, size_t n)
+{
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const bool second = i >= na;
+        const pad_job &j = second ? b : a;
+        const size_t k = second ? i - na : i, r = k / j.cols8, c = (k - r * j.cols8) * 8;
+        const uint16_t *p = j.src + r * j.cols + c;
+        uint16_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = r < j.rows && c + e < j.cols ? p[e] : (uint16_t)0;
+        ((uint4 *)j.dst)[k] = make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16,
+                                         v[6] | (uint32_t)v[7] << 16);
+    }
+}
+
 // ---------------------------------------------------------------- forward
 
 // A tile of the product holds columns of Wg beside the same columns of Wu
@@ -142,7 +168,14 @@ __global__ void __launch_bounds__(kFewWaves * 64, 1) k_gated_few(gemm_kargs g)
             gv += *(const LDS f32x4 *)(part + (w * 16 + row) * RP + c4);
             uv += *(const LDS f32x4 *)(part + (w * 16 + row) * RP + 16 + c4);
         }
-        gate_store(g.epi, g.C, g.N, row, n0 + c4, gv, uv);
+        if (gate_whole(g.epi, g.C, g.N)) {
+            gate_store4(g.epi, g.C, g.N, row, n0 + c4, gv, uv);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n0 + c4 + q < g.N)
+                    gate_store1(g.epi, g.C, g.N, row, n0 + c4 + q, gv[q], uv[q]);
+        }
     }
 }
 
@@ -251,7 +284,7 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// The blocks of rows: enough to fill the chip, at most 32 where they leave
+// The blocks of rows: enough to fill the chip, at most 64 where they leave
 // partial column sums, which one more launch adds one after the other.
 struct bwd_plan {
     int v;
@@ -262,8 +295,8 @@ bwd_plan plan_bwd(size_t m, size_t f, bool v4, bool sums)
 {
     const int v = v4 ? 4 : 1;
     const size_t gx = (f + 64 * v - 1) / (64 * v);
-    size_t gy = (sums ? 1024 : 4096) / gx;
-    gy = gy < 1 ? 1 : sums && gy > 32 ? 32 : gy > 16384 ? 16384 : gy;
+    size_t gy = (sums ? 2048 : 4096) / gx;
+    gy = gy < 1 ? 1 : sums && gy > 64 ? 64 : gy > 16384 ? 16384 : gy;
     size_t rows = (m + gy - 1) / gy;
     rows = (rows + 3) / 4 * 4;
     return {v, (unsigned)gx, (unsigned)((m + rows - 1) / rows), (int)rows};
@@ -301,6 +334,20 @@ bool rows_of_four(const void *dh, int dh_dtype, const float *z, size_t f)
 }
 
 } // namespace
+
+extern "C" int pgk_gated_pad(const uint16_t *x, size_t m, size_t k, uint16_t *x16, const uint16_t *w, size_t f, uint16_t *w16,
+                             pgk_stream s)
+{
+    const size_t k8 = (k + 7) / 8, f8 = (f + 7) / 8;
+    const pad_job a = {x, x16, m, k, m, k8}, b = {w, w16, 2 * k, f, 16 * k8, f8};
+    const size_t na = x16 ? a.rows_pad * a.cols8 : 0, n = na + (w16 ? b.rows_pad * b.cols8 : 0);
+    if (!n)
+        return 0;
+    const size_t blocks = (n + 255) / 256;
+    hipLaunchKernelGGL(k_gated_pad, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, (hipStream_t)s, a, b, na,
+                       n);
+    return (int)hipGetLastError();
+}
 
 extern "C" int pgk_gated_forward(int dtype, int act, size_t m, size_t f, size_t k8, const uint16_t *x, size_t ldx,
                                  const uint16_t *w, size_t f8, const float *bias, float *z, float *h32, uint16_t *h16,

@@ -1024,7 +1024,9 @@ extern "C" int pgk_gemm16_cu(int dtype, int ta, int tb, size_t m, size_t n, size
     if (!m || !n || !batch)
         return 0;
     const bool has_epi = epi && (epi->bias || epi->act != PGK_ACT_NONE || epi->z || epi->c16);
-    if (has_epi && (beta || batch != 1 || (epi->c16 && epi->dtype16 != 1 && epi->dtype16 != 2)))
+    // of a batch only the 16-bit form, where one launch finishes it
+    const bool only16 = has_epi && epi->c16 && epi->skip_out && !epi->bias && epi->act == PGK_ACT_NONE && !epi->z;
+    if (has_epi && (beta || (batch != 1 && !only16) || (epi->c16 && epi->dtype16 != 1 && epi->dtype16 != 2)))
         return (int)hipErrorInvalidValue;
     // an unwritten C needs the epilogue on the GEMM or the split-K sum: the
     // k-tail and empty-k paths apply it over C's accumulated values
@@ -1094,7 +1096,7 @@ extern "C" int pgk_gemm16_cu(int dtype, int ta, int tb, size_t m, size_t n, size
     } else if (has_epi && !sp && !ktail && (tb || !ta)) {
         // a forward product's epilogue, or a grad's rounded to 16 bits
         gemm_args g = {a, lda, stride_a, (int)a_extent, b, ldb, stride_b, (int)b_extent, c, ldc, stride_c,
-                       (int)m, (int)n, (int)kmain, 0, 1u, pl.tile};
+                       (int)m, (int)n, (int)kmain, 0, (unsigned)batch, pl.tile};
         if (!tb)
             return f16 ? launch_layout<false, false, true, true>(g, st, *epi)
                        : launch_layout<false, false, false, true>(g, st, *epi);

@@ -318,17 +318,20 @@ struct gcfg {
     static constexpr int LDS_U4 = S * (BM * KB / 8 + BN * KB / 8); // uint4 of LDS
 };
 
-// Four outputs of a gated layer, row `row`, columns col .. col + 3 of the n: z = [g | u]
-// and h = act(g) u, in f32 (c) unless skip_out and in 16 bits.  The stores are
-// whole pieces where the rows keep their alignment.
-__device__ __forceinline__ void gate_store(const pgk_epi &epi, float *c, int n, int row, int col, f32x4 gv, f32x4 uv)
+// Outputs of a gated layer: z = [g | u] (biases added here) and h = act(g) u, in
+// f32 (c) unless skip_out and in 16 bits.  gate_store4: columns col .. col + 3 of
+// the n (a multiple of 4) of row `row`, whole pieces; gate_store1: one column.
+__device__ __forceinline__ bool gate_whole(const pgk_epi &epi, const float *c, int n)
 {
-    const size_t h = (size_t)row * n + col, zg = (size_t)row * 2 * n + col, zu = zg + n;
-    const bool v4 = (n & 3) == 0 && ((((uintptr_t)c) | (uintptr_t)epi.z) & 15) == 0 && (((uintptr_t)epi.c16) & 7) == 0;
+    return (n & 3) == 0 && ((((uintptr_t)c) | (uintptr_t)epi.z) & 15) == 0 && (((uintptr_t)epi.c16) & 7) == 0;
+}
+__device__ __forceinline__ void gate_store4(const pgk_epi &epi, float *c, int n, int row, int col, f32x4 gv, f32x4 uv)
+{
+    const size_t h = (size_t)row * n + col, zg = (size_t)row * 2 * n + col;
     f32x4 o;
+    if (epi.bias)
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-        if (epi.bias && col + q < n) {
+        for (int q = 0; q < 4; ++q) {
             gv[q] += epi.bias[col + q];
             uv[q] += epi.bias[n + col + q];
         }
@@ -337,30 +340,32 @@ __device__ __forceinline__ void gate_store(const pgk_epi &epi, float *c, int n, 
         for (int q = 0; q < 4; ++q)
             o[q] = gate_f<decltype(code)::value>(gv[q]) * uv[q];
     });
-    if (v4) {
-        if (epi.z) { // read again only by the backward, much later
-            __builtin_nontemporal_store(gv, (f32x4 *)(epi.z + zg));
-            __builtin_nontemporal_store(uv, (f32x4 *)(epi.z + zu));
-        }
-        if (!epi.skip_out)
-            *(f32x4 *)(c + h) = o;
-        if (epi.c16)
-            *(uint2 *)(epi.c16 + h) = make_uint2(to16x2(epi.dtype16, o[0], o[1]), to16x2(epi.dtype16, o[2], o[3]));
-        return;
+    if (epi.z) { // read again only by the backward, much later
+        __builtin_nontemporal_store(gv, (f32x4 *)(epi.z + zg));
+        __builtin_nontemporal_store(uv, (f32x4 *)(epi.z + zg + n));
     }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        if (col + q >= n)
-            break;
-        if (epi.z) {
-            epi.z[zg + q] = gv[q];
-            epi.z[zu + q] = uv[q];
-        }
-        if (!epi.skip_out)
-            c[h + q] = o[q];
-        if (epi.c16)
-            epi.c16[h + q] = to16(epi.dtype16, o[q]);
+    if (!epi.skip_out)
+        *(f32x4 *)(c + h) = o;
+    if (epi.c16)
+        *(uint2 *)(epi.c16 + h) = make_uint2(to16x2(epi.dtype16, o[0], o[1]), to16x2(epi.dtype16, o[2], o[3]));
+}
+__device__ __forceinline__ void gate_store1(const pgk_epi &epi, float *c, int n, int row, int col, float gv, float uv)
+{
+    const size_t h = (size_t)row * n + col, zg = (size_t)row * 2 * n + col;
+    if (epi.bias) {
+        gv += epi.bias[col];
+        uv += epi.bias[n + col];
     }
+    float o = 0.0f;
+    gate_switch(epi.act, [&](auto code) { o = gate_f<decltype(code)::value>(gv) * uv; });
+    if (epi.z) {
+        epi.z[zg] = gv;
+        epi.z[zg + n] = uv;
+    }
+    if (!epi.skip_out)
+        c[h] = o;
+    if (epi.c16)
+        epi.c16[h] = to16(epi.dtype16, o);
 }
 
 // One block tile of problem g: tile pid of the nb tiles of batch entry (or
@@ -587,11 +592,13 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
     const int lrow = lane & 31, lk = lane >> 5;
     if constexpr (GATE) {
         // through LDS as below: the wave's first 32 columns are g, the others u of
-        // the same 32 outputs, four outputs a lane
+        // the same 32 outputs; four outputs a lane, or one where rows of n do
+        // not keep whole pieces (then neighbouring lanes store neighbours)
         static_assert(WN == 64 && EPI && TB && !TA, "one group of g and one of u per wave");
         constexpr int RS = WN + 8;
         LDS float *reg = (LDS float *)((LDS char *)lds + wave * (32 * RS * 4));
-        const int c4 = (lane & 7) * 4, col = n0 + wn * 32 + c4;
+        const bool v4 = gate_whole(epi, g.C, N);
+        const int cl = v4 ? (lane & 7) * 4 : lrow, col = n0 + wn * 32 + cl;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             __syncthreads();
@@ -601,12 +608,18 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
                 for (int e = 0; e < 16; ++e)
                     reg[((e >> 2) * 8 + lk * 4 + (e & 3)) * RS + j * 32 + lrow] = acc[i][j][e];
             __syncthreads();
+            const int grow0 = m0 + wm * WM + i * 32;
+            if (col >= N)
+                continue;
+            if (v4) {
 #pragma unroll 1
-            for (int row = lane >> 3; row < 32; row += 8) {
-                const int grow = m0 + wm * WM + i * 32 + row;
-                if (grow < M && col < N)
-                    gate_store(epi, g.C, N, grow, col, *(const LDS f32x4 *)(reg + row * RS + c4),
-                               *(const LDS f32x4 *)(reg + row * RS + 32 + c4));
+                for (int row = lane >> 3; row < 32 && grow0 + row < M; row += 8)
+                    gate_store4(epi, g.C, N, grow0 + row, col, *(const LDS f32x4 *)(reg + row * RS + cl),
+                                *(const LDS f32x4 *)(reg + row * RS + 32 + cl));
+            } else {
+#pragma unroll 1
+                for (int row = lk; row < 32 && grow0 + row < M; row += 2)
+                    gate_store1(epi, g.C, N, grow0 + row, col, reg[row * RS + cl], reg[row * RS + 32 + cl]);
             }
         }
     } else if constexpr (EPI) {
@@ -626,8 +639,9 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             bias4[q] = (epi.bias && gcol + q < N) ? epi.bias[gcol + q] : 0.0f;
+        uint16_t *const c16 = epi.c16 ? epi.c16 + (size_t)z * sC : nullptr;
         const bool v4 = (ldc & 3) == 0 && gcol + 3 < N && (((uintptr_t)Cb) & 15) == 0 &&
-                        (((uintptr_t)epi.z) & 15) == 0 && (((uintptr_t)epi.c16) & 7) == 0;
+                        (((uintptr_t)epi.z) & 15) == 0 && (((uintptr_t)c16) & 7) == 0;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             __syncthreads(); // the k-loop's (or the previous pass') LDS reads are done
@@ -656,8 +670,8 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
                         const f32x4 zz = {zv[0], zv[1], zv[2], zv[3]};
                         __builtin_nontemporal_store(zz, reinterpret_cast<f32x4 *>(epi.z + off));
                     }
-                    if (epi.c16)
-                        *reinterpret_cast<uint2 *>(epi.c16 + off) =
+                    if (c16)
+                        *reinterpret_cast<uint2 *>(c16 + off) =
                             make_uint2(to16x2(epi.dtype16, o[0], o[1]), to16x2(epi.dtype16, o[2], o[3]));
                 } else {
 #pragma unroll
@@ -668,8 +682,8 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
                             Cb[off + q] = o[q];
                         if (epi.z)
                             epi.z[off + q] = zv[q];
-                        if (epi.c16)
-                            epi.c16[off + q] = to16(epi.dtype16, o[q]);
+                        if (c16)
+                            c16[off + q] = to16(epi.dtype16, o[q]);
                     }
                 }
             }
@@ -883,23 +897,41 @@ __device__ __forceinline__ void ks_block(const gemm_kargs &g, int has_epi, int p
                 part[(wave * TM + i * 32 + (e >> 2) * 8 + lk * 4 + (e & 3)) * CF::RS + j * 32 + lrow] = acc[0][i][j][e];
     __syncthreads();
     if constexpr (CF::GATE) {
+        if (gate_whole(g.epi, g.C, g.N)) {
 #pragma unroll 1
-        for (int i = (int)threadIdx.x; i < TM * TN / 8; i += CF::NT) {
-            const int row = i / (TN / 8), c4 = i % (TN / 8) * 4, gr = m0 + row, gc = n0 + c4;
-            if (gr >= g.M || gc >= g.N)
-                continue;
-            f32x4 gv = {0.0f, 0.0f, 0.0f, 0.0f}, uv = gv;
+            for (int i = (int)threadIdx.x; i < TM * TN / 8; i += CF::NT) {
+                const int row = i / (TN / 8), c4 = i % (TN / 8) * 4, gr = m0 + row, gc = n0 + c4;
+                if (gr >= g.M || gc >= g.N)
+                    continue;
+                f32x4 gv = {0.0f, 0.0f, 0.0f, 0.0f}, uv = gv;
 #pragma unroll
-            for (int w = 0; w < KG; ++w) {
-                gv += *(const LDS f32x4 *)(part + (w * TM + row) * CF::RS + c4);
-                uv += *(const LDS f32x4 *)(part + (w * TM + row) * CF::RS + TN / 2 + c4);
+                for (int w = 0; w < KG; ++w) {
+                    gv += *(const LDS f32x4 *)(part + (w * TM + row) * CF::RS + c4);
+                    uv += *(const LDS f32x4 *)(part + (w * TM + row) * CF::RS + TN / 2 + c4);
+                }
+                gate_store4(g.epi, g.C, g.N, gr, gc, gv, uv);
             }
-            gate_store(g.epi, g.C, g.N, gr, gc, gv, uv);
+        } else {
+#pragma unroll 1
+            for (int i = (int)threadIdx.x; i < TM * TN / 2; i += CF::NT) {
+                const int row = i / (TN / 2), c = i % (TN / 2), gr = m0 + row, gc = n0 + c;
+                if (gr >= g.M || gc >= g.N)
+                    continue;
+                float gv = 0.0f, uv = 0.0f;
+#pragma unroll
+                for (int w = 0; w < KG; ++w) {
+                    gv += part[(w * TM + row) * CF::RS + c];
+                    uv += part[(w * TM + row) * CF::RS + TN / 2 + c];
+                }
+                gate_store1(g.epi, g.C, g.N, gr, gc, gv, uv);
+            }
         }
         return;
     }
     float *C = g.C + (size_t)z * g.sC;
-    const pgk_epi &epi = g.epi;
+    pgk_epi epi = g.epi;
+    if (epi.c16)
+        epi.c16 += (size_t)z * g.sC;
     const bool v4 = (g.ldc & 3) == 0 && (((uintptr_t)C | (uintptr_t)epi.z) & 15) == 0 && (((uintptr_t)epi.c16) & 7) == 0;
 #pragma unroll
     for (int i = (int)threadIdx.x; i < TM * TN / 4; i += CF::NT) {

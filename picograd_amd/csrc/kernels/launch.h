@@ -138,7 +138,8 @@ int pgk_copy_to16(int dtype, int src_dtype, const void *src, size_t rows, size_t
  */
 size_t pgk_gemm16_workspace(int ta, int tb, size_t m, size_t n, size_t k, size_t batch);
 
-/* Optional epilogue of pgk_gemm16 (one matrix, beta = 0): with
+/* Optional epilogue of pgk_gemm16 (one matrix, or with c16 and skip_out alone
+ * a batch; beta = 0): with
  * v = sum_p A(i, p) B(p, j) + bias[j], it writes C[i, j] = act(v),
  * z[i, j] = v and c16[i, j] = RNE-16-bit(act(v)) (z, c16 at C's leading
  * dim; each NULL to skip).  act codes follow the reference's
@@ -267,6 +268,8 @@ int pgk_act_bwd16n(int act, const uint16_t *dn, const uint16_t *wn, int kw, int 
 
 /* Gated feed-forward layer (gated.hip), z = x W + bias = [g | u] [m, 2 f] f32:
  * h = act(g) u [m, f], acts PGK_ACT_* and the two below.
+ * _pad: 16-bit x [m, k] and W [k, 2 f] as [m, k8] and [k8, 2, f8], zeros between
+ * (x16 or w16 NULL: not wanted).
  * _forward: from x [m, k8] (ldx) and W [k8, 2, f8] 16-bit of dtype, k8 and f8
  * multiples of 8 (zeros past the layer's own sizes), one launch: h in f32 (h32)
  * and / or 16 bits (h16, RNE), and z unless NULL.
@@ -276,6 +279,8 @@ int pgk_act_bwd16n(int act, const uint16_t *dn, const uint16_t *wn, int kw, int 
  * sums db [2 f] (beta ? += : =) in a fixed order (ws: pgk_gated_bwd_workspace
  * bytes). */
 enum { PGK_ACT_SILU = 3, PGK_ACT_SIGMOID = 4 };
+int pgk_gated_pad(const uint16_t *x, size_t m, size_t k, uint16_t *x16, const uint16_t *w, size_t f, uint16_t *w16,
+                  pgk_stream s);
 int pgk_gated_forward(int dtype, int act, size_t m, size_t f, size_t k8, const uint16_t *x, size_t ldx, const uint16_t *w,
                       size_t f8, const float *bias, float *z, float *h32, uint16_t *h16, pgk_stream s);
 size_t pgk_gated_bwd_workspace(size_t m, size_t f);
