@@ -16,8 +16,8 @@ namespace {
 // ---------------------------------------------------------------- operands
 
 // Two matrices of 16-bit values with their rows padded by zeros to whole 16-byte
-// pieces, in one launch: eight values a thread, read one by one (the rows'
-// own alignment is any).
+// pieces, in one launch: eight values a thread, a whole piece as one load at
+// whatever address it has, the last piece of a row one by one.
 struct pad_job {
     const uint16_t *src;
     uint16_t *dst;
@@ -30,12 +30,17 @@ __global__ void __launch_bounds__(256) k_gated_pad(pad_job a, pad_job b, size_t 
         const pad_job &j = second ? b : a;
         const size_t k = second ? i - na : i, r = k / j.cols8, c = (k - r * j.cols8) * 8;
         const uint16_t *p = j.src + r * j.cols + c;
-        uint16_t v[8];
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (r < j.rows && c + 8 <= j.cols) {
+            __builtin_memcpy(&q, p, sizeof(q));
+        } else if (r < j.rows) {
+            uint16_t v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = r < j.rows && c + e < j.cols ? p[e] : (uint16_t)0;
-        ((uint4 *)j.dst)[k] = make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16,
-                                         v[6] | (uint32_t)v[7] << 16);
+            for (int e = 0; e < 8; ++e)
+                v[e] = c + e < j.cols ? p[e] : (uint16_t)0;
+            __builtin_memcpy(&q, v, sizeof(q));
+        }
+        ((uint4 *)j.dst)[k] = q;
     }
 }
 
@@ -59,9 +64,14 @@ __global__ void __launch_bounds__(CF::NT, CF::KG == 4 ? 2 : 1) k_gated_ks(gemm_k
 }
 
 // Up to 16 rows: a block owns 16 outputs, whose 32 columns of W it streams past
-// once, its eight waves splitting the reduction, each with a ring of three
-// 64-deep chunks of its own and no block barrier until the waves' partial tiles
-// (16 x 16, one of g and one of u) are added through LDS in wave order.
+// once, its four waves splitting the reduction, each with a ring of two 64-deep
+// chunks of its own and no block barrier until the waves' partial tiles (16 x 16,
+// one of g and one of u) are added through LDS in wave order.  Bound by W's
+// stream; the block being small, the chip fills at few outputs.  One row, k x f,
+// this kernel against the tiles below: 1024 x 1024 4.5 : 6.1 us, 1024 x 4096
+// 7.2 : 8.4, 4096 x 4096 18.7 : 20.9 (3.6 TB/s of W); 4096 x 8192, whose
+// blocks come in two rounds, 50.4 : 35.5, so it is taken up to
+// 256 blocks.  Eight waves and three chunks: 8.0, 19.2 and 52.3 us.
 typedef float f32x4m __attribute__((ext_vector_type(4)));
 template <bool F16>
 __device__ __forceinline__ f32x4m mfma16(const uint4 &a, const uint4 &b, const f32x4m &c)
@@ -73,11 +83,12 @@ __device__ __forceinline__ f32x4m mfma16(const uint4 &a, const uint4 &b, const f
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);
 }
-constexpr int kFewWaves = 8, kFewStages = 3, kFewK = 64;
+constexpr int kFewWaves = 4, kFewStages = 2, kFewK = 64;
+constexpr int kFewBlocks = 256;
 constexpr int kFewA = 16 * kFewK / 8, kFewB = kFewK * 32 / 8; // uint4 of one A and one B stage
 
 template <bool F16>
-__global__ void __launch_bounds__(kFewWaves * 64, 1) k_gated_few(gemm_kargs g)
+__global__ void __launch_bounds__(kFewWaves * 64, 2) k_gated_few(gemm_kargs g)
 {
     __shared__ uint4 smem[kFewWaves * kFewStages * (kFewA + kFewB)];
     const int lane = (int)threadIdx.x & 63;
@@ -197,7 +208,7 @@ int launch_split(gemm_kargs g, hipStream_t s)
 template <bool F16>
 int launch_forward(int tile, const gemm_kargs &g, hipStream_t s)
 {
-    if (g.M <= 16) {
+    if (g.M <= 16 && (g.N + 15) / 16 <= kFewBlocks) {
         hipLaunchKernelGGL(k_gated_few<F16>, dim3((unsigned)((g.N + 15) / 16)), dim3(kFewWaves * 64), 0, s, g);
         return (int)hipGetLastError();
     }
