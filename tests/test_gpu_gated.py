@@ -108,6 +108,32 @@ def test_forward_and_backward(bench, dtype, m, k, f):
         check(bench.read(db), ref["db"], F32, "db")
 
 
+# Large enough for every tile of the forward (few outputs of one row beside many;
+# 128 x 128, 128 x 256 and 256 x 256 tiles at whole and odd widths), and for
+# several strips of rows in the backward.
+LARGE = [(1, 40, 4100), (3, 64, 5000), (16, 37, 4501), (300, 80, 1500), (512, 104, 4096), (500, 72, 4001), (1024, 64, 2048),
+         (1023, 50, 2049), (1024, 72, 8192), (1001, 33, 8001), (2100, 48, 130)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("m,k,f", LARGE)
+def test_every_tile(bench, dtype, m, k, f):
+    L, act = bench.L, sorted(ACTS)[(m + f) % 5]
+    x, w, b, dh = data(m, k, f, dtype, bias=f % 3 != 0, seed=7)
+    ref = model(x, w, b, dh, act, dtype)
+    tx, tw, tb, th = bench.tensor(x, dtype), bench.tensor(w, dtype), None if b is None else bench.tensor(b), bench.tensor(dh, dtype)
+    h, z = bench.unset((m, f), dtype), bench.unset((m, 2 * f))
+    bench.ok(L.pg_amd_gated(tx, tw, tb, ACTS[act], h, z))
+    check(bench.read(h), ref["h"], dtype, "h")
+    check(bench.read(z), ref["z"], F32, "z")
+    for gd in (dtype, F32):
+        dx, dw, db = bench.unset((m, k), gd), bench.unset((k, 2 * f), gd), bench.unset((2 * f,))
+        bench.ok(L.pg_amd_gated_backward(tx, tw, z, th, ACTS[act], dx, dw, db))
+        check(bench.read(dx), ref["dx"], gd, "dx")
+        check(bench.read(dw), ref["dw"], gd, "dw")
+        check(bench.read(db), ref["db"], F32, "db")
+
+
 @pytest.mark.parametrize("act", sorted(ACTS))
 @pytest.mark.parametrize("m,f", [(3, 24), (40, 24), (200, 130)])
 def test_every_activation(bench, act, m, f):

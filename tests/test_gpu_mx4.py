@@ -126,6 +126,26 @@ def test_product(bench, dtype, out, m, k, n):
     within(product(bench, x, w, dtype, out), want, bound, "y")
 
 
+# Sizes of every tile: 64 x 32 and 64 x 64 split eight ways, 64 x 64 split four
+# ways, 128 x 128 in stages (one, two and several steps of 256 along the reduction).
+TILES = [(640, 300, 640), (900, 260, 901), (1100, 900, 1210), (1100, 40, 1185), (1500, 100, 1600), (1601, 300, 1503),
+         (1500, 700, 1601), (2000, 1025, 1300), (5000, 31, 600)]
+
+
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F32, F16)], ids=lambda d: NAMES[d])
+@pytest.mark.parametrize("m,k,n", TILES)
+def test_product_of_many_tiles(bench, dtype, out, m, k, n):
+    g = np.random.default_rng(m + k + n)
+    x = rounded(g.standard_normal((m, k)) * np.exp(g.standard_normal(k)), dtype)
+    w = rounded(g.uniform(-1, 1, (k, n)) * k ** -0.5, F32)
+    qx, qw = quantized(x), quantized(w.T).T
+    want, size = qx @ qw, np.abs(qx) @ np.abs(qw)
+    bound = (k + 2) * 2.0 ** -24 * size + TINY[F32]
+    if out != F32:
+        bound = bound + UNIT[out] * (np.abs(want) + bound) + TINY[out]
+    within(product(bench, x, w, dtype, out), want, bound, "y")
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_a_block_that_is_nan_spoils_its_row_or_column_only(bench, m):
     g = np.random.default_rng(1)
