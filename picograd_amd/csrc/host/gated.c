@@ -55,26 +55,48 @@ static bool product(const char *what, int dt, int t, size_t m, size_t n, size_t 
     return pgm_gemm16x(dt, t, t, m, n, k, a, lda, 0, aext, b, ldb, 0, bext, NULL, ldc, 0, 1, 0, &epi, what);
 }
 
-/* dx = dz W^T and dW = x^T dz from dz16 [M, 2, F8]; M, K, F > 0 */
+/* both grads in one launch; false: not for these sizes (nothing launched) or an
+ * error, which the products alone then meet again */
+static bool both_grads(int dt, const pgk_gemm_desc *dd, uint16_t *d16, const pgk_gemm_desc *dw, uint16_t *w16)
+{
+    const size_t wb = pgk_gemm16_grads_workspace(dd, dw);
+    void *ws = wb ? pgd_malloc(wb) : NULL;
+    if (wb && !ws)
+        return false;
+    int tk = pgd_tbegin(PGD_T_GEMM16);
+    const int rc = pgk_gemm16_grads(dt, dd, d16, dw, w16, ws, pgd_stream());
+    pgd_tend(tk);
+    if (ws)
+        pgd_free(ws, wb);
+    return rc == 0;
+}
+
+/* dx = dz W^T and dW = x^T dz from dz16 [M, 2, F8]; M, K, F > 0.  An odd F's dW
+ * is a batch of two halves, F apart in its rows. */
 static bool grads(const char *what, int dt, const gated_dims *d, const uint16_t *x16, const uint16_t *w16,
                   const uint16_t *dz16, const gated_out *dx, const gated_out *dw)
 {
-    const size_t N = 2 * d->F, N8 = 2 * d->F8;
-    if (dx->p && dw->p && dx->p != dw->p && !dx->is16 && !dw->is16 && N == N8) {
-        const pgk_gemm_desc dd = {d->M, d->K, N8, dz16, N8, 0, d->M, w16, N8, 0, d->K, dx->p, d->K, 0, 1, dx->beta};
-        const pgk_gemm_desc dg = {d->K, N, d->M, x16, d->K8, 0, d->K8, dz16, N8, 0, N8, dw->p, N, 0, 1, dw->beta};
-        if (pgm_pair_ks(dt, &dd, &dg, what) || pgm_pair_full(dt, &dd, &dg, what))
+    const size_t N = 2 * d->F, N8 = 2 * d->F8, halves = N == N8 ? 1 : 2, n = N / halves, n8 = N8 / halves;
+    if (dx->p && dw->p && dx->p != dw->p) {
+        const pgk_gemm_desc dd = {d->M, d->K, N8, dz16, N8, 0, d->M, w16, N8, 0, d->K, dx->is16 ? NULL : dx->p, d->K, 0, 1,
+                                  dx->beta};
+        const pgk_gemm_desc dg = {d->K, n, d->M, x16, d->K8, 0, d->K8, dz16, N8, n8, n8, dw->is16 ? NULL : dw->p, N, n, halves,
+                                  dw->beta};
+        const bool f32 = !dx->is16 && !dw->is16 && halves == 1;
+        if ((f32 && pgm_pair_ks(dt, &dd, &dg, what)) ||
+            both_grads(dt, &dd, dx->is16 ? dx->p : NULL, &dg, dw->is16 ? dw->p : NULL) ||
+            (f32 && pgm_pair_full(dt, &dd, &dg, what)))
             return true;
     }
     bool ok = true;
     if (dx->p)
         ok = product(what, dt, 0, d->M, d->K, N8, dz16, N8, d->M, w16, N8, d->K, dx, d->K);
-    if (dw->p && N == N8) {
+    if (dw->p && halves == 1) {
         ok = ok && product(what, dt, 1, d->K, N, d->M, x16, d->K8, d->K8, dz16, N8, N8, dw, N);
-    } else if (ok && dw->p) { /* the halves of dW as a batch of two, F apart in its rows */
+    } else if (ok && dw->p) {
         const pgk_epi epi = {.act = PGK_ACT_NONE, .c16 = dw->p, .dtype16 = dt, .skip_out = 1};
-        ok = pgm_gemm16x(dt, 1, 1, d->K, d->F, d->M, x16, d->K8, 0, d->K8, dz16, N8, d->F8, d->F8,
-                         dw->is16 ? NULL : dw->p, N, d->F, 2, dw->is16 ? 0 : dw->beta, dw->is16 ? &epi : NULL, what);
+        ok = pgm_gemm16x(dt, 1, 1, d->K, n, d->M, x16, d->K8, 0, d->K8, dz16, N8, n8, n8, dw->is16 ? NULL : dw->p, N, n, 2,
+                         dw->is16 ? 0 : dw->beta, dw->is16 ? &epi : NULL, what);
     }
     return ok;
 }

@@ -213,7 +213,9 @@ int launch_forward(int tile, const gemm_kargs &g, hipStream_t s)
         return (int)hipGetLastError();
     }
     switch (tile) {
-    case 1: return launch_tiles<gcfg<128, 128, 2, 2, false, true, F16, true, 64, 2, true>>(g, s);
+    // four stages of 32 rather than the plain product's two of 64: 512 x 1024 x
+    // 4096 18.6 : 19.8 us, 200 x 4096 x 4096 35.9 : 43.4
+    case 1: return launch_tiles<gcfg<128, 128, 2, 2, false, true, F16, true, 32, 4, true>>(g, s);
     case 2: return launch_tiles<gcfg<256, 256, 2, 4, false, true, F16, true, 32, 4, true>>(g, s);
     case 3: return launch_tiles<gcfg<128, 256, 2, 4, false, true, F16, true, 32, 4, true>>(g, s);
     case 5: return launch_split<kscfg<32, 32, 8, 64, 2, false, true, F16, true>>(g, s);
@@ -225,59 +227,72 @@ int launch_forward(int tile, const gemm_kargs &g, hipStream_t s)
 
 // ---------------------------------------------------------------- backward
 
-// The gate's backward over a strip of 64 V columns of f and a run of rows per block:
-// its four waves take every fourth row each, V neighbouring columns a lane (4
-// where every row keeps that alignment, else 1), and keep the strip's column
-// sums, joined through LDS in wave order into the block's row of part.  Bound by
-// the stream of z and dh in and dz out (4096 x 8192: 470 MB).
-template <int V, class T>
-__device__ __forceinline__ void load_as(const T *p, float *v)
+// The gate's backward over a strip of 256 columns of f and a run of rows per
+// block: its four waves take every fourth row each, four neighbouring columns a
+// lane, and keep the strip's column sums, joined through LDS in wave order into
+// the block's row of part.  Bound by the stream of z and dh in and dz out (4096 x
+// 8192 in bf16: 470 MB in 91 us, 5.1 TB/s).  A piece of four is one load at
+// whatever address an odd f gives it (1023 x 2049: one value a lane took 11 us).
+constexpr int kBwdV = 4;
+template <bool WHOLE, class T>
+__device__ __forceinline__ void load_piece(const T *p, size_t left, float *v)
 {
-    typedef T tv __attribute__((ext_vector_type(V)));
-    const tv q = __builtin_nontemporal_load((const tv *)p); // read once
+    typedef T tv __attribute__((ext_vector_type(kBwdV), aligned(sizeof(T))));
+    if constexpr (WHOLE) {
+        const tv q = __builtin_nontemporal_load((const tv *)p); // read once
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        v[i] = (float)q[i];
+        for (int i = 0; i < kBwdV; ++i)
+            v[i] = (float)q[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kBwdV; ++i)
+            v[i] = i < left ? (float)p[i] : 0.0f;
+    }
 }
 
-template <int V, int ACT, class D>
+template <int ACT, class D>
 __global__ void __launch_bounds__(256)
     k_gated_bwd(const D *__restrict__ dh, const float *__restrict__ z, size_t m, size_t f, size_t f8,
                 uint16_t *__restrict__ dz, int dtype, float *__restrict__ part, int rows)
 {
+    constexpr int V = kBwdV;
     __shared__ float sums[4][2][64 * V];
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
     const size_t c = ((size_t)blockIdx.x * 64 + lane) * V;
     const size_t r0 = (size_t)blockIdx.y * rows, r1 = r0 + rows < m ? r0 + rows : m;
     float sg[V] = {}, su[V] = {};
-    if (c < f8)
-#pragma unroll 2
+    // the rows of a lane whose piece lies within f, or of f's last columns (past
+    // them zeros, whose grads are zeros)
+    auto run = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        const size_t left = f - c;
+#pragma unroll WHOLE ? 4 : 1
         for (size_t r = r0 + wave; r < r1; r += 4) {
-            float dg[V] = {}, du[V] = {};
-            if (c < f) {
-                float d[V], g[V], u[V];
-                load_as<V>(dh + r * f + c, d);
-                load_as<V>(z + r * 2 * f + c, g);
-                load_as<V>(z + r * 2 * f + f + c, u);
+            float d[V], g[V], u[V], dg[V], du[V];
+            load_piece<WHOLE>(dh + r * f + c, left, d);
+            load_piece<WHOLE>(z + r * 2 * f + c, left, g);
+            load_piece<WHOLE>(z + r * 2 * f + f + c, left, u);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float da;
-                    const float a = gate_fd<ACT>(g[i], da);
-                    dg[i] = d[i] * u[i] * da;
-                    du[i] = d[i] * a;
-                    sg[i] += dg[i];
-                    su[i] += du[i];
-                }
+            for (int i = 0; i < V; ++i) {
+                float da;
+                const float a = gate_fd<ACT>(g[i], da);
+                dg[i] = d[i] * u[i] * da;
+                du[i] = d[i] * a;
+                sg[i] += dg[i];
+                su[i] += du[i];
             }
             uint16_t *p = dz + r * 2 * f8 + c;
-            if constexpr (V == 4) {
-                *(uint2 *)p = make_uint2(to16x2(dtype, dg[0], dg[1]), to16x2(dtype, dg[2], dg[3]));
-                *(uint2 *)(p + f8) = make_uint2(to16x2(dtype, du[0], du[1]), to16x2(dtype, du[2], du[3]));
-            } else {
-                p[0] = to16(dtype, dg[0]);
-                p[f8] = to16(dtype, du[0]);
-            }
+            *(uint2 *)p = make_uint2(to16x2(dtype, dg[0], dg[1]), to16x2(dtype, dg[2], dg[3]));
+            *(uint2 *)(p + f8) = make_uint2(to16x2(dtype, du[0], du[1]), to16x2(dtype, du[2], du[3]));
         }
+    };
+    if (c + V <= f)
+        run(std::true_type{});
+    else if (c < f)
+        run(std::false_type{});
+    else if (c < f8) // the zeros past an odd f
+        for (size_t r = r0 + wave; r < r1; r += 4)
+            *(uint2 *)(dz + r * 2 * f8 + c) = *(uint2 *)(dz + r * 2 * f8 + f8 + c) = make_uint2(0, 0);
     if (!part)
         return;
 #pragma unroll
@@ -298,19 +313,17 @@ __global__ void __launch_bounds__(256)
 // The blocks of rows: enough to fill the chip, at most 64 where they leave
 // partial column sums, which one more launch adds one after the other.
 struct bwd_plan {
-    int v;
     unsigned gx, gy;
     int rows;
 };
-bwd_plan plan_bwd(size_t m, size_t f, bool v4, bool sums)
+bwd_plan plan_bwd(size_t m, size_t f, bool sums)
 {
-    const int v = v4 ? 4 : 1;
-    const size_t gx = (f + 64 * v - 1) / (64 * v);
+    const size_t gx = (f + 64 * kBwdV - 1) / (64 * kBwdV);
     size_t gy = (sums ? 2048 : 4096) / gx;
     gy = gy < 1 ? 1 : sums && gy > 64 ? 64 : gy > 16384 ? 16384 : gy;
     size_t rows = (m + gy - 1) / gy;
     rows = (rows + 3) / 4 * 4;
-    return {v, (unsigned)gx, (unsigned)((m + rows - 1) / rows), (int)rows};
+    return {(unsigned)gx, (unsigned)((m + rows - 1) / rows), (int)rows};
 }
 
 struct bwd_args {
@@ -321,27 +334,17 @@ struct bwd_args {
     int dtype;
     float *part;
 };
-template <int V, int ACT, class D>
+template <int ACT, class D>
 void launch_bwd(const bwd_args &a, const bwd_plan &p, hipStream_t s)
 {
-    hipLaunchKernelGGL((k_gated_bwd<V, ACT, D>), dim3(p.gx, p.gy), dim3(256), 0, s, (const D *)a.dh, a.z, a.m, a.f,
+    hipLaunchKernelGGL((k_gated_bwd<ACT, D>), dim3(p.gx, p.gy), dim3(256), 0, s, (const D *)a.dh, a.z, a.m, a.f,
                        (a.f + 7) & ~(size_t)7, a.dz, a.dtype, a.part, p.rows);
 }
 template <int ACT>
 void launch_bwd(const bwd_args &a, int dh_dtype, const bwd_plan &p, hipStream_t s)
 {
-    if (p.v == 4)
-        dh_dtype == 0 ? launch_bwd<4, ACT, float>(a, p, s)
-                      : dh_dtype == 1 ? launch_bwd<4, ACT, _Float16>(a, p, s) : launch_bwd<4, ACT, __bf16>(a, p, s);
-    else
-        dh_dtype == 0 ? launch_bwd<1, ACT, float>(a, p, s)
-                      : dh_dtype == 1 ? launch_bwd<1, ACT, _Float16>(a, p, s) : launch_bwd<1, ACT, __bf16>(a, p, s);
-}
-
-// whether rows of dh and z keep pieces of four values aligned
-bool rows_of_four(const void *dh, int dh_dtype, const float *z, size_t f)
-{
-    return f % 4 == 0 && ((uintptr_t)z & 15) == 0 && ((uintptr_t)dh & (dh_dtype == 0 ? 15 : 7)) == 0;
+    dh_dtype == 0 ? launch_bwd<ACT, float>(a, p, s)
+                  : dh_dtype == 1 ? launch_bwd<ACT, _Float16>(a, p, s) : launch_bwd<ACT, __bf16>(a, p, s);
 }
 
 } // namespace
@@ -384,8 +387,7 @@ extern "C" size_t pgk_gated_bwd_workspace(size_t m, size_t f)
 {
     if (!m || !f)
         return 0;
-    const size_t a = plan_bwd(m, f, true, true).gy, b = plan_bwd(m, f, false, true).gy;
-    return (a > b ? a : b) * 2 * f * sizeof(float);
+    return plan_bwd(m, f, true).gy * 2 * f * sizeof(float);
 }
 
 extern "C" int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float *z, size_t m, size_t f, uint16_t *dz16,
@@ -395,7 +397,7 @@ extern "C" int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float 
         return 0;
     if (m > 0x7fffffff || f > 0x1fffffff || (db && !ws) || ((uintptr_t)dz16 & 15) || act < 0 || act > PGK_ACT_SIGMOID)
         return (int)hipErrorInvalidValue;
-    const bwd_plan p = plan_bwd(m, f, rows_of_four(dh, dh_dtype, z, f), db != nullptr);
+    const bwd_plan p = plan_bwd(m, f, db != nullptr);
     const bwd_args a = {dh, z, m, f, dz16, dtype, db ? (float *)ws : nullptr};
     hipStream_t st = (hipStream_t)s;
     switch (act) {

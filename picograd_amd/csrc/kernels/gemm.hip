@@ -681,6 +681,37 @@ int launch_pair_dw(const gemm_args &gd, const gemm_args &gw, hipStream_t s)
     return (int)hipGetLastError();
 }
 
+// A dgrad in `splits` slices of its reduction and a wgrad, each finished by an
+// epilogue (or, in slices, left as dense f32 partials), in one launch on 128 x
+// 256 tiles.  A slice's blocks, and neighbouring tiles of the wgrad, go to one
+// XCD: with every slice on every XCD each L2 would read the whole of both
+// operands.
+template <class C1, class C2>
+__global__ void __launch_bounds__(C1::NT, 1) k_gemm16_grads(gemm_kargs g1, gemm_kargs g2, int nb1, int n1, int n2)
+{
+    static_assert(C1::NT == C2::NT, "one block size");
+    __shared__ uint4 smem[C1::LDS_U4 > C2::LDS_U4 ? C1::LDS_U4 : C2::LDS_U4];
+    const int b = (int)blockIdx.x;
+    if (b < n1) {
+        const int t = xcd_tile(b, n1);
+        gemm16_block<C1>(g1, t % nb1, nb1, false, t / nb1, (LDS uint4 *)smem);
+    } else {
+        const int t = xcd_tile(b - n1, n2), nb2 = g2.tiles_m * g2.tiles_n;
+        gemm16_block<C2>(g2, t % nb2, nb2, false, t / nb2, (LDS uint4 *)smem);
+    }
+}
+
+template <bool F16>
+int launch_grads(const gemm_args &gd, const pgk_epi &ed, const gemm_args &gw, const pgk_epi &ew, hipStream_t s)
+{
+    using CD = layout_cfg<false, false, F16, true, 3>;
+    using CW = layout_cfg<true, true, F16, true, 3>;
+    const gemm_kargs kd = make_kargs<CD>(gd, ed), kw = make_kargs<CW>(gw, ew);
+    const int nb1 = kd.tiles_m * kd.tiles_n, n1 = nb1 * (int)gd.batch, n2 = kw.tiles_m * kw.tiles_n * (int)gw.batch;
+    hipLaunchKernelGGL((k_gemm16_grads<CD, CW>), dim3((unsigned)(n1 + n2)), dim3(CD::NT), 0, s, kd, kw, nb1, n1, n2);
+    return (int)hipGetLastError();
+}
+
 // both problems on tile `tile`
 template <bool F16>
 int launch_pair_tiles(int tile, const gemm_args &gd, const gemm_args &gw, hipStream_t s)
@@ -1242,6 +1273,100 @@ extern "C" int pgk_gemm16_pair_dw(int dtype, const pgk_gemm_desc *d, const pgk_g
     const splitk_desc s1 = pd.sp > 1 ? splitk_of(part_d, pd.sp, d->m, d->n, d->c, d->ldc, d->beta) : splitk_desc{};
     const splitk_desc s2 = pw.sp > 1 ? splitk_of(part_w, pw.sp, w->m, w->n, w->c, w->ldc, w->beta) : splitk_desc{};
     hipLaunchKernelGGL(k_splitk_sum, splitk_grid(s1, s2), dim3(256), 0, st, s1, s2);
+    return (int)hipGetLastError();
+}
+
+// The slices of the dgrad in k_gemm16_grads, 0 when the two products are better
+// alone.  Depths in the reduction, a block costing its own and some 800 of
+// start and epilogue; the dgrad's blocks run first, the wgrad's fill the CUs
+// that they leave; a launch takes some 8 us per 1024 of its longest CU and 10
+// more per 1024 of the mean, a sum 5 us and its bytes at 5 TB/s.  Together
+// against alone, M x K x F (dgrad of depth 2F, wgrad of depth M), us:
+//   512 x 1024 x 4096   36 : 46      1024 x 768 x 2048   28 : 40
+//   1023 x 777 x 2049   37 : 51      2048 x 1024 x 2048  46 : 66
+//   256 x 2048 x 4096   44 : 51      512 x 4096 x 1024   34 : 43
+//   2048 x 2048 x 2048  75 : 92      4096 x 1024 x 4096 157 : 178
+//   20 x 1024 x 8192    35 : 50      1000 x 1000 x 3001  46 : 66
+// and with more work than the last the larger tiles of the products alone
+// gain on it (2048 x 2048 x 4096 172 : 168); with few tiles of either, or where
+// both are small enough for the split-over-waves tiles, it loses (100 x 512 x
+// 2048 23 : 17, 512 x 512 x 2048 24 : 20, 8192 x 256 x 512 83 : 37).
+static int grads_plan(const pgk_gemm_desc *d, const pgk_gemm_desc *w)
+{
+    const size_t nd = ((d->m + 127) / 128) * ((d->n + 255) / 256);
+    const size_t nw = ((w->m + 127) / 128) * ((w->n + 255) / 256) * w->batch;
+    if (d->batch != 1 || nd < 4 || nw < 64 || nd * d->k + nw * w->k > (size_t)8192 * kCUs ||
+        (ks_tile({{d->m, d->n, 1, d->k}}, false) && ks_tile({{w->m, w->n, w->batch, w->k}}, true)))
+        return 0;
+    int best = 0;
+    double best_t = 1e300;
+    for (int sp : {1, 2, 3, 4, 6, 8}) {
+        const size_t ks = ((d->k + sp - 1) / sp + BK - 1) / BK * BK, n1 = nd * sp;
+        if (ks * (size_t)(sp - 1) >= d->k)
+            break; // the last slice would be empty
+        const double a = (double)ks + 800, b = (double)w->k + 800;
+        // CUs with one dgrad block more than the rest, and the time at which
+        // all the wgrad's blocks have had their place
+        const double r = (double)(n1 / kCUs), more = (double)(n1 % kCUs), la = (r + (more > 0 ? 1 : 0)) * a, lb = r * a;
+        double ca = la, cb = lb + ceil((la - lb) / b) * b, t = la;
+        while (more * floor((t - la) / b) + (kCUs - more) * floor((t - lb) / b) < (double)nw) {
+            (ca <= cb ? ca : cb) += b;
+            t = ca < cb ? ca : cb;
+        }
+        t = (t * 8e-6 + ((double)n1 * a + (double)nw * b) / kCUs * 10e-6) / 1024;
+        if (sp > 1)
+            t += 5e-6 + 2.0 * sp * (double)d->m * (double)d->n * 4.0 / 5.0e12;
+        if (t < best_t) {
+            best_t = t;
+            best = sp;
+        }
+    }
+    return nd * best < 32 ? 0 : best;
+}
+
+extern "C" size_t pgk_gemm16_grads_workspace(const pgk_gemm_desc *d, const pgk_gemm_desc *w)
+{
+    const int sp = grads_plan(d, w);
+    return sp > 1 ? (size_t)sp * d->m * d->n * sizeof(float) : 0;
+}
+
+extern "C" int pgk_gemm16_grads(int dtype, const pgk_gemm_desc *d, uint16_t *d16, const pgk_gemm_desc *w, uint16_t *w16,
+                                void *ws, pgk_stream s)
+{
+    if (d->beta || w->beta || !d->m || !d->n || !d->k || !w->m || !w->n || !w->k || !w->batch || d->k % 8)
+        return PGK_GEMM_NOT_PAIRED;
+    const int sp = grads_plan(d, w);
+    if (!sp)
+        return PGK_GEMM_NOT_PAIRED;
+    int bad = check_gemm_args(0, 0, d->m, d->n, d->k, d->a, d->lda, d->stride_a, d->a_extent, d->b, d->ldb,
+                              d->stride_b, d->b_extent, d->batch);
+    if (!bad)
+        bad = check_gemm_args(1, 1, w->m, w->n, w->k, w->a, w->lda, w->stride_a, w->a_extent, w->b, w->ldb,
+                              w->stride_b, w->b_extent, w->batch);
+    if (bad || (sp > 1 && !ws))
+        return bad ? bad : (int)hipErrorInvalidValue;
+    pgk_epi ed = {}, ew = {};
+    if (w16)
+        ew.c16 = w16, ew.dtype16 = dtype, ew.skip_out = 1;
+    if (d16)
+        ed.c16 = d16, ed.dtype16 = dtype, ed.skip_out = 1;
+    const gemm_args gw = {w->a, w->lda, w->stride_a, (int)w->a_extent, w->b, w->ldb, w->stride_b, (int)w->b_extent, w->c,
+                          w->ldc, w->stride_c, (int)w->m, (int)w->n, (int)w->k, 0, (unsigned)w->batch, 3};
+    gemm_args gd = {d->a, d->lda, 0, (int)d->a_extent, d->b, d->ldb, 0, (int)d->b_extent, d->c, d->ldc, 0, (int)d->m,
+                    (int)d->n, (int)d->k, 0, 1u, 3};
+    hipStream_t st = (hipStream_t)s;
+    float *const part = (float *)ws;
+    if (sp > 1) {
+        const size_t ks = ((d->k + sp - 1) / sp + BK - 1) / BK * BK;
+        gd.sa = gd.sb = ks, gd.c = part, gd.ldc = d->n, gd.sc = d->m * d->n, gd.k = (int)ks, gd.batch = (unsigned)sp;
+        gd.k_total = (int)d->k, gd.kz_step = (int)ks;
+    }
+    const pgk_epi e1 = sp > 1 ? pgk_epi{} : ed;
+    int rc = dtype == 1 ? launch_grads<true>(gd, e1, gw, ew, st) : launch_grads<false>(gd, e1, gw, ew, st);
+    if (rc || sp == 1)
+        return rc;
+    const splitk_desc sd = splitk_of(part, sp, d->m, d->n, d->c, d->ldc, 0, d16 ? &ed : nullptr);
+    hipLaunchKernelGGL(k_splitk_sum, splitk_grid(sd, sd), dim3(256), 0, st, sd, sd);
     return (int)hipGetLastError();
 }
 

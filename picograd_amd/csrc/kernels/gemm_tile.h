@@ -640,8 +640,9 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
         for (int q = 0; q < 4; ++q)
             bias4[q] = (epi.bias && gcol + q < N) ? epi.bias[gcol + q] : 0.0f;
         uint16_t *const c16 = epi.c16 ? epi.c16 + (size_t)z * sC : nullptr;
-        const bool v4 = (ldc & 3) == 0 && gcol + 3 < N && (((uintptr_t)Cb) & 15) == 0 &&
-                        (((uintptr_t)epi.z) & 15) == 0 && (((uintptr_t)c16) & 7) == 0;
+        const bool v4 = gcol + 3 < N; // at any alignment: rows of an odd width start anywhere
+        typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+        typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             __syncthreads(); // the k-loop's (or the previous pass') LDS reads are done
@@ -665,14 +666,14 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
                 const size_t off = (size_t)grow * ldc + gcol;
                 if (v4) {
                     if (!epi.skip_out)
-                        *reinterpret_cast<float4 *>(Cb + off) = make_float4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<f32x4u *>(Cb + off) = f32x4u{o[0], o[1], o[2], o[3]};
                     if (epi.z) { // read again only by the backward, much later
-                        const f32x4 zz = {zv[0], zv[1], zv[2], zv[3]};
-                        __builtin_nontemporal_store(zz, reinterpret_cast<f32x4 *>(epi.z + off));
+                        const f32x4u zz = {zv[0], zv[1], zv[2], zv[3]};
+                        __builtin_nontemporal_store(zz, reinterpret_cast<f32x4u *>(epi.z + off));
                     }
                     if (c16)
-                        *reinterpret_cast<uint2 *>(c16 + off) =
-                            make_uint2(to16x2(epi.dtype16, o[0], o[1]), to16x2(epi.dtype16, o[2], o[3]));
+                        *reinterpret_cast<u32x2u *>(c16 + off) =
+                            u32x2u{to16x2(epi.dtype16, o[0], o[1]), to16x2(epi.dtype16, o[2], o[3])};
                 } else {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {

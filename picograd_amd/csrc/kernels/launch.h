@@ -211,6 +211,14 @@ int pgk_gemm16_ks_pair(int dtype, const pgk_gemm_desc *d, const pgk_gemm_desc *w
 size_t pgk_gemm16_pair_dw_workspace(const pgk_gemm_desc *d, const pgk_gemm_desc *w, int cu_d, size_t *off_w);
 int pgk_gemm16_pair_dw(int dtype, const pgk_gemm_desc *d, const pgk_gemm_desc *w, int cu_d, void *ws,
                        pgk_stream s);
+/* The pair of middle sizes in one launch, d in slices of its reduction (one
+ * more launch adds them); d16, w16: the output rounded to the operands' type,
+ * or NULL for f32 at the desc's c.  Written, not added to (beta 0), w a batch of
+ * any size.  PGK_GEMM_NOT_PAIRED (nothing launched) where the products alone
+ * are faster.  ws: _workspace bytes. */
+size_t pgk_gemm16_grads_workspace(const pgk_gemm_desc *d, const pgk_gemm_desc *w);
+int pgk_gemm16_grads(int dtype, const pgk_gemm_desc *d, uint16_t *d16, const pgk_gemm_desc *w, uint16_t *w16,
+                     void *ws, pgk_stream s);
 
 /* MFMA rate probe: `blocks` x 512 threads, each wave 8 x iters bf16
  * 32x32x16 MFMAs, operands from registers (lds 0) or LDS (lds 1); sink

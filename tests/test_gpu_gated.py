@@ -134,6 +134,26 @@ def test_every_tile(bench, dtype, m, k, f):
         check(bench.read(db), ref["db"], F32, "db")
 
 
+# Sizes at which both products of the backward are one launch: in one to eight
+# slices of the dgrad's reduction, at whole and odd widths.
+BOTH = [(300, 1000, 1031), (257, 1030, 2048), (1000, 520, 2060), (1600, 2050, 600), (20, 1024, 2048), (129, 777, 1501),
+        (520, 512, 1000)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("m,k,f", BOTH)
+def test_both_grads(bench, dtype, m, k, f):
+    L = bench.L
+    x, w, _, dh = data(m, k, f, dtype, False, seed=9)
+    ref = model(x, w, None, dh, "silu", dtype)
+    tx, tw, th, z = bench.tensor(x, dtype), bench.tensor(w, dtype), bench.tensor(dh, dtype), bench.tensor(ref["z"][0])
+    for xd, wd in ((dtype, dtype), (F32, F32), (dtype, F32), (F32, dtype)):
+        dx, dw = bench.unset((m, k), xd), bench.unset((k, 2 * f), wd)
+        bench.ok(L.pg_amd_gated_backward(tx, tw, z, th, ACTS["silu"], dx, dw, None))
+        check(bench.read(dx), ref["dx"], xd, "dx")
+        check(bench.read(dw), ref["dw"], wd, "dw")
+
+
 @pytest.mark.parametrize("act", sorted(ACTS))
 @pytest.mark.parametrize("m,f", [(3, 24), (40, 24), (200, 130)])
 def test_every_activation(bench, act, m, f):
