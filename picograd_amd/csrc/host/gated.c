@@ -119,6 +119,35 @@ static uint16_t *make_dz(const char *what, int dt, const gated_dims *d, int act,
     return ok ? dz : NULL;
 }
 
+/* few rows (pgk_gated_few_grads_ok): all grads from f32 dz, x and W as they lie (x
+ * rows ldx apart, W's halves `half`) */
+static bool few_rows(const char *what, int dt, const gated_dims *d, int act, const pg_tensor *dh, const float *z, float *db,
+                     int db_beta, const uint16_t *x, size_t ldx, const uint16_t *w, size_t half, const gated_out *dx,
+                     const gated_out *dw)
+{
+    const size_t bytes = d->M * 2 * d->F * sizeof(float);
+    const size_t wb = dx->p ? pgk_gated_few_grads_workspace(d->M, d->K, d->F) : 0;
+    float *dz = pgd_malloc(bytes);
+    void *ws = wb ? pgd_malloc(wb) : NULL;
+    pgk_stream st = pgd_stream();
+    int tk = pgd_tbegin(PGD_T_GEMM16);
+    bool ok = dz && (ws || !wb) &&
+              pgd_check(pgk_gated_few_dz(act, dh->dev, (int)dh->dtype, z, d->M, d->F, dz, db, db_beta, st), what);
+    /* x and W in one storage: its grads one after the other */
+    const bool apart = dx->p && dx->p == dw->p;
+    for (int i = apart ? 0 : 1; ok && i < 2 && (dx->p || dw->p); i++)
+        ok = pgd_check(pgk_gated_few_grads(dt, dz, d->M, d->K, d->F, x, ldx, w, half, apart && i ? NULL : dx->p,
+                                           dx->is16 ? dt : 0, dx->beta, apart && !i ? NULL : dw->p, dw->is16 ? dt : 0,
+                                           dw->beta, ws, st),
+                       what);
+    pgd_tend(tk);
+    if (ws)
+        pgd_free(ws, wb);
+    if (dz)
+        pgd_free(dz, bytes);
+    return ok;
+}
+
 /* ---------------------------------------------------------------- on tensors */
 
 static bool aligned16(const void *p) { return !((uintptr_t)p & 15); }
@@ -273,14 +302,20 @@ bool pg_amd_gated_backward(const pg_tensor *x, const pg_tensor *w, const pg_tens
     bool ok = hc != NULL;
     if (ok) {
         const int dt = (int)x->dtype;
-        gated_ops o = {0};
-        uint16_t *dz = make_dz(what, dt, &d, act, hc, zc->dev, db ? db->dev : NULL, 0);
+        float *const b = db ? db->dev : NULL;
         const gated_out ox = {dx && d.K ? dx->dev : NULL, dx && dx->dtype != PG_DTYPE_F32, 0};
         const gated_out ow = {dw && d.K ? dw->dev : NULL, dw && dw->dtype != PG_DTYPE_F32, 0};
-        ok = done(what, dz && stage(&d, xc, wc, &o) && grads(what, dt, &d, o.x, o.w, dz, &ox, &ow));
-        unstage(&o);
-        if (dz)
-            pgd_free(dz, d.M * 2 * d.F8 * 2);
+        if (pgk_gated_few_grads_ok(d.M, d.K, d.F)) {
+            ok = few_rows(what, dt, &d, act, hc, zc->dev, b, 0, xc->dev, d.K, wc->dev, d.F, &ox, &ow);
+        } else {
+            gated_ops o = {0};
+            uint16_t *dz = make_dz(what, dt, &d, act, hc, zc->dev, b, 0);
+            ok = dz && stage(&d, xc, wc, &o) && grads(what, dt, &d, o.x, o.w, dz, &ox, &ow);
+            unstage(&o);
+            if (dz)
+                pgd_free(dz, d.M * 2 * d.F8 * 2);
+        }
+        done(what, ok);
     }
     for (int i = 0; i < 4; i++)
         pg_tensor_free(own[i]);
@@ -334,18 +369,24 @@ void pgo_gated_backward(pg_node *n)
     pgt_materialize(n->grad);
     int bb = 0, bx = 0, bw = 0;
     pg_tensor *gb = pb && pb->requires_grad ? pga_grad_for_write(pb, &bb) : NULL;
-    uint16_t *dz = make_dz(what, cx->dt, &d, cx->act, n->grad, cx->z->dev, gb ? gb->dev : NULL, bb);
-    if (!dz)
+    float *const db = gb ? gb->dev : NULL;
+    const bool few = pgk_gated_few_grads_ok(d.M, d.K, d.F);
+    uint16_t *dz = few ? NULL : make_dz(what, cx->dt, &d, cx->act, n->grad, cx->z->dev, db, bb);
+    if (!dz && !few)
         return;
     pg_tensor *gx = d.K && px->requires_grad ? pga_grad_for_write(px, &bx) : NULL;
     pg_tensor *gw = d.K && pw->requires_grad ? pga_grad_for_write(pw, &bw) : NULL;
     gated_ops o;
     if (operands(&d, cx->dt, px->value, pw->value, gw != NULL, gx != NULL, &o)) {
         const gated_out ox = {gx ? gx->dev : NULL, false, bx}, ow = {gw ? gw->dev : NULL, false, bw};
-        grads(what, cx->dt, &d, o.x, o.w, dz, &ox, &ow);
+        if (few)
+            few_rows(what, cx->dt, &d, cx->act, n->grad, cx->z->dev, db, bb, o.x, d.K8, o.w, d.F8, &ox, &ow);
+        else
+            grads(what, cx->dt, &d, o.x, o.w, dz, &ox, &ow);
     }
     unstage(&o);
-    pgd_free(dz, d.M * 2 * d.F8 * 2);
+    if (dz)
+        pgd_free(dz, d.M * 2 * d.F8 * 2);
 }
 
 pg_node *pg_amd_ag_gated16(pg_node *x, pg_node *w, pg_node *b, int act, pg_dtype dtype)

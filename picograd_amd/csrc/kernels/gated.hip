@@ -347,6 +347,218 @@ void launch_bwd(const bwd_args &a, int dh_dtype, const bwd_plan &p, hipStream_t 
                   : dh_dtype == 1 ? launch_bwd<ACT, _Float16>(a, p, s) : launch_bwd<ACT, __bf16>(a, p, s);
 }
 
+// Up to 16 rows: dz stays in f32 (rounded to 16 bits it is half of the error of so
+// few sums) and both grads are one launch over the matrices where they lie.
+// One thread per column of f: dz and, over the rows in turn, db.
+template <int ACT, class D>
+__global__ void __launch_bounds__(64)
+    k_gated_few_dz(const D *__restrict__ dh, const float *__restrict__ z, int m, size_t f, float *__restrict__ dz,
+                   float *__restrict__ db, int db_beta)
+{
+    const size_t c = (size_t)blockIdx.x * 64 + threadIdx.x;
+    if (c >= f)
+        return;
+    float sg = 0.0f, su = 0.0f;
+#pragma unroll 4
+    for (int r = 0; r < m; ++r) {
+        const float d = (float)dh[r * f + c], g = z[r * 2 * f + c], u = z[r * 2 * f + f + c];
+        float da;
+        const float a = gate_fd<ACT>(g, da), dg = d * u * da, du = d * a;
+        dz[r * 2 * f + c] = dg;
+        dz[r * 2 * f + f + c] = du;
+        sg += dg;
+        su += du;
+    }
+    if (db) {
+        db[c] = db_beta ? db[c] + sg : sg;
+        db[f + c] = db_beta ? db[f + c] + su : su;
+    }
+}
+
+// dx[:, k] = dz W[k, :] and dW[k, :] = x[:, k] dz for 16 rows k of W and a part of
+// its columns per block, by 16 x 16 x 4 products in f32 (W and x widened).  A wave
+// takes every eighth piece of 64 columns: W's piece once, in the order of dx's
+// product (lane l: row l % 16, columns 8 (l / 16) .. + 7), dz in that order and again
+// in dW's (rows 4 s + l / 16, columns 4 (l % 16) .. + 3) from the caches; the waves'
+// sums of dx are joined through LDS in wave order, the parts' in one more small
+// launch.  Bound by the latency of a piece's loads, then by dz from the caches
+// (loads a piece ahead cost more in registers than they hid, two and four row
+// groups a wave gained at 4096 x 8192 alone).
+constexpr int kFgWaves = 8;
+struct few_grads {
+    const uint16_t *x, *w;
+    size_t ldx, ldw, half; // of W: a row, and from g's columns to u's in it
+    const float *dz;
+    int m;
+    size_t k, f;
+    void *dx, *dw; // NULL: not wanted
+    int dx_dtype, dw_dtype, dx_beta, dw_beta;
+    float *part; // [parts, m, k] of dx where the columns are in more than one part
+};
+
+// the parts of the columns: a block for each CU, a piece a wave at least
+unsigned few_parts(size_t k, size_t f)
+{
+    const size_t rows = (k + 15) / 16, pieces = 2 * ((f + 63) / 64), most = pieces / kFgWaves;
+    const size_t want = 256 / rows, n = want < most ? want : most;
+    return n > 1 ? (unsigned)n : 1;
+}
+
+template <bool F16>
+__device__ __forceinline__ float widened(uint32_t bits)
+{
+    if constexpr (F16)
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+    else
+        return __builtin_bit_cast(float, bits << 16);
+}
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4h __attribute__((ext_vector_type(4), aligned(2)));
+
+// N values at p, those at or past `left` and of an absent row as zeros (p is then
+// another row's)
+template <int N>
+__device__ __forceinline__ void load_f32(const float *p, long left, bool row, float *v)
+{
+    if (left >= N) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const f32x4u q = *(const f32x4u *)(p + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[i + e] = row ? q[e] : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = row && i < left ? p[i] : 0.0f;
+    }
+}
+
+// v as the output type at p[i], or added to an f32 there
+__device__ __forceinline__ void put(void *p, int dtype, int beta, size_t i, float v)
+{
+    if (dtype == 0) {
+        float *const q = (float *)p + i;
+        *q = beta ? *q + v : v;
+    } else {
+        ((uint16_t *)p)[i] = to16(dtype, v);
+    }
+}
+
+template <bool F16>
+__global__ void __launch_bounds__(kFgWaves * 64, 2) k_gated_few_grads(few_grads a)
+{
+    __shared__ float sums[kFgWaves][16][17];
+    const int lane = (int)threadIdx.x & 63, q = lane & 15, grp = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const size_t k0 = (size_t)blockIdx.x * 16, kr = k0 + q < a.k ? k0 + q : a.k - 1;
+    const size_t per = (a.f + 63) / 64, pieces = 2 * per;
+    float xv[4]; // x[4 s + l / 16][k0 + l % 16]
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+        xv[s] = a.dw && 4 * s + grp < a.m ? widened<F16>(a.x[(4 * s + grp) * a.ldx + kr]) : 0.0f;
+    f32x4m acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (size_t p = blockIdx.y * kFgWaves + wave; p < pieces; p += (size_t)kFgWaves * gridDim.y) {
+        const size_t h = p >= per, c0 = (p - h * per) * 64;
+        const float *dz = a.dz + h * a.f + c0;
+        const long left = (long)(a.f - c0);
+        u32x4 w[2];    // W's row kr at columns 8 grp .. + 7 of both halves
+        float da[2][8]; // dz of row q there
+        float db[4][4]; // dz of rows 4 s + grp at columns 4 q .. + 3
+        if (a.dx) {
+            const uint16_t *src = a.w + kr * a.ldw + h * a.half + c0;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int c = 32 * t + 8 * grp;
+                if (left - c >= 8) {
+                    w[t] = __builtin_bit_cast(u32x4, *(const u32x4h *)(src + c));
+                } else {
+                    uint16_t e16[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        e16[e] = c + e < left ? src[c + e] : (uint16_t)0;
+                    __builtin_memcpy(&w[t], e16, 16);
+                }
+                load_f32<8>(dz + (size_t)(q < a.m ? q : 0) * 2 * a.f + c, left - c, q < a.m, da[t]);
+            }
+        }
+        if (a.dw)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (4 * s < a.m) {
+                    const int m = 4 * s + grp;
+                    load_f32<4>(dz + (size_t)(m < a.m ? m : 0) * 2 * a.f + 4 * q, left - 4 * q, m < a.m, db[s]);
+                }
+        if (a.dx)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(da[t][e], widened<F16>(w[t][e >> 1] >> 16 * (e & 1) & 0xffffu), acc,
+                                                               0, 0, 0);
+        if (!a.dw)
+            continue;
+        f32x4m o[4] = {};
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (4 * s < a.m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) // columns 4 q + e of rows k
+                    o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[s], db[s][e], o[e], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { // lane: rows 4 grp + r
+            const size_t row = k0 + 4 * grp + r, at = row * 2 * a.f + h * a.f + c0 + 4 * q;
+            if (row >= a.k)
+                continue;
+            const float v[4] = {o[0][r], o[1][r], o[2][r], o[3][r]};
+            if (left >= 4 * q + 4 && !a.dw_beta) {
+                if (a.dw_dtype == 0) {
+                    *(f32x4u *)((float *)a.dw + at) = f32x4u{v[0], v[1], v[2], v[3]};
+                } else {
+                    typedef uint32_t u32x2h __attribute__((ext_vector_type(2), aligned(2)));
+                    *(u32x2h *)((uint16_t *)a.dw + at) = u32x2h{to16x2(a.dw_dtype, v[0], v[1]), to16x2(a.dw_dtype, v[2], v[3])};
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (4 * q + e < left)
+                        put(a.dw, a.dw_dtype, a.dw_beta, at + e, v[e]);
+            }
+        }
+    }
+    if (!a.dx)
+        return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        sums[wave][4 * grp + r][q] = acc[r]; // row of x, row of W
+    __syncthreads();
+    const int row = (int)threadIdx.x >> 4, col = (int)threadIdx.x & 15;
+    if (row < a.m && k0 + col < a.k) {
+        float v = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kFgWaves; ++t)
+            v += sums[t][row][col];
+        const size_t at = (size_t)row * a.k + k0 + col;
+        if (a.part)
+            a.part[(size_t)blockIdx.y * a.m * a.k + at] = v;
+        else
+            put(a.dx, a.dx_dtype, a.dx_beta, at, v);
+    }
+}
+// the parts of dx, added in their order
+__global__ void __launch_bounds__(256) k_gated_few_join(few_grads a, unsigned parts)
+{
+    const size_t n = (size_t)a.m * a.k, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n)
+        return;
+    float v = 0.0f;
+    for (unsigned t = 0; t < parts; ++t)
+        v += a.part[t * n + i];
+    put(a.dx, a.dx_dtype, a.dx_beta, i, v);
+}
+
 } // namespace
 
 extern "C" int pgk_gated_pad(const uint16_t *x, size_t m, size_t k, uint16_t *x16, const uint16_t *w, size_t f, uint16_t *w16,
@@ -412,4 +624,68 @@ extern "C" int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float 
         return rc;
     const pgk_colsum_job job = {(const float *)ws, p.gy, 2 * f, db, db_beta};
     return pgk_colsum_run(&job, s);
+}
+
+// Against the 16-bit products, us for k x f in bf16 with 1, 4, 16 rows (those:
+// 17): 64 x 64 6.2, 6.2, 7.8 (10.5), 64 x 8192 16, 16, 19 (36), 1024 x 4096 20, 21,
+// 29 (29), 4096 x 8192 112, 115, 159 (112).
+extern "C" int pgk_gated_few_grads_ok(size_t m, size_t k, size_t f)
+{
+    return m <= 4 || (m <= 16 && (!k || f <= ((size_t)1 << 22) / k));
+}
+
+extern "C" size_t pgk_gated_few_grads_workspace(size_t m, size_t k, size_t f)
+{
+    const unsigned parts = k && f ? few_parts(k, f) : 1;
+    return parts > 1 ? parts * m * k * sizeof(float) : 0;
+}
+
+namespace {
+template <int ACT>
+void launch_few_dz(const void *dh, int dh_dtype, const float *z, int m, size_t f, float *dz, float *db, int db_beta, hipStream_t s)
+{
+    const dim3 grid((unsigned)((f + 63) / 64));
+    if (dh_dtype == 0)
+        hipLaunchKernelGGL((k_gated_few_dz<ACT, float>), grid, dim3(64), 0, s, (const float *)dh, z, m, f, dz, db, db_beta);
+    else if (dh_dtype == 1)
+        hipLaunchKernelGGL((k_gated_few_dz<ACT, _Float16>), grid, dim3(64), 0, s, (const _Float16 *)dh, z, m, f, dz, db, db_beta);
+    else
+        hipLaunchKernelGGL((k_gated_few_dz<ACT, __bf16>), grid, dim3(64), 0, s, (const __bf16 *)dh, z, m, f, dz, db, db_beta);
+}
+} // namespace
+
+extern "C" int pgk_gated_few_dz(int act, const void *dh, int dh_dtype, const float *z, size_t m, size_t f, float *dz, float *db,
+                                int db_beta, pgk_stream s)
+{
+    if (m > 16 || !f || f > 0x1fffffff)
+        return (int)hipErrorInvalidValue;
+    hipStream_t st = (hipStream_t)s;
+    switch (act) {
+    case PGK_ACT_RELU: launch_few_dz<PGK_ACT_RELU>(dh, dh_dtype, z, (int)m, f, dz, db, db_beta, st); break;
+    case PGK_ACT_GELU: launch_few_dz<PGK_ACT_GELU>(dh, dh_dtype, z, (int)m, f, dz, db, db_beta, st); break;
+    case PGK_ACT_SILU: launch_few_dz<PGK_ACT_SILU>(dh, dh_dtype, z, (int)m, f, dz, db, db_beta, st); break;
+    case PGK_ACT_SIGMOID: launch_few_dz<PGK_ACT_SIGMOID>(dh, dh_dtype, z, (int)m, f, dz, db, db_beta, st); break;
+    default: launch_few_dz<PGK_ACT_NONE>(dh, dh_dtype, z, (int)m, f, dz, db, db_beta, st); break;
+    }
+    return (int)hipGetLastError();
+}
+
+extern "C" int pgk_gated_few_grads(int dtype, const float *dz, size_t m, size_t k, size_t f, const uint16_t *x, size_t ldx,
+                                   const uint16_t *w, size_t half, void *dx, int dx_dtype, int dx_beta, void *dw, int dw_dtype,
+                                   int dw_beta, void *ws, pgk_stream s)
+{
+    if (!m || m > 16 || !k || k > 0x3fffffff || !f || f > 0x1fffffff || (dtype != 1 && dtype != 2) || (dx_beta && dx_dtype) ||
+        (dw_beta && dw_dtype) || half < f || (dw && ldx < k) ||
+        (dx && !ws && few_parts(k, f) > 1))
+        return (int)hipErrorInvalidValue;
+    const few_grads a = {x, w, ldx, 2 * half, half, dz, (int)m, k, f, dx, dw, dx_dtype, dw_dtype, dx_beta, dw_beta,
+                         few_parts(k, f) > 1 ? (float *)ws : nullptr};
+    const dim3 grid((unsigned)((k + 15) / 16), few_parts(k, f));
+    if (dtype == 1)
+        hipLaunchKernelGGL(k_gated_few_grads<true>, grid, dim3(kFgWaves * 64), 0, (hipStream_t)s, a);
+    else
+        hipLaunchKernelGGL(k_gated_few_grads<false>, grid, dim3(kFgWaves * 64), 0, (hipStream_t)s, a);
+    if (dx && grid.y > 1)
+        hipLaunchKernelGGL(k_gated_few_join, dim3((unsigned)((m * k + 255) / 256)), dim3(256), 0, (hipStream_t)s, a, grid.y);
+    return (int)hipGetLastError();
 }

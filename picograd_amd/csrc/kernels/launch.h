@@ -294,6 +294,18 @@ int pgk_gated_forward(int dtype, int act, size_t m, size_t f, size_t k8, const u
 size_t pgk_gated_bwd_workspace(size_t m, size_t f);
 int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float *z, size_t m, size_t f, uint16_t *dz16, int dtype,
                   float *db, int db_beta, void *ws, pgk_stream s);
+/* The backward of few rows (_ok): dz [m, 2 f] stays f32, db as above; then dx =
+ * dz W^T [m, k] and dw = x^T dz [k, 2 f] from 16-bit x (rows ldx apart) and W [k, 2,
+ * half] at any alignment, either NULL, written as the dtype says or added to
+ * an f32 (beta), in one launch, two where dx's sums are in parts.  dx and dw do
+ * not overlap.  ws: _workspace bytes. */
+size_t pgk_gated_few_grads_workspace(size_t m, size_t k, size_t f);
+int pgk_gated_few_grads_ok(size_t m, size_t k, size_t f);
+int pgk_gated_few_dz(int act, const void *dh, int dh_dtype, const float *z, size_t m, size_t f, float *dz, float *db,
+                     int db_beta, pgk_stream s);
+int pgk_gated_few_grads(int dtype, const float *dz, size_t m, size_t k, size_t f, const uint16_t *x, size_t ldx,
+                        const uint16_t *w, size_t half, void *dx, int dx_dtype, int dx_beta, void *dw, int dw_dtype,
+                        int dw_beta, void *ws, pgk_stream s);
 
 /* 4-bit matrices with a power of two per 32 values along the reduction
  * (mx4.hip), in the order in which the 16 x 16 x 128 matrix instruction takes
