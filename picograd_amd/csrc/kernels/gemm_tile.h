@@ -671,9 +671,13 @@ __device__ __forceinline__ void gemm16_block(const gemm_kargs &g, int pid, int n
                         const f32x4u zz = {zv[0], zv[1], zv[2], zv[3]};
                         __builtin_nontemporal_store(zz, reinterpret_cast<f32x4u *>(epi.z + off));
                     }
-                    if (c16)
-                        *reinterpret_cast<u32x2u *>(c16 + off) =
-                            u32x2u{to16x2(epi.dtype16, o[0], o[1]), to16x2(epi.dtype16, o[2], o[3])};
+                    if (c16) {
+                        const u32x2u q2 = {to16x2(epi.dtype16, o[0], o[1]), to16x2(epi.dtype16, o[2], o[3])};
+                        if constexpr (TA == TB) // a grad: past the caches, as below
+                            __builtin_nontemporal_store(q2, reinterpret_cast<u32x2u *>(c16 + off));
+                        else
+                            *reinterpret_cast<u32x2u *>(c16 + off) = q2;
+                    }
                 } else {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
