@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) k_mx4_columns(pgk_mx4 q, const T *__restr
         float v[kBlock];
 #pragma unroll
         for (int j = 0; j < kBlock; ++j)
-            v[j] = row < q.rows && c0 + j < q.cols ? (float)src[(c0 + j) * q.rows + row] : 0.0f;
+            v[j] = row < q.rows && c0 + j < q.cols ? (float)__builtin_nontemporal_load(src + (c0 + j) * q.rows + row) : 0.0f;
         uint32_t byte;
         ((uint4 *)codes_at(q, t, s + h))[entry] = round_block(v, byte);
         both |= byte << (8 * h);
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(256) k_mx4_back_columns(pgk_mx4 q, O *__restri
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (c0 + j * 8 + e < q.cols)
-                    dst[(c0 + j * 8 + e) * q.rows + row] = (O)v[e];
+                    __builtin_nontemporal_store((O)v[e], dst + (c0 + j * 8 + e) * q.rows + row);
         }
     }
 }
