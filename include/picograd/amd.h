@@ -165,8 +165,8 @@ pg_node *pg_amd_ag_gated16(pg_node *x, pg_node *w, pg_node *b, int act, pg_dtype
  * for NaN.  The reference has no form below 16 bits. */
 typedef struct pg_amd_mx4 pg_amd_mx4;
 /* t [rows, cols] of any dtype in 4 bits, the blocks along dimension `axis`
- * (0 or 1); for the weights [K, N] of a product x W that is 0.  t is read,
- * not kept.  NULL and pg_autograd_last_error() on bad arguments or a device
+ * (0 or 1), which is at most 2^24 long; for the weights [K, N] of a
+ * product x W that is 0.  t is read, not kept.  NULL and pg_autograd_last_error() on bad arguments or a device
  * error.  Freed with pg_amd_mx4_free. */
 pg_amd_mx4 *pg_amd_mx4_quantize(const pg_tensor *t, int axis);
 void pg_amd_mx4_free(pg_amd_mx4 *q);

@@ -49,7 +49,10 @@ __global__ void __launch_bounds__(256) k_gated_pad(pad_job a, pad_job b, size_t 
 // A tile of the product holds columns of Wg beside the same columns of Wu
 // (TileGate), so its epilogue has g and u of each output and z need not be
 // read back; z itself is written only for a backward.  Tiles and k-loops are
-// the 16-bit GEMM's.
+// the 16-bit GEMM's, and what bounds it is what bounds that: in rounds of full
+// tiles the matrix units (4096 x 4096 x 8192 in bf16 518 us, 1.06 PFLOP/s, z's 268 MB
+// among them), with one round the loads' latency and the epilogue (512 x 1024 x
+// 4096 17 us, 0.5 PFLOP/s).
 template <class CF>
 __global__ void __launch_bounds__(CF::NT, 1) k_gated(gemm_kargs g)
 {
@@ -230,8 +233,9 @@ int launch_forward(int tile, const gemm_kargs &g, hipStream_t s)
 // The gate's backward over a strip of 256 columns of f and a run of rows per
 // block: its four waves take every fourth row each, four neighbouring columns a
 // lane, and keep the strip's column sums, joined through LDS in wave order into
-// the block's row of part.  Bound by the stream of z and dh in and dz out (4096 x
-// 8192 in bf16: 470 MB in 91 us, 5.1 TB/s).  A piece of four is one load at
+// the block's row of part.  dz is rounded to the operands' 16 bits, in which both
+// products take it; the sums take it before.  Bound by the stream of z and dh in
+// and dz out (4096 x 8192 in bf16: 470 MB in 90 us, 5.2 TB/s).  A piece of four is one load at
 // whatever address an odd f gives it (1023 x 2049: one value a lane took 11 us).
 constexpr int kBwdV = 4;
 template <bool WHOLE, class T>

@@ -106,7 +106,8 @@ __device__ __forceinline__ void load_block(const T *p, int left, float *v)
 
 // Blocks along the source's rows: a wave makes two steps of one tile, lane l
 // the blocks that are entry l of each, so a lane rounds a block by itself and
-// the codes leave as whole kilobytes.  Bound by the stream of the source.
+// the codes leave as whole kilobytes.  Bound by the stream of the source (8192 x
+// 4096 in bf16, 84 MB with the codes: 14 us, 6 TB/s with a part still cached).
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) k_mx4_rows(pgk_mx4 q, const T *__restrict__ src)
 {
@@ -131,7 +132,8 @@ __global__ void __launch_bounds__(256) k_mx4_rows(pgk_mx4 q, const T *__restrict
 
 // Blocks down the source's columns ([cols, rows]): a thread takes block `wave`
 // of two steps of one column, so that a wave reads whole row pieces of 64
-// columns (four tiles).  Bound by the stream of the source.
+// columns (four tiles).  Bound by the stream of the source (4096 x 4096 in f32,
+// 76 MB with the codes: 13.9 us).
 template <class T>
 __global__ void __launch_bounds__(256) k_mx4_columns(pgk_mx4 q, const T *__restrict__ src)
 {
@@ -255,7 +257,7 @@ __device__ __forceinline__ bool rows_keep_four(const O *y, size_t n)
 // the reduction, so the weights stream past once.  A lane rounds its own blocks of x
 // on the way (entry l of a step is one block of one row): no other launch.  The
 // waves' partial tiles are added through LDS in wave order.  Bound by the loads'
-// latency and the launch at 4096 x 4096.
+// latency and the launch: one row by 4096 x 4096, 8.9 MB, 4.7 us.
 constexpr int kFewWaves = 8;
 
 template <class T, class O, bool VEC>
@@ -312,7 +314,8 @@ __global__ void __launch_bounds__(kFewWaves * 64, 1) k_mx4_few(const T *__restri
 // pairs of steps v, v + KG, ... straight from memory into registers, the next
 // pair's loads in flight.  LDS only for the sum of the partial tiles: the upper
 // half of the waves leaves its own, the lower half adds them and leaves the
-// sums, which are added in wave order.  Bound by the loads' latency.
+// sums, which are added in wave order.  Bound by the loads' latency: 333 x 1000 x
+// 2049 takes 5.9 us, 0.23 PFLOP/s, beside 4.9 for rounding x.
 template <int FM, int FN>
 struct pair_of_steps {
     uint4 a[2][FM], b[2][FN];
@@ -424,7 +427,8 @@ __global__ void __launch_bounds__(KG * 64, 1) k_mx4_split(pgk_mx4 x, pgk_mx4 w, 
 // set.  A stage is refilled during the step that follows its last read, behind
 // the step's one barrier, so its loads have three steps to land.  Tiles of
 // 128 x 128 on four waves, two blocks to a CU, of which one computes while the
-// other waits at its barrier.  8192 x 4096 x 4096 takes 92 us, 3.0 PFLOP/s where the matrix
+// other waits at its barrier.  8192 x 4096 x 4096 takes 72 us and the
+// rounding of x 14, 3.8 PFLOP/s of the product where the matrix
 // units alone reach 6.0 on random codes; two stages of two steps take 109 and
 // 256 x 256 tiles, whose eight waves run out of registers, 90 to 111.
 template <int BM, int BN, int WGM, int WGN, class O>
