@@ -154,6 +154,25 @@ def test_both_grads(bench, dtype, m, k, f):
         check(bench.read(dw), ref["dw"], wd, "dw")
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("m,k,f", [(1, 64, 64), (3, 30, 68), (4, 700, 2000), (9, 129, 333), (16, 1024, 1030)])
+def test_few_rows_round_once(bench, dtype, m, k, f):
+    """Up to 16 rows [dg | du] is not rounded on the way to dx and dW: the bounds are those of f32."""
+    L = bench.L
+    x, w, _, dh = data(m, k, f, dtype, False, seed=13)
+    z = rounded(x @ w, F32)
+    a, da = act64(z[:, :f], "silu")
+    u = z[:, f:]
+    dz = np.concatenate([dh * u * da, dh * a], 1)
+    e = np.abs(dh) * MATH * (1 + np.abs(z[:, :f]) * 2.0 ** -2)
+    e = np.concatenate([np.abs(u) * e, e], 1) + 3 * F * np.abs(dz) + TINY[F32]
+    dx, dw = bench.unset((m, k)), bench.unset((k, 2 * f))
+    bench.ok(L.pg_amd_gated_backward(bench.tensor(x, dtype), bench.tensor(w, dtype), bench.tensor(z), bench.tensor(dh, dtype), 3,
+                                     dx, dw, None))
+    within(bench.read(dx), dz @ w.T, e @ np.abs(w).T + (2 * f + 4) * F * ((np.abs(dz) + e) @ np.abs(w).T), "dx")
+    within(bench.read(dw), x.T @ dz, np.abs(x).T @ e + (m + 4) * F * (np.abs(x).T @ (np.abs(dz) + e)), "dw")
+
+
 @pytest.mark.parametrize("act", sorted(ACTS))
 @pytest.mark.parametrize("m,f", [(3, 24), (40, 24), (200, 130)])
 def test_every_activation(bench, act, m, f):
