@@ -820,8 +820,8 @@ static bool g_narrow = true;
 /* The bias grad of the last activation pass whose row-block partials are
  * not yet added: the next activation pass adds them in a row of extra
  * blocks of its own launch (one launch less per layer), or
- * pgm_colsum_flush does, at the end of the backward walk and before that
- * grad is taken for writing again.  The partials sit in scratch slot
+ * pgm_colsum_flush does, at the end of the backward walk, before that grad is
+ * taken for writing again and before the backward of the node whose it is.  The partials sit in scratch slot
  * g_fin_slot; the next pass writes its own into the other slot.  The
  * additions are k_colsum_fin's either way (the same bits). */
 #define PGM_FIN_SLOT_A 3

@@ -204,7 +204,8 @@ const uint16_t *pgm_operand16(pg_tensor *t, int dt, size_t rows, size_t cols, si
 int pgm_grad_split(size_t M, size_t K, size_t N, size_t N8, size_t B, size_t Mw, size_t Bw, bool *streams);
 /* a linear16 bias grad whose last step (the sum of its row-block partials)
  * the next activation pass was to run: run it now (the walk's end), or now
- * if it writes into t's storage (t is about to be written) */
+ * if it writes into t's storage (t is about to be written, or read by the
+ * backward of the node whose grad it is) */
 void pgm_colsum_flush(void);
 void pgm_colsum_flush_for(const pg_tensor *t);
 /* pg_amd_ag_linear16's backward and the destructor of its node context

@@ -599,6 +599,9 @@ static bool walk(pg_node *loss, const pg_tensor *seed, wmode mode)
             pg_node *x = order.v[kk];
             if (w.done[kk] || !x->backward || !x->grad)
                 continue;
+            /* x may be a linear16 bias: the last sums of its grad, deferred to
+             * a later pass, are read here */
+            pgm_colsum_flush_for(x->grad);
             if (x->grad->pg_flags & PG_TENSOR_ZERO_PENDING) {
                 /* a zero upstream grad contributes nothing, but the parents'
                  * grads still come into existence (as zeros) */

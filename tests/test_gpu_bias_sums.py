@@ -92,3 +92,42 @@ def test_shared_bias(lib):
     # the out layer's grad is written first (beta 0), the first layer's added
     want = (db2 + db1).astype(np.float32)
     assert np.array_equal(db.view(np.uint32), want.view(np.uint32))
+
+
+@pytest.mark.parametrize("via", ["mul", "gelu", "sum", "linear16"])
+@pytest.mark.parametrize("M", [1537, 4000])
+def test_bias_made_by_another_node(lib, via, M):
+    """A bias that is itself a node's value: its grad, whose last step waits
+    for a later pass, is read by that node's backward.  The seed holds
+    sixteenths, so the column sums are exact in f32."""
+    print("bias sums: made by", via, flush=True)
+    rng = np.random.default_rng(M)
+    K, N = 64, 384
+    x, w = rng.standard_normal((M, K)).astype(np.float32), rng.standard_normal((K, N)).astype(np.float32)
+    g = (rng.integers(-8, 9, (M, N)) / 16).astype(np.float32)
+    db = g.sum(0, dtype=np.float64)
+    nx, nw = lib.var(x, False), lib.var(w)
+    if via == "mul":
+        c = rng.integers(1, 9, N).astype(np.float32)
+        leaves = [lib.var(rng.standard_normal(N).astype(np.float32)), lib.var(c, False)]
+        b, want = lib.op("mul", *leaves), db * c
+    elif via == "gelu":
+        leaves = [lib.var(np.zeros(N, np.float32))]  # gelu'(0) is 0.5
+        b, want = lib.op("gelu", leaves[0]), db * 0.5
+    elif via == "sum":
+        leaves = [lib.var(rng.standard_normal((3, N)).astype(np.float32))]
+        b, want = lib.op("sum", leaves[0], 0, False), np.tile(db, (3, 1))
+    else:  # one row of ones: the grad of its weights' first row is the bias grad in bf16
+        leaves = [lib.var(rng.standard_normal((8, N)).astype(np.float32)), lib.var(np.eye(1, 8, dtype=np.float32), False)]
+        b = lib._check(lib.pg_amd_ag_linear16(leaves[1], leaves[0], None, NONE, BF16))
+        want = np.zeros((8, N))
+        want[0] = db
+    y = lib._check(lib.pg_amd_ag_linear16(nx, nw, b, NONE, BF16))
+    seed = lib.tensor(g)
+    lib.pg_amd_backward_from(y, seed)
+    got = lib.grad(leaves[0]).astype(np.float64)
+    unit = 2.0 ** -8 if via == "linear16" else 2.0 ** -22
+    assert (np.abs(got - want) <= unit * np.abs(want)).all(), np.abs(got - want).max()
+    lib.pg_tensor_free(seed)
+    for n in [y, b, nx, nw] + leaves:
+        lib.pg_node_free(n)

@@ -348,3 +348,20 @@ def test_refusals(bench):
                       ((nx, nw, None, 9, BF16), "act"), ((nx, nx, None, 3, BF16), "x [M, K]")):
         assert not L.pg_amd_ag_gated16(*bad)
         assert word in L.pg_autograd_last_error().decode()
+
+
+@pytest.mark.parametrize("m,k2", [(40, 24), (512, 64), (3000, 40)])
+def test_a_gated_row_as_the_bias_of_a_linear_layer(bench, m, k2):
+    """The bias grad, whose last sums may wait for a later pass, is the gated node's upstream one."""
+    L, k, f = bench.L, 24, 64
+    r = np.random.default_rng(m)
+    x, w, _, _ = data(1, k, f, BF16, False, seed=15)
+    dy = r.integers(-8, 9, (m, f)) / 16.0  # its column sums are exact
+    nodes = [bench.var(v) for v in (x, w, r.standard_normal((m, k2)), r.standard_normal((k2, f)))]
+    h = bench.node(L.pg_amd_ag_gated16(nodes[0], nodes[1], None, 3, BF16))
+    y = bench.node(L.pg_amd_ag_linear16(nodes[2], nodes[3], h, 0, BF16))
+    L.pg_amd_backward_from(y, bench.tensor(dy))
+    ref = model(x, w, None, dy.sum(0)[None], "silu", BF16)
+    within(L.grad(h), dy.sum(0)[None], 0, "the bias grad")
+    within(L.grad(nodes[0]), *ref["dx"], "dx")
+    within(L.grad(nodes[1]), *ref["dw"], "dw")
