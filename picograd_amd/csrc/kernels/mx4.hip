@@ -30,6 +30,11 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kBlock = 32; // values under one power of two
 
+// A launch holds under 2^32 threads in x and 65536 blocks in y: longer grids are
+// several launches, each told the first block of its own (a loop over the blocks
+// within the kernels costs a 4096 x 4096 matrix taken to 4 bits and back 11 us of 30).
+constexpr size_t kMostX = (size_t)1 << 22, kMostY = 65535;
+
 // the bytes of step s of tile t, and of its powers (of the pair of steps s / 2)
 __device__ __forceinline__ uint8_t *codes_at(const pgk_mx4 &q, size_t t, size_t s)
 {
@@ -135,10 +140,10 @@ __global__ void __launch_bounds__(256) k_mx4_rows(pgk_mx4 q, const T *__restrict
 // columns (four tiles).  Bound by the stream of the source (4096 x 4096 in f32,
 // 76 MB with the codes: 13.9 us).
 template <class T>
-__global__ void __launch_bounds__(256) k_mx4_columns(pgk_mx4 q, const T *__restrict__ src)
+__global__ void __launch_bounds__(256) k_mx4_columns(pgk_mx4 q, const T *__restrict__ src, size_t x0, size_t y0)
 {
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const size_t row = (size_t)blockIdx.x * 64 + lane, s = (size_t)blockIdx.y * 2, t = row >> 4;
+    const size_t row = (x0 + blockIdx.x) * 64 + lane, s = (y0 + blockIdx.y) * 2, t = row >> 4;
     if (t >= q.tiles)
         return;
     const int entry = wave * 16 + (lane & 15);
@@ -192,10 +197,10 @@ __global__ void __launch_bounds__(256) k_mx4_back_rows(pgk_mx4 q, O *__restrict_
 
 // Columns back, as k_mx4_columns reads them.
 template <class O>
-__global__ void __launch_bounds__(256) k_mx4_back_columns(pgk_mx4 q, O *__restrict__ dst)
+__global__ void __launch_bounds__(256) k_mx4_back_columns(pgk_mx4 q, O *__restrict__ dst, size_t x0, size_t y0)
 {
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const size_t row = (size_t)blockIdx.x * 64 + lane, s = (size_t)blockIdx.y * 2, t = row >> 4;
+    const size_t row = (x0 + blockIdx.x) * 64 + lane, s = (y0 + blockIdx.y) * 2, t = row >> 4;
     if (row >= q.rows)
         return;
     const int entry = wave * 16 + (lane & 15);
@@ -261,12 +266,13 @@ __device__ __forceinline__ bool rows_keep_four(const O *y, size_t n)
 constexpr int kFewWaves = 8;
 
 template <class T, class O, bool VEC>
-__global__ void __launch_bounds__(kFewWaves * 64, 1) k_mx4_few(const T *__restrict__ x, int m, pgk_mx4 w, O *__restrict__ y)
+__global__ void __launch_bounds__(kFewWaves * 64, 1)
+    k_mx4_few(const T *__restrict__ x, int m, pgk_mx4 w, O *__restrict__ y, int t0)
 {
     constexpr int U = 4; // steps in flight
     __shared__ float part[kFewWaves][16][17];
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    const int t = xcd_tile((int)blockIdx.x, (int)gridDim.x), steps = (int)w.steps, k = (int)w.cols;
+    const int t = t0 + xcd_tile((int)blockIdx.x, (int)gridDim.x), steps = (int)w.steps, k = (int)w.cols;
     // runs of U neighbouring steps, dealt to the waves in turn
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = wave * U; s0 < steps; s0 += kFewWaves * U) {
@@ -613,16 +619,28 @@ bool vector_rows(const T *p, size_t cols)
     return ((uintptr_t)p & 15) == 0 && cols * sizeof(T) % 16 == 0;
 }
 
+// fn(grid, first x, first y) for parts of an x by y grid
+template <class FN>
+int by_parts(size_t x, size_t y, FN fn)
+{
+    for (size_t x0 = 0; x0 < x; x0 += kMostX)
+        for (size_t y0 = 0; y0 < y; y0 += kMostY) {
+            const size_t nx = x - x0 < kMostX ? x - x0 : kMostX, ny = y - y0 < kMostY ? y - y0 : kMostY;
+            fn(dim3((unsigned)nx, (unsigned)ny), x0, y0);
+            const int rc = (int)hipGetLastError();
+            if (rc)
+                return rc;
+        }
+    return 0;
+}
+
 template <class T>
 int quantize(const pgk_mx4 &q, const T *src, int trans, hipStream_t st)
 {
-    if (trans) {
-        if (q.steps / 2 > 65535)
-            return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL(k_mx4_columns<T>, dim3((unsigned)((q.tiles + 3) / 4), (unsigned)(q.steps / 2)), dim3(256), 0, st,
-                           q, src);
-        return (int)hipGetLastError();
-    }
+    if (trans)
+        return by_parts((q.tiles + 3) / 4, q.steps / 2, [&](const dim3 &grid, size_t x0, size_t y0) {
+            hipLaunchKernelGGL(k_mx4_columns<T>, grid, dim3(256), 0, st, q, src, x0, y0);
+        });
     const dim3 grid(blocks_for(q.tiles * q.steps / 2 * 64));
     if (vector_rows(src, q.cols))
         hipLaunchKernelGGL((k_mx4_rows<T, true>), grid, dim3(256), 0, st, q, src);
@@ -634,25 +652,23 @@ int quantize(const pgk_mx4 &q, const T *src, int trans, hipStream_t st)
 template <class O>
 int dequantize(const pgk_mx4 &q, O *dst, int trans, hipStream_t st)
 {
-    if (!trans)
-        hipLaunchKernelGGL(k_mx4_back_rows<O>, dim3(blocks_for(q.rows * ((q.cols + 7) / 8))), dim3(256), 0, st, q, dst);
-    else if (q.steps / 2 > 65535)
-        return (int)hipErrorInvalidValue;
-    else
-        hipLaunchKernelGGL(k_mx4_back_columns<O>, dim3((unsigned)((q.tiles + 3) / 4), (unsigned)(q.steps / 2)), dim3(256), 0,
-                           st, q, dst);
+    if (trans)
+        return by_parts((q.tiles + 3) / 4, q.steps / 2, [&](const dim3 &grid, size_t x0, size_t y0) {
+            hipLaunchKernelGGL(k_mx4_back_columns<O>, grid, dim3(256), 0, st, q, dst, x0, y0);
+        });
+    hipLaunchKernelGGL(k_mx4_back_rows<O>, dim3(blocks_for(q.rows * ((q.cols + 7) / 8))), dim3(256), 0, st, q, dst);
     return (int)hipGetLastError();
 }
 
 template <class T, class O>
 int few(const T *x, size_t m, const pgk_mx4 &w, O *y, hipStream_t st)
 {
-    const dim3 grid((unsigned)w.tiles), block(kFewWaves * 64);
-    if (vector_rows(x, w.cols))
-        hipLaunchKernelGGL((k_mx4_few<T, O, true>), grid, block, 0, st, x, (int)m, w, y);
-    else
-        hipLaunchKernelGGL((k_mx4_few<T, O, false>), grid, block, 0, st, x, (int)m, w, y);
-    return (int)hipGetLastError();
+    return by_parts(w.tiles, 1, [&](const dim3 &grid, size_t t0, size_t) {
+        if (vector_rows(x, w.cols))
+            hipLaunchKernelGGL((k_mx4_few<T, O, true>), grid, dim3(kFewWaves * 64), 0, st, x, (int)m, w, y, (int)t0);
+        else
+            hipLaunchKernelGGL((k_mx4_few<T, O, false>), grid, dim3(kFewWaves * 64), 0, st, x, (int)m, w, y, (int)t0);
+    });
 }
 
 template <int FM, int FN, int KG, class O>
@@ -666,7 +682,7 @@ template <class O>
 int product(const pgk_mx4 &x, const pgk_mx4 &w, O *y, hipStream_t st)
 {
     auto tiles = [&](size_t bm, size_t bn) { return (x.rows + bm - 1) / bm * ((w.rows + bn - 1) / bn); };
-    if (tiles(128, 128) > 0x7fffffff)
+    if (tiles(128, 128) >> 24) // 2^32 threads
         return (int)hipErrorInvalidValue;
     if (tiles(32, 32) <= 256)
         split<2, 2, 8>(x, w, y, st);

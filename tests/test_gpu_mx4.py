@@ -222,3 +222,40 @@ def test_refusals(bench):
     bench.refused(L.pg_amd_mx4_matmul(wide, q64, wide), "overlaps")
     for p in (q, other, q64):
         L.pg_amd_mx4_free(p)
+
+
+@pytest.mark.parametrize("k", [2 ** 24, 2 ** 24 - 33, 65535 * 256 + 1])
+@pytest.mark.parametrize("axis", [0, 1])
+def test_the_longest_blocked_dimension(bench, axis, k):
+    """Up to 2^24 along the blocks, down a column as along a row: a pattern of 32 blocks, each times its own power."""
+    g = np.random.default_rng(k)
+    some = rounded(g.standard_normal((1, 1024)), F32)
+    blocks = (k + 31) // 32
+    power = np.repeat(2.0 ** (np.arange(blocks) % 61 - 30), 32)[:k]
+    v = np.resize(some[0], k) * power
+    want = np.resize(quantized(some)[0], k) * power
+    if k % 32:
+        want[blocks * 32 - 32:] = quantized(v[None, blocks * 32 - 32:])[0]
+    shape = (k, 1) if axis == 0 else (1, k)
+    assert np.array_equal(keep(bench, bench.tensor(v.reshape(shape)), axis, shape), want.reshape(shape))
+
+
+@pytest.mark.parametrize("m", [1, 17])
+def test_the_longest_reduction(bench, m):
+    """2^24 terms of 0 or 1: every partial sum is exact."""
+    k = 2 ** 24
+    w = (np.arange(k) % 3 == 0).astype(np.float32)[:, None]
+    assert (product(bench, np.ones((m, k), np.float32), w, BF16, F32) == w.sum(dtype=np.float64)).all()
+
+
+def test_more_columns_than_a_launch_has_threads_for(bench):
+    """2^27 columns of one value, 16 of them a tile of 512 threads."""
+    n = 2 ** 27 + 40
+    w = (np.arange(n, dtype=np.uint32) % 5).astype(np.float32)[None]
+    x = bench.tensor(np.ones((1, 1)), BF16)
+    q = bench.L.pg_amd_mx4_quantize(bench.tensor(w), 0)
+    assert q, bench.L.pg_autograd_last_error().decode()
+    y = bench.unset((1, n))
+    bench.ok(bench.L.pg_amd_mx4_matmul(x, q, y))
+    bench.L.pg_amd_mx4_free(q)
+    assert np.array_equal(bench.L.read(y), w)
