@@ -839,6 +839,42 @@ size_t parts_of(const pgk_distill_args &a)
     return (a.v / chunk_of<T>::N + kPartChunks - 1) / kPartChunks;
 }
 
+// A launch holds under 2^32 threads: fn(args of a run of rows) for runs of at most
+// `most`.
+template <class FN>
+void by_runs(const pgk_distill_args &a, size_t most, FN fn)
+{
+    auto size = [](int dtype) { return dtype == 0 ? (size_t)4 : (size_t)2; };
+    for (size_t r = 0; r < a.n; r += most) {
+        pgk_distill_args b = a;
+        b.n = a.n - r < most ? a.n - r : most;
+        b.s = (const char *)a.s + r * a.v * size(a.dtype);
+        b.t = (const char *)a.t + r * a.top * size(a.top_dtype);
+        b.idx = a.idx + r * a.top;
+        b.label = a.label ? a.label + r : nullptr;
+        b.loss = a.loss ? a.loss + r : nullptr;
+        b.ds = a.ds ? (char *)a.ds + r * a.v * size(a.ds_dtype) : nullptr;
+        fn(b);
+    }
+}
+
+template <class T, class O, int G>
+void launch_short(const pgk_distill_args &all, hipStream_t st)
+{
+    constexpr size_t R = 256 / G; // rows of a block
+    by_runs(all, R << 22, [&](const pgk_distill_args &a) {
+        hipLaunchKernelGGL((k_distill_short<T, O, G>), dim3((unsigned)((a.n + R - 1) / R)), dim3(256), 0, st, a);
+    });
+}
+
+template <class T, class O>
+void launch_stream(const pgk_distill_args &all, hipStream_t st)
+{
+    by_runs(all, (size_t)1 << 21, [&](const pgk_distill_args &a) {
+        hipLaunchKernelGGL((k_distill_stream<T, O>), dim3((unsigned)a.n), dim3(kStreamThreads), 0, st, a);
+    });
+}
+
 // The rows' blocks would leave most of the chip idle, or cannot hold a row.  Up
 // to 2^21 chunks of 16 bytes in all the two reads of a split row cost less than
 // the idle CUs: 16 rows of 131072 f16 take 9.9 us split and 28.0 whole, 128 26.9
@@ -856,11 +892,11 @@ int launch(const pgk_distill_args &a, float *ws, hipStream_t st)
     const size_t chunks = a.v / chunk_of<T>::N;
     const bool one = a.label && a.alpha < 1.0f && a.temperature != 1.0f;
     if (a.v <= 64 && a.top <= 16) {
-        hipLaunchKernelGGL((k_distill_short<T, O, 16>), dim3((unsigned)((a.n + 15) / 16)), dim3(256), 0, st, a);
+        launch_short<T, O, 16>(a, st);
     } else if (a.v <= 256 && a.top <= 64) {
-        hipLaunchKernelGGL((k_distill_short<T, O, 64>), dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, st, a);
+        launch_short<T, O, 64>(a, st);
     } else if (!chunks_match<T, O>(a) || a.beta) {
-        hipLaunchKernelGGL((k_distill_stream<T, O>), dim3((unsigned)a.n), dim3(kStreamThreads), 0, st, a);
+        launch_stream<T, O>(a, st);
     } else if (split<T>(a)) {
         const int parts = (int)parts_of<T>(a);
         const dim3 grid((unsigned)parts, (unsigned)a.n);
@@ -872,7 +908,7 @@ int launch(const pgk_distill_args &a, float *ws, hipStream_t st)
         else
             hipLaunchKernelGGL((k_distill_finish<T, O, true, false>), grid, dim3(kPartThreads), 0, st, a, ws, parts);
     } else if (chunks > 16384) {
-        hipLaunchKernelGGL((k_distill_stream<T, O>), dim3((unsigned)a.n), dim3(kStreamThreads), 0, st, a);
+        launch_stream<T, O>(a, st);
     } else if (chunks > 8192) {
         launch_rows<T, O, 1024, 16>(a, 1, st);
     } else if (chunks > 4096) {

@@ -355,3 +355,50 @@ def test_refusals(bench):
     assert not L.pg_amd_ag_distill(None, t, idx, lab, C.byref(DistillCfg(1.0, 0.5, 1.0)))
     assert not L.pg_amd_ag_distill(bench.var(np.zeros((4, 9))), t, idx, bench.tensor(np.zeros(5)),
                                    C.byref(DistillCfg(1.0, 0.5, 1.0)))
+
+
+def test_more_rows_than_a_launch_has_threads_for(bench):
+    """Past 2^32 threads at 16, 64 and 1024 a row.  One entry and equal logits: the loss is log V, the grad 1 / V,
+    less 1 at the entry."""
+    L = bench.L
+    cfg = DistillCfg(1.0, 1.0, 1.0)
+
+    def full(shape, dtype, value):
+        nd, sh = shape_arg(shape)
+        t = L.pg_tensor_full_dtype(dtype, nd, sh, value)
+        assert t, L.pg_amd_last_error().decode()
+        return t
+
+    def at(t, *i):
+        return bench.get(t, (C.c_size_t * len(i))(*i))
+
+    bench.get = L.lib.pg_tensor_get
+    bench.get.restype, bench.get.argtypes = C.c_float, [C.c_void_p, C.POINTER(C.c_size_t)]
+    for n, v, dtype in ((2 ** 28 + 17, 2, BF16), (2 ** 26 + 5, 65, BF16)):
+        made = [full((n, v), dtype, 0.5), full((n, 1), BF16, 3.0), full((n, 1), F32, 1.0), full((n,), F32, 777.0)]
+        done = L.pg_amd_distill(*made[:3], None, C.byref(cfg), made[3], None)
+        got = [at(made[3], i) for i in (0, 1, n // 2, n - 17, n - 1)] if done else []
+        L.sync()
+        for t in made:
+            L.pg_tensor_free(t)
+        bench.ok(done)
+        within(got, np.full(5, np.log(v)), (v / 256 + 64 + 16) * 2.0 ** -24 * (np.log(v) + 4), (n, v))
+        L.lib.pg_tensor_pool_clear()
+    # two losses over one node: the second adds to the grad
+    n, v = 2 ** 22 + 3, 257
+    top, idx = full((n, 1), BF16, 3.0), full((n, 1), F32, 2.0)
+    nd, sh = shape_arg((n, v))
+    x = L._check(L.pg_var_full(nd, sh, 0.5, True))
+    parts = [L._check(L.pg_amd_ag_distill(x, top, idx, None, C.byref(cfg))) for _ in range(2)]
+    total = L._check(L.pg_ag_add(*parts))
+    L.pg_backward(total)
+    g = L.node(x).grad
+    got = [at(g, i, j) for i in (0, 2 ** 22 - 1, 2 ** 22, n - 1) for j in (0, 2, 256)]
+    L.sync()
+    for node in (total, *parts, x):
+        L.pg_node_free(node)
+    for t in (top, idx):
+        L.pg_tensor_free(t)
+    L.lib.pg_tensor_pool_clear()
+    want = np.array([2 / v, 2 / v - 2, 2 / v] * 4)
+    within(got, want, 2 * (v / 256 + 64 + 16) * 2.0 ** -24 * np.array([1 / v, 1 + 1 / v, 1 / v] * 4), "two losses")
