@@ -25,7 +25,7 @@ static bool dims_ok(const pg_tensor *x, const pg_tensor *w, const pg_tensor *b, 
         (b && b->numel != w->shape[1]))
         return false;
     *d = (gated_dims){x->shape[0], x->shape[1], w->shape[1] / 2, up8(x->shape[1]), up8(w->shape[1] / 2)};
-    return d->M <= 0x7fffffff && d->K <= 0x3fffffff && d->F <= 0x1fffffff;
+    return d->M <= 0x7fffff00 && d->K <= 0x3fffffff && d->F <= 0x1fffffff;
 }
 
 /* z (when given) and h of the layer; h in f32 (h32) and / or 16 bits (h16) */

@@ -394,7 +394,7 @@ struct few_grads {
     size_t ldx, ldw, half; // of W: a row, and from g's columns to u's in it
     const float *dz;
     int m;
-    size_t k, f;
+    size_t k, f, first; // the launch's first 16 rows of W
     void *dx, *dw; // NULL: not wanted
     int dx_dtype, dw_dtype, dx_beta, dw_beta;
     float *part; // [parts, m, k] of dx where the columns are in more than one part
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kFgWaves * 64, 2) k_gated_few_grads(few_grads 
     __shared__ float sums[kFgWaves][16][17];
     const int lane = (int)threadIdx.x & 63, q = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const size_t k0 = (size_t)blockIdx.x * 16, kr = k0 + q < a.k ? k0 + q : a.k - 1;
+    const size_t k0 = (a.first + blockIdx.x) * 16, kr = k0 + q < a.k ? k0 + q : a.k - 1;
     const size_t per = (a.f + 63) / 64, pieces = 2 * per;
     float xv[4]; // x[4 s + l / 16][k0 + l % 16]
 #pragma unroll
@@ -588,6 +588,8 @@ extern "C" int pgk_gated_forward(int dtype, int act, size_t m, size_t f, size_t 
     if (m > 0x7fffffff || f > 0x1fffffff || k8 > 0x7fff0000 || (k8 & 7) || (ldx & 7) || (f8 & 7) || f8 < f || ldx < k8 ||
         ((((uintptr_t)x) | (uintptr_t)w) & 15) || (dtype != 1 && dtype != 2))
         return (int)hipErrorInvalidValue;
+    if (((m + 127) / 128) * ((f + 63) / 64) >> 24) // a launch holds under 2^32 threads, a tile has 256
+        return (int)hipErrorInvalidValue;
     gemm_kargs g = {};
     g.A = x, g.lda = ldx, g.a_extent = (int)m;
     g.B = w, g.ldb = 2 * f8, g.b_extent = (int)f8;
@@ -682,14 +684,19 @@ extern "C" int pgk_gated_few_grads(int dtype, const float *dz, size_t m, size_t 
         (dw_beta && dw_dtype) || half < f || (dw && ldx < k) ||
         (dx && !ws && few_parts(k, f) > 1))
         return (int)hipErrorInvalidValue;
-    const few_grads a = {x, w, ldx, 2 * half, half, dz, (int)m, k, f, dx, dw, dx_dtype, dw_dtype, dx_beta, dw_beta,
-                         few_parts(k, f) > 1 ? (float *)ws : nullptr};
-    const dim3 grid((unsigned)((k + 15) / 16), few_parts(k, f));
-    if (dtype == 1)
-        hipLaunchKernelGGL(k_gated_few_grads<true>, grid, dim3(kFgWaves * 64), 0, (hipStream_t)s, a);
-    else
-        hipLaunchKernelGGL(k_gated_few_grads<false>, grid, dim3(kFgWaves * 64), 0, (hipStream_t)s, a);
-    if (dx && grid.y > 1)
-        hipLaunchKernelGGL(k_gated_few_join, dim3((unsigned)((m * k + 255) / 256)), dim3(256), 0, (hipStream_t)s, a, grid.y);
+    few_grads a = {x, w, ldx, 2 * half, half, dz, (int)m, k, f, 0, dx, dw, dx_dtype, dw_dtype, dx_beta, dw_beta,
+                   few_parts(k, f) > 1 ? (float *)ws : nullptr};
+    // a launch holds under 2^32 threads
+    const size_t blocks = (k + 15) / 16, most = (size_t)1 << 22;
+    const unsigned parts = few_parts(k, f);
+    for (; a.first < blocks; a.first += most) {
+        const dim3 grid((unsigned)(blocks - a.first < most ? blocks - a.first : most), parts);
+        if (dtype == 1)
+            hipLaunchKernelGGL(k_gated_few_grads<true>, grid, dim3(kFgWaves * 64), 0, (hipStream_t)s, a);
+        else
+            hipLaunchKernelGGL(k_gated_few_grads<false>, grid, dim3(kFgWaves * 64), 0, (hipStream_t)s, a);
+    }
+    if (dx && parts > 1)
+        hipLaunchKernelGGL(k_gated_few_join, dim3((unsigned)((m * k + 255) / 256)), dim3(256), 0, (hipStream_t)s, a, parts);
     return (int)hipGetLastError();
 }

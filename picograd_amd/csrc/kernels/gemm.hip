@@ -953,7 +953,9 @@ static size_t k_inkernel(int ta, int tb, size_t k) { return (ta && tb) || k % 8 
 // its 16-row blocks; the rest keep the tiled plans (split-K among them)
 static bool skinny_ok(int ta, int tb, size_t m, size_t n, size_t k, size_t batch)
 {
-    return tb && n <= 16 && batch == 1 && k && (ta || k % 8 == 0) && (m + 15) / 16 >= 64;
+    // (a launch holds under 2^32 threads, a block has 512)
+    return tb && n <= 16 && batch == 1 && k && (ta || k % 8 == 0) && (m + 15) / 16 >= 64 &&
+           (m + 15) / 16 < (size_t)1 << 23;
 }
 
 // k_few_rows's products: one 16-row tile with a block per CU at most (past
@@ -984,6 +986,10 @@ int check_gemm_args(int ta, int tb, size_t m, size_t n, size_t k, const uint16_t
     // k leaves headroom for the k offsets of the tiles the kernel loads
     // past the end (from the zero page) to stay within int
     if (m > 0x7fffffff || n > 0x7fffffff || k > 0x7fff0000 || batch > 65535)
+        return (int)hipErrorInvalidValue;
+    // a launch holds under 2^32 threads (more of them wrap with no error), a
+    // 128 x 128 tile has 256
+    if (((m + 127) / 128) * ((n + 127) / 128) >> 24)
         return (int)hipErrorInvalidValue;
     // 16-byte global loads: aligned bases, leading dims and batch strides
     if ((((uintptr_t)a | (uintptr_t)b) & 15) || (lda & 7) || (ldb & 7) || (stride_a & 7) || (stride_b & 7))

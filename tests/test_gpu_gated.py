@@ -7,6 +7,8 @@ the sum of its terms' magnitudes; act and act' are within 2^-20 of their
 argument's scale (a few units of f32 over an exponential); every rounding to
 16 bits adds half a unit in the last place of what it rounds.
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 from scipy.special import ndtr
@@ -365,3 +367,39 @@ def test_a_gated_row_as_the_bias_of_a_linear_layer(bench, m, k2):
     within(L.grad(h), dy.sum(0)[None], 0, "the bias grad")
     within(L.grad(nodes[0]), *ref["dx"], "dx")
     within(L.grad(nodes[1]), *ref["dw"], "dw")
+
+
+@pytest.mark.parametrize("m,f", [(1, 1), (17, 8)])
+def test_more_inputs_than_a_launch_has_threads_for(bench, m, f):
+    """K past 2^27: 2^32 threads at 512 for 16 rows of W.  Operands of one value each, so that every sum is exact."""
+    L, k = bench.L, 2 ** 27 + 40
+    made = {}
+    for name, shape, dtype, value in (("x", (m, k), F16, 0.5), ("w", (k, 2 * f), F16, 0.25), ("z", (m, 2 * f), F32, 2.0),
+                                      ("dh", (m, f), F16, 1.0), ("dx", (m, k), F16, 777.0), ("dw", (k, 2 * f), F16, 777.0)):
+        nd, sh = shape_arg(shape)
+        made[name] = L.pg_tensor_full_dtype(dtype, nd, sh, value)
+        assert made[name], L.pg_amd_last_error().decode()
+    done = L.pg_amd_gated_backward(*(made[n] for n in ("x", "w", "z", "dh")), 0, made["dx"], made["dw"], None)
+    get = L.lib.pg_tensor_get
+    get.restype, get.argtypes = C.c_float, [C.c_void_p, C.POINTER(C.c_size_t)]
+    at = [0, 5, 2 ** 26 - 1, 2 ** 26, 2 ** 27 - 17, 2 ** 27, k - 1]
+    dx = [get(made["dx"], (C.c_size_t * 2)(m - 1, i)) for i in at] if done else []
+    dw = [get(made["dw"], (C.c_size_t * 2)(i, 2 * f - 1)) for i in at] if done else []
+    L.sync()
+    for t in made.values():
+        L.pg_tensor_free(t)
+    L.lib.pg_tensor_pool_clear()
+    bench.ok(done)
+    # act NONE: [dg | du] = dh [u | g] = 2
+    assert dx == [2 * 0.25 * 2 * f] * len(at) and dw == [0.5 * 2 * m] * len(at)
+
+
+def test_more_rows_than_a_launch_has_threads_for_are_refused(bench):
+    L = bench.L
+    made = [L.pg_tensor_empty_dtype(F16, *shape_arg(s)) for s in ((2 ** 31 - 1, 1), (1, 2), (2 ** 31 - 1, 1))]
+    assert all(made), L.pg_amd_last_error().decode()
+    done = L.pg_amd_gated(made[0], made[1], None, 3, made[2], None)
+    for t in made:
+        L.pg_tensor_free(t)
+    L.lib.pg_tensor_pool_clear()
+    bench.refused(done, "x [M, K]")
