@@ -402,3 +402,34 @@ def test_more_rows_than_a_launch_has_threads_for(bench):
     L.lib.pg_tensor_pool_clear()
     want = np.array([2 / v, 2 / v - 2, 2 / v] * 4)
     within(got, want, 2 * (v / 256 + 64 + 16) * 2.0 ** -24 * np.array([1 / v, 1 + 1 / v, 1 / v] * 4), "two losses")
+
+
+@pytest.mark.parametrize("dtype,n,v", ROWS)
+def test_many_rows_in_place(bench, dtype, n, v):
+    """The grad of a row is stored while the next row's logits are fetched."""
+    s, t, idx, lab = data(n, v, 5, dtype, True, seed=10)
+    check(bench, s, t, idx, lab, 1.7, 0.5, 1.0 / n if dtype != F16 else 1.0, dtype, inplace=True)
+
+
+@pytest.mark.parametrize("dtype,n,v", ROWS)
+def test_many_rows_without_labels(bench, dtype, n, v):
+    """One exponential a value, in place too; entries enough that several waves correct the row before."""
+    s, t, idx, _ = data(n, v, 130, dtype, False, seed=11)
+    idx[:, 1] = 0
+    idx[:, 2] = v - 1
+    check(bench, s, t, idx, None, 1.0, 1.0, 1.0 / n if dtype != F16 else 1.0, dtype, inplace=n in (600, 1900))
+
+
+@pytest.mark.parametrize("dtype,n,v", ROWS)
+@pytest.mark.parametrize("labels", [False, True])
+def test_many_rows_with_f32_grads(bench, dtype, n, v, labels):
+    """Two stored pieces for each one loaded, with one exponential and with two."""
+    s, t, idx, lab = data(n, v, 7, dtype, labels, seed=12)
+    check(bench, s, t, idx, lab, 1.7 if labels else 1.0, 0.5 if labels else 1.0, 1.0, dtype, out=F32)
+
+
+@pytest.mark.parametrize("n,v", [(300, 33001), (600, 16501), (1100, 4203), (1700, 1030), (1900, 301)])
+def test_many_f32_rows_in_place_and_without_labels(bench, n, v):
+    s, t, idx, lab = data(n, v, 9, F32, True, seed=13)
+    check(bench, s, t, idx, lab, 1.7, 0.5, 1.0, F32, inplace=True)
+    check(bench, s, t, idx, None, 1.0, 1.0, 1.0, F32)
