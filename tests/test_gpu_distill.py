@@ -404,6 +404,11 @@ def test_more_rows_than_a_launch_has_threads_for(bench):
     within(got, want, 2 * (v / 256 + 64 + 16) * 2.0 ** -24 * np.array([1 / v, 1 + 1 / v, 1 / v] * 4), "two losses")
 
 
+# Each block of k_distill_rows at rows of an odd length, more of them than blocks:
+# 1024 x 16, 512 x 16, 256 x 16, 256 x 4 and 256 x 1 pieces of 16 bytes.
+ROWS = [(BF16, 300, 66001), (F16, 600, 33003), (BF16, 1100, 8301), (F16, 1700, 2101), (BF16, 1900, 601)]
+
+
 @pytest.mark.parametrize("dtype,n,v", ROWS)
 def test_many_rows_in_place(bench, dtype, n, v):
     """The grad of a row is stored while the next row's logits are fetched."""
