@@ -438,3 +438,35 @@ def test_many_f32_rows_in_place_and_without_labels(bench, n, v):
     s, t, idx, lab = data(n, v, 9, F32, True, seed=13)
     check(bench, s, t, idx, lab, 1.7, 0.5, 1.0, F32, inplace=True)
     check(bench, s, t, idx, None, 1.0, 1.0, 1.0, F32)
+
+
+def inside(bench, a, dtype, skip):
+    """A tensor of a's values that starts `skip` elements into its storage."""
+    L, size = bench.L, np.asarray(a).size
+    store = bench.tensor(np.concatenate([np.full(skip, 5.0), np.ravel(a)]), dtype)
+    t = L.pg_tensor_view(store)
+    bench.frees.append((L.pg_tensor_free, t))
+    i = L.tinfo(t)
+    i.dev += skip * i.elem_size
+    i.numel, i.ndim = size, np.ndim(a)
+    stride = size
+    for d, n in enumerate(np.shape(a)):
+        stride //= n
+        i.shape[d], i.stride[d] = n, stride
+    return t
+
+
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (F16, F16), (BF16, BF16), (BF16, F32)], ids=lambda d: NAMES[d])
+@pytest.mark.parametrize("n,v", [(5, 30), (40, 3001), (3, 70001)])
+@pytest.mark.parametrize("skip", [(1, 1), (3, 0), (0, 5)])
+def test_tensors_that_start_inside_their_storage(bench, dtype, out, n, v, skip):
+    """Logits and grad whose 16-byte pieces fall together, and not."""
+    L, T, alpha = bench.L, 2.0, 0.5
+    s, t, idx, lab = data(n, v, 6, dtype, True, seed=14)
+    cfg = DistillCfg(T, alpha, 1.0)
+    loss, ds = inside(bench, np.full(n, 777.0), F32, 3), inside(bench, np.full((n, v), 777.0), out, skip[1])
+    bench.ok(L.pg_amd_distill(inside(bench, s, dtype, skip[0]), inside(bench, t, F32, 1), inside(bench, idx, F32, 3),
+                              inside(bench, lab, F32, 1), C.byref(cfg), loss, ds))
+    wl, el, wd, ed = model(s, t, idx, lab, T, alpha, 1.0)
+    within(bench.read(loss), wl, el, "loss")
+    within(bench.read(ds), wd, ed + (0 if out == F32 else UNIT[out] * (np.abs(wd) + ed) + TINY[out]), "grad")

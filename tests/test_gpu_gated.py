@@ -403,3 +403,94 @@ def test_more_rows_than_a_launch_has_threads_for_are_refused(bench):
         L.pg_tensor_free(t)
     L.lib.pg_tensor_pool_clear()
     bench.refused(done, "x [M, K]")
+
+
+@pytest.mark.parametrize("k", [4, 8, 16])
+def test_one_tensor_as_both_operands_of_few_rows(bench, k):
+    """Up to 16 rows, where both grads could be one launch: x's is added to W's in the one storage."""
+    L = bench.L
+    r = np.random.default_rng(k)
+    v = rounded(r.standard_normal((k, k)) * 0.4, F16)
+    dh = rounded(r.standard_normal((k, k // 2)), F16)
+    n = bench.var(v)
+    h = bench.node(L.pg_amd_ag_gated16(n, n, None, 3, F16))
+    ref = model(v, v, None, dh, "silu", F16)
+    check(L.value(h), ref["h"], F32, "h")
+    L.pg_amd_backward_from(h, bench.tensor(dh))
+    within(L.grad(n), ref["dx"][0] + ref["dw"][0], ref["dx"][1] + ref["dw"][1] + 2 * F * np.abs(ref["dx"][0] + ref["dw"][0]),
+           "grad")
+
+
+@pytest.mark.parametrize("m,f", [(3, 24), (40, 24), (40, 129)])
+def test_an_empty_reduction(bench, m, f):
+    """x [m, 0]: z is the bias, db what it is for any other layer."""
+    L = bench.L
+    _, _, b, dh = data(m, 1, f, BF16, True, seed=16)
+    nd, sh = shape_arg((m, 0))
+    x, w, dx, dw = (L.pg_tensor_empty_dtype(BF16, *shape_arg(s)) for s in ((m, 0), (0, 2 * f), (m, 0), (0, 2 * f)))
+    if not (x and w and dx and dw):
+        pytest.skip("no tensors without elements")
+    ref = model(np.zeros((m, 0)), np.zeros((0, 2 * f)), b, dh, "gelu", BF16)
+    h, z, db = bench.unset((m, f)), bench.unset((m, 2 * f)), bench.unset((2 * f,))
+    bench.ok(L.pg_amd_gated(x, w, bench.tensor(b), 2, h, z))
+    check(bench.read(z), (np.tile(b, (m, 1)), 0 * ref["z"][1]), F32, "z")
+    check(bench.read(h), ref["h"], F32, "h")
+    bench.ok(L.pg_amd_gated_backward(x, w, z, bench.tensor(dh, BF16), 2, dx, dw, db))
+    check(bench.read(db), ref["db"], F32, "db")
+    for t in (x, w, dx, dw):
+        L.pg_tensor_free(t)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("f", [1, 4, 8])
+def test_narrow_layers_of_many_inputs(bench, dtype, f):
+    """dW of at most 16 columns and 1100 rows, in 16 bits and in f32."""
+    L, m, k = bench.L, 40, 1100
+    x, w, b, dh = data(m, k, f, dtype, True, seed=17)
+    ref = model(x, w, b, dh, "silu", dtype)
+    tx, tw, th = bench.tensor(x, dtype), bench.tensor(w, dtype), bench.tensor(dh, dtype)
+    h, z = bench.unset((m, f), dtype), bench.unset((m, 2 * f))
+    bench.ok(L.pg_amd_gated(tx, tw, bench.tensor(b), 3, h, z))
+    check(bench.read(h), ref["h"], dtype, "h")
+    for gd in (dtype, F32):
+        dx, dw, db = bench.unset((m, k), gd), bench.unset((k, 2 * f), gd), bench.unset((2 * f,))
+        bench.ok(L.pg_amd_gated_backward(tx, tw, z, th, 3, dx, dw, db))
+        check(bench.read(dx), ref["dx"], gd, "dx")
+        check(bench.read(dw), ref["dw"], gd, "dw")
+        check(bench.read(db), ref["db"], F32, "db")
+
+
+def inside(bench, a, dtype, skip):
+    """A tensor of a's values that starts `skip` elements into its storage."""
+    L, size = bench.L, np.asarray(a).size
+    store = bench.tensor(np.concatenate([np.full(skip, 5.0), np.ravel(a)]), dtype)
+    t = L.pg_tensor_view(store)
+    bench.frees.append((L.pg_tensor_free, t))
+    i = L.tinfo(t)
+    i.dev += skip * i.elem_size
+    i.numel, i.ndim = size, np.ndim(a)
+    stride = size
+    for d, n in enumerate(np.shape(a)):
+        stride //= n
+        i.shape[d], i.stride[d] = n, stride
+    return t
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("m,k,f", [(3, 64, 40), (40, 64, 40), (300, 136, 520), (512, 1024, 2048)])
+def test_tensors_that_start_inside_their_storage(bench, dtype, m, k, f):
+    """Operands and outputs none of which starts on 16 bytes."""
+    L = bench.L
+    x, w, b, dh = data(m, k, f, dtype, True, seed=18)
+    ref = model(x, w, b, dh, "silu", dtype)
+    tx, tw, th = (inside(bench, v, dtype, s) for v, s in ((x, 1), (w, 3), (dh, 5)))
+    h, z = inside(bench, np.full((m, f), 777.0), dtype, 7), inside(bench, np.full((m, 2 * f), 777.0), F32, 1)
+    bench.ok(L.pg_amd_gated(tx, tw, inside(bench, b, F32, 1), 3, h, z))
+    check(bench.read(h), ref["h"], dtype, "h")
+    check(bench.read(z), ref["z"], F32, "z")
+    for gd in (dtype, F32):
+        dx, dw, db = (inside(bench, np.full(s, 777.0), d, n) for s, d, n in (((m, k), gd, 3), ((k, 2 * f), gd, 1), (2 * f, F32, 1)))
+        bench.ok(L.pg_amd_gated_backward(tx, tw, z, th, 3, dx, dw, db))
+        check(bench.read(dx), ref["dx"], gd, "dx")
+        check(bench.read(dw), ref["dw"], gd, "dw")
+        check(bench.read(db), ref["db"], F32, "db")

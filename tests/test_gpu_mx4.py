@@ -259,3 +259,39 @@ def test_more_columns_than_a_launch_has_threads_for(bench):
     bench.ok(bench.L.pg_amd_mx4_matmul(x, q, y))
     bench.L.pg_amd_mx4_free(q)
     assert np.array_equal(bench.L.read(y), w)
+
+
+def inside(bench, a, dtype, skip):
+    """A tensor of a's values that starts `skip` elements into its storage."""
+    L, size = bench.L, np.asarray(a).size
+    store = bench.tensor(np.concatenate([np.full(skip, 5.0), np.ravel(a)]), dtype)
+    t = L.pg_tensor_view(store)
+    bench.frees.append((L.pg_tensor_free, t))
+    i = L.tinfo(t)
+    i.dev += skip * i.elem_size
+    i.numel, i.ndim = size, np.ndim(a)
+    stride = size
+    for d, n in enumerate(np.shape(a)):
+        stride //= n
+        i.shape[d], i.stride[d] = n, stride
+    return t
+
+
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F32)], ids=lambda d: NAMES[d])
+@pytest.mark.parametrize("m,k,n", [(3, 256, 64), (100, 256, 64), (1100, 128, 1600)])
+def test_tensors_that_start_inside_their_storage(bench, dtype, out, m, k, n):
+    """Rows whose lengths keep 16 bytes, but not where they start."""
+    L = bench.L
+    g = np.random.default_rng(m)
+    x, w = rounded(g.standard_normal((m, k)), dtype), rounded(g.standard_normal((k, n)), dtype)
+    qx, qw = quantized(x), quantized(w.T).T
+    q, back, y = L.pg_amd_mx4_quantize(inside(bench, w, dtype, 1), 0), inside(bench, np.full((k, n), 777.0), out, 3), inside(
+        bench, np.full((m, n), 777.0), out, 1)
+    bench.ok(L.pg_amd_mx4_dequantize(q, back))
+    bench.ok(L.pg_amd_mx4_matmul(inside(bench, x, dtype, 3), q, y))
+    L.pg_amd_mx4_free(q)
+    within(bench.read(back), rounded(qw, out), 0, "read back")
+    bound = (k + 2) * 2.0 ** -24 * (np.abs(qx) @ np.abs(qw)) + TINY[F32]
+    if out != F32:
+        bound = bound + UNIT[out] * (np.abs(qx @ qw) + bound) + TINY[out]
+    within(bench.read(y), qx @ qw, bound, "y")
