@@ -36,8 +36,9 @@ void pg_amd_release_cached(void);
 
 /* pg_backward() with the root's upstream gradient given explicitly instead
  * of 1 (like torch's backward(gradient)).  seed must have the root value's
- * shape, f32; it is read, not kept, and must stay valid until the stream has
- * run the backward.  The fused loss-suffix JIT does not apply here. */
+ * shape, f32, and may be strided; it is read, not kept, and must stay valid
+ * until the stream has run the backward.  The fused loss-suffix JIT does not
+ * apply here. */
 void pg_amd_backward_from(pg_node *root, const pg_tensor *seed);
 
 /* Mixed-precision matmul of f32 nodes, A [M, K] . B [K, N] -> f32 [M, N],

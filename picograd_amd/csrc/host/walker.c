@@ -669,7 +669,15 @@ void pg_amd_backward_from(pg_node *root, const pg_tensor *seed)
         pga_set_err("pg_amd_backward_from: seed must be f32 with the root's shape");
         return;
     }
+    /* the nodes read their upstream grads in row-major order */
+    pg_tensor *own = NULL;
+    const pg_tensor *rows = pgt_contiguous(seed, &own);
+    if (!rows) {
+        pga_set_err("pg_amd_backward_from: %s", pg_amd_last_error());
+        return;
+    }
     pg_tensor_free(root->grad);
     root->grad = NULL;
-    walk(root, seed, MODE_SEEDED);
+    walk(root, rows, MODE_SEEDED);
+    pg_tensor_free(own);
 }
