@@ -113,14 +113,9 @@ pg_node *pg_var_from_tensor(const pg_tensor *t, bool rg)
 {
     if (!t)
         return NULL;
-    pg_tensor *c = pgt_alloc(t->dtype, t->ndim, t->shape);
-    if (!c)
-        return NULL;
-    if (t->pg_flags & PG_TENSOR_ZERO_PENDING)
-        pg_tensor_fill(c, 0.0f);
-    else
-        pgd_d2d(c->dev, t->dev, t->numel * t->elem_size);
-    return node_wrap(c, rg);
+    /* (also of elements that are strided or not yet written) */
+    pg_tensor *c = pg_tensor_clone(t);
+    return c ? node_wrap(c, rg) : NULL;
 }
 
 pg_node *pg_var_zeros(size_t ndim, const size_t *shape, bool rg) { return node_wrap(pg_tensor_zeros(ndim, shape), rg); }

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from op_tools import Bench
-from picograd_amd.capi import BF16, F16
+from picograd_amd.capi import BF16, F16, F32
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,30 @@ def test_strided_seed(bench, kind):
         bench.L.pg_amd_backward_from(n, t)
         grads.append(bench.L.grad(nx))
     assert np.array_equal(grads[0].view(np.uint32), grads[1].view(np.uint32))
+
+
+@pytest.mark.parametrize("act", [1, 2])
+def test_leaf_of_a_value_not_yet_written(bench, act):
+    """A linear16 layer's output whose elements are pending until they are read."""
+    L = bench.L
+    r = np.random.default_rng(2)
+    n = bench.node(L.pg_amd_ag_linear16(bench.var(r.standard_normal((M, K))), bench.var(r.standard_normal((K, N))), None, act,
+                                        BF16))
+    leaf = bench.node(L.pg_var_from_tensor(L.node(n).value, False))
+    got = L.value(leaf)
+    assert np.array_equal(got.view(np.uint32), L.value(n).view(np.uint32)) and np.abs(got).max() > 0
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_leaf_of_a_strided_tensor(bench, dtype):
+    v = np.arange(M * N, dtype=np.float32).reshape(M, N)
+    leaf = bench.node(bench.L.pg_var_from_tensor(bench.transposed(v, dtype), False))
+    assert np.array_equal(bench.read(bench.L.node(leaf).value), v)
+
+
+def test_leaf_of_a_grad(bench):
+    L = bench.L
+    x = bench.var(np.ones((M, N)))
+    L.pg_backward(bench.node(L.pg_ag_sum_all(x)))
+    leaf = bench.node(L.pg_var_from_tensor(L.node(x).grad, False))
+    assert (L.value(leaf) == 1).all()
