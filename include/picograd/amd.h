@@ -134,8 +134,13 @@ void pg_amd_linear16_narrow(bool on);
  *   dg = dh u act'(g), du = dh act(g), dx = [dg | du] W^T,
  *   dW = x^T [dg | du], db = column sums of [dg | du].
  * The products run on the MFMA units with f32 accumulation; z, act, act' and
- * the column sums are f32; [dg | du] is rounded to the 16-bit type for the
- * two products.  The reference's layers (nn.c:46-125) have no gated form. */
+ * the column sums are f32.  For the two products of the backward [dg | du] is
+ * rounded to the 16-bit type, which makes the grads' error some 1.4 times that of
+ * one rounding; in f16 a value of it past 65504 is then infinite, whatever the
+ * types of dh, dx and dW (scale the loss, or use bf16).  Only with at most 4
+ * rows, or 16 where K F is at most 2^22, does it stay f32.  M is at most 2^31 -
+ * 256, K under 2^30, F under 2^29.  The reference's layers (nn.c:46-125) have no
+ * gated form. */
 #define PG_ACT_SILU 3
 #define PG_ACT_SIGMOID 4
 /* On tensors that the caller holds: x and w of one 16-bit dtype, b f32, h [M,
@@ -166,9 +171,10 @@ pg_node *pg_amd_ag_gated16(pg_node *x, pg_node *w, pg_node *b, int act, pg_dtype
  * for NaN.  The reference has no form below 16 bits. */
 typedef struct pg_amd_mx4 pg_amd_mx4;
 /* t [rows, cols] of any dtype in 4 bits, the blocks along dimension `axis`
- * (0 or 1), which is at most 2^24 long; for the weights [K, N] of a
- * product x W that is 0.  t is read, not kept.  NULL and pg_autograd_last_error() on bad arguments or a device
- * error.  Freed with pg_amd_mx4_free. */
+ * (0 or 1), which is at most 2^24 long, the other under 2^30; for the weights
+ * [K, N] of a product x W that is 0.  t is read, not kept.  NULL and
+ * pg_autograd_last_error() on bad arguments or a device error.  Freed with
+ * pg_amd_mx4_free. */
 pg_amd_mx4 *pg_amd_mx4_quantize(const pg_tensor *t, int axis);
 void pg_amd_mx4_free(pg_amd_mx4 *q);
 /* The device bytes q holds. */
@@ -209,15 +215,17 @@ typedef struct pg_amd_distill_cfg {
  * 1 <= k <= 256; labels [N] f32 or NULL; loss [N] f32, a value per row;
  * dlogits [N, V], of logits' dtype or f32, or NULL for the loss alone.  dlogits
  * may be logits itself: the grad then replaces them.  Otherwise the outputs
- * must not overlap the inputs.  Both are written whole, in one pass over the
- * logits.  Enqueued on the library stream.  false and
- * pg_autograd_last_error() on bad arguments or a device error. */
+ * must not overlap the inputs.  Both are written whole.  The logits are read
+ * once by rows that a block holds (up to 16384 pieces of 16 bytes), twice by
+ * longer ones and by few long rows, which several blocks share.  Enqueued on
+ * the library stream.  false and pg_autograd_last_error() on bad arguments or a
+ * device error. */
 bool pg_amd_distill(const pg_tensor *logits, const pg_tensor *top, const pg_tensor *top_idx, const pg_tensor *labels,
                     const pg_amd_distill_cfg *cfg, pg_tensor *loss, pg_tensor *dlogits);
 /* The loss as a node [1], the sum of the rows': its backward adds the grad to
- * the logits node's.  logits is an f32 node [N, V]; top, top_idx and
- * labels are read again by the backward, so they are kept (retained) and must
- * not change until it has run.  NULL (pg_autograd_last_error) on bad
+ * the logits node's.  logits is an f32 node [N, V]; it, top, top_idx and labels
+ * are read again by the backward, which takes the sums anew, so the last three
+ * are kept (retained) and none may change until it has run.  NULL (pg_autograd_last_error) on bad
  * arguments. */
 pg_node *pg_amd_ag_distill(pg_node *logits, const pg_tensor *top, const pg_tensor *top_idx, const pg_tensor *labels,
                            const pg_amd_distill_cfg *cfg);

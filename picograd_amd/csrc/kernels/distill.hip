@@ -494,8 +494,9 @@ __device__ __forceinline__ void store_chunks(const span<T> &sp, const uint4 (&r)
 // grad's store.  A block takes every gridDim-th row, and each register is
 // refilled from the next row as soon as it has been read for the last time, so
 // that loads are in flight while the grad (or, for the loss alone, the sums)
-// is computed.  The entries of a row are put right one row later: the waits
-// for the refills, which were issued behind the row's stores, order the two.
+// is computed.  The entries of a row are put right one row later, behind that
+// row's barrier: a block's accesses pass its CU's L1 in the order of their issue,
+// so the row's stores, issued before the barrier by any wave, land before these.
 // ONE: the second exponential may be there.  Bound by the stream of the rows in
 // and out: 4096 x 131072 bf16 467 us, 4.6 TB/s, 1000 x 50001 f32 91 us, 4.4 TB/s.
 template <class T, class O, int NT, int PER, bool GRAD, bool ONE>
@@ -683,9 +684,10 @@ __global__ void __launch_bounds__(kPartThreads) k_distill_finish(pgk_distill_arg
 
 constexpr int kStreamThreads = 1024;
 
-// Logits and a grad whose 16-byte chunks do not fall together, a grad that is
-// added to, and rows past what a block holds: one block per row, value by value, the row read once for
-// its stats and once for the grad.
+// Logits and a grad whose 16-byte chunks do not fall together (tensors that start
+// inside their storage), a grad that is added to, and more than 65535 rows past what a
+// block holds: one block per row, value by value, the row read once for its stats and
+// once for the grad.
 template <class T, class O>
 __global__ void __launch_bounds__(kStreamThreads) k_distill_stream(pgk_distill_args a)
 {

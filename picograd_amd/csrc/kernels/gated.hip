@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(256) k_gated_pad(pad_job a, pad_job b, size_t 
 // (TileGate), so its epilogue has g and u of each output and z need not be
 // read back; z itself is written only for a backward.  Tiles and k-loops are
 // the 16-bit GEMM's, and what bounds it is what bounds that: in rounds of full
-// tiles the matrix units (4096 x 4096 x 8192 in bf16 518 us, 1.06 PFLOP/s, z's 268 MB
+// tiles the matrix units (4096 x 4096 x 8192 in bf16 509 us, 1.08 PFLOP/s, z's 268 MB
 // among them), with one round the loads' latency and the epilogue (512 x 1024 x
 // 4096 17 us, 0.5 PFLOP/s).
 template <class CF>
@@ -234,7 +234,8 @@ int launch_forward(int tile, const gemm_kargs &g, hipStream_t s)
 // block: its four waves take every fourth row each, four neighbouring columns a
 // lane, and keep the strip's column sums, joined through LDS in wave order into
 // the block's row of part.  dz is rounded to the operands' 16 bits, in which both
-// products take it; the sums take it before.  Bound by the stream of z and dh in
+// products take it (in f32 the matrix units run at an eighth of the rate, and a dz
+// split into two halves doubles the products); the sums take it before.  Bound by the stream of z and dh in
 // and dz out (4096 x 8192 in bf16: 470 MB in 90 us, 5.2 TB/s).  A piece of four is one load at
 // whatever address an odd f gives it (1023 x 2049: one value a lane took 11 us).
 constexpr int kBwdV = 4;
@@ -351,7 +352,7 @@ void launch_bwd(const bwd_args &a, int dh_dtype, const bwd_plan &p, hipStream_t 
                   : dh_dtype == 1 ? launch_bwd<ACT, _Float16>(a, p, s) : launch_bwd<ACT, __bf16>(a, p, s);
 }
 
-// Up to 16 rows: dz stays in f32 (rounded to 16 bits it is half of the error of so
+// Few rows (pgk_gated_few_grads_ok): dz stays in f32 (rounded to 16 bits it is half of the error of so
 // few sums) and both grads are one launch over the matrices where they lie.
 // One thread per column of f: dz and, over the rows in turn, db.
 template <int ACT, class D>
@@ -633,8 +634,9 @@ extern "C" int pgk_gated_bwd(int act, const void *dh, int dh_dtype, const float 
 }
 
 // Against the 16-bit products, us for k x f in bf16 with 1, 4, 16 rows (those:
-// 17): 64 x 64 6.2, 6.2, 7.8 (10.5), 64 x 8192 16, 16, 19 (36), 1024 x 4096 20, 21,
-// 29 (29), 4096 x 8192 112, 115, 159 (112).
+// 17): 64 x 64 6.1, 6.2, 7.5 (10.5), 64 x 8192 16, 16, 19 (36), 1024 x 4096 20, 21,
+// 29 (28), 4096 x 8192 107, 110, 159 (103).  Up to four rows it is taken at the last
+// sizes too, for the error of so few sums.
 extern "C" int pgk_gated_few_grads_ok(size_t m, size_t k, size_t f)
 {
     return m <= 4 || (m <= 16 && (!k || f <= ((size_t)1 << 22) / k));

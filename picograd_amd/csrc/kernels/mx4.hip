@@ -433,10 +433,11 @@ __global__ void __launch_bounds__(KG * 64, 1) k_mx4_split(pgk_mx4 x, pgk_mx4 w, 
 // set.  A stage is refilled during the step that follows its last read, behind
 // the step's one barrier, so its loads have three steps to land.  Tiles of
 // 128 x 128 on four waves, two blocks to a CU, of which one computes while the
-// other waits at its barrier.  8192 x 4096 x 4096 takes 72 us and the
-// rounding of x 14, 3.8 PFLOP/s of the product where the matrix
+// other waits at its barrier.  8192 x 4096 x 4096 takes 75 us and the
+// rounding of x 14, 3.7 PFLOP/s of the product where the matrix
 // units alone reach 6.0 on random codes; two stages of two steps take 109 and
-// 256 x 256 tiles, whose eight waves run out of registers, 90 to 111.
+// 256 x 256 tiles, whose eight waves run out of registers, 90 to 111.  Bound by
+// LDS: a wave's 64 x 64 reads 8 KB for 16 matrix instructions.
 template <int BM, int BN, int WGM, int WGN, class O>
 __global__ void __launch_bounds__(64 * WGM *WGN, 1) k_mx4_tiles(pgk_mx4 x, pgk_mx4 w, O *__restrict__ y)
 {
