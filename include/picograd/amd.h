@@ -161,6 +161,30 @@ bool pg_amd_gated_backward(const pg_tensor *x, const pg_tensor *w, const pg_tens
  * act. */
 pg_node *pg_amd_ag_gated16(pg_node *x, pg_node *w, pg_node *b, int act, pg_dtype dtype);
 
+/* ---- layer norm ----
+ * Over the last dimension of x [.., D], M rows of D:
+ *   n = (x - mean) rstd, rstd = 1 / sqrt(var + eps), var the mean of (x - mean)^2
+ *   y = n w + b
+ * and with h = dy w:
+ *   dx = rstd (h - mean(h) - n mean(h n)), dw = sum over rows of dy n, db = of dy.
+ * Statistics and sums are f32; y and dx round once.  A row that holds a NaN or an
+ * infinity becomes NaN whole, and so do dw and (where dy is) db.  M is under 2^31, D
+ * from 1 to 2^28, eps finite and at least 0 (with 0 a row of equal values is NaN).
+ * pg_ag_layernorm is the node of it. */
+/* x of any dtype, w and b f32 [D] or NULL (1 and 0), y of x's shape, of its dtype
+ * or f32; y may be x itself.  stats (f32, 2 M elements) receives each row's mean
+ * and rstd for the backward; NULL when there is none (serving).  Inputs may be
+ * strided; outputs are contiguous, written whole and otherwise overlap no input.
+ * Enqueued on the library stream.  false and pg_autograd_last_error() on bad
+ * arguments or a device error. */
+bool pg_amd_layernorm(const pg_tensor *x, const pg_tensor *w, const pg_tensor *b, float eps, pg_tensor *y,
+                      pg_tensor *stats);
+/* The grads for dy (x's shape, of x's dtype or f32), with the stats that
+ * pg_amd_layernorm kept and the x that it read: dx of x's shape, of x's dtype or
+ * f32, dw and db f32 [D]; each may be NULL. */
+bool pg_amd_layernorm_backward(const pg_tensor *x, const pg_tensor *w, const pg_tensor *stats, const pg_tensor *dy,
+                               pg_tensor *dx, pg_tensor *dw, pg_tensor *db);
+
 /* ---- products with matrices held in 4 bits ----
  * A matrix rounded to the values 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives
  * (e2m1) times one power of two for each block of 32 along the dimension that

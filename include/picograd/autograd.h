@@ -11,7 +11,7 @@
  *     synchronised (pg_tensor_sync_host() does that);
  *   - the fused backward covers every maximal chain of elementwise nodes,
  *     GELU/ERF/ABS included, not only the chain under the loss.
- * Ops that are not part of the MI355X build (softmax, norms, conv,
+ * Ops that are not part of the MI355X build (softmax, RMS and batch norm, conv,
  * embedding, dropout, cross-entropy, BCE, pow, transpose) keep their
  * declarations for link compatibility, return NULL and set last_error.
  */
@@ -126,6 +126,9 @@ pg_node *pg_ag_mean_all(pg_node *a);
 
 pg_node *pg_ag_softmax(pg_node *a, size_t axis);
 pg_node *pg_ag_transpose(pg_node *a, size_t axis0, size_t axis1);
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over x's last dimension [D],
+ * var the mean of (x - mean)^2; weight and bias [D], each may be NULL.  f32 nodes,
+ * contiguous; eps >= 0. */
 pg_node *pg_ag_layernorm(pg_node *x, pg_node *weight, pg_node *bias, float eps);
 pg_node *pg_ag_rmsnorm(pg_node *x, pg_node *weight, float eps);
 pg_node *pg_ag_batchnorm(pg_node *x, pg_node *weight, pg_node *bias, float eps);

@@ -100,6 +100,7 @@ _PROTOS = {
     "pg_ag_mse": (vp, [vp, vp, bo]),
     "pg_ag_leaky_relu": (vp, [vp, fl]),
     "pg_ag_clamp": (vp, [vp, fl, fl]),
+    "pg_ag_layernorm": (vp, [vp, vp, vp, fl]),
     "pg_backward": (None, [vp]),
     "pg_backward_jit": (bo, [vp]),
     "pg_autograd_set_jit": (None, [bo]),
@@ -194,6 +195,8 @@ _AMD_PROTOS = {
     "pg_amd_gated": (bo, [vp, vp, vp, ip, vp, vp]),
     "pg_amd_gated_backward": (bo, [vp, vp, vp, vp, ip, vp, vp, vp]),
     "pg_amd_ag_gated16": (vp, [vp, vp, vp, ip, ip]),
+    "pg_amd_layernorm": (bo, [vp, vp, vp, fl, vp, vp]),
+    "pg_amd_layernorm_backward": (bo, [vp, vp, vp, vp, vp, vp, vp]),
     "pg_amd_mx4_quantize": (vp, [vp, ip]),
     "pg_amd_mx4_free": (None, [vp]),
     "pg_amd_mx4_bytes": (sz, [vp]),

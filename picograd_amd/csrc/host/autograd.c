@@ -162,6 +162,8 @@ void pg_node_free(pg_node *n)
             pgo_gated_free_ctx(t->ctx);
         else if (t->backward == pgo_distill_backward)
             pgo_distill_free_ctx(t->ctx);
+        else if (t->backward == pgo_layernorm_backward)
+            pgo_layernorm_free_ctx(t->ctx);
         else
             free(t->ctx);
         if (sp + t->nparents > cap) {
@@ -1275,7 +1277,6 @@ static pg_node *unsupported(const char *what)
 pg_node *pg_ag_pow(pg_node *a, pg_node *b) { (void)a; (void)b; return unsupported("pg_ag_pow"); }
 pg_node *pg_ag_softmax(pg_node *a, size_t axis) { (void)a; (void)axis; return unsupported("pg_ag_softmax"); }
 pg_node *pg_ag_transpose(pg_node *a, size_t x, size_t y) { (void)a; (void)x; (void)y; return unsupported("pg_ag_transpose"); }
-pg_node *pg_ag_layernorm(pg_node *x, pg_node *w, pg_node *b, float e) { (void)x; (void)w; (void)b; (void)e; return unsupported("pg_ag_layernorm"); }
 pg_node *pg_ag_rmsnorm(pg_node *x, pg_node *w, float e) { (void)x; (void)w; (void)e; return unsupported("pg_ag_rmsnorm"); }
 pg_node *pg_ag_batchnorm(pg_node *x, pg_node *w, pg_node *b, float e) { (void)x; (void)w; (void)b; (void)e; return unsupported("pg_ag_batchnorm"); }
 pg_node *pg_ag_batchnorm2d(pg_node *x, pg_node *w, pg_node *b, pg_tensor *rm, pg_tensor *rv, float e, float m, bool t)

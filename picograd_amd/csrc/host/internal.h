@@ -219,6 +219,9 @@ void pgo_gated_backward(pg_node *n);
 void pgo_gated_free_ctx(void *ctx);
 void pgo_distill_backward(pg_node *n);
 void pgo_distill_free_ctx(void *ctx);
+/* pg_ag_layernorm's backward and the destructor of its node context */
+void pgo_layernorm_backward(pg_node *n);
+void pgo_layernorm_free_ctx(void *ctx);
 
 /* ---- operands of the calls that write to tensors of the caller ----
  * t as an input: its elements current and in row-major order (*owned a copy

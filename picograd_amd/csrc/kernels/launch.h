@@ -362,6 +362,36 @@ typedef struct {
 size_t pgk_distill_workspace(const pgk_distill_args *a);
 int pgk_distill(const pgk_distill_args *a, void *ws, pgk_stream s);
 
+/* Layer norm (norm.hip) of the dense rows of x [m, d], d at most PGK_NORM_MAX_D,
+ * m > 0; dtypes 0 = f32, 1 = f16, 2 = bf16, y_dtype, dy_dtype and dx_dtype being
+ * dtype or 0.  w, b [d] f32 or NULL; stats [m, 2] f32: mean and rstd of each row.
+ * pgk_norm: y = (x - mean) rstd w + b (y may be x, of one dtype), stats unless
+ * NULL.  ws: pgk_norm_workspace bytes.
+ * pgk_norm_bwd: from dy and stats dx (NULL: not wanted; beta_x: added to, f32),
+ * dw, db [d] f32 (either NULL; beta_*: added to), which do not overlap.
+ * ws: pgk_norm_bwd_workspace bytes (sums: dw or db is wanted). */
+#define PGK_NORM_MAX_D ((size_t)1 << 28)
+typedef struct {
+    const void *x;
+    int dtype;
+    size_t m, d;
+    const float *w, *b;
+    float eps;
+    void *y;
+    int y_dtype;
+    float *stats;
+    const void *dy;
+    int dy_dtype;
+    void *dx;
+    int dx_dtype, beta_x;
+    float *dw, *db;
+    int beta_w, beta_b;
+} pgk_norm_args;
+size_t pgk_norm_workspace(int dtype, size_t m, size_t d);
+int pgk_norm(const pgk_norm_args *a, void *ws, pgk_stream s);
+size_t pgk_norm_bwd_workspace(int dtype, size_t m, size_t d, int sums);
+int pgk_norm_bwd(const pgk_norm_args *a, void *ws, pgk_stream s);
+
 /* multi-tensor SGD */
 typedef struct {
     float *p;
