@@ -214,6 +214,34 @@ bool pg_amd_mx4_dequantize(const pg_amd_mx4 *q, pg_tensor *out);
  * library stream.  false and pg_autograd_last_error() on failure. */
 bool pg_amd_mx4_matmul(const pg_tensor *x, const pg_amd_mx4 *w, pg_tensor *y);
 
+/* ---- products with matrices held in 8 bits ----
+ * Every line of a matrix along the dimension that a product sums over is rounded
+ * to whole numbers q of -127 .. 127 times a scale of its own: s = max |v| / 127 in
+ * f32, q = v / s to nearest, ties to even (a line whose s is 0 becomes 0).  A line
+ * that holds a NaN or an infinity stands for NaN.  Beside the 4-bit form above it
+ * takes twice the room and rounds some 10 times finer.  The reference has no form
+ * below 16 bits. */
+typedef struct pg_amd_q8 pg_amd_q8;
+/* t [rows, cols] of any dtype in 8 bits, a scale for each line along dimension
+ * `axis` (0 or 1), which is at most 2^17 long, the other under 2^30; for the weights
+ * [K, N] of a product x W that is 0.  t is read, not kept.  NULL and
+ * pg_autograd_last_error() on bad arguments or a device error.  Freed with
+ * pg_amd_q8_free. */
+pg_amd_q8 *pg_amd_q8_quantize(const pg_tensor *t, int axis);
+void pg_amd_q8_free(pg_amd_q8 *q);
+/* The device bytes q holds. */
+size_t pg_amd_q8_bytes(const pg_amd_q8 *q);
+/* out (the shape of q's source, any dtype; rounded to it) = the values that q
+ * stands for.  false and pg_autograd_last_error() on failure. */
+bool pg_amd_q8_dequantize(const pg_amd_q8 *q, pg_tensor *out);
+/* y [M, N] = Q(x) W for x [M, K] of any dtype, each row rounded to 8 bits in the
+ * call as above, and W [K, N] held in 8 bits (axis 0): (sum of qx qw) sx sw, the sum
+ * of whole numbers exact, y (any dtype) rounded from f32.  x may be strided; y is
+ * contiguous, written whole and does not overlap x.  Forward only: for frozen
+ * layers.  Enqueued on the library stream.  false and pg_autograd_last_error() on
+ * failure. */
+bool pg_amd_q8_matmul(const pg_tensor *x, const pg_amd_q8 *w, pg_tensor *y);
+
 /* ---- distillation from a teacher's top logits ----
  * Per row s of the student's logits [N, V], with the teacher's logits t_k at
  * the indices i_k of its top entries and a label:

@@ -202,6 +202,11 @@ _AMD_PROTOS = {
     "pg_amd_mx4_bytes": (sz, [vp]),
     "pg_amd_mx4_dequantize": (bo, [vp, vp]),
     "pg_amd_mx4_matmul": (bo, [vp, vp, vp]),
+    "pg_amd_q8_quantize": (vp, [vp, ip]),
+    "pg_amd_q8_free": (None, [vp]),
+    "pg_amd_q8_bytes": (sz, [vp]),
+    "pg_amd_q8_dequantize": (bo, [vp, vp]),
+    "pg_amd_q8_matmul": (bo, [vp, vp, vp]),
     "pg_amd_distill": (bo, [vp, vp, vp, vp, C.POINTER(DistillCfg), vp, vp]),
     "pg_amd_ag_distill": (vp, [vp, vp, vp, vp, C.POINTER(DistillCfg)]),
     "pg_amd_sgd_buffer": (vp, [vp, sz]),

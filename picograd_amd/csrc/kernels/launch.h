@@ -362,6 +362,34 @@ typedef struct {
 size_t pgk_distill_workspace(const pgk_distill_args *a);
 int pgk_distill(const pgk_distill_args *a, void *ws, pgk_stream s);
 
+/* 8-bit matrices (q8.hip): whole numbers of -127 .. 127 at rows of ld bytes (cols
+ * rounded up to 128, zeros behind the end), a scale per row; cols, along the
+ * reduction, at most PGK_Q8_MAX_K (32 bits hold its sums), rows under 2^30, both
+ * positive */
+#define PGK_Q8_MAX_K ((size_t)1 << 17)
+typedef struct {
+    size_t rows, cols, ld;
+    int8_t *codes;
+    float *scale;
+} pgk_q8;
+/* sets rows, cols and ld; the byte sizes of codes and scale */
+void pgk_q8_shape(pgk_q8 *q, size_t rows, size_t cols, size_t *code_bytes, size_t *scale_bytes);
+/* q = src, dense of dtype 0 = f32, 1 = f16, 2 = bf16: [rows, cols], or with `trans`
+ * [cols, rows]; ws: pgk_q8_workspace bytes */
+size_t pgk_q8_workspace(const pgk_q8 *q, int trans);
+int pgk_q8_quantize(const pgk_q8 *q, const void *src, int dtype, int trans, void *ws, pgk_stream s);
+/* dst (dense, as src above) = the values q stands for */
+int pgk_q8_dequantize(const pgk_q8 *q, void *dst, int dtype, int trans, pgk_stream s);
+/* y [x->rows, w->rows] of y_dtype = x w^T over their shared cols; _few: for the m
+ * that pgk_q8_few_rows takes, x in 8 bits (xq), or with xq NULL dense of dtype, [m,
+ * w->cols], rounded in the launch (by every block: pgk_q8_few_fused says where that
+ * is faster) */
+int pgk_q8_few_rows(size_t m);
+int pgk_q8_few_fused(size_t m, size_t k);
+int pgk_q8_matmul_few(const void *x, int dtype, const pgk_q8 *xq, size_t m, const pgk_q8 *w, void *y, int y_dtype,
+                      pgk_stream s);
+int pgk_q8_matmul(const pgk_q8 *x, const pgk_q8 *w, void *y, int y_dtype, pgk_stream s);
+
 /* Layer norm (norm.hip) of the dense rows of x [m, d], d at most PGK_NORM_MAX_D,
  * m > 0; dtypes 0 = f32, 1 = f16, 2 = bf16, y_dtype, dy_dtype and dx_dtype being
  * dtype or 0.  w, b [d] f32 or NULL; stats [m, 2] f32: mean and rstd of each row.
