@@ -255,7 +255,11 @@ def _prepare_own(s) -> None:
             s.tensor("w%d" % i, v["w%d" % i])
             n = L._check(L.pg_var_from_tensor(s.t["w%d" % i], True))
             s.frees.append((L.pg_node_free, n))
-            L.pg_amd_backward_from(n, s.t["g%d" % i])  # the node's grad
+            zero = L._check(L.pg_var_scalar(0.0, False))
+            loss = L.op("add", n, zero)
+            L.pg_amd_backward_from(loss, s.t["g%d" % i])  # the node's grad
+            for node in (loss, zero):
+                L.pg_node_free(node)
             if L.pg_amd_muon_add_param(s.opt, n) != 0:
                 raise RuntimeError(L.pg_autograd_last_error().decode())
             s.out["w%d" % i] = s.view(L.node(n).value, shape)
