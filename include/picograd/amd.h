@@ -282,6 +282,68 @@ bool pg_amd_distill(const pg_tensor *logits, const pg_tensor *top, const pg_tens
 pg_node *pg_amd_ag_distill(pg_node *logits, const pg_tensor *top, const pg_tensor *top_idx, const pg_tensor *labels,
                            const pg_amd_distill_cfg *cfg);
 
+/* ---- orthogonalised updates ----
+ * The orthogonal factor of a matrix G by Newton-Schulz products, its singular
+ * values taken towards 1 with their directions kept: X = G / ||G||_F, then `steps`
+ * times X <- a X + (b S + c S S) X with S = X X^T (of a G with more rows than
+ * columns the transpose is taken) and (a, b, c) = (3.4445, -4.7750, 2.0315).  After
+ * 5 steps singular values over some 1/500 of the norm lie between 0.6 and 1.21.
+ * The norm is summed in 64 bits; the products run on the f16 MFMA units from two
+ * pieces of each operand, which keeps them as exact as f32 ones.  G of zeros gives
+ * zeros, one that holds a NaN or an infinity NaN whole. */
+/* g [K, N] of any dtype, sides of 1 to 2^16; out of g's shape, any dtype, rounded
+ * to it once; steps 1 to 100.  g may be strided; out is contiguous, written whole
+ * and may be g itself, otherwise it does not overlap g.  Enqueued on the library
+ * stream.  false and pg_autograd_last_error() on bad arguments or a device error. */
+bool pg_amd_orthogonalise(const pg_tensor *g, int steps, pg_tensor *out);
+
+/* The optimiser that steps along the orthogonal factor of the momentum (Muon), for
+ * weight matrices W [K, N] beside pg_sgd or pg_adam for the other parameters:
+ *   m <- momentum m + g, u = nesterov ? g + momentum m : m, O = factor of u
+ *   W <- (1 - lr weight_decay) W - lr size O
+ * with size = sqrt(max(1, N / K)), or rms sqrt(max(K, N)) where rms > 0 (entries of
+ * an update then have about that root mean square). */
+typedef struct {
+    float lr, momentum, weight_decay; /* at least 0 */
+    float rms;                        /* at least 0 */
+    int steps;                        /* of the factor, 1 to 100 */
+    bool nesterov;
+} pg_amd_muon_cfg;
+/* lr 0.02, momentum 0.95, no decay, rms 0, 5 steps, nesterov */
+pg_amd_muon_cfg pg_amd_muon_cfg_default(void);
+typedef struct pg_amd_muon pg_amd_muon;
+/* a NULL cfg takes the defaults; NULL (pg_autograd_last_error) for values out of
+ * range */
+pg_amd_muon *pg_amd_muon_new(const pg_amd_muon_cfg *cfg);
+void pg_amd_muon_free(pg_amd_muon *opt);
+/* Retains a node that requires grads and whose value is a contiguous f32 matrix
+ * with sides of 1 to 2^16; with momentum its buffer is made here, zero.  0, or -1
+ * (pg_autograd_last_error) otherwise, also for a value that overlaps an earlier
+ * parameter's. */
+int pg_amd_muon_add_param(pg_amd_muon *opt, pg_node *param);
+size_t pg_amd_muon_num_params(const pg_amd_muon *opt);
+/* The momentum of the i-th parameter, owned by the optimiser; NULL without momentum
+ * or for i out of range. */
+pg_tensor *pg_amd_muon_buffer(pg_amd_muon *opt, size_t i);
+bool pg_amd_muon_set_lr(pg_amd_muon *opt, float lr);
+float pg_amd_muon_get_lr(const pg_amd_muon *opt);
+/* frees the grads, as pg_sgd_zero_grad does */
+void pg_amd_muon_zero_grad(pg_amd_muon *opt);
+/* Steps every parameter that has a grad, up to 12 of them in shared launches, and
+ * rewrites kept 16-bit copies with them; workspace of some 16 bytes per element
+ * comes from the allocator's cache.  Enqueued on the library stream.  false and
+ * pg_autograd_last_error() on a grad of another shape (nothing is stepped) or a
+ * device error. */
+bool pg_amd_muon_step(pg_amd_muon *opt);
+/* The momenta as "PGMU", u32 version 1, u64 nparams, per parameter u32 has_buf (0
+ * or 1) then the buffer's PGT1 record when has_buf.  load_into is for an optimiser
+ * of the same parameters (count and shapes checked, false on a mismatch); one saved
+ * without momentum is zero afterwards. */
+bool pg_amd_muon_save(const pg_amd_muon *opt, const char *path);
+bool pg_amd_muon_save_fp(const pg_amd_muon *opt, FILE *fp);
+bool pg_amd_muon_load_into(pg_amd_muon *opt, const char *path);
+bool pg_amd_muon_load_into_fp(pg_amd_muon *opt, FILE *fp);
+
 /* The 16-bit operand copies of matmul16 (pg_amd_ag_matmul16) written by the
  * fused elementwise kernels beside their f32 outputs, in place of a cast
  * pass over them: a deferred forward run whose output a matmul16 takes as

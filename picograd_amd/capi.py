@@ -66,6 +66,11 @@ class DistillCfg(C.Structure):
     _fields_ = [("temperature", C.c_float), ("alpha", C.c_float), ("scale", C.c_float)]
 
 
+class MuonCfg(C.Structure):
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("rms", C.c_float),
+                ("steps", C.c_int), ("nesterov", C.c_bool)]
+
+
 vp, sz, fl, bo, ip = C.c_void_p, C.c_size_t, C.c_float, C.c_bool, C.c_int
 SZP = C.POINTER(C.c_size_t)
 
@@ -209,6 +214,19 @@ _AMD_PROTOS = {
     "pg_amd_q8_matmul": (bo, [vp, vp, vp]),
     "pg_amd_distill": (bo, [vp, vp, vp, vp, C.POINTER(DistillCfg), vp, vp]),
     "pg_amd_ag_distill": (vp, [vp, vp, vp, vp, C.POINTER(DistillCfg)]),
+    "pg_amd_orthogonalise": (bo, [vp, ip, vp]),
+    "pg_amd_muon_cfg_default": (MuonCfg, []),
+    "pg_amd_muon_new": (vp, [C.POINTER(MuonCfg)]),
+    "pg_amd_muon_free": (None, [vp]),
+    "pg_amd_muon_add_param": (ip, [vp, vp]),
+    "pg_amd_muon_num_params": (sz, [vp]),
+    "pg_amd_muon_buffer": (vp, [vp, sz]),
+    "pg_amd_muon_set_lr": (bo, [vp, fl]),
+    "pg_amd_muon_get_lr": (fl, [vp]),
+    "pg_amd_muon_zero_grad": (None, [vp]),
+    "pg_amd_muon_step": (bo, [vp]),
+    "pg_amd_muon_save": (bo, [vp, C.c_char_p]),
+    "pg_amd_muon_load_into": (bo, [vp, C.c_char_p]),
     "pg_amd_sgd_buffer": (vp, [vp, sz]),
     "pg_tensor_clone": (vp, [vp]),
     "pg_tensor_view": (vp, [vp]),

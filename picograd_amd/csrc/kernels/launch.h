@@ -460,6 +460,31 @@ typedef struct {
 } pgk_adam_hyper;
 int pgk_adam_multi(const pgk_adam_seg *segs, int nseg, const pgk_adam_hyper *h, pgk_stream s);
 
+/* Orthogonal factors by Newton-Schulz products (muon.hip) of up to PGK_MUON_MAX
+ * matrices in as many launches as one takes; sides from 1 to PGK_MUON_MAX_SIDE */
+#define PGK_MUON_MAX 12
+#define PGK_MUON_MAX_SIDE ((size_t)1 << 16)
+typedef struct {
+    size_t rows, cols;
+    const void *g; /* dense */
+    int g_dtype;   /* 0 = f32, 1 = f16, 2 = bf16 */
+    /* gclip (f32): g is read as (g * gmul) * ginv (a pending clip-by-norm scale) */
+    int gclip;
+    float gmul, ginv;
+    float *m; /* momentum (f32 g): m = mu m + g, and g + mu m (nesterov) or m is factored; NULL: g is */
+    void *out; /* the factor, of out_dtype; unused with w */
+    int out_dtype;
+    float *w; /* w = decay w - step factor; NULL: out is written */
+    float decay, step;
+    uint16_t *shadow; /* optional 16-bit copy of w, as pgk_sgd_seg's */
+    int shadow_dtype;
+    size_t shadow_cols, shadow_ld;
+} pgk_muon_seg;
+size_t pgk_muon_workspace(const pgk_muon_seg *segs, int n);
+/* outputs, momenta and shadows of different matrices must not overlap; out may be
+ * g.  ws: _workspace bytes */
+int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov, int steps, void *ws, pgk_stream s);
+
 /* gradient clipping over a list of f32 grads (optim.hip) */
 typedef struct {
     float *g;

@@ -169,13 +169,13 @@ __device__ __forceinline__ void piece_loop(const piece_operand &A, const piece_o
     __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(0)); // the loads past the end land before the LDS is used anew
 }
 
-// The sums' way out: 32 rows of each wave's tile at a time through LDS; f(row,
-// column, four neighbouring sums) for every row < M and column < N (a multiple
-// of 4 behind n0), or with `down` the same four sums down a column, f(row, column)
-// naming the first.  Both orders of a pass see one barrier.
+// The sums' way out: 32 rows of each wave's tile at a time through LDS.  f(row,
+// column, v, false) takes four neighbouring sums of a row, for every row < M and
+// column < N (a multiple of 4 behind n0), and may change them; with `down`
+// f(row, column, v, true) then takes what it left, four down a column.
 template <class CF, class V4, class FN_>
 __device__ __forceinline__ void piece_out(typename CF::ACC (&acc)[CF::FM][CF::FN], int m0, int n0, int M, int N,
-                                          LDS uint4 *const lds, bool across, bool down, FN_ f)
+                                          LDS uint4 *const lds, bool down, FN_ f)
 {
     constexpr int RS = CF::RS, WN = CF::WN, CL = WN / 4;
     typedef LDS int *lds_int;
@@ -194,22 +194,26 @@ __device__ __forceinline__ void piece_out(typename CF::ACC (&acc)[CF::FM][CF::FN
                 reg[((e >> 2) * 8 + lk * 4 + (e & 3)) * RS + j * 32 + lrow] = __builtin_bit_cast(int, one);
             }
         __syncthreads();
-        const int row0 = m0 + wm * CF::WM + i * 32;
-        if (across) {
-            const int c4 = (lane % CL) * 4;
+        const int row0 = m0 + wm * CF::WM + i * 32, c4 = (lane % CL) * 4;
 #pragma unroll 1
-            for (int r = lane / CL; r < 32; r += 64 / CL)
-                if (row0 + r < M && col0 + c4 < N)
-                    f(row0 + r, col0 + c4, __builtin_bit_cast(V4, *(const LDS i32x4 *)(reg + r * RS + c4)), false);
-        }
+        for (int r = lane / CL; r < 32; r += 64 / CL)
+            if (row0 + r < M && col0 + c4 < N) {
+                LDS i32x4 *const at = (LDS i32x4 *)(reg + r * RS + c4);
+                V4 v = __builtin_bit_cast(V4, *at);
+                f(row0 + r, col0 + c4, v, false);
+                if (down)
+                    *at = __builtin_bit_cast(i32x4, v);
+            }
         if (down) {
+            __syncthreads();
             const int r4 = (lane & 7) * 4;
 #pragma unroll 1
             for (int c = lane >> 3; c < WN; c += 8) {
                 if (row0 + r4 >= M || col0 + c >= N)
                     continue;
-                const i32x4 v = {reg[r4 * RS + c], reg[(r4 + 1) * RS + c], reg[(r4 + 2) * RS + c], reg[(r4 + 3) * RS + c]};
-                f(row0 + r4, col0 + c, __builtin_bit_cast(V4, v), true);
+                const i32x4 q = {reg[r4 * RS + c], reg[(r4 + 1) * RS + c], reg[(r4 + 2) * RS + c], reg[(r4 + 3) * RS + c]};
+                V4 v = __builtin_bit_cast(V4, q);
+                f(row0 + r4, col0 + c, v, true);
             }
         }
     }
