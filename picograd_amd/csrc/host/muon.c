@@ -26,8 +26,13 @@ static bool run(const char *what, const pgk_muon_seg *segs, size_t n, float mu, 
 {
     for (size_t i = 0; i < n;) {
         size_t k = 1, wb = pgk_muon_workspace(segs + i, 1);
-        while (i + k < n && k < PGK_MUON_MAX && wb + pgk_muon_workspace(segs + i + k, 1) <= MOST_WORKSPACE)
-            wb += pgk_muon_workspace(segs + i + k++, 1);
+        while (i + k < n && k < PGK_MUON_MAX) {
+            const size_t more = pgk_muon_workspace(segs + i, (int)k + 1);
+            if (more > MOST_WORKSPACE)
+                break;
+            wb = more;
+            k++;
+        }
         pgk_stream st = pgd_stream();
         void *ws = pgd_malloc(wb);
         const bool ok = ws && pgd_check(pgk_muon(segs + i, (int)k, mu, nesterov, steps, ws, st), what);

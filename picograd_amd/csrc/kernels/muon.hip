@@ -26,6 +26,7 @@
 #include <math.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "launch.h"
 #include "piece_tile.h"
@@ -46,13 +47,18 @@ struct ns_prob {
     int m, n, mp, np, parts;
     uint32_t per_part; // elements
 };
+// Tiles are numbered through all matrices; those from `whole` on are split along
+// the reduction in z slices, whose sums go to partial and are joined by a launch of
+// their own
 struct ns_table {
-    int n;
+    int n, whole, z;
+    float *partial;
     int first[kMost + 1]; // blocks
     ns_prob p[kMost];
 };
 struct seg_table {
-    int n;
+    int n, whole, z;
+    float *partial;
     int first[kMost + 1];
     float mu;
     int nesterov;
@@ -71,14 +77,46 @@ __device__ __forceinline__ int which(const TAB &t, int block)
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-__device__ __forceinline__ float grad_at(const pgk_muon_seg &s, size_t i)
+// n (1 to 4) neighbours of the grad from element i
+__device__ __forceinline__ void grad4(const pgk_muon_seg &s, size_t i, int n, float (&g)[4])
 {
+    auto from = [&](auto *p) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+        typedef T v4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        if (n == 4) {
+            const v4 v = *(const v4 *)(p + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                g[e] = (float)v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                g[e] = e < n ? (float)p[i + e] : 0.0f;
+        }
+    };
     if (s.g_dtype == 1)
-        return (float)((const _Float16 *)s.g)[i];
-    if (s.g_dtype == 2)
-        return (float)((const __bf16 *)s.g)[i];
-    const float g = ((const float *)s.g)[i];
-    return s.gclip ? g * s.gmul * s.ginv : g;
+        from((const _Float16 *)s.g);
+    else if (s.g_dtype == 2)
+        from((const __bf16 *)s.g);
+    else
+        from((const float *)s.g);
+    if (s.gclip)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            g[e] = g[e] * s.gmul * s.ginv; // as a pending scale is written
+}
+__device__ __forceinline__ void momentum4(const float *p, int n, float (&m)[4])
+{
+    if (n == 4) {
+        const f32x4u v = *(const f32x4u *)p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            m[e] = v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            m[e] = e < n ? p[e] : 0.0f;
+    }
 }
 
 // The momentum, and the blocks' sums of u's squares in 64 bits.
@@ -91,14 +129,29 @@ __global__ void __launch_bounds__(256) k_ns_size(seg_table t)
     const size_t n = s.rows * s.cols, begin = (size_t)part * p.per_part;
     const size_t end = begin + p.per_part < n ? begin + p.per_part : n;
     double sum = 0.0;
-    for (size_t i = begin + tid; i < end; i += 256) {
-        float u = grad_at(s, i);
+#pragma unroll 2
+    for (size_t i = begin + tid * 4; i < end; i += 1024) {
+        const int some = end - i < 4 ? (int)(end - i) : 4;
+        float u[4], m[4];
+        grad4(s, i, some, u);
         if (s.m) {
-            const float g = u, m = t.mu * s.m[i] + g;
-            s.m[i] = m;
-            u = t.nesterov ? g + t.mu * m : m;
+            momentum4(s.m + i, some, m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m[e] = t.mu * m[e] + u[e];
+                u[e] = t.nesterov ? u[e] + t.mu * m[e] : m[e];
+            }
+            if (some == 4)
+                *(f32x4u *)(s.m + i) = f32x4u{m[0], m[1], m[2], m[3]};
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < some)
+                        s.m[i + e] = m[e];
         }
-        sum += (double)u * (double)u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            sum += (double)u[e] * (double)u[e];
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
@@ -142,35 +195,52 @@ __global__ void __launch_bounds__(256) k_ns_start(seg_table t)
     sum = sums[0] + sums[1] + sums[2] + sums[3];
     const double scale = sum == 0.0 ? 0.0 : (double)kUnit / sqrt(sum);
     const bool tall = s.rows > s.cols;
-    const int c = tid & 63;
-#pragma unroll 4
-    for (int r = tid >> 6; r < 64; r += 4) {
-        // row and column of u
-        const int row = (tall ? j0 : i0) + r, col = (tall ? i0 : j0) + c;
-        float x = 0.0f;
-        if ((size_t)row < s.rows && (size_t)col < s.cols) {
-            const size_t i = (size_t)row * s.cols + col;
-            float u;
-            if (s.m)
-                u = t.nesterov ? grad_at(s, i) + t.mu * s.m[i] : s.m[i];
-            else
-                u = grad_at(s, i);
-            x = (float)((double)u * scale);
-        }
-        tile[tall ? c : r][tall ? r : c] = x;
-    }
-    __syncthreads();
     const size_t plane = (size_t)p.mp * p.np;
-#pragma unroll
-    for (int r = tid >> 4; r < 64; r += 16) {
-        const int c4 = (tid & 15) * 4;
+    auto put = [&](int r, int c4, const float (&x)[4]) { // four neighbours of X
         uint16_t h[4], l[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            pieces(tile[r][c4 + e], h[e], l[e]);
+            pieces(x[e], h[e], l[e]);
         uint16_t *const d = p.x + (size_t)(i0 + r) * p.np + j0 + c4;
         *(uint2 *)d = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
         *(uint2 *)(d + plane) = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
+    };
+    const int c4 = (tid & 15) * 4;
+#pragma unroll
+    for (int r = tid >> 4; r < 64; r += 16) {
+        // row and columns of u
+        const int row = (tall ? j0 : i0) + r, col = (tall ? i0 : j0) + c4;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if ((size_t)row < s.rows && (size_t)col < s.cols) {
+            const size_t i = (size_t)row * s.cols + col;
+            const int some = s.cols - col < 4 ? (int)(s.cols - col) : 4;
+            float m[4];
+            if (!s.m || t.nesterov)
+                grad4(s, i, some, x);
+            if (s.m) {
+                momentum4(s.m + i, some, m);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[e] = t.nesterov ? x[e] + t.mu * m[e] : m[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[e] = (float)((double)x[e] * scale);
+        }
+        if (tall)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                tile[c4 + e][r] = x[e];
+        else
+            put(r, c4, x);
+    }
+    if (!tall)
+        return;
+    __syncthreads();
+#pragma unroll
+    for (int r = tid >> 4; r < 64; r += 16) {
+        const float x[4] = {tile[r][c4], tile[r][c4 + 1], tile[r][c4 + 2], tile[r][c4 + 3]};
+        put(r, c4, x);
     }
 }
 
@@ -222,7 +292,7 @@ __device__ __forceinline__ void finish4(const pgk_muon_seg &s, size_t i, const f
         }
 }
 
-enum { NS_S = 0, NS_B = 1, NS_X = 2 };
+enum { NS_S = 0, NS_B = 1, NS_X = 2, NS_LAST = 3 };
 
 // row and column of tile i of a lower triangle, row by row
 __device__ __forceinline__ void triangle(int i, int &r, int &c)
@@ -235,41 +305,40 @@ __device__ __forceinline__ void triangle(int i, int &r, int &c)
     c = i - r * (r + 1) / 2;
 }
 
-// One product for every matrix: S, B or the next X.
+// tile `at` of a matrix: its first row and column
 template <class CF, int WHAT>
-__global__ void __launch_bounds__(CF::NT, 1) k_ns_product(ns_table t)
+__device__ __forceinline__ void tile_of(const ns_prob &p, int at, int &m0, int &n0)
 {
-    __shared__ uint4 smem[CF::LDS_U4];
-    LDS uint4 *const lds = (LDS uint4 *)smem;
-    const int pid = xcd_tile((int)blockIdx.x, (int)gridDim.x);
-    const ns_prob &p = t.p[which(t, pid)];
-    const int at = pid - t.first[which(t, pid)];
-    const size_t px = (size_t)p.mp * p.np, ps = (size_t)p.mp * p.mp;
-    f32x16 acc[CF::FM][CF::FN];
-    if constexpr (WHAT == NS_X) {
+    if constexpr (WHAT == NS_S || WHAT == NS_B) {
+        triangle(at, m0, n0);
+        m0 *= CF::BM;
+        n0 *= CF::BN;
+    } else { // eight tile-rows at a time
         const int tiles_m = (p.mp + CF::BM - 1) / CF::BM, tiles_n = (p.np + CF::BN - 1) / CF::BN;
         const int per_group = 8 * tiles_n, group = at / per_group, first = group * 8;
         const int gsz = tiles_m - first < 8 ? tiles_m - first : 8, in = at - group * per_group;
-        const int m0 = (first + in % gsz) * CF::BM, n0 = in / gsz * CF::BN;
-        piece_loop<CF>({p.b, (size_t)p.mp, ps, p.mp}, {p.x, (size_t)p.np, px, p.np}, p.mp, m0, n0, lds, acc);
-        piece_out<CF, f32x4>(acc, m0, n0, p.mp, p.np, lds, false, [&](int row, int col, f32x4 &v, bool) {
-            float x[4];
-            load4(p.x + (size_t)row * p.np + col, px, x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = kA * x[e] + v[e] * (1.0f / kUnit);
-            store4(p.to + (size_t)row * p.np + col, px, v);
-        });
-    } else {
-        int r, c;
-        triangle(at, r, c);
-        const int m0 = r * CF::BM, n0 = c * CF::BN;
-        if constexpr (WHAT == NS_S)
-            piece_loop<CF>({p.x, (size_t)p.np, px, p.mp}, {p.x, (size_t)p.np, px, p.mp}, p.np, m0, n0, lds, acc);
-        else
-            piece_loop<CF>({p.s, (size_t)p.mp, ps, p.mp}, {p.s, (size_t)p.mp, ps, p.mp}, p.mp, m0, n0, lds, acc);
+        m0 = (first + in % gsz) * CF::BM;
+        n0 = in / gsz * CF::BN;
+    }
+}
+
+// the reduction of a product
+template <int WHAT>
+__device__ __forceinline__ int depth_of(const ns_prob &p)
+{
+    return WHAT == NS_S ? p.np : p.mp;
+}
+
+// strip i of the tile at (m0, n0): what becomes of the sums
+template <class CF, int WHAT, class TAB>
+__device__ __forceinline__ void strip_out(const TAB &t, int k, f32x16 (&acc)[CF::FN], int i, int m0, int n0,
+                                          LDS uint4 *const lds)
+{
+    const ns_prob &p = t.p[k];
+    const size_t px = (size_t)p.mp * p.np, ps = (size_t)p.mp * p.mp;
+    if constexpr (WHAT == NS_S || WHAT == NS_B) {
         uint16_t *const to = WHAT == NS_S ? p.s : p.b;
-        piece_out<CF, f32x4>(acc, m0, n0, p.mp, p.mp, lds, r != c, [&](int row, int col, f32x4 &v, bool mirror) {
+        piece_out_strip<CF, f32x4>(acc, i, m0, n0, p.mp, p.mp, lds, m0 != n0, [&](int row, int col, f32x4 &v, bool mirror) {
             if (mirror) {
                 store4(to + (size_t)col * p.mp + row, ps, v);
                 return;
@@ -284,47 +353,140 @@ __global__ void __launch_bounds__(CF::NT, 1) k_ns_product(ns_table t)
             }
             store4(to + (size_t)row * p.mp + col, ps, v);
         });
+    } else {
+        bool tall = false; // only the last X is written as u lies
+        if constexpr (WHAT == NS_LAST)
+            tall = t.seg[k].rows > t.seg[k].cols;
+        piece_out_strip<CF, f32x4>(acc, i, m0, n0, p.mp, p.np, lds, tall, [&](int row, int col, f32x4 &v, bool mirror) {
+            if (!mirror) {
+                float x[4];
+                load4(p.x + (size_t)row * p.np + col, px, x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = kA * x[e] + v[e] * (1.0f / kUnit);
+            }
+            if constexpr (WHAT == NS_X) {
+                store4(p.to + (size_t)row * p.np + col, px, v);
+            } else {
+                if (mirror != tall || row >= p.m || col >= p.n)
+                    return;
+                const int left = tall ? p.m - row : p.n - col;
+                finish4(t.seg[k], tall ? (size_t)col * p.m + row : (size_t)row * p.n + col, v, left < 4 ? left : 4);
+            }
+        });
     }
 }
 
-// The last X, straight to where it goes.
+// a slice's part of a tile's sums, in the order in which the lanes hold them
 template <class CF>
-__global__ void __launch_bounds__(CF::NT, 1) k_ns_last(seg_table t)
+__device__ __forceinline__ f32x4 *partial_at(float *p, size_t unit, int i, int j)
+{
+    const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
+    return (f32x4 *)p + ((unit * (CF::NT / 64) + wave) * (CF::FM * CF::FN) + i * CF::FN + j) * 256 + lane;
+}
+
+// One product for every matrix: S, B, the next X or the last.  The 256 x 256 tiles of
+// 4096 x 4096 run at 1300 TFLOP/s of the three f16 products, where a large f16
+// product alone reaches 1060 on the same card: a k-step's three products share
+// the operands of two, so less is moved for each.  Bound by the matrix units at the
+// clock that they hold.
+template <class CF, int WHAT, class TAB>
+__global__ void __launch_bounds__(CF::NT, 1) k_ns_product(TAB t)
 {
     __shared__ uint4 smem[CF::LDS_U4];
     LDS uint4 *const lds = (LDS uint4 *)smem;
-    const int pid = xcd_tile((int)blockIdx.x, (int)gridDim.x), k = which(t, pid), at = pid - t.first[k];
+    int tile = (int)blockIdx.x, slice = 0;
+    const bool split = tile >= t.whole;
+    if (split) {
+        const int r = tile - t.whole;
+        tile = t.whole + r / t.z;
+        slice = r % t.z;
+    } else { // neighbours on one XCD, within what the chip runs at a time
+        constexpr int round = CF::BM == 256 ? 256 : 512;
+        const int first = tile / round * round, left = t.whole - first;
+        tile = first + xcd_tile(tile - first, left < round ? left : round);
+    }
+    const int k = which(t, tile);
     const ns_prob &p = t.p[k];
-    const pgk_muon_seg &s = t.seg[k];
     const size_t px = (size_t)p.mp * p.np, ps = (size_t)p.mp * p.mp;
-    const int tiles_m = (p.mp + CF::BM - 1) / CF::BM, tiles_n = (p.np + CF::BN - 1) / CF::BN;
-    const int per_group = 8 * tiles_n, group = at / per_group, first = group * 8;
-    const int gsz = tiles_m - first < 8 ? tiles_m - first : 8, in = at - group * per_group;
-    const int m0 = (first + in % gsz) * CF::BM, n0 = in / gsz * CF::BN;
-    const bool tall = s.rows > s.cols;
-    f32x16 acc[CF::FM][CF::FN];
-    piece_loop<CF>({p.b, (size_t)p.mp, ps, p.mp}, {p.x, (size_t)p.np, px, p.np}, p.mp, m0, n0, lds, acc);
-    piece_out<CF, f32x4>(acc, m0, n0, p.mp, p.np, lds, tall, [&](int row, int col, f32x4 &v, bool mirror) {
-        if (!mirror) {
-            float x[4];
-            load4(p.x + (size_t)row * p.np + col, px, x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = kA * x[e] + v[e] * (1.0f / kUnit);
-        }
-        if (mirror != tall || row >= p.m || col >= p.n)
+    int m0, n0;
+    tile_of<CF, WHAT>(p, tile - t.first[k], m0, n0);
+    int begin = 0, end = depth_of<WHAT>(p);
+    if (split) {
+        const int kt = end / CF::KB;
+        begin = kt * slice / t.z * CF::KB;
+        end = kt * (slice + 1) / t.z * CF::KB;
+        if (begin == end) // fewer tiles of the reduction than slices
             return;
-        const int left = tall ? p.m - row : p.n - col;
-        finish4(s, tall ? (size_t)col * p.m + row : (size_t)row * p.n + col, v, left < 4 ? left : 4);
-    });
+    }
+    f32x16 acc[CF::FM][CF::FN];
+    if constexpr (WHAT == NS_S)
+        piece_loop<CF>({p.x, (size_t)p.np, px, p.mp}, {p.x, (size_t)p.np, px, p.mp}, begin, end - begin, m0, n0, lds, acc);
+    else if constexpr (WHAT == NS_B)
+        piece_loop<CF>({p.s, (size_t)p.mp, ps, p.mp}, {p.s, (size_t)p.mp, ps, p.mp}, begin, end - begin, m0, n0, lds, acc);
+    else
+        piece_loop<CF>({p.b, (size_t)p.mp, ps, p.mp}, {p.x, (size_t)p.np, px, p.np}, begin, end - begin, m0, n0, lds, acc);
+    if (split) {
+        const size_t unit = blockIdx.x - t.whole;
+#pragma unroll
+        for (int i = 0; i < CF::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < CF::FN; ++j) {
+                f32x4 *const to = partial_at<CF>(t.partial, unit, i, j);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    to[q * 64] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < CF::FM; ++i)
+        strip_out<CF, WHAT>(t, k, acc[i], i, m0, n0, lds);
+}
+
+// The slices of split tiles joined in their order, a strip a block.
+template <class CF, int WHAT, class TAB>
+__global__ void __launch_bounds__(CF::NT, 1) k_ns_join(TAB t)
+{
+    __shared__ uint4 smem[CF::OUT_U4];
+    LDS uint4 *const lds = (LDS uint4 *)smem;
+    const int r = (int)blockIdx.x / CF::FM, i = (int)blockIdx.x % CF::FM, tile = t.whole + r, k = which(t, tile);
+    const ns_prob &p = t.p[k];
+    int m0, n0;
+    tile_of<CF, WHAT>(p, tile - t.first[k], m0, n0);
+    const int kt = depth_of<WHAT>(p) / CF::KB;
+    f32x16 acc[CF::FN];
+#pragma unroll
+    for (int j = 0; j < CF::FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            acc[j][e] = 0.0f;
+    for (int s = 0; s < t.z; ++s) {
+        if (kt * s / t.z == kt * (s + 1) / t.z)
+            continue;
+#pragma unroll
+        for (int j = 0; j < CF::FN; ++j) {
+            const f32x4 *const from = partial_at<CF>(t.partial, (size_t)r * t.z + s, i, j);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = from[q * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[j][4 * q + e] += v[e];
+            }
+        }
+    }
+    strip_out<CF, WHAT>(t, k, acc, i, m0, n0, lds);
 }
 
 // ---------------------------------------------------------------- launches
 
 template <bool TB>
+using T256 = pcfg<f32x16, 2, 256, 256, 2, 4, TB, 32, 2>;
+template <bool TB>
 using T128 = pcfg<f32x16, 2, 128, 128, 2, 2, TB, 32, 2>;
 template <bool TB>
-using T64 = pcfg<f32x16, 2, 64, 64, 2, 2, TB, 32, 2>;
+using T64 = pcfg<f32x16, 2, 64, 64, 2, 2, TB, 64, 2>;
 
 size_t up64(size_t v) { return (v + 63) & ~(size_t)63; }
 
@@ -341,19 +503,6 @@ void shape(const pgk_muon_seg &s, ns_prob *p)
     p->per_part = (uint32_t)per;
     p->parts = (int)((all + per - 1) / per);
 }
-size_t bytes_of(const ns_prob &p)
-{
-    return ((size_t)p.mp * p.np * 2 + (size_t)p.mp * p.mp * 2) * 4 + kMostParts * sizeof(double);
-}
-
-// tiles of a side: below the diagonal, or all of X
-template <class CF>
-int tiles(const ns_prob &p, bool sym)
-{
-    const int r = (p.mp + CF::BM - 1) / CF::BM;
-    return sym ? r * (r + 1) / 2 : r * ((p.np + CF::BN - 1) / CF::BN);
-}
-
 template <class TAB, class FN>
 int number(TAB &t, FN blocks)
 {
@@ -366,36 +515,120 @@ int number(TAB &t, FN blocks)
     return all;
 }
 
-template <class TAB, template <bool> class CF, bool TB>
-int total(TAB &t, bool sym)
+// tiles of a side: below the diagonal, or all of X
+int tiles_of(const ns_prob &p, int what, int side)
 {
-    return number(t, [&](const ns_prob &p) { return tiles<CF<TB>>(p, sym); });
+    const int r = (p.mp + side - 1) / side;
+    return what == NS_S || what == NS_B ? r * (r + 1) / 2 : r * ((p.np + side - 1) / side);
 }
 
-template <int WHAT>
-int product(ns_table &t, hipStream_t st)
+// How a product of all matrices is cut.  Whole rounds of tiles over the chip run
+// as they are; what is left, less than a round, is split along the reduction
+// where that is faster.  The time of 32 along the reduction was measured with one
+// block on a CU and with as many as fit (two of 128 and 64), in us: 1.7 and 2.4 for a
+// side of 256, 0.76 and 1.4 for 128, 0.36 and 0.44 for 64; a joining launch takes
+// some 5 us and the partial sums' way at 3.5 TB/s.  1024 x 4096, S: 36 tiles of 128
+// in 7 slices 22 us, whole 81; 64: 46.
+struct ns_plan {
+    int side, whole, z, tiles;
+};
+ns_plan plan_of(const ns_prob *p, int n, int what)
 {
-    constexpr bool TB = WHAT == NS_X, sym = !TB;
-    const int big = total<ns_table, T128, TB>(t, sym);
-    if (big >= 256) {
-        hipLaunchKernelGGL((k_ns_product<T128<TB>, WHAT>), dim3((unsigned)big), dim3(T128<TB>::NT), 0, st, t);
-    } else {
-        const int n = total<ns_table, T64, TB>(t, sym);
-        hipLaunchKernelGGL((k_ns_product<T64<TB>, WHAT>), dim3((unsigned)n), dim3(T64<TB>::NT), 0, st, t);
+    static const struct {
+        int side, blocks;
+        double alone, full;
+    } kinds[3] = {{256, 1, 1.7, 2.4}, {128, 2, 0.76, 1.4}, {64, 2, 0.36, 0.44}};
+    ns_plan best = {};
+    double least = 0.0;
+    for (const auto &c : kinds) {
+        int tiles = 0;
+        double work = 0.0; // of the reduction, in 32s
+        for (int i = 0; i < n; ++i) {
+            tiles += tiles_of(p[i], what, c.side);
+            work += (double)tiles_of(p[i], what, c.side) * ((what == NS_S ? p[i].np : p[i].mp) / 32);
+        }
+        const int slots = 256 * c.blocks, whole = tiles / slots * slots, rest = tiles - whole;
+        // the longest reduction among the last tiles
+        int depth = 0;
+        double left = 0.0;
+        for (int i = n - 1, seen = 0; i >= 0 && seen < rest; --i) {
+            const int t = tiles_of(p[i], what, c.side), d = (what == NS_S ? p[i].np : p[i].mp) / 32;
+            left += (double)(t < rest - seen ? t : rest - seen) * d;
+            depth = d > depth ? d : depth;
+            seen += t;
+        }
+        for (int z = 1; rest ? z <= 16 && rest * z <= slots && (z == 1 || depth / z >= 4) : z == 1; ++z) {
+            const int units = rest * z;
+            const double steps = (double)((depth + z - 1) / z);
+            double time = (work - left) / slots * c.full;
+            if (rest)
+                time += 2.0 + steps * (units <= 256 ? c.alone + (c.full / c.blocks - c.alone) * (c.blocks == 1 ? units / 256.0 : 0.0)
+                                                    : c.full);
+            if (z > 1)
+                time += 5.0 + units * (double)c.side * c.side * 8.0 / 3.5e6;
+            if (!best.side || time < least) {
+                least = time;
+                best = {c.side, z == 1 ? tiles : whole, z, tiles};
+            }
+        }
     }
+    return best;
+}
+size_t partial_bytes(const ns_plan &q) { return (size_t)(q.tiles - q.whole) * q.z * q.side * q.side * sizeof(float); }
+
+template <template <bool> class TILE, int WHAT, class TAB>
+int launch(TAB &t, const ns_plan &q, hipStream_t st)
+{
+    using CF = TILE<(WHAT == NS_X || WHAT == NS_LAST)>;
+    number(t, [&](const ns_prob &p) { return tiles_of(p, WHAT, q.side); });
+    t.whole = q.whole;
+    t.z = q.z;
+    const int rest = q.tiles - q.whole;
+    hipLaunchKernelGGL((k_ns_product<CF, WHAT, TAB>), dim3((unsigned)(q.whole + rest * q.z)), dim3(CF::NT), 0, st, t);
+    if (rest)
+        hipLaunchKernelGGL((k_ns_join<CF, WHAT, TAB>), dim3((unsigned)(rest * CF::FM)), dim3(CF::NT), 0, st, t);
     return (int)hipGetLastError();
 }
 
-int last(seg_table &t, hipStream_t st)
+template <int WHAT, class TAB>
+int product(TAB &t, hipStream_t st)
 {
-    const int big = total<seg_table, T128, true>(t, false);
-    if (big >= 256) {
-        hipLaunchKernelGGL((k_ns_last<T128<true>>), dim3((unsigned)big), dim3(T128<true>::NT), 0, st, t);
-    } else {
-        const int n = total<seg_table, T64, true>(t, false);
-        hipLaunchKernelGGL((k_ns_last<T64<true>>), dim3((unsigned)n), dim3(T64<true>::NT), 0, st, t);
+    const ns_plan q = plan_of(t.p, t.n, WHAT);
+    return q.side == 256 ? launch<T256, WHAT>(t, q, st) : q.side == 128 ? launch<T128, WHAT>(t, q, st) : launch<T64, WHAT>(t, q, st);
+}
+
+// the matrices' own places and the partial sums'
+size_t places(ns_prob *p, int n, char *at, float **partial)
+{
+    char *const begin = at;
+    size_t most = 0;
+    for (int what = NS_S; what <= NS_X; ++what) {
+        const size_t b = partial_bytes(plan_of(p, n, what));
+        most = b > most ? b : most;
     }
-    return (int)hipGetLastError();
+    *partial = (float *)at;
+    at += most;
+    for (int i = 0; i < n; ++i) {
+        const size_t px = (size_t)p[i].mp * p[i].np * 4, ps = (size_t)p[i].mp * p[i].mp * 4;
+        p[i].x = (uint16_t *)at;
+        p[i].to = (uint16_t *)(at + px);
+        p[i].s = (uint16_t *)(at + 2 * px);
+        p[i].b = (uint16_t *)(at + 2 * px + ps);
+        p[i].part = (double *)(at + 2 * px + 2 * ps);
+        at += 2 * px + 2 * ps + kMostParts * sizeof(double);
+    }
+    return (size_t)(at - begin);
+}
+
+// the largest first, so that the tiles left over are the shortest
+void order(ns_prob *p, pgk_muon_seg *seg, int n)
+{
+    for (int i = 1; i < n; ++i)
+        for (int j = i; j > 0 && (size_t)p[j].mp * p[j].np > (size_t)p[j - 1].mp * p[j - 1].np; --j) {
+            std::swap(p[j], p[j - 1]);
+            if (seg)
+                std::swap(seg[j], seg[j - 1]);
+        }
 }
 
 bool fits(const pgk_muon_seg &s)
@@ -407,13 +640,14 @@ bool fits(const pgk_muon_seg &s)
 
 extern "C" size_t pgk_muon_workspace(const pgk_muon_seg *segs, int n)
 {
-    size_t all = 0;
-    for (int i = 0; i < n; ++i) {
-        ns_prob p;
-        shape(segs[i], &p);
-        all += bytes_of(p);
-    }
-    return all;
+    if (n < 1 || n > kMost)
+        return 0;
+    ns_prob p[kMost];
+    for (int i = 0; i < n; ++i)
+        shape(segs[i], &p[i]);
+    order(p, NULL, n);
+    float *partial;
+    return places(p, n, NULL, &partial);
 }
 
 extern "C" int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov, int steps, void *ws, pgk_stream s)
@@ -426,21 +660,14 @@ extern "C" int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov,
     t.n = n;
     t.mu = mu;
     t.nesterov = nesterov;
-    char *at = (char *)ws;
     for (int i = 0; i < n; ++i) {
         if (!fits(segs[i]))
             return (int)hipErrorInvalidValue;
         t.seg[i] = segs[i];
-        ns_prob &p = t.p[i];
-        shape(segs[i], &p);
-        const size_t px = (size_t)p.mp * p.np * 4, ps = (size_t)p.mp * p.mp * 4;
-        p.x = (uint16_t *)at;
-        p.to = (uint16_t *)(at + px);
-        p.s = (uint16_t *)(at + 2 * px);
-        p.b = (uint16_t *)(at + 2 * px + ps);
-        p.part = (double *)(at + 2 * px + 2 * ps);
-        at += bytes_of(p);
+        shape(segs[i], &t.p[i]);
     }
+    order(t.p, t.seg, n);
+    places(t.p, n, (char *)ws, &t.partial);
     int blocks = number(t, [](const ns_prob &p) { return p.parts; });
     hipLaunchKernelGGL(k_ns_size, dim3((unsigned)blocks), dim3(256), 0, st, t);
     if (const int rc = (int)hipGetLastError())
@@ -451,6 +678,7 @@ extern "C" int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov,
         return rc;
     ns_table q = {};
     q.n = n;
+    q.partial = t.partial;
     for (int i = 0; i < n; ++i)
         q.p[i] = t.p[i];
     for (int k = 0; k < steps; ++k) {
@@ -470,5 +698,5 @@ extern "C" int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov,
     }
     for (int i = 0; i < n; ++i)
         t.p[i] = q.p[i];
-    return last(t, st);
+    return product<NS_LAST>(t, st);
 }

@@ -45,21 +45,26 @@ struct piece_operand {
     int ext;
 };
 
-// The sums of the tile at (m0, n0) over K, a positive multiple of KB.  The ring of
-// S stages works as the 16-bit products' (gemm16_block): a tile's last k-step
-// starts behind the one barrier of the tile, refills the stage that every wave
-// has read and reads the next tile's first operands, in slots between the
-// matrix instructions.  LDS is free again afterwards (behind a barrier).
+// The sums of the tile at (m0, n0) over [k0, k0 + K), both multiples of KB, K
+// positive.  The ring of S stages works as the 16-bit products' (gemm16_block): one
+// barrier a tile, behind which the stage that every wave has read is refilled and
+// the next tile's first operands are read, in slots between the matrix
+// instructions.  LDS is free again afterwards (behind a barrier).
+//
+// One piece: a k-step's operands are read a step ahead into a second set.  Two
+// pieces: its three products run one after the other, Ah Bh beside which Al is read,
+// Ah Bl, Al Bh, and the next step's Bh, Ah and Bl are read as soon as the last
+// product with the ones that they replace is issued; only Bh has a second set.  In
+// a tile's last step the barrier stands behind the first product.
 template <class CF>
-__device__ __forceinline__ void piece_loop(const piece_operand &A, const piece_operand &B, int K, int m0, int n0,
+__device__ __forceinline__ void piece_loop(const piece_operand &A, const piece_operand &B, int k0, int K, int m0, int n0,
                                            LDS uint4 *const lds, typename CF::ACC (&acc)[CF::FM][CF::FN])
 {
     constexpr int P = CF::P, BM = CF::BM, BN = CF::BN, WM = CF::WM, WN = CF::WN, KB = CF::KB, S = CF::S, NT = CF::NT;
     constexpr int FM = CF::FM, FN = CF::FN, SA = CF::SA, SB = CF::SB;
     using OA = TileK<BM, NT, KB>;
     using OB = typename std::conditional<CF::TB, TileMN<BN, NT, KB>, TileK<BN, NT, KB>>::type;
-    constexpr int LPT = P * (OA::NQ + OB::NQ), KS = KB / 16;
-    constexpr int NP = P == 1 ? 1 : 3, NM = NP * FM * FN, NF = P * (FM + FN); // products and operands of a k-step
+    constexpr int LPT = P * (OA::NQ + OB::NQ), KS = KB / 16, NM = FM * FN;
     static_assert(P == 1 || P == 2, "one piece or two");
     static_assert(S >= 2 && KS % 2 == 0, "two or more stages, an even number of k-steps per tile");
     static_assert((S - 1) * LPT < 64, "the loads in flight fit the vmcnt counter");
@@ -77,13 +82,13 @@ __device__ __forceinline__ void piece_loop(const piece_operand &A, const piece_o
     for (int q = 0; q < OB::NQ; ++q)
         fB[q] = OB::fast_q(q, B.ld, n0, B.ext, wave, lane);
     auto dma = [&](int q, int t, int st) {
-        const int k0 = (t < KT ? t : KT - 1) * KB; // stages past the end are read by none
+        const int k = k0 + (t < KT ? t : KT - 1) * KB; // stages past the end are read by none
         if (q < P * OA::NQ) {
             const int p = q / OA::NQ, i = q % OA::NQ;
-            OA::load_fast(i, fA[i], A.p + p * A.plane, A.ld, m0, k0, stA(st, p), wave);
+            OA::load_fast(i, fA[i], A.p + p * A.plane, A.ld, m0, k, stA(st, p), wave);
         } else {
             const int p = (q - P * OA::NQ) / OB::NQ, i = (q - P * OA::NQ) % OB::NQ;
-            OB::load_fast(i, fB[i], B.p + p * B.plane, B.ld, n0, k0, stB(st, p), wave);
+            OB::load_fast(i, fB[i], B.p + p * B.plane, B.ld, n0, k, stB(st, p), wave);
         }
     };
     auto sync_tile = [&](auto newer) { // all but the newest tiles' loads have landed, every wave has read its operands
@@ -92,14 +97,14 @@ __device__ __forceinline__ void piece_loop(const piece_operand &A, const piece_o
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
     };
-    uint4 fa[2][P][FM], fb[2][P][FN];
-    // operand r of k-step s of the tile in stage st
-    auto read = [&](int r, int st, int s, int to) {
-        if (r < P * FM)
-            fa[to][r / FM][r % FM] = OA::frag(stA(st, r / FM), wm * WM + (r % FM) * 32, s, lane);
-        else
-            fb[to][(r - P * FM) / FN][(r - P * FM) % FN] =
-                OB::frag(stB(st, (r - P * FM) / FN), wn * WN + ((r - P * FM) % FN) * 32, s, lane);
+    auto fragA = [&](int st, int p, int i, int s) { return OA::frag(stA(st, p), wm * WM + i * 32, s, lane); };
+    auto fragB = [&](int st, int p, int j, int s) { return OB::frag(stB(st, p), wn * WN + j * 32, s, lane); };
+    // part g of n of `all` things, in slots between the matrix instructions
+    auto slots = [&](int g, int n, int all, auto f) {
+#pragma unroll
+        for (int r = g * all / n; r < (g + 1) * all / n; ++r)
+            f(r);
+        __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -108,52 +113,97 @@ __device__ __forceinline__ void piece_loop(const piece_operand &A, const piece_o
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 acc[i][j][e] = 0;
-    // k-step s; `next`: k-step ns of the tile in stage nst is read beside it;
-    // `tail`: tile `reload` goes to stage rst
-    auto step = [&](int s, bool next, int nst, int ns, bool tail, int reload, int rst) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int pr = 0; pr < NP; ++pr)
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    acc[i][j] = piece_mma(fa[s & 1][pr == 2][i], fb[s & 1][pr == 1][j], acc[i][j]);
-                    const int g = (pr * FM + i) * FN + j;
-                    if (next) {
-#pragma unroll
-                        for (int r = g * NF / NM; r < (g + 1) * NF / NM; ++r)
-                            read(r, nst, ns, (s + 1) & 1);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    if (tail) {
-#pragma unroll
-                        for (int q = g * LPT / NM; q < (g + 1) * LPT / NM; ++q)
-                            dma(q, reload, rst);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    auto head = [&](int st) {
-#pragma unroll
-        for (int s = 0; s < KS - 1; ++s)
-            step(s, true, st, s + 1, false, 0, 0);
-    };
 #pragma unroll
     for (int t = 0; t < S; ++t)
 #pragma unroll
         for (int q = 0; q < LPT; ++q)
             dma(q, t, t);
     sync_tile(std::integral_constant<int, S - 1>{});
+    // ah, al: A's pieces; bh: B's high piece of even and odd steps (with one piece,
+    // ah and al those of even and odd steps); bl: B's low piece
+    uint4 ah[FM], al[FM], bh[2][FN], bl[FN];
 #pragma unroll
-    for (int r = 0; r < NF; ++r)
-        read(r, 0, 0, 0);
+    for (int i = 0; i < FM; ++i)
+        ah[i] = fragA(0, 0, i, 0);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        bh[0][j] = fragB(0, 0, j, 0);
+        if constexpr (P == 2)
+            bl[j] = fragB(0, 1, j, 0);
+    }
+    // k-step s of the tile in stage st; `next`: the operands of step ns of the tile in
+    // stage nst are read beside it; `tail`: its barrier, and tile `reload` to stage st
+    auto step = [&](int s, int st, bool next, int nst, int ns, bool tail, int reload) {
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (P == 1) {
+            if (tail)
+                sync_tile(std::integral_constant<int, S - 2>{});
+            uint4(&a)[FM] = s & 1 ? al : ah;
+            uint4(&na)[FM] = s & 1 ? ah : al;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    acc[i][j] = piece_mma(a[i], bh[s & 1][j], acc[i][j]);
+                    if (next)
+                        slots(i * FN + j, NM, FM + FN, [&](int r) {
+                            if (r < FM)
+                                na[r] = fragA(nst, 0, r, ns);
+                            else
+                                bh[s + 1 & 1][r - FM] = fragB(nst, 0, r - FM, ns);
+                        });
+                    if (tail)
+                        slots(i * FN + j, NM, LPT, [&](int q) { dma(q, reload, st); });
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    acc[i][j] = piece_mma(ah[i], bh[s & 1][j], acc[i][j]);
+                    slots(i * FN + j, NM, FM, [&](int r) { al[r] = fragA(st, 1, r, s); });
+                }
+            if (tail)
+                sync_tile(std::integral_constant<int, S - 2>{});
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    acc[i][j] = piece_mma(ah[i], bl[j], acc[i][j]);
+                    const int g = i * FN + j;
+                    if (next)
+                        slots(g, NM, FN, [&](int r) { bh[s + 1 & 1][r] = fragB(nst, 0, r, ns); });
+                    if (tail)
+                        slots(g, 2 * NM, LPT, [&](int q) { dma(q, reload, st); });
+                }
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    acc[i][j] = piece_mma(al[i], bh[s & 1][j], acc[i][j]);
+                    const int g = i * FN + j;
+                    if (next)
+                        slots(g, NM, FM + FN, [&](int r) {
+                            if (r < FM)
+                                ah[r] = fragA(nst, 0, r, ns);
+                            else
+                                bl[r - FM] = fragB(nst, 1, r - FM, ns);
+                        });
+                    if (tail)
+                        slots(NM + g, 2 * NM, LPT, [&](int q) { dma(q, reload, st); });
+                }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto head = [&](int st) {
+#pragma unroll
+        for (int s = 0; s < KS - 1; ++s)
+            step(s, st, true, st, s + 1, false, 0);
+    };
     head(0);
-    // the tail of tile t in stage u and the head of tile t + 1
+    // the last step of tile t in stage u and the others of tile t + 1
     auto link = [&](int t, int u) {
-        sync_tile(std::integral_constant<int, S - 2>{});
-        step(KS - 1, true, (u + 1) % S, 0, true, t + S, u);
+        step(KS - 1, u, true, (u + 1) % S, 0, true, t + S);
         head((u + 1) % S);
     };
     int t = 0;
@@ -165,17 +215,17 @@ __device__ __forceinline__ void piece_loop(const piece_operand &A, const piece_o
     for (int u = 0; u < S - 1; ++u)
         if (t + u < KT - 1)
             link(t + u, u);
-    step(KS - 1, false, 0, 0, false, 0, 0);
+    step(KS - 1, (KT - 1) % S, false, 0, 0, false, 0);
     __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(0)); // the loads past the end land before the LDS is used anew
 }
 
-// The sums' way out: 32 rows of each wave's tile at a time through LDS.  f(row,
-// column, v, false) takes four neighbouring sums of a row, for every row < M and
-// column < N (a multiple of 4 behind n0), and may change them; with `down`
+// The way out of strip i of the sums, 32 rows of each wave's tile, through LDS.
+// f(row, column, v, false) takes four neighbouring sums of a row, for every row <
+// M and column < N (a multiple of 4 behind n0), and may change them; with `down`
 // f(row, column, v, true) then takes what it left, four down a column.
 template <class CF, class V4, class FN_>
-__device__ __forceinline__ void piece_out(typename CF::ACC (&acc)[CF::FM][CF::FN], int m0, int n0, int M, int N,
-                                          LDS uint4 *const lds, bool down, FN_ f)
+__device__ __forceinline__ void piece_out_strip(typename CF::ACC (&acc)[CF::FN], int i, int m0, int n0, int M, int N,
+                                                LDS uint4 *const lds, bool down, FN_ f)
 {
     constexpr int RS = CF::RS, WN = CF::WN, CL = WN / 4;
     typedef LDS int *lds_int;
@@ -183,40 +233,45 @@ __device__ __forceinline__ void piece_out(typename CF::ACC (&acc)[CF::FM][CF::FN
     const int lrow = lane & 31, lk = lane >> 5;
     const lds_int reg = (lds_int)lds + wave * 32 * RS;
     const int col0 = n0 + wn * WN;
+    __syncthreads(); // the stages' (or the previous strip's) reads are done
 #pragma unroll
-    for (int i = 0; i < CF::FM; ++i) {
-        __syncthreads(); // the stages' (or the previous pass's) reads are done
+    for (int j = 0; j < CF::FN; ++j)
 #pragma unroll
-        for (int j = 0; j < CF::FN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const auto one = acc[i][j][e]; // (a bit cast of a vector's element itself takes its first)
-                reg[((e >> 2) * 8 + lk * 4 + (e & 3)) * RS + j * 32 + lrow] = __builtin_bit_cast(int, one);
-            }
+        for (int e = 0; e < 16; ++e) {
+            const auto one = acc[j][e]; // (a bit cast of a vector's element itself takes its first)
+            reg[((e >> 2) * 8 + lk * 4 + (e & 3)) * RS + j * 32 + lrow] = __builtin_bit_cast(int, one);
+        }
+    __syncthreads();
+    const int row0 = m0 + wm * CF::WM + i * 32, c4 = (lane % CL) * 4;
+#pragma unroll 1
+    for (int r = lane / CL; r < 32; r += 64 / CL)
+        if (row0 + r < M && col0 + c4 < N) {
+            LDS i32x4 *const at = (LDS i32x4 *)(reg + r * RS + c4);
+            V4 v = __builtin_bit_cast(V4, *at);
+            f(row0 + r, col0 + c4, v, false);
+            if (down)
+                *at = __builtin_bit_cast(i32x4, v);
+        }
+    if (down) {
         __syncthreads();
-        const int row0 = m0 + wm * CF::WM + i * 32, c4 = (lane % CL) * 4;
+        const int r4 = (lane & 7) * 4;
 #pragma unroll 1
-        for (int r = lane / CL; r < 32; r += 64 / CL)
-            if (row0 + r < M && col0 + c4 < N) {
-                LDS i32x4 *const at = (LDS i32x4 *)(reg + r * RS + c4);
-                V4 v = __builtin_bit_cast(V4, *at);
-                f(row0 + r, col0 + c4, v, false);
-                if (down)
-                    *at = __builtin_bit_cast(i32x4, v);
-            }
-        if (down) {
-            __syncthreads();
-            const int r4 = (lane & 7) * 4;
-#pragma unroll 1
-            for (int c = lane >> 3; c < WN; c += 8) {
-                if (row0 + r4 >= M || col0 + c >= N)
-                    continue;
-                const i32x4 q = {reg[r4 * RS + c], reg[(r4 + 1) * RS + c], reg[(r4 + 2) * RS + c], reg[(r4 + 3) * RS + c]};
-                V4 v = __builtin_bit_cast(V4, q);
-                f(row0 + r4, col0 + c, v, true);
-            }
+        for (int c = lane >> 3; c < WN; c += 8) {
+            if (row0 + r4 >= M || col0 + c >= N)
+                continue;
+            const i32x4 q = {reg[r4 * RS + c], reg[(r4 + 1) * RS + c], reg[(r4 + 2) * RS + c], reg[(r4 + 3) * RS + c]};
+            V4 v = __builtin_bit_cast(V4, q);
+            f(row0 + r4, col0 + c, v, true);
         }
     }
+}
+template <class CF, class V4, class FN_>
+__device__ __forceinline__ void piece_out(typename CF::ACC (&acc)[CF::FM][CF::FN], int m0, int n0, int M, int N,
+                                          LDS uint4 *const lds, bool down, FN_ f)
+{
+#pragma unroll
+    for (int i = 0; i < CF::FM; ++i)
+        piece_out_strip<CF, V4>(acc[i], i, m0, n0, M, N, lds, down, f);
 }
 
 } // namespace

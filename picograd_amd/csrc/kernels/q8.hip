@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(CF::NT, 1) k_q8_tiles(pgk_q8 x, pgk_q8 w, O *_
     const int gsz = tiles_m - first < 8 ? tiles_m - first : 8, in = pid - group * per_group;
     const int m0 = (first + in % gsz) * CF::BM, n0 = in / gsz * CF::BN;
     i32x16 acc[CF::FM][CF::FN];
-    piece_loop<CF>({(const uint16_t *)x.codes, x.ld / 2, 0, M}, {(const uint16_t *)w.codes, w.ld / 2, 0, N}, (int)(x.ld / 2),
+    piece_loop<CF>({(const uint16_t *)x.codes, x.ld / 2, 0, M}, {(const uint16_t *)w.codes, w.ld / 2, 0, N}, 0, (int)(x.ld / 2),
                    m0, n0, lds, acc);
     piece_out<CF, i32x4>(acc, m0, n0, M, N, lds, false, [&](int row, int col, const i32x4 &v, bool) {
         const float sx = x.scale[row];
