@@ -34,8 +34,8 @@ static bool run(const char *what, const pgk_muon_seg *segs, size_t n, float mu, 
             k++;
         }
         pgk_stream st = pgd_stream();
-        void *ws = pgd_malloc(wb);
-        const bool ok = ws && pgd_check(pgk_muon(segs + i, (int)k, mu, nesterov, steps, ws, st), what);
+        void *ws = wb ? pgd_malloc(wb) : NULL;
+        const bool ok = (ws || !wb) && pgd_check(pgk_muon(segs + i, (int)k, mu, nesterov, steps, ws, st), what);
         if (ws)
             pgd_free(ws, wb); /* in stream order */
         if (!ok) {

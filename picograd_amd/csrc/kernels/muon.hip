@@ -25,6 +25,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(CF::NT, 1) k_ns_product(TAB t)
         tile = t.whole + r / t.z;
         slice = r % t.z;
     } else { // neighbours on one XCD, within what the chip runs at a time
-        constexpr int round = CF::BM == 256 ? 256 : 512;
+        constexpr int round = CF::BM == 64 ? 512 : 256;
         const int first = tile / round * round, left = t.whole - first;
         tile = first + xcd_tile(tile - first, left < round ? left : round);
     }
@@ -479,12 +480,170 @@ __global__ void __launch_bounds__(CF::NT, 1) k_ns_join(TAB t)
     strip_out<CF, WHAT>(t, k, acc, i, m0, n0, lds);
 }
 
+// ---------------------------------------------------------------- small matrices, a block each
+
+// Short sides of up to 64, long ones of up to NP: everything in LDS, X as rows of
+// both sides so that each product's operands lie along its reduction.  Sixteen
+// waves, one 16 x 16 tile of S and B each.  Bound by the chain of dependent
+// products: 64 x 64 in five steps takes 15 of them, where launches of their own
+// take 4 us each.
+constexpr int kSmallM = 64, kSmallN = 256;
+
+__device__ __forceinline__ f32x4 mma16(const uint4 &a, const uint4 &b, const f32x4 &c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <int NP>
+__global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
+{
+    constexpr int M = kSmallM, PX = NP + 8, PM = M + 8, T = NP / 64; // pitches; tiles of X per wave
+    constexpr int XP = M * PX, YP = NP * PM, SP = M * PM;            // a piece of X, of its transpose, of S
+    __shared__ uint4 mem[(2 * XP + 2 * YP + 2 * SP) / 8];
+    __shared__ double sums[16];
+    uint16_t *const X = (uint16_t *)mem, *const Y = X + 2 * XP, *const S = Y + 2 * YP;
+    const pgk_muon_seg &s = t.seg[blockIdx.x];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
+    const int rows = (int)s.rows, cols = (int)s.cols;
+    const bool tall = rows > cols;
+    for (int i = tid; i < (2 * XP + 2 * YP) / 8; i += 1024)
+        mem[i] = make_uint4(0, 0, 0, 0);
+    // up to four pieces of four values a thread
+    const int per = (cols + 3) / 4;
+    float u[4][4];
+    double sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int at = tid + q * 1024, row = at / per, col = (at - row * per) * 4;
+        if (row >= rows)
+            break;
+        const size_t i = (size_t)row * cols + col;
+        const int some = cols - col < 4 ? cols - col : 4;
+        grad4(s, i, some, u[q]);
+        if (s.m) {
+            float m[4];
+            momentum4(s.m + i, some, m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m[e] = t.mu * m[e] + u[q][e];
+                u[q][e] = t.nesterov ? u[q][e] + t.mu * m[e] : m[e];
+                if (e < some)
+                    s.m[i + e] = m[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            sum += (double)u[q][e] * (double)u[q][e];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        sum += __shfl_xor(sum, o);
+    if (lane == 0)
+        sums[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w)
+        sum += sums[w];
+    const double scale = sum == 0.0 ? 0.0 : (double)kUnit / sqrt(sum);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int at = tid + q * 1024, row = at / per, col = (at - row * per) * 4;
+        if (row >= rows)
+            break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < cols) {
+                const int i = tall ? col + e : row, j = tall ? row : col + e;
+                uint16_t h, l;
+                pieces((float)((double)u[q][e] * scale), h, l);
+                X[i * PX + j] = h;
+                X[XP + i * PX + j] = l;
+                Y[j * PM + i] = h;
+                Y[YP + j * PM + i] = l;
+            }
+    }
+    __syncthreads();
+    // the sums over k of rows a0 + lr of A and b0 + lr of B: lane gets column lr of
+    // rows 4 lg .. + 3
+    auto product = [&](const uint16_t *A, int pa, int planeA, int a0, const uint16_t *B, int pb, int planeB, int b0, int k) {
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint16_t *const a = A + (a0 + lr) * pa + lg * 8, *const b = B + (b0 + lr) * pb + lg * 8;
+#pragma unroll
+        for (int i = 0; i < k; i += 32) {
+            const uint4 ah = *(const uint4 *)(a + i), al = *(const uint4 *)(a + planeA + i);
+            const uint4 bh = *(const uint4 *)(b + i), bl = *(const uint4 *)(b + planeB + i);
+            acc = mma16(ah, bh, acc);
+            acc = mma16(ah, bl, acc);
+            acc = mma16(al, bh, acc);
+        }
+        return acc;
+    };
+    const int ti = wave >> 2 << 4, tj = (wave & 3) << 4;
+    uint16_t *const mine = S + (tj + lr) * PM + ti + 4 * lg; // S and B are symmetric: down a column is along a row
+    for (int step = 0; step < steps; ++step) {
+        f32x4 v = product(X, PX, XP, ti, X, PX, XP, tj, NP) * (1.0f / kUnit);
+        store4(mine, SP, v);
+        __syncthreads();
+        v = product(S, PM, SP, ti, S, PM, SP, tj, M) * (1.0f / kUnit);
+        float x[4];
+        load4(mine, SP, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[e] = kB * x[e] + kC * v[e];
+        __syncthreads(); // S is read
+        store4(mine, SP, v);
+        __syncthreads();
+        f32x4 next[T];
+#pragma unroll
+        for (int q = 0; q < T; ++q) {
+            const int j0 = (tj >> 4) * (NP / 4) + q * 16;
+            next[q] = product(S, PM, SP, ti, Y, PM, YP, j0, M) * (1.0f / kUnit);
+            load4(Y + (j0 + lr) * PM + ti + 4 * lg, YP, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                next[q][e] = kA * x[e] + next[q][e];
+        }
+        if (step + 1 == steps) {
+#pragma unroll
+            for (int q = 0; q < T; ++q) {
+                const int i = ti + 4 * lg, j = (tj >> 4) * (NP / 4) + q * 16 + lr, m = tall ? cols : rows, n = tall ? rows : cols;
+                if (i >= m || j >= n)
+                    continue;
+                if (tall) {
+                    finish4(s, (size_t)j * m + i, next[q], m - i < 4 ? m - i : 4);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (i + e < m)
+                            finish4(s, (size_t)(i + e) * n + j, f32x4{next[q][e], 0.0f, 0.0f, 0.0f}, 1);
+                }
+            }
+            break;
+        }
+        __syncthreads(); // X is read
+#pragma unroll
+        for (int q = 0; q < T; ++q) {
+            const int j = (tj >> 4) * (NP / 4) + q * 16 + lr, i = ti + 4 * lg;
+            uint16_t h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pieces(next[q][e], h[e], l[e]);
+                X[(i + e) * PX + j] = h[e];
+                X[XP + (i + e) * PX + j] = l[e];
+            }
+            store4(Y + j * PM + i, YP, next[q]);
+        }
+        __syncthreads();
+    }
+}
+
 // ---------------------------------------------------------------- launches
 
 template <bool TB>
 using T256 = pcfg<f32x16, 2, 256, 256, 2, 4, TB, 32, 2>;
 template <bool TB>
-using T128 = pcfg<f32x16, 2, 128, 128, 2, 2, TB, 32, 2>;
+using T128 = pcfg<f32x16, 2, 128, 128, 4, 2, TB, 32, 4>;
 template <bool TB>
 using T64 = pcfg<f32x16, 2, 64, 64, 2, 2, TB, 64, 2>;
 
@@ -524,11 +683,10 @@ int tiles_of(const ns_prob &p, int what, int side)
 
 // How a product of all matrices is cut.  Whole rounds of tiles over the chip run
 // as they are; what is left, less than a round, is split along the reduction
-// where that is faster.  The time of 32 along the reduction was measured with one
-// block on a CU and with as many as fit (two of 128 and 64), in us: 1.7 and 2.4 for a
-// side of 256, 0.76 and 1.4 for 128, 0.36 and 0.44 for 64; a joining launch takes
-// some 5 us and the partial sums' way at 3.5 TB/s.  1024 x 4096, S: 36 tiles of 128
-// in 7 slices 22 us, whole 81; 64: 46.
+// where that is faster.  The time of 32 along the reduction was measured with few
+// blocks and with as many as fit (two on a CU of 64, else one), in us: 1.7 and 2.4
+// for a side of 256, 0.5 and 0.75 for 128, 0.36 and 0.44 for 64; a joining launch
+// takes some 5 us and the partial sums' way at 3.5 TB/s.
 struct ns_plan {
     int side, whole, z, tiles;
 };
@@ -537,7 +695,7 @@ ns_plan plan_of(const ns_prob *p, int n, int what)
     static const struct {
         int side, blocks;
         double alone, full;
-    } kinds[3] = {{256, 1, 1.7, 2.4}, {128, 2, 0.76, 1.4}, {64, 2, 0.36, 0.44}};
+    } kinds[3] = {{256, 1, 1.7, 2.4}, {128, 1, 0.5, 0.75}, {64, 2, 0.36, 0.44}};
     ns_plan best = {};
     double least = 0.0;
     for (const auto &c : kinds) {
@@ -638,16 +796,23 @@ bool fits(const pgk_muon_seg &s)
 
 } // namespace
 
+// matrices that a block holds
+bool small(const pgk_muon_seg &s)
+{
+    const size_t lo = s.rows < s.cols ? s.rows : s.cols, hi = s.rows < s.cols ? s.cols : s.rows;
+    return lo <= kSmallM && hi <= kSmallN;
+}
+
 extern "C" size_t pgk_muon_workspace(const pgk_muon_seg *segs, int n)
 {
-    if (n < 1 || n > kMost)
-        return 0;
     ns_prob p[kMost];
-    for (int i = 0; i < n; ++i)
-        shape(segs[i], &p[i]);
-    order(p, NULL, n);
+    int k = 0;
+    for (int i = 0; i < n && i < kMost; ++i)
+        if (!small(segs[i]))
+            shape(segs[i], &p[k++]);
+    order(p, NULL, k);
     float *partial;
-    return places(p, n, NULL, &partial);
+    return k ? places(p, k, NULL, &partial) : 0;
 }
 
 extern "C" int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov, int steps, void *ws, pgk_stream s)
@@ -657,15 +822,33 @@ extern "C" int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov,
     static_assert(sizeof(seg_table) <= 4096, "the table fits the kernels' arguments");
     const hipStream_t st = (hipStream_t)s;
     seg_table t = {};
-    t.n = n;
     t.mu = mu;
     t.nesterov = nesterov;
+    size_t longest = 0;
     for (int i = 0; i < n; ++i) {
         if (!fits(segs[i]))
             return (int)hipErrorInvalidValue;
-        t.seg[i] = segs[i];
-        shape(segs[i], &t.p[i]);
+        if (small(segs[i])) {
+            t.seg[t.n++] = segs[i];
+            longest = std::max({longest, segs[i].rows, segs[i].cols});
+        }
     }
+    if (t.n) {
+        if (longest <= 64)
+            hipLaunchKernelGGL(k_ns_small<64>, dim3((unsigned)t.n), dim3(1024), 0, st, t, steps);
+        else
+            hipLaunchKernelGGL(k_ns_small<kSmallN>, dim3((unsigned)t.n), dim3(1024), 0, st, t, steps);
+        if (const int rc = (int)hipGetLastError())
+            return rc;
+    }
+    t.n = 0;
+    for (int i = 0; i < n; ++i)
+        if (!small(segs[i])) {
+            t.seg[t.n] = segs[i];
+            shape(segs[i], &t.p[t.n++]);
+        }
+    if (!(n = t.n))
+        return 0;
     order(t.p, t.seg, n);
     places(t.p, n, (char *)ws, &t.partial);
     int blocks = number(t, [](const ns_prob &p) { return p.parts; });
