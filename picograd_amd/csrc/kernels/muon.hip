@@ -245,14 +245,22 @@ __global__ void __launch_bounds__(256) k_ns_start(seg_table t)
     }
 }
 
-__device__ __forceinline__ void load4(const uint16_t *p, size_t plane, float (&v)[4])
+// four neighbours in two pieces
+struct pieces4 {
+    uint2 h, l;
+    __device__ __forceinline__ void values(float (&v)[4]) const
+    {
+        v[0] = whole((uint16_t)h.x, (uint16_t)l.x);
+        v[1] = whole((uint16_t)(h.x >> 16), (uint16_t)(l.x >> 16));
+        v[2] = whole((uint16_t)h.y, (uint16_t)l.y);
+        v[3] = whole((uint16_t)(h.y >> 16), (uint16_t)(l.y >> 16));
+    }
+};
+__device__ __forceinline__ pieces4 raw4(const uint16_t *p, size_t plane)
 {
-    const uint2 h = *(const uint2 *)p, l = *(const uint2 *)(p + plane);
-    v[0] = whole((uint16_t)h.x, (uint16_t)l.x);
-    v[1] = whole((uint16_t)(h.x >> 16), (uint16_t)(l.x >> 16));
-    v[2] = whole((uint16_t)h.y, (uint16_t)l.y);
-    v[3] = whole((uint16_t)(h.y >> 16), (uint16_t)(l.y >> 16));
+    return {*(const uint2 *)p, *(const uint2 *)(p + plane)};
 }
+__device__ __forceinline__ void load4(const uint16_t *p, size_t plane, float (&v)[4]) { raw4(p, plane).values(v); }
 __device__ __forceinline__ void store4(uint16_t *p, size_t plane, const f32x4 &v)
 {
     uint16_t h[4], l[4];
@@ -263,33 +271,52 @@ __device__ __forceinline__ void store4(uint16_t *p, size_t plane, const f32x4 &v
     *(uint2 *)(p + plane) = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
 }
 
-// four neighbours of the result, X times kUnit, at element i of the matrix
-__device__ __forceinline__ void finish4(const pgk_muon_seg &s, size_t i, const f32x4 &x, int n)
+// n (1 to 4) neighbours of w from element i; of an output without w nothing is read
+__device__ __forceinline__ f32x4 weights4(const pgk_muon_seg &s, size_t i, int n)
 {
-    float o[4];
-    if (s.w) {
-        const float step = s.step / kUnit;
+    f32x4 w = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!s.w)
+        return w;
+    if (n == 4) {
+        const f32x4u v = *(const f32x4u *)(s.w + i);
+        return f32x4{v[0], v[1], v[2], v[3]};
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < n) {
-                o[e] = s.decay * s.w[i + e] - step * x[e];
-                s.w[i + e] = o[e];
-                if (s.shadow) {
-                    const size_t j = i + e;
-                    s.shadow[s.shadow_cols ? j / s.shadow_cols * s.shadow_ld + j % s.shadow_cols : j] =
-                        to16(s.shadow_dtype, o[e]);
-                }
-            }
+    for (int e = 0; e < 4; ++e)
+        if (e < n)
+            w[e] = s.w[i + e];
+    return w;
+}
+// what becomes of them, from the last X times kUnit
+__device__ __forceinline__ void finish4(const pgk_muon_seg &s, size_t i, const f32x4 &w, const f32x4 &x, int n)
+{
+    typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+    f32x4 o = x * (1.0f / kUnit);
+    if (s.w)
+        o = s.decay * w - s.step * o;
+    float *const wide = s.w ? s.w : s.out_dtype == 0 ? (float *)s.out : nullptr;
+    if (wide) {
+        if (n == 4)
+            *(f32x4u *)(wide + i) = f32x4u{o[0], o[1], o[2], o[3]};
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < n)
+                    wide[i + e] = o[e];
+    }
+    uint16_t *const narrow = s.w ? s.shadow : (uint16_t *)s.out;
+    const int dt = s.w ? s.shadow_dtype : s.out_dtype;
+    if (!narrow || dt == 0)
+        return;
+    if (n == 4 && !s.shadow_cols) {
+        *(u32x2u *)(narrow + i) = u32x2u{to16x2(dt, o[0], o[1]), to16x2(dt, o[2], o[3])};
         return;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (e < n) {
-            const float v = x[e] / kUnit;
-            if (s.out_dtype == 0)
-                ((float *)s.out)[i + e] = v;
-            else
-                ((uint16_t *)s.out)[i + e] = to16(s.out_dtype, v);
+            const size_t j = i + e;
+            narrow[s.shadow_cols ? j / s.shadow_cols * s.shadow_ld + j % s.shadow_cols : j] = to16(dt, o[e]);
         }
 }
 
@@ -339,42 +366,70 @@ __device__ __forceinline__ void strip_out(const TAB &t, int k, f32x16 (&acc)[CF:
     const size_t px = (size_t)p.mp * p.np, ps = (size_t)p.mp * p.mp;
     if constexpr (WHAT == NS_S || WHAT == NS_B) {
         uint16_t *const to = WHAT == NS_S ? p.s : p.b;
-        piece_out_strip<CF, f32x4>(acc, i, m0, n0, p.mp, p.mp, lds, m0 != n0, [&](int row, int col, f32x4 &v, bool mirror) {
-            if (mirror) {
-                store4(to + (size_t)col * p.mp + row, ps, v);
-                return;
-            }
-            v *= 1.0f / kUnit;
-            if constexpr (WHAT == NS_B) {
-                float x[4];
-                load4(p.s + (size_t)row * p.mp + col, ps, x);
+        piece_out_strip<CF, f32x4>(
+            acc, i, m0, n0, p.mp, p.mp, lds, m0 != n0,
+            [&](int row, int col) {
+                if constexpr (WHAT == NS_B)
+                    return raw4(p.s + (size_t)row * p.mp + col, ps);
+                else
+                    return 0;
+            },
+            [&](int row, int col, f32x4 &v, const auto &with, bool mirror) {
+                if (mirror) {
+                    store4(to + (size_t)col * p.mp + row, ps, v);
+                    return;
+                }
+                v *= 1.0f / kUnit;
+                if constexpr (WHAT == NS_B) {
+                    float x[4];
+                    with.values(x);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] = kB * x[e] + kC * v[e];
-            }
-            store4(to + (size_t)row * p.mp + col, ps, v);
-        });
-    } else {
-        bool tall = false; // only the last X is written as u lies
-        if constexpr (WHAT == NS_LAST)
-            tall = t.seg[k].rows > t.seg[k].cols;
-        piece_out_strip<CF, f32x4>(acc, i, m0, n0, p.mp, p.np, lds, tall, [&](int row, int col, f32x4 &v, bool mirror) {
-            if (!mirror) {
+                    for (int e = 0; e < 4; ++e)
+                        v[e] = kB * x[e] + kC * v[e];
+                }
+                store4(to + (size_t)row * p.mp + col, ps, v);
+            });
+    } else if constexpr (WHAT == NS_X) {
+        piece_out_strip<CF, f32x4>(
+            acc, i, m0, n0, p.mp, p.np, lds, false,
+            [&](int row, int col) { return raw4(p.x + (size_t)row * p.np + col, px); },
+            [&](int row, int col, f32x4 &v, const pieces4 &with, bool) {
                 float x[4];
-                load4(p.x + (size_t)row * p.np + col, px, x);
+                with.values(x);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     v[e] = kA * x[e] + v[e] * (1.0f / kUnit);
-            }
-            if constexpr (WHAT == NS_X) {
                 store4(p.to + (size_t)row * p.np + col, px, v);
-            } else {
+            });
+    } else { // as u lies
+        const pgk_muon_seg &s = t.seg[k];
+        const bool tall = s.rows > s.cols;
+        struct from4 {
+            pieces4 x;
+            f32x4 w;
+        };
+        piece_out_strip<CF, f32x4, 2>(
+            acc, i, m0, n0, p.mp, p.np, lds, tall,
+            [&](int row, int col) {
+                from4 q = {raw4(p.x + (size_t)row * p.np + col, px), {}};
+                if (!tall && row < p.m && col < p.n)
+                    q.w = weights4(s, (size_t)row * p.n + col, p.n - col < 4 ? p.n - col : 4);
+                return q;
+            },
+            [&](int row, int col, f32x4 &v, const from4 &with, bool mirror) {
+                if (!mirror) {
+                    float x[4];
+                    with.x.values(x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        v[e] = kA * x[e] + v[e] * (1.0f / kUnit);
+                }
                 if (mirror != tall || row >= p.m || col >= p.n)
                     return;
-                const int left = tall ? p.m - row : p.n - col;
-                finish4(t.seg[k], tall ? (size_t)col * p.m + row : (size_t)row * p.n + col, v, left < 4 ? left : 4);
-            }
-        });
+                const int left = tall ? p.m - row : p.n - col, n = left < 4 ? left : 4;
+                const size_t at = tall ? (size_t)col * p.m + row : (size_t)row * p.n + col;
+                finish4(s, at, tall ? weights4(s, at, n) : with.w, v, n);
+            });
     }
 }
 
@@ -462,6 +517,7 @@ __global__ void __launch_bounds__(CF::NT, 1) k_ns_join(TAB t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
             acc[j][e] = 0.0f;
+#pragma unroll 2
     for (int s = 0; s < t.z; ++s) {
         if (kt * s / t.z == kt * (s + 1) / t.z)
             continue;
@@ -611,12 +667,16 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
                 if (i >= m || j >= n)
                     continue;
                 if (tall) {
-                    finish4(s, (size_t)j * m + i, next[q], m - i < 4 ? m - i : 4);
+                    const size_t at = (size_t)j * m + i;
+                    const int some = m - i < 4 ? m - i : 4;
+                    finish4(s, at, weights4(s, at, some), next[q], some);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (i + e < m)
-                            finish4(s, (size_t)(i + e) * n + j, f32x4{next[q][e], 0.0f, 0.0f, 0.0f}, 1);
+                        if (i + e < m) {
+                            const size_t at = (size_t)(i + e) * n + j;
+                            finish4(s, at, weights4(s, at, 1), f32x4{next[q][e], 0.0f, 0.0f, 0.0f}, 1);
+                        }
                 }
             }
             break;

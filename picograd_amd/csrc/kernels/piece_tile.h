@@ -220,19 +220,32 @@ __device__ __forceinline__ void piece_loop(const piece_operand &A, const piece_o
 }
 
 // The way out of strip i of the sums, 32 rows of each wave's tile, through LDS.
-// f(row, column, v, false) takes four neighbouring sums of a row, for every row <
-// M and column < N (a multiple of 4 behind n0), and may change them; with `down`
-// f(row, column, v, true) then takes what it left, four down a column.
-template <class CF, class V4, class FN_>
+// f(row, column, v, from(row, column), false) takes four neighbouring sums of a
+// row, for every row < M and column < N (a multiple of 4 behind n0), and may change
+// them; `from` is asked for all of a thread's places before the first f, so that
+// its loads wait for none of f's stores (f loading what it needs by itself took 26 us
+// of each round of 256 x 256 tiles, now 11); U > 0: of U places at a time.  With
+// `down` f(row, column, v, {}, true) then takes what it left, four down a column.
+template <class CF, class V4, int U_ = 0, class FROM, class FN_>
 __device__ __forceinline__ void piece_out_strip(typename CF::ACC (&acc)[CF::FN], int i, int m0, int n0, int M, int N,
-                                                LDS uint4 *const lds, bool down, FN_ f)
+                                                LDS uint4 *const lds, bool down, FROM from, FN_ f)
 {
-    constexpr int RS = CF::RS, WN = CF::WN, CL = WN / 4;
+    constexpr int RS = CF::RS, WN = CF::WN, CL = WN / 4, STEP = 64 / CL, NR = 32 / STEP;
+    constexpr int U = U_ && U_ < NR ? U_ : NR;
+    static_assert(NR % U == 0, "whole groups of places");
     typedef LDS int *lds_int;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / CF::WGN, wn = wave % CF::WGN;
     const int lrow = lane & 31, lk = lane >> 5;
     const lds_int reg = (lds_int)lds + wave * 32 * RS;
-    const int col0 = n0 + wn * WN;
+    const int col0 = n0 + wn * WN, row0 = m0 + wm * CF::WM + i * 32, r0 = lane / CL, c4 = (lane % CL) * 4;
+    decltype(from(0, 0)) with[U] = {};
+    auto ask = [&](int r1) {
+#pragma unroll
+        for (int r = 0; r < U; ++r)
+            if (row0 + r0 + (r1 + r) * STEP < M && col0 + c4 < N)
+                with[r] = from(row0 + r0 + (r1 + r) * STEP, col0 + c4);
+    };
+    ask(0);
     __syncthreads(); // the stages' (or the previous strip's) reads are done
 #pragma unroll
     for (int j = 0; j < CF::FN; ++j)
@@ -242,36 +255,34 @@ __device__ __forceinline__ void piece_out_strip(typename CF::ACC (&acc)[CF::FN],
             reg[((e >> 2) * 8 + lk * 4 + (e & 3)) * RS + j * 32 + lrow] = __builtin_bit_cast(int, one);
         }
     __syncthreads();
-    const int row0 = m0 + wm * CF::WM + i * 32, c4 = (lane % CL) * 4;
 #pragma unroll 1
-    for (int r = lane / CL; r < 32; r += 64 / CL)
-        if (row0 + r < M && col0 + c4 < N) {
-            LDS i32x4 *const at = (LDS i32x4 *)(reg + r * RS + c4);
+    for (int r1 = 0; r1 < NR; r1 += U) {
+        if (r1)
+            ask(r1);
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+            const int row = r0 + (r1 + r) * STEP;
+            if (row0 + row >= M || col0 + c4 >= N)
+                continue;
+            LDS i32x4 *const at = (LDS i32x4 *)(reg + row * RS + c4);
             V4 v = __builtin_bit_cast(V4, *at);
-            f(row0 + r, col0 + c4, v, false);
+            f(row0 + row, col0 + c4, v, with[r], false);
             if (down)
                 *at = __builtin_bit_cast(i32x4, v);
         }
+    }
     if (down) {
         __syncthreads();
         const int r4 = (lane & 7) * 4;
-#pragma unroll 1
+#pragma unroll 4
         for (int c = lane >> 3; c < WN; c += 8) {
             if (row0 + r4 >= M || col0 + c >= N)
                 continue;
             const i32x4 q = {reg[r4 * RS + c], reg[(r4 + 1) * RS + c], reg[(r4 + 2) * RS + c], reg[(r4 + 3) * RS + c]};
             V4 v = __builtin_bit_cast(V4, q);
-            f(row0 + r4, col0 + c, v, true);
+            f(row0 + r4, col0 + c, v, decltype(from(0, 0)){}, true);
         }
     }
-}
-template <class CF, class V4, class FN_>
-__device__ __forceinline__ void piece_out(typename CF::ACC (&acc)[CF::FM][CF::FN], int m0, int n0, int M, int N,
-                                          LDS uint4 *const lds, bool down, FN_ f)
-{
-#pragma unroll
-    for (int i = 0; i < CF::FM; ++i)
-        piece_out_strip<CF, V4>(acc[i], i, m0, n0, M, N, lds, down, f);
 }
 
 } // namespace

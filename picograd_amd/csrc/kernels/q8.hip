@@ -205,42 +205,90 @@ __global__ void __launch_bounds__(256) k_q8_tops(pgk_q8 q, const T *__restrict__
     }
 }
 
-// Codes of 64 columns by kSlab of the reduction: a thread rounds 64 values down a
-// column, LDS turns them into pieces of the column's row.
+// Codes of columns: a thread takes 16 bytes of 16 neighbouring rows of src, so that
+// it has a whole piece of each of its columns' codes; four lanes (two of 16-bit
+// types) side by side, the others down a wave, the waves below each other.  HELD:
+// a block holds its 16 columns whole (kHeld long) and finds their scales by itself,
+// src is read once; else the tops are there.  Bound by the stream of the source: 4096 x
+// 4096 in f32, 84 MB with the codes, 18.6 us; the search and the rounding in passes
+// of their own took 28.
+constexpr int kColumns = 16; // of a block
 template <class T>
-__global__ void __launch_bounds__(256) k_q8_columns(pgk_q8 q, const T *__restrict__ src, const uint32_t *__restrict__ part,
-                                                    int slabs, size_t nx, size_t ny)
+constexpr int kHeld = 64 / (kColumns * sizeof(T) / 16) * 16 * 16; // rows of 16 waves
+
+template <class T, bool HELD>
+__global__ void __launch_bounds__(1024, 1) k_q8_columns(pgk_q8 q, const T *__restrict__ src, const uint32_t *__restrict__ part,
+                                                        int slabs, size_t nx, size_t ny)
 {
-    constexpr int PITCH = kSlab + 16;
-    __shared__ uint4 piece[64 * PITCH / 16];
-    const int lane = (int)threadIdx.x & 63, w = (int)threadIdx.x >> 6;
+    constexpr int C = 16 / sizeof(T), A = kColumns / C; // columns of a thread; lanes side by side
+    typedef T tv __attribute__((ext_vector_type(C), aligned(sizeof(T))));
+    __shared__ uint32_t tops[16][kColumns];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
+    const int lc = lane % A * C, lrow = (wave * (64 / A) + lane / A) * 16;
     for (size_t job = blockIdx.x; job < nx * ny; job += gridDim.x) {
-        const size_t slab = job / nx, c0 = (job - slab * nx) * 64, col = c0 + lane, k0 = slab * kSlab;
-        uint32_t top = 0;
-        if (col < q.rows)
-            for (int i = 0; i < slabs; ++i) {
-                const uint32_t a = part[(size_t)i * q.rows + col];
-                top = a > top ? a : top;
-            }
-        const float s = scale_of(top), inv = 1.0f / s;
-        if (slab == 0 && w == 0 && col < q.rows)
-            q.scale[col] = s;
+        // neighbouring columns share lines: on one XCD
+        const size_t at = gridDim.x == nx * ny ? (size_t)xcd_tile((int)job, (int)gridDim.x) : job, x = at % nx;
+        const size_t col = x * kColumns + lc, k0 = at / nx * kHeld<T> + lrow;
+        const int left = col < q.rows ? (int)(q.rows - col < C ? q.rows - col : C) : 0;
+        tv raw[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v[16];
+        for (int i = 0; i < 16; ++i) {
+            const size_t k = k0 + i;
+            raw[i] = tv{};
+            if (k < q.cols) {
+                const T *const p = src + k * q.rows + col;
+                if (left == C)
+                    raw[i] = *(const tv *)p;
+                else
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const size_t k = k0 + w * 64 + i * 16 + e;
-                v[e] = col < q.rows && k < q.cols ? (float)src[k * q.rows + col] : 0.0f;
+                    for (int e = 0; e < C; ++e)
+                        if (e < left)
+                            raw[i][e] = p[e];
             }
-            piece[(lane * PITCH + w * 64) / 16 + i] = codes16(v, s, inv);
+        }
+        if constexpr (HELD) {
+#pragma unroll
+            for (int e = 0; e < C; ++e) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t a = magnitude((float)raw[i][e]);
+                    top = a > top ? a : top;
+                }
+#pragma unroll
+                for (int o = A; o < 64; o <<= 1) {
+                    const uint32_t a = (uint32_t)__shfl_xor((int)top, o);
+                    top = a > top ? a : top;
+                }
+                if (lane < A)
+                    tops[wave][lc + e] = top;
+            }
+        } else if (tid < kColumns) {
+            uint32_t top = 0;
+            if (x * kColumns + tid < q.rows)
+                for (int i = 0; i < slabs; ++i) {
+                    const uint32_t a = part[(size_t)i * q.rows + x * kColumns + tid];
+                    top = a > top ? a : top;
+                }
+            tops[0][tid] = top;
         }
         __syncthreads();
 #pragma unroll
-        for (int i = (int)threadIdx.x; i < 64 * (kSlab / 16); i += 256) {
-            const int r = i / (kSlab / 16), c = i % (kSlab / 16);
-            if (c0 + r < q.rows && k0 + c * 16 < q.ld)
-                *(uint4 *)(q.codes + (c0 + r) * q.ld + k0 + c * 16) = piece[r * PITCH / 16 + c];
+        for (int e = 0; e < C; ++e) {
+            if (e >= left)
+                break;
+            uint32_t top = tops[0][lc + e];
+            for (int i = 1; HELD && i < waves; ++i)
+                top = tops[i][lc + e] > top ? tops[i][lc + e] : top;
+            const float s = scale_of(top);
+            if (k0 == 0)
+                q.scale[col + e] = s;
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                v[i] = (float)raw[i][e];
+            if (k0 < q.ld)
+                *(uint4 *)(q.codes + (col + e) * q.ld + k0) = codes16(v, s, 1.0f / s);
         }
         __syncthreads();
     }
@@ -331,77 +379,96 @@ __device__ __forceinline__ void put4(O *p, const float (&v)[4], int n)
 }
 
 // Up to 16 rows of x: a thread block owns 16 columns of y and its waves split the
-// reduction, so the weights stream past once.  FUSED: every block finds the rows'
-// scales and rounds x by itself, no other launch; else xq holds them.  Bound by
-// the loads' latency and the launch.
-constexpr int kFewWaves = 8;
+// reduction, so the weights stream past once.  FUSED: every block rounds x into LDS by
+// itself while its first weights are on their way, no other launch; else xq holds
+// it.  Bound by the loads' latency and the launch.
+constexpr int kFewWaves = 8, kFewFused = 16384; // values of x that every block rounds
 
 template <class T, class O, bool FUSED>
 __global__ void __launch_bounds__(kFewWaves * 64, 1)
     k_q8_few(const T *__restrict__ x, pgk_q8 xq, int m, pgk_q8 w, O *__restrict__ y, size_t tiles)
 {
-    constexpr int U = 4; // steps of 64 in flight
+    constexpr int U = 8, MOST = FUSED ? kFewFused / 16 + 16 * 8 : 1; // steps of 64 in flight; pieces of x
+    constexpr int PER = (MOST + kFewWaves * 64 - 1) / (kFewWaves * 64);
     __shared__ int part[kFewWaves][16][17];
-    __shared__ uint32_t tops[kFewWaves][16];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    __shared__ uint4 xs[MOST];
+    __shared__ uint32_t tops[16];
+    // (the wave's number is uniform to the compiler: a matrix instruction heeds no mask)
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
     const size_t steps = w.ld / 64, k = w.cols;
+    const int nc = (int)(w.ld / 16), xr = r < m ? r : m - 1; // (rows past the last give sums that no one takes)
     for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const size_t n0 = tile * 16, wr = n0 + r < w.rows ? n0 + r : w.rows - 1;
         const uint8_t *const pw = (const uint8_t *)w.codes + wr * w.ld + g * 16;
-        float s = 0.0f, inv = 0.0f;
-        if constexpr (FUSED) {
-            uint32_t top = 0;
-            if (r < m)
-                for (size_t st = wave; st < steps; st += kFewWaves) {
-                    float v[16];
-                    load16(x + r * k, st * 4 + g, k, v);
-                    top = top16(v, top);
-                }
-#pragma unroll
-            for (int o = 16; o < 64; o <<= 1) {
-                const uint32_t a = (uint32_t)__shfl_xor((int)top, o);
-                top = a > top ? a : top;
-            }
-            if (g == 0)
-                tops[wave][r] = top;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kFewWaves; ++i)
-                top = tops[i][r] > top ? tops[i][r] : top;
-            s = scale_of(top);
-            inv = 1.0f / s;
-        }
-        i32x4 acc = {0, 0, 0, 0};
-        for (size_t s0 = (size_t)wave * U; s0 < steps; s0 += kFewWaves * U) {
-            uint4 b[U];
+        uint4 b[U];
+        auto load = [&](size_t s0) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (s0 + u < steps)
                     b[u] = *(const uint4 *)(pw + (s0 + u) * 64);
+        };
+        size_t s0 = (size_t)wave * U;
+        load(s0);
+        if (FUSED && tile == blockIdx.x) {
+            if (tid < 16)
+                tops[tid] = 0;
+            float v[PER][16];
+            uint32_t top[PER];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (s0 + u >= steps)
-                    break;
-                uint4 a = make_uint4(0, 0, 0, 0);
-                if (r < m) {
-                    if constexpr (FUSED) {
-                        float v[16];
-                        load16(x + r * k, (s0 + u) * 4 + g, k, v);
-                        a = codes16(v, s, inv);
-                    } else {
-                        a = *(const uint4 *)(xq.codes + r * xq.ld + (s0 + u) * 64 + g * 16);
-                    }
+            for (int i = 0; i < PER; ++i) {
+                const int c = tid + i * kFewWaves * 64, row = c / nc;
+                top[i] = 0;
+                if (row < m) {
+                    load16(x + row * k, c - row * nc, k, v[i]);
+                    top[i] = top16(v[i], 0);
                 }
-                acc = mma16(a, b[u], acc);
             }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int c = tid + i * kFewWaves * 64, row = c / nc;
+                // a wave within one row has one largest
+                if (__all(row == __builtin_amdgcn_readfirstlane(row))) {
+                    const uint32_t t = wave_top(top[i]);
+                    if (lane == 0 && row < m)
+                        atomicMax(&tops[row], t);
+                } else if (row < m) {
+                    atomicMax(&tops[row], top[i]);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int c = tid + i * kFewWaves * 64, row = c / nc;
+                if (row < m) {
+                    const float s = scale_of(tops[row]);
+                    xs[c] = codes16(v[i], s, 1.0f / s);
+                }
+            }
+            __syncthreads();
+        }
+        i32x4 acc = {0, 0, 0, 0};
+        while (s0 < steps) {
+            uint4 a[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s0 + u < steps) {
+                    if constexpr (FUSED)
+                        a[u] = xs[xr * nc + (s0 + u) * 4 + g];
+                    else
+                        a[u] = *(const uint4 *)(xq.codes + xr * xq.ld + (s0 + u) * 64 + g * 16);
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s0 + u < steps)
+                    acc = mma16(a[u], b[u], acc);
+            s0 += kFewWaves * U;
+            load(s0);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             part[wave][4 * g + e][r] = acc[e];
-        // (lanes of the first wave with g == 0 hold the rows' scales)
-        __shared__ float scales[16];
-        if (FUSED && wave == 0 && g == 0)
-            scales[r] = s;
         __syncthreads();
         const int row = tid >> 4, col = tid & 15;
         if (row < m && row < 16 && n0 + col < w.rows) {
@@ -409,119 +476,16 @@ __global__ void __launch_bounds__(kFewWaves * 64, 1)
 #pragma unroll
             for (int i = 0; i < kFewWaves; ++i)
                 sum += part[i][row][col];
-            const float sx = FUSED ? scales[row] : xq.scale[row];
+            const float sx = FUSED ? scale_of(tops[row]) : xq.scale[row];
             y[(size_t)row * w.rows + n0 + col] = (O)((float)sum * sx * w.scale[n0 + col]);
         }
         __syncthreads();
     }
 }
 
-// Products that the tiles below would not spread over the chip: a thread block owns
-// FM x FN tiles of 16 and its KG waves split the reduction, wave v taking the
-// pairs of steps v, v + KG, ... straight from memory into registers, the next
-// pair's loads in flight.  LDS only for the exact sum of the partial tiles.
-template <int FM, int FN>
-struct pair_of_steps {
-    uint4 a[2][FM], b[2][FN];
-    __device__ __forceinline__ void load(const uint8_t *const (&pa)[FM], const uint8_t *const (&pb)[FN], size_t s)
-    {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-                a[h][i] = *(const uint4 *)(pa[i] + (s + h) * 64);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-                b[h][j] = *(const uint4 *)(pb[j] + (s + h) * 64);
-        }
-    }
-    __device__ __forceinline__ void multiply(i32x4 (&acc)[FM][FN]) const
-    {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j)
-                    acc[i][j] = mma16(a[h][i], b[h][j], acc[i][j]);
-    }
-};
-
-template <int FM, int FN, int KG, class O>
-__global__ void __launch_bounds__(KG * 64, 1) k_q8_split(pgk_q8 x, pgk_q8 w, O *__restrict__ y)
-{
-    constexpr int TM = 16 * FM, TN = 16 * FN, RS = TN + 4;
-    __shared__ int part[KG / 2][TM * RS];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lr = lane & 15, lg = lane >> 4;
-    const int tiles_n = (int)((w.rows + TN - 1) / TN);
-    const int pid = xcd_tile((int)blockIdx.x, (int)gridDim.x);
-    const size_t m0 = (size_t)(pid / tiles_n) * TM, n0 = (size_t)(pid % tiles_n) * TN;
-    const size_t steps = x.ld / 64; // an even number
-    const uint8_t *pa[FM], *pb[FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const size_t r = m0 + i * 16 + lr;
-        pa[i] = (const uint8_t *)x.codes + (r < x.rows ? r : x.rows - 1) * x.ld + lg * 16;
-    }
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const size_t r = n0 + j * 16 + lr;
-        pb[j] = (const uint8_t *)w.codes + (r < w.rows ? r : w.rows - 1) * w.ld + lg * 16;
-    }
-    i32x4 acc[FM][FN] = {};
-    pair_of_steps<FM, FN> cur, next;
-    size_t s = wave * 2;
-    if (s < steps)
-        cur.load(pa, pb, s);
-    for (; s < steps; s += 2 * KG) {
-        const size_t ahead = s + 2 * KG;
-        if (ahead < steps)
-            next.load(pa, pb, ahead);
-        cur.multiply(acc);
-        cur = next;
-    }
-    auto at = [&](int slot, int i, int j, int e) -> int & { return part[slot][(i * 16 + 4 * lg + e) * RS + j * 16 + lr]; };
-    if (wave >= KG / 2)
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    at(wave - KG / 2, i, j, e) = acc[i][j][e];
-    __syncthreads();
-    if (wave < KG / 2) // each in its own slot
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    at(wave, i, j, e) += acc[i][j][e];
-    __syncthreads();
-    const size_t M = x.rows, N = w.rows;
-#pragma unroll 1
-    for (int i = tid; i < TM * TN / 4; i += KG * 64) {
-        const int row = i / (TN / 4), c4 = i % (TN / 4) * 4;
-        const size_t gm = m0 + row, gn = n0 + c4;
-        if (gm >= M || gn >= N)
-            continue;
-        i32x4 v = *(const i32x4 *)&part[0][row * RS + c4];
-#pragma unroll
-        for (int p = 1; p < KG / 2; ++p)
-            v += *(const i32x4 *)&part[p][row * RS + c4];
-        const float sx = x.scale[gm];
-        const int n = N - gn < 4 ? (int)(N - gn) : 4;
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            o[e] = e < n ? (float)v[e] * sx * w.scale[gn + e] : 0.0f;
-        put4(y + gm * N + gn, o, n);
-    }
-}
-
-// Large products on the tiles of piece_loop.
+// More rows on the tiles of piece_loop: bound by loads' latency where there are few
+// tiles, by LDS and the matrix units where there are many (8192 x 4096 x 4096: 126 us,
+// 2.2 POP/s; along the reduction alone 2.7 of the 3.0 that the instruction reaches).
 template <class CF, class O>
 __global__ void __launch_bounds__(CF::NT, 1) k_q8_tiles(pgk_q8 x, pgk_q8 w, O *__restrict__ y)
 {
@@ -537,15 +501,24 @@ __global__ void __launch_bounds__(CF::NT, 1) k_q8_tiles(pgk_q8 x, pgk_q8 w, O *_
     i32x16 acc[CF::FM][CF::FN];
     piece_loop<CF>({(const uint16_t *)x.codes, x.ld / 2, 0, M}, {(const uint16_t *)w.codes, w.ld / 2, 0, N}, 0, (int)(x.ld / 2),
                    m0, n0, lds, acc);
-    piece_out<CF, i32x4>(acc, m0, n0, M, N, lds, false, [&](int row, int col, const i32x4 &v, bool) {
-        const float sx = x.scale[row];
-        const int n = N - col < 4 ? N - col : 4;
-        float o[4];
+    // a lane's columns are the same in every strip
+    const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
+    const int col0 = n0 + wave % CF::WGN * CF::WN + lane % (CF::WN / 4) * 4;
+    float sw[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            o[e] = e < n ? (float)v[e] * sx * w.scale[col + e] : 0.0f;
-        put4(y + (size_t)row * N + col, o, n);
-    });
+    for (int e = 0; e < 4; ++e)
+        sw[e] = col0 + e < N ? w.scale[col0 + e] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < CF::FM; ++i)
+        piece_out_strip<CF, i32x4>(
+            acc[i], i, m0, n0, M, N, lds, false, [&](int row, int) { return x.scale[row]; },
+            [&](int row, int col, const i32x4 &v, float sx, bool) {
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    o[e] = (float)v[e] * sx * sw[e];
+                put4(y + (size_t)row * N + col, o, N - col < 4 ? N - col : 4);
+            });
 }
 
 // ---------------------------------------------------------------- launches
@@ -581,26 +554,26 @@ int quantize_rows(const pgk_q8 &q, const T *src, hipStream_t st)
 template <class T>
 int quantize_columns(const pgk_q8 &q, const T *src, uint32_t *ws, hipStream_t st)
 {
-    const size_t nx = (q.rows + 63) / 64, ny = slabs_of(&q);
-    hipLaunchKernelGGL(k_q8_tops<T>, dim3(grid_of(nx * ny)), dim3(256), 0, st, q, src, ws, nx, ny);
+    constexpr size_t per = kHeld<T> / 16; // rows of a wave
+    const size_t nx = (q.rows + kColumns - 1) / kColumns, ny = (q.ld + kHeld<T> - 1) / kHeld<T>;
+    if (ny == 1) {
+        hipLaunchKernelGGL((k_q8_columns<T, true>), dim3(grid_of(nx)), dim3((unsigned)((q.ld + per - 1) / per) * 64), 0, st, q,
+                           src, (const uint32_t *)nullptr, 0, nx, ny);
+        return (int)hipGetLastError();
+    }
+    const size_t sx = (q.rows + 63) / 64, slabs = slabs_of(&q);
+    hipLaunchKernelGGL(k_q8_tops<T>, dim3(grid_of(sx * slabs)), dim3(256), 0, st, q, src, ws, sx, slabs);
     if (const int rc = (int)hipGetLastError())
         return rc;
-    hipLaunchKernelGGL(k_q8_columns<T>, dim3(grid_of(nx * ny)), dim3(256), 0, st, q, src, ws, (int)ny, nx, ny);
+    hipLaunchKernelGGL((k_q8_columns<T, false>), dim3(grid_of(nx * ny)), dim3(1024), 0, st, q, src, ws, (int)slabs, nx, ny);
     return (int)hipGetLastError();
-}
-
-template <int FM, int FN, int KG, class O>
-void split(const pgk_q8 &x, const pgk_q8 &w, O *y, hipStream_t st)
-{
-    const size_t blocks = (x.rows + 16 * FM - 1) / (16 * FM) * ((w.rows + 16 * FN - 1) / (16 * FN));
-    hipLaunchKernelGGL((k_q8_split<FM, FN, KG, O>), dim3((unsigned)blocks), dim3(KG * 64), 0, st, x, w, y);
 }
 
 template <class O>
 int product(const pgk_q8 &x, const pgk_q8 &w, O *y, hipStream_t st)
 {
     auto tiles = [&](size_t bm, size_t bn) { return (x.rows + bm - 1) / bm * ((w.rows + bn - 1) / bn); };
-    if (tiles(128, 128) >> 22) { // a grid holds under 2^32 threads: the rows in two halves
+    if (tiles(64, 64) >> 24) { // a grid holds under 2^32 threads: the rows in two halves
         if (x.rows <= 256) // over 2^28 columns
             return (int)hipErrorInvalidValue;
         pgk_q8 a = x, b = x;
@@ -611,20 +584,35 @@ int product(const pgk_q8 &x, const pgk_q8 &w, O *y, hipStream_t st)
         const int rc = product(a, w, y, st);
         return rc ? rc : product(b, w, y + a.rows * w.rows, st);
     }
-    using T128 = pcfg<i32x16, 1, 128, 128, 2, 2, false, 64, 2>;
+    using T64 = pcfg<i32x16, 1, 64, 64, 2, 2, false, 64, 4>;
+    using T128 = pcfg<i32x16, 1, 128, 128, 4, 2, false, 64, 4>;
+    using TWO = pcfg<i32x16, 1, 128, 128, 2, 2, false, 64, 2>; // of 128 x 128 to a CU
+    using TALL = pcfg<i32x16, 1, 256, 128, 4, 2, false, 64, 3>;
     using T256 = pcfg<i32x16, 1, 256, 256, 2, 4, false, 64, 2>;
-    if (tiles(32, 32) <= 256)
-        split<2, 2, 8>(x, w, y, st);
-    else if (tiles(64, 32) <= 256)
-        split<4, 2, 8>(x, w, y, st);
-    else if (tiles(64, 64) <= 256)
-        split<4, 4, 8>(x, w, y, st);
-    else if (tiles(64, 64) <= 512)
-        split<4, 4, 4>(x, w, y, st);
-    else if (tiles(256, 256) < 192)
-        hipLaunchKernelGGL((k_q8_tiles<T128, O>), dim3((unsigned)tiles(128, 128)), dim3(T128::NT), 0, st, x, w, y);
+    auto go = [&](auto cf) {
+        using CF = decltype(cf);
+        hipLaunchKernelGGL((k_q8_tiles<CF, O>), dim3((unsigned)tiles(CF::BM, CF::BN)), dim3(CF::NT), 0, st, x, w, y);
+    };
+    // The largest tile that fills the chip; over K = N = 4096 with M rows, in us:
+    //   M       512    1000   1024   1500   2048   3000   4096   5000
+    //   64     15.8     29   29.6     43     57     83    110    141
+    //   128    17.6     23   23.4     39     46     66     89    108
+    //   TALL   25.8     29   29.6     33     39     65     76    102
+    //   TWO    23.4     28   27.8     37     42     66     77     98
+    //   256    43.1     47   47.5     50     53     57     68    109
+    // Past those: whole rounds of 256-tiles against half rounds of two 128-tiles a
+    // CU, each 0.68 of one.
+    const size_t big = (tiles(256, 256) + 255) / 256, half = (tiles(128, 128) + 255) / 256;
+    if (tiles(128, 128) <= 128)
+        go(T64{});
+    else if (tiles(128, 128) <= 256)
+        go(T128{});
+    else if (tiles(256, 128) <= 256)
+        go(TALL{});
+    else if ((double)big <= 0.34 * (double)half)
+        go(T256{});
     else
-        hipLaunchKernelGGL((k_q8_tiles<T256, O>), dim3((unsigned)tiles(256, 256)), dim3(T256::NT), 0, st, x, w, y);
+        go(TWO{});
     return (int)hipGetLastError();
 }
 
@@ -641,7 +629,10 @@ extern "C" void pgk_q8_shape(pgk_q8 *q, size_t rows, size_t cols, size_t *code_b
     *scale_bytes = rows * sizeof(float);
 }
 
-extern "C" size_t pgk_q8_workspace(const pgk_q8 *q, int trans) { return trans ? slabs_of(q) * q->rows * sizeof(uint32_t) : 0; }
+extern "C" size_t pgk_q8_workspace(const pgk_q8 *q, int trans)
+{
+    return trans && q->ld > kHeld<float> ? slabs_of(q) * q->rows * sizeof(uint32_t) : 0;
+}
 
 extern "C" int pgk_q8_quantize(const pgk_q8 *q, const void *src, int dtype, int trans, void *ws, pgk_stream s)
 {
@@ -671,7 +662,7 @@ extern "C" int pgk_q8_dequantize(const pgk_q8 *q, void *dst, int dtype, int tran
 }
 
 extern "C" int pgk_q8_few_rows(size_t m) { return m <= 16; }
-extern "C" int pgk_q8_few_fused(size_t m, size_t k) { return m * k <= 16384; }
+extern "C" int pgk_q8_few_fused(size_t m, size_t k) { return m * k <= kFewFused; }
 
 extern "C" int pgk_q8_matmul_few(const void *x, int dtype, const pgk_q8 *xq, size_t m, const pgk_q8 *w, void *y, int y_dtype,
                                  pgk_stream s)
