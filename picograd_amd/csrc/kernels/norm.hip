@@ -20,29 +20,59 @@
 
 namespace {
 
-constexpr int kChunks = 4;            // of 16 bytes of x, per thread
+constexpr int kChunks = 2; // of 16 bytes of x, per thread of a slice
 constexpr unsigned kMostBlocks = 1u << 20; // of a grid; kernels loop past it
 
-// 16 bytes of x's type, at any alignment of an element
+// as many values of S as 16 bytes hold of T, at any alignment of an element
+template <class T, class S>
+struct piece {
+    static constexpr int E = 16 / sizeof(T);
+    typedef S sv __attribute__((ext_vector_type(E), aligned(sizeof(S))));
+    sv q;
+    // elements c E .. of the row p [d]; past the end: 0
+    __device__ __forceinline__ void load(const S *p, int c, int d)
+    {
+        const int at = c * E, left = d - at;
+        if (left >= E) {
+            q = *(const sv *)(p + at);
+        } else {
+            q = sv{};
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e < left)
+                    q[e] = p[at + e];
+        }
+    }
+    __device__ __forceinline__ float operator[](int e) const { return (float)q[e]; }
+    // new to the compiler: the values read from here on are converted anew, where
+    // those converted before would be kept in twice the registers
+    __device__ __forceinline__ void again()
+    {
+        typedef uint32_t words __attribute__((ext_vector_type(sizeof(sv) / 4)));
+        words v = __builtin_bit_cast(words, q);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(sv) / 4); ++i) {
+            uint32_t one = v[i];
+            __asm__("" : "+v"(one));
+            v[i] = one;
+        }
+        q = __builtin_bit_cast(sv, v);
+    }
+};
+
+// the same as f32
 template <class T>
 struct chunk {
     static constexpr int E = 16 / sizeof(T);
     float v[E];
-    template <class S> // elements c E .. of the row p [d]; past the end: 0
+    template <class S>
     __device__ __forceinline__ void load(const S *p, int c, int d)
     {
-        typedef S sv __attribute__((ext_vector_type(E), aligned(sizeof(S))));
-        const int at = c * E, left = d - at;
-        if (left >= E) {
-            const sv q = *(const sv *)(p + at);
+        piece<T, S> q;
+        q.load(p, c, d);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                v[e] = (float)q[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                v[e] = e < left ? (float)p[at + e] : 0.0f;
-        }
+        for (int e = 0; e < E; ++e)
+            v[e] = q[e];
     }
     template <class O>
     __device__ __forceinline__ void store(O *p, int c, int d) const
@@ -99,9 +129,10 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float (*red)[N], int tid)
 
 // ---------------------------------------------------------------- rows that a block holds
 
-// TPR threads per row, kChunks chunks each; a block of 256 threads takes 256 / TPR
-// rows, one of 1024 threads one.
-template <class T, class O, int TPR>
+// TPR threads per row, R chunks each; a block of 256 threads takes 256 / TPR rows at a
+// time, one of 1024 threads one.  The next rows are on their way while a row is
+// worked on; HOLD: the weights stay in registers.
+template <class T, class O, int TPR, int R, bool HOLD>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, const float *__restrict__ w,
                                                                 const float *__restrict__ b, float eps, size_t m, int d,
                                                                 O *y, float *__restrict__ stats)
@@ -111,159 +142,193 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
     __shared__ float red[4][TPR > 64 ? TPR / 64 : 1][1];
     const int tid = (int)threadIdx.x, lane = tid % TPR;
     const int nc = (d + ch::E - 1) / ch::E;
+    const float inv = 1.0f / (float)d;
+    ch wv[HOLD ? R : 1], bv[HOLD ? R : 1];
+    auto weights = [&](int i, ch &wi, ch &bi) {
+        const int c = lane + i * TPR;
+        if (w && c < nc)
+            wi.load(w, c, d);
+        else
+            wi.fill(1.0f);
+        if (b && c < nc)
+            bi.load(b, c, d);
+        else
+            bi.fill(0.0f);
+    };
+    piece<T, T> cur[R];
+    auto ask = [&](size_t row, piece<T, T>(&q)[R]) {
+        const T *p = x + row * d;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            q[i].q = {};
+            if (row < m && lane + i * TPR < nc)
+                q[i].load(p, lane + i * TPR, d);
+        }
+    };
+    const size_t step = (size_t)gridDim.x * RPB;
+    size_t row = (size_t)blockIdx.x * RPB + tid / TPR;
+    ask(row, cur);
+    if constexpr (HOLD)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            weights(i, wv[i], bv[i]);
     int turn = 0;
-    for (size_t r0 = (size_t)blockIdx.x * RPB; r0 < m; r0 += (size_t)gridDim.x * RPB, turn ^= 2) {
-        const size_t row = r0 + tid / TPR;
-        const bool in = row < m;
-        const T *p = x + (in ? row : 0) * d;
-        ch v[kChunks];
+    for (size_t r0 = (size_t)blockIdx.x * RPB; r0 < m; r0 += step, row += step, turn ^= 2) {
+        piece<T, T> next[R];
+        if (r0 + step < m)
+            ask(row + step, next);
         float s[1] = {0.0f};
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i)
-            if (lane + i * TPR < nc)
-                v[i].load(p, lane + i * TPR, d);
-            else
-                v[i].fill(0.0f);
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int e = 0; e < ch::E; ++e)
-                s[0] += v[i].v[e];
+                s[0] += cur[i][e];
         row_sum<TPR>(s, red[turn], tid);
         const float mean = s[0] / (float)d;
         s[0] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i)
+        for (int i = 0; i < R; ++i) {
+            cur[i].again();
+            const bool whole = (lane + i * TPR + 1) * ch::E <= d;
 #pragma unroll
             for (int e = 0; e < ch::E; ++e) {
-                const float c = v[i].v[e] - mean;
-                s[0] += (lane + i * TPR) * ch::E + e < d ? c * c : 0.0f;
+                const float c = cur[i][e] - mean;
+                s[0] += whole || (lane + i * TPR) * ch::E + e < d ? c * c : 0.0f;
             }
-        row_sum<TPR>(s, red[turn + 1], tid);
-        const float rstd = 1.0f / sqrtf(s[0] / (float)d + eps);
-        if (!in)
-            continue;
-        if (stats && lane == 0)
-            *(float2 *)(stats + row * 2) = make_float2(mean, rstd);
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int c = lane + i * TPR;
-            if (c >= nc)
-                break;
-            ch wv, bv;
-            if (w)
-                wv.load(w, c, d);
-            else
-                wv.fill(1.0f);
-            if (b)
-                bv.load(b, c, d);
-            else
-                bv.fill(0.0f);
-#pragma unroll
-            for (int e = 0; e < ch::E; ++e)
-                v[i].v[e] = (v[i].v[e] - mean) * rstd * wv.v[e] + bv.v[e];
-            v[i].store(y + row * d, c, d);
         }
+        row_sum<TPR>(s, red[turn + 1], tid);
+        const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+        if (row < m) {
+            if (stats && lane == 0)
+                *(float2 *)(stats + row * 2) = make_float2(mean, rstd);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int c = lane + i * TPR;
+                if (c >= nc)
+                    break;
+                if constexpr (!HOLD)
+                    weights(i, wv[0], bv[0]);
+                cur[i].again();
+                ch o;
+#pragma unroll
+                for (int e = 0; e < ch::E; ++e)
+                    o.v[e] = (cur[i][e] - mean) * rstd * wv[HOLD ? i : 0].v[e] + bv[HOLD ? i : 0].v[e];
+                o.store(y + row * d, c, d);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            cur[i] = next[i];
     }
 }
 
 // The grads of a block's rows: dx, and the block's own sums of dw and db to part
-// [blocks][2][d] (NULL: not wanted), each thread those of its own columns.
-template <class T, class G, class O, int TPR>
-__global__ void __launch_bounds__(256) k_norm_bwd(const T *__restrict__ x, const float *__restrict__ w,
-                                                  const float *__restrict__ stats, const G *__restrict__ dy, size_t m,
-                                                  int d, O *__restrict__ dx, int beta, float *__restrict__ part)
+// [blocks][2][d] (NULL: not wanted), each thread those of its own columns.  The
+// next rows are on their way while a row is worked on.
+template <class T, class G, class O, int TPR, int R>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_bwd(const T *__restrict__ x, const float *__restrict__ w,
+                                                     const float *__restrict__ stats, const G *__restrict__ dy, size_t m,
+                                                     int d, O *__restrict__ dx, int beta, float *__restrict__ part)
 {
     using ch = chunk<T>;
-    constexpr int RPB = 256 / TPR, COLS = TPR * kChunks * ch::E;
+    constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR, COLS = TPR * R * ch::E;
     __shared__ float red[2][TPR > 64 ? TPR / 64 : 1][2];
     __shared__ float sums[RPB > 1 ? RPB : 1][RPB > 1 ? COLS : 1];
     const int tid = (int)threadIdx.x, lane = tid % TPR, group = tid / TPR;
     const int nc = (d + ch::E - 1) / ch::E;
     const float inv = 1.0f / (float)d;
-    ch gw[kChunks], gb[kChunks];
+    ch gw[R], gb[R], wv[R];
+    struct rows {
+        piece<T, T> x[R];
+        piece<T, G> dy[R];
+        float2 st;
+    } cur;
+    auto ask = [&](size_t row, rows &q) { // (past the end of a row and of all rows dy is 0)
+        const size_t at = row * d;
+        q.st = row < m ? *(const float2 *)(stats + row * 2) : make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-        gw[i].fill(0.0f);
-        gb[i].fill(0.0f);
-    }
-    int turn = 0;
-    for (size_t r0 = (size_t)blockIdx.x * RPB; r0 < m; r0 += (size_t)gridDim.x * RPB, turn ^= 1) {
-        const size_t row = r0 + group;
-        const bool in = row < m;
-        const size_t at = (in ? row : 0) * d;
-        const float2 st = in ? *(const float2 *)(stats + row * 2) : make_float2(0.0f, 0.0f);
-        ch n[kChunks], h[kChunks];
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
+        for (int i = 0; i < R; ++i) {
             const int c = lane + i * TPR;
-            if (in && c < nc) {
-                n[i].load(x + at, c, d);
-                h[i].load(dy + at, c, d);
-            } else {
-                n[i].fill(st.x);
-                h[i].fill(0.0f);
+            q.x[i].q = {};
+            q.dy[i].q = {};
+            if (row < m && c < nc) {
+                q.x[i].load(x + at, c, d);
+                q.dy[i].load(dy + at, c, d);
             }
         }
+    };
+    const size_t step = (size_t)gridDim.x * RPB;
+    size_t row = (size_t)blockIdx.x * RPB + group;
+    ask(row, cur);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        gw[i].fill(0.0f);
+        gb[i].fill(0.0f);
+        if (w && lane + i * TPR < nc)
+            wv[i].load(w, lane + i * TPR, d);
+        else
+            wv[i].fill(1.0f);
+    }
+    int turn = 0;
+    for (size_t r0 = (size_t)blockIdx.x * RPB; r0 < m; r0 += step, row += step, turn ^= 1) {
+        rows next;
+        if (r0 + step < m)
+            ask(row + step, next);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int c = lane + i * TPR;
-            ch wv;
-            if (w && c < nc)
-                wv.load(w, c, d);
-            else
-                wv.fill(1.0f);
+        for (int i = 0; i < R; ++i) {
+            const bool whole = (lane + i * TPR + 1) * ch::E <= d;
 #pragma unroll
             for (int e = 0; e < ch::E; ++e) {
-                // (past the end of a row dy is 0 and n is never stored)
-                const float g = h[i].v[e];
-                n[i].v[e] = c * ch::E + e < d ? (n[i].v[e] - st.x) * st.y : 0.0f;
-                gw[i].v[e] += g * n[i].v[e];
+                const float g = cur.dy[i][e], h = g * wv[i].v[e];
+                const float n = whole || (lane + i * TPR) * ch::E + e < d ? (cur.x[i][e] - cur.st.x) * cur.st.y : 0.0f;
+                gw[i].v[e] += g * n;
                 gb[i].v[e] += g;
-                h[i].v[e] = g * wv.v[e];
-                s[0] += h[i].v[e];
-                s[1] += h[i].v[e] * n[i].v[e];
+                s[0] += h;
+                s[1] += h * n;
             }
         }
         row_sum<TPR>(s, red[turn], tid);
-        if (!dx || !in)
-            continue;
-        const float c1 = s[0] * inv, c2 = s[1] * inv;
+        if (dx && row < m) {
+            const float c1 = s[0] * inv, c2 = s[1] * inv;
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int c = lane + i * TPR;
-            if (c >= nc)
-                break;
-            ch o;
-            if (beta)
-                o.load(dx + at, c, d);
-            else
-                o.fill(0.0f);
+            for (int i = 0; i < R; ++i) {
+                const int c = lane + i * TPR;
+                if (c >= nc)
+                    break;
+                cur.x[i].again();
+                cur.dy[i].again();
+                ch o;
+                if (beta)
+                    o.load(dx + row * d, c, d);
+                else
+                    o.fill(0.0f);
 #pragma unroll
-            for (int e = 0; e < ch::E; ++e)
-                o.v[e] += st.y * (h[i].v[e] - c1 - n[i].v[e] * c2);
-            o.store(dx + at, c, d);
+                for (int e = 0; e < ch::E; ++e)
+                    o.v[e] += cur.st.y * (cur.dy[i][e] * wv[i].v[e] - c1 - (cur.x[i][e] - cur.st.x) * cur.st.y * c2);
+                o.store(dx + row * d, c, d);
+            }
         }
+        cur = next;
     }
     if (!part)
         return;
     // the groups' sums of a column in the groups' order
-    auto leave = [&](ch(&g)[kChunks], float *out) {
+    auto leave = [&](ch(&g)[R], float *out) {
         if constexpr (RPB == 1) {
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i)
+            for (int i = 0; i < R; ++i)
                 if (lane + i * TPR < nc)
                     g[i].store(out, lane + i * TPR, d);
         } else {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i)
+            for (int i = 0; i < R; ++i)
 #pragma unroll
                 for (int e = 0; e < ch::E; ++e)
                     sums[group][(lane + i * TPR) * ch::E + e] = g[i].v[e];
             __syncthreads();
-            for (int c = tid; c < d; c += 256) {
+            for (int c = tid; c < d; c += NT) {
                 float t = 0.0f;
 #pragma unroll 4
                 for (int r = 0; r < RPB; ++r)
@@ -277,14 +342,16 @@ __global__ void __launch_bounds__(256) k_norm_bwd(const T *__restrict__ x, const
     leave(gb, out + d);
 }
 
-// dw and db (either NULL) from the blocks' sums, in a fixed order: 16 threads
-// take every 16th block's of a column
-__global__ void __launch_bounds__(1024) k_norm_fin(const float *__restrict__ part, int blocks, int d, float *dw, int beta_w,
-                                                   float *db, int beta_b)
+// dw and db (either NULL) from the blocks' sums [blocks][2][d], in a fixed order: 64
+// columns of one of them a job, NT / 64 threads taking every (NT / 64)'th block's
+template <int NT>
+__device__ __forceinline__ void join_sums(const float *__restrict__ part, int blocks, int d, int job, float *dw, int beta_w,
+                                          float *db, int beta_b)
 {
-    __shared__ float s[16][64];
-    const int col = (int)blockIdx.x * 64 + ((int)threadIdx.x & 63), k = (int)threadIdx.x >> 6;
-    const bool second = blockIdx.y != 0;
+    constexpr int K = NT / 64;
+    __shared__ float s[K][64];
+    const int across = (d + 63) / 64, col = job % across * 64 + ((int)threadIdx.x & 63), k = (int)threadIdx.x >> 6;
+    const bool second = job >= across;
     float *out = second ? db : dw;
     const int beta = second ? beta_b : beta_w;
     if (!out)
@@ -292,8 +359,8 @@ __global__ void __launch_bounds__(1024) k_norm_fin(const float *__restrict__ par
     float t = 0.0f;
     if (col < d) {
         const float *p = part + (second ? d : 0) + col;
-#pragma unroll 4
-        for (int i = k; i < blocks; i += 16)
+#pragma unroll 16
+        for (int i = k; i < blocks; i += K)
             t += p[(size_t)i * 2 * d];
     }
     s[k][threadIdx.x & 63] = t;
@@ -302,9 +369,14 @@ __global__ void __launch_bounds__(1024) k_norm_fin(const float *__restrict__ par
         return;
     t = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < K; ++i)
         t += s[i][threadIdx.x];
     out[col] = beta ? out[col] + t : t;
+}
+__global__ void __launch_bounds__(1024) k_norm_fin(const float *__restrict__ part, int blocks, int d, float *dw, int beta_w,
+                                                   float *db, int beta_b)
+{
+    join_sums<1024>(part, blocks, d, (int)blockIdx.x, dw, beta_w, db, beta_b);
 }
 
 // ---------------------------------------------------------------- longer rows, in slices
@@ -443,110 +515,127 @@ __global__ void __launch_bounds__(256) k_norm_long(const T *x, const float *__re
     }
 }
 
-// each slice's sums of h and h n
+// What the backward sums: a block owns 256 chunks of columns and every gridDim.y'th row,
+// four of them on their way at a time.  Each row's sums of h and h n over these
+// columns go to rows [m][gridDim.x], the block's own of dw and db (unless NULL) to
+// part [gridDim.y][2][d].
 template <class T, class G>
-__global__ void __launch_bounds__(256) k_norm_bwd_slices(const T *__restrict__ x, const float *__restrict__ w,
-                                                         const float *__restrict__ stats, const G *__restrict__ dy,
-                                                         size_t m, int d, int slices, float2 *__restrict__ part)
+__global__ void __launch_bounds__(256) k_norm_sums(const T *__restrict__ x, const float *__restrict__ w,
+                                                   const float *__restrict__ stats, const G *__restrict__ dy, size_t m, int d,
+                                                   float2 *__restrict__ rows, float *__restrict__ part)
 {
     using ch = chunk<T>;
-    __shared__ float red[2][4][2];
-    const int tid = (int)threadIdx.x;
+    constexpr int U = 4;
+    __shared__ float red[2][4][2 * U];
+    const int tid = (int)threadIdx.x, c = (int)blockIdx.x * 256 + tid;
+    ch gw, gb, wv;
+    gw.fill(0.0f);
+    gb.fill(0.0f);
+    wv.fill(1.0f);
+    const bool in = c * ch::E < d, whole = (c + 1) * ch::E <= d;
+    if (w && in)
+        wv.load(w, c, d);
     int turn = 0;
-    for (size_t job = blockIdx.x; job < m * slices; job += gridDim.x, turn ^= 1) {
+    for (size_t r0 = blockIdx.y; r0 < m; r0 += (size_t)gridDim.y * U, turn ^= 1) {
+        piece<T, T> n[U];
+        piece<T, G> g[U];
+        float2 st[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t row = r0 + (size_t)u * gridDim.y;
+            n[u].q = {};
+            g[u].q = {};
+            st[u] = make_float2(0.0f, 0.0f);
+            if (row < m && in) {
+                n[u].load(x + row * d, c, d);
+                g[u].load(dy + row * d, c, d);
+                st[u] = *(const float2 *)(stats + row * 2);
+            }
+        }
+        float s[2 * U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[2 * u] = s[2 * u + 1] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < ch::E; ++e) {
+                const float f = whole || c * ch::E + e < d ? (n[u][e] - st[u].x) * st[u].y : 0.0f, h = g[u][e] * wv.v[e];
+                gw.v[e] += g[u][e] * f;
+                gb.v[e] += g[u][e];
+                s[2 * u] += h;
+                s[2 * u + 1] += h * f;
+            }
+        }
+        row_sum<256>(s, red[turn], tid);
+        if (tid < U) {
+            const size_t row = r0 + (size_t)tid * gridDim.y;
+            if (row < m) {
+                float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (u == tid)
+                        v = make_float2(s[2 * u], s[2 * u + 1]);
+                rows[row * gridDim.x + blockIdx.x] = v;
+            }
+        }
+    }
+    if (part && in) {
+        float *out = part + (size_t)blockIdx.y * 2 * d;
+        gw.store(out, c, d);
+        gb.store(out + d, c, d);
+    }
+}
+
+// dx of a slice, and behind the slices' blocks the joining of dw and db
+template <class T, class G, class O>
+__global__ void __launch_bounds__(256) k_norm_bwd_long(const T *__restrict__ x, const float *__restrict__ w,
+                                                       const float *__restrict__ stats, const G *__restrict__ dy, size_t m,
+                                                       int d, int slices, int blocks, const float2 *__restrict__ rows,
+                                                       int across, O *__restrict__ dx, int beta,
+                                                       const float *__restrict__ part, int parts, float *dw, int beta_w,
+                                                       float *db, int beta_b)
+{
+    using ch = chunk<T>;
+    if ((int)blockIdx.x >= blocks) {
+        join_sums<256>(part, parts, d, (int)blockIdx.x - blocks, dw, beta_w, db, beta_b);
+        return;
+    }
+    const int tid = (int)threadIdx.x, lane = tid & 63;
+    const float inv = 1.0f / (float)d;
+    for (size_t job = blockIdx.x; job < m * slices; job += blocks) {
         const size_t row = job / slices;
         const int first = (int)(job - row * slices) * kSlice<T>, len = d - first < kSlice<T> ? d - first : kSlice<T>;
         const size_t at = row * d + first;
         const int nc = (len + ch::E - 1) / ch::E;
-        const float2 st = *(const float2 *)(stats + row * 2);
-        float s[2] = {0.0f, 0.0f};
+        piece<T, T> n[kChunks];
+        piece<T, G> g[kChunks];
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int c = tid + i * 256;
-            if (c >= nc)
-                break;
-            ch n, h, wv;
-            n.load(x + at, c, len);
-            h.load(dy + at, c, len);
-            if (w)
-                wv.load(w + first, c, len);
-            else
-                wv.fill(1.0f);
-#pragma unroll
-            for (int e = 0; e < ch::E; ++e)
-                if (c * ch::E + e < len) {
-                    const float f = h.v[e] * wv.v[e];
-                    s[0] += f;
-                    s[1] += f * ((n.v[e] - st.x) * st.y);
-                }
-        }
-        row_sum<256>(s, red[turn], tid);
-        if (tid == 0)
-            part[job] = make_float2(s[0], s[1]);
-    }
-}
-
-// A block owns a slice's columns and every gridDim.y'th row; its sums of dw and db
-// to part [gridDim.y][2][d].
-template <class T, class G, class O>
-__global__ void __launch_bounds__(256) k_norm_bwd_long(const T *__restrict__ x, const float *__restrict__ w,
-                                                       const float *__restrict__ stats, const G *__restrict__ dy, size_t m,
-                                                       int d, int slices, const float2 *__restrict__ sums,
-                                                       O *__restrict__ dx, int beta, float *__restrict__ part)
-{
-    using ch = chunk<T>;
-    const int tid = (int)threadIdx.x, lane = tid & 63, first = (int)blockIdx.x * kSlice<T>;
-    const int len = d - first < kSlice<T> ? d - first : kSlice<T>, nc = (len + ch::E - 1) / ch::E;
-    const float inv = 1.0f / (float)d;
-    ch gw[kChunks], gb[kChunks];
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-        gw[i].fill(0.0f);
-        gb[i].fill(0.0f);
-    }
-    for (size_t row = blockIdx.y; row < m; row += gridDim.y) {
-        const size_t at = row * d + first;
-        const float2 st = *(const float2 *)(stats + row * 2);
-        float2 s = make_float2(0.0f, 0.0f);
-        if (dx)
-            s = slice_sums(sums + row * slices, slices, lane);
+        for (int i = 0; i < kChunks; ++i)
+            if (tid + i * 256 < nc) {
+                n[i].load(x + at, tid + i * 256, len);
+                g[i].load(dy + at, tid + i * 256, len);
+            }
+        const float2 st = *(const float2 *)(stats + row * 2), s = slice_sums(rows + row * across, across, lane);
         const float c1 = s.x * inv, c2 = s.y * inv;
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) {
             const int c = tid + i * 256;
             if (c >= nc)
                 break;
-            ch n, h, wv, o;
-            n.load(x + at, c, len);
-            h.load(dy + at, c, len);
+            ch wv, o;
             if (w)
                 wv.load(w + first, c, len);
             else
                 wv.fill(1.0f);
-            if (dx && beta)
+            if (beta)
                 o.load(dx + at, c, len);
             else
                 o.fill(0.0f);
 #pragma unroll
-            for (int e = 0; e < ch::E; ++e) {
-                const float f = (n.v[e] - st.x) * st.y, g = h.v[e];
-                gw[i].v[e] += g * f;
-                gb[i].v[e] += g;
-                o.v[e] += st.y * (g * wv.v[e] - c1 - f * c2);
-            }
-            if (dx)
-                o.store(dx + at, c, len);
+            for (int e = 0; e < ch::E; ++e)
+                o.v[e] += st.y * (g[i][e] * wv.v[e] - c1 - (n[i][e] - st.x) * st.y * c2);
+            o.store(dx + at, c, len);
         }
     }
-    if (!part)
-        return;
-    float *out = part + (size_t)blockIdx.y * 2 * d + first;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i)
-        if (tid + i * 256 < nc) {
-            gw[i].store(out, tid + i * 256, len);
-            gb[i].store(out + d, tid + i * 256, len);
-        }
 }
 
 // ---------------------------------------------------------------- launches
@@ -557,24 +646,41 @@ size_t slices_of(int dtype, size_t d) { return (chunks(dtype, d) + 256 * kChunks
 
 unsigned grid_of(size_t n) { return (unsigned)(n < kMostBlocks ? n : kMostBlocks); }
 
-// threads per row, of the rows that 1024 (forward) or 256 threads (backward)
-// hold; 0: longer
-int threads_per_row(size_t c, bool backward)
+// Threads per row, of two chunks each (more would not leave registers for the next
+// row), as the row's c chunks need them; 1024 of up to eight each for many longer rows
+// of the forward (a block's row of 50000 takes 15 us, so that slices of it on every CU
+// are faster for few).  0: slices.
+int threads_per_row(size_t m, size_t c, bool backward)
 {
-    return c <= 8 * kChunks ? 8 : c <= 64 * kChunks ? 64 : c <= 256 * kChunks ? 256 : !backward && c <= 1024 * kChunks ? 1024 : 0;
+    return c <= 8 * 2 ? 8 : c <= 64 * 2 ? 64 : c <= 256 * 2 ? 256 : c <= 512 * 2 ? 512 : !backward && c <= 1024 * 8 && m >= 256 ? 1024 : 0;
+}
+template <class FN>
+void by_row(int tpr, FN fn)
+{
+    using std::integral_constant;
+    if (tpr == 8)
+        fn(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+    else if (tpr == 64)
+        fn(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    else if (tpr == 256)
+        fn(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    else
+        fn(integral_constant<int, 512>{}, integral_constant<int, 2>{});
 }
 
-// blocks of the backward: each leaves its sums of 2 d floats, so no more than two per CU
+// Blocks of the backward, each of which leaves its sums of 2 d floats: two per CU, of
+// the longest rows one (8192 x 8192 in bf16: 94 us, with two 101, with four 115)
 size_t bwd_blocks(size_t m, int tpr)
 {
-    const size_t rows = 256 / tpr, n = (m + rows - 1) / rows;
-    return n < 512 ? n : 512;
+    const size_t rows = tpr < 256 ? 256 / tpr : 1, n = (m + rows - 1) / rows, most = tpr == 512 ? 256 : 512;
+    return n < most ? n : most;
 }
-// row groups of the backward of long rows: some 1024 blocks
-size_t long_groups(size_t m, size_t slices)
+// row groups of the sums of longer rows: some 512 blocks, four rows each at least
+size_t across_of(int dtype, size_t d) { return (chunks(dtype, d) + 255) / 256; }
+size_t long_groups(int dtype, size_t m, size_t d)
 {
-    const size_t n = slices < 1024 ? 1024 / slices : 1;
-    return m < n ? m : n;
+    const size_t a = across_of(dtype, d), n = a < 512 ? 512 / a : 1, most = (m + 3) / 4;
+    return most < n ? most : n;
 }
 
 template <class FN>
@@ -592,22 +698,24 @@ int type_or_f32(int dtype, FN fn)
 template <class T, class O>
 int forward(const pgk_norm_args &a, const T *x, O *y, float2 *ws, hipStream_t st)
 {
-    const int tpr = threads_per_row(chunks(a.dtype, a.d), false);
+    const size_t c = chunks(a.dtype, a.d);
+    const int tpr = threads_per_row(a.m, c, false);
     if (tpr) {
         const int nt = tpr < 256 ? 256 : tpr;
-        const dim3 grid(grid_of((a.m + nt / tpr - 1) / (nt / tpr)));
-        auto go = [&](auto n) {
-            hipLaunchKernelGGL((k_norm<T, O, decltype(n)::value>), grid, dim3(nt), 0, st, x, a.w, a.b, a.eps, a.m, (int)a.d, y,
+        // a few rows to a block, so that the weights are read less often than x
+        const size_t blocks = (a.m + nt / tpr - 1) / (nt / tpr), most = 2048 * 256 / nt;
+        const dim3 grid((unsigned)(blocks < most ? blocks : most));
+        auto go = [&](auto n, auto r) {
+            constexpr int TPR = decltype(n)::value, R = decltype(r)::value;
+            hipLaunchKernelGGL((k_norm<T, O, TPR, R, (TPR < 1024)>), grid, dim3(nt), 0, st, x, a.w, a.b, a.eps, a.m, (int)a.d, y,
                                a.stats);
         };
-        if (tpr == 8)
-            go(std::integral_constant<int, 8>{});
-        else if (tpr == 64)
-            go(std::integral_constant<int, 64>{});
-        else if (tpr == 256)
-            go(std::integral_constant<int, 256>{});
+        if (tpr < 1024)
+            by_row(tpr, go);
+        else if (c <= 1024 * 4)
+            go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
         else
-            go(std::integral_constant<int, 1024>{});
+            go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
         return (int)hipGetLastError();
     }
     const size_t slices = slices_of(a.dtype, a.d);
@@ -623,41 +731,34 @@ int forward(const pgk_norm_args &a, const T *x, O *y, float2 *ws, hipStream_t st
 template <class T, class G, class O>
 int backward(const pgk_norm_args &a, const T *x, const G *dy, O *dx, void *ws, hipStream_t st)
 {
-    const int tpr = threads_per_row(chunks(a.dtype, a.d), true);
+    const int tpr = threads_per_row(a.m, chunks(a.dtype, a.d), true);
     const bool sums = a.dw || a.db;
-    size_t parts;
-    float *part = NULL;
+    const int fin = sums ? 2 * (int)((a.d + 63) / 64) : 0;
     if (tpr) {
-        parts = bwd_blocks(a.m, tpr);
-        part = sums ? (float *)ws : NULL;
-        auto go = [&](auto n) {
-            hipLaunchKernelGGL((k_norm_bwd<T, G, O, decltype(n)::value>), dim3((unsigned)parts), dim3(256), 0, st, x, a.w,
-                               a.stats, dy, a.m, (int)a.d, dx, a.beta_x, part);
-        };
-        if (tpr == 8)
-            go(std::integral_constant<int, 8>{});
-        else if (tpr == 64)
-            go(std::integral_constant<int, 64>{});
-        else
-            go(std::integral_constant<int, 256>{});
-    } else {
-        const size_t slices = slices_of(a.dtype, a.d);
-        float2 *const s = (float2 *)ws;
-        parts = long_groups(a.m, slices);
-        part = sums ? (float *)(s + a.m * slices) : NULL;
-        if (dx)
-            hipLaunchKernelGGL((k_norm_bwd_slices<T, G>), dim3(grid_of(a.m * slices)), dim3(256), 0, st, x, a.w, a.stats, dy,
-                               a.m, (int)a.d, (int)slices, s);
+        const size_t parts = bwd_blocks(a.m, tpr);
+        float *const part = sums ? (float *)ws : NULL;
+        by_row(tpr, [&](auto n, auto r) {
+            hipLaunchKernelGGL((k_norm_bwd<T, G, O, decltype(n)::value, decltype(r)::value>), dim3((unsigned)parts),
+                               dim3(tpr < 256 ? 256 : tpr), 0, st, x, a.w, a.stats, dy, a.m, (int)a.d, dx, a.beta_x, part);
+        });
         if (const int rc = (int)hipGetLastError())
             return rc;
-        hipLaunchKernelGGL((k_norm_bwd_long<T, G, O>), dim3((unsigned)slices, (unsigned)parts), dim3(256), 0, st, x, a.w,
-                           a.stats, dy, a.m, (int)a.d, (int)slices, s, dx, a.beta_x, part);
+        if (sums)
+            hipLaunchKernelGGL(k_norm_fin, dim3((unsigned)fin), dim3(1024), 0, st, part, (int)parts, (int)a.d, a.dw, a.beta_w,
+                               a.db, a.beta_b);
+        return (int)hipGetLastError();
     }
+    const size_t slices = slices_of(a.dtype, a.d), across = across_of(a.dtype, a.d), groups = long_groups(a.dtype, a.m, a.d);
+    float2 *const rows = (float2 *)ws;
+    float *const part = sums ? (float *)(rows + a.m * across) : NULL;
+    hipLaunchKernelGGL((k_norm_sums<T, G>), dim3((unsigned)across, (unsigned)groups), dim3(256), 0, st, x, a.w, a.stats, dy, a.m,
+                       (int)a.d, rows, part);
     if (const int rc = (int)hipGetLastError())
         return rc;
-    if (sums)
-        hipLaunchKernelGGL(k_norm_fin, dim3((unsigned)((a.d + 63) / 64), 2), dim3(1024), 0, st, part, (int)parts, (int)a.d,
-                           a.dw, a.beta_w, a.db, a.beta_b);
+    const unsigned blocks = dx ? grid_of(a.m * slices) : 0;
+    hipLaunchKernelGGL((k_norm_bwd_long<T, G, O>), dim3(blocks + (unsigned)fin), dim3(256), 0, st, x, a.w, a.stats, dy, a.m,
+                       (int)a.d, (int)slices, (int)blocks, rows, (int)across, dx, a.beta_x, part, (int)groups, a.dw, a.beta_w,
+                       a.db, a.beta_b);
     return (int)hipGetLastError();
 }
 
@@ -667,7 +768,7 @@ bool fits(const pgk_norm_args *a) { return a->m && a->m <= 0x7fffffff && a->d &&
 
 extern "C" size_t pgk_norm_workspace(int dtype, size_t m, size_t d)
 {
-    return threads_per_row(chunks(dtype, d), false) ? 0 : m * slices_of(dtype, d) * sizeof(float2);
+    return threads_per_row(m, chunks(dtype, d), false) ? 0 : m * slices_of(dtype, d) * sizeof(float2);
 }
 
 extern "C" int pgk_norm(const pgk_norm_args *a, void *ws, pgk_stream s)
@@ -684,11 +785,10 @@ extern "C" int pgk_norm(const pgk_norm_args *a, void *ws, pgk_stream s)
 
 extern "C" size_t pgk_norm_bwd_workspace(int dtype, size_t m, size_t d, int sums)
 {
-    const int tpr = threads_per_row(chunks(dtype, d), true);
+    const int tpr = threads_per_row(m, chunks(dtype, d), true);
     if (tpr)
         return sums ? bwd_blocks(m, tpr) * 2 * d * sizeof(float) : 0;
-    const size_t slices = slices_of(dtype, d);
-    return m * slices * sizeof(float2) + (sums ? long_groups(m, slices) * 2 * d * sizeof(float) : 0);
+    return m * across_of(dtype, d) * sizeof(float2) + (sums ? long_groups(dtype, m, d) * 2 * d * sizeof(float) : 0);
 }
 
 extern "C" int pgk_norm_bwd(const pgk_norm_args *a, void *ws, pgk_stream s)
