@@ -540,9 +540,10 @@ __global__ void __launch_bounds__(CF::NT, 1) k_ns_join(TAB t)
 
 // Short sides of up to 64, long ones of up to NP: everything in LDS, X as rows of
 // both sides so that each product's operands lie along its reduction.  Sixteen
-// waves, one 16 x 16 tile of S and B each.  Bound by the chain of dependent
-// products: 64 x 64 in five steps takes 15 of them, where launches of their own
-// take 4 us each.
+// waves, one 16 x 16 tile of S and B each, which keep their tiles of S and X in f32
+// beside the pieces that the others read; tiles and parts of the reduction past the
+// matrix's own sizes are left out.  Bound by the chain of dependent products: 64 x 64
+// in five steps takes 15 of them, where launches of their own take 4 us each.
 constexpr int kSmallM = 64, kSmallN = 256;
 
 __device__ __forceinline__ f32x4 mma16(const uint4 &a, const uint4 &b, const f32x4 &c)
@@ -559,17 +560,20 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
     __shared__ double sums[16];
     uint16_t *const X = (uint16_t *)mem, *const Y = X + 2 * XP, *const S = Y + 2 * YP;
     const pgk_muon_seg &s = t.seg[blockIdx.x];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
+    const int tid = (int)threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6); // (uniform to the compiler: matrix instructions heed no mask)
     const int rows = (int)s.rows, cols = (int)s.cols;
     const bool tall = rows > cols;
-    for (int i = tid; i < (2 * XP + 2 * YP) / 8; i += 1024)
+    const int sm = tall ? cols : rows, sn = tall ? rows : cols;
+    for (int i = tid; i < (2 * XP + 2 * YP + 2 * SP) / 8; i += 1024)
         mem[i] = make_uint4(0, 0, 0, 0);
-    // up to four pieces of four values a thread
+    // up to Q pieces of four values a thread
+    constexpr int Q = M * NP / 4096;
     const int per = (cols + 3) / 4;
-    float u[4][4];
+    float u[Q][4];
     double sum = 0.0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < Q; ++q) {
         const int at = tid + q * 1024, row = at / per, col = (at - row * per) * 4;
         if (row >= rows)
             break;
@@ -603,7 +607,7 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
         sum += sums[w];
     const double scale = sum == 0.0 ? 0.0 : (double)kUnit / sqrt(sum);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < Q; ++q) {
         const int at = tid + q * 1024, row = at / per, col = (at - row * per) * 4;
         if (row >= rows)
             break;
@@ -620,13 +624,16 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
             }
     }
     __syncthreads();
-    // the sums over k of rows a0 + lr of A and b0 + lr of B: lane gets column lr of
-    // rows 4 lg .. + 3
-    auto product = [&](const uint16_t *A, int pa, int planeA, int a0, const uint16_t *B, int pb, int planeB, int b0, int k) {
+    // the sums over k <= MOST of rows a0 + lr of A and b0 + lr of B: lane gets column lr
+    // of rows 4 lg .. + 3
+    auto product = [&](const uint16_t *A, int pa, int planeA, int a0, const uint16_t *B, int pb, int planeB, int b0, auto most,
+                       int k) {
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         const uint16_t *const a = A + (a0 + lr) * pa + lg * 8, *const b = B + (b0 + lr) * pb + lg * 8;
 #pragma unroll
-        for (int i = 0; i < k; i += 32) {
+        for (int i = 0; i < decltype(most)::value; i += 32) {
+            if (i >= k)
+                break;
             const uint4 ah = *(const uint4 *)(a + i), al = *(const uint4 *)(a + planeA + i);
             const uint4 bh = *(const uint4 *)(b + i), bl = *(const uint4 *)(b + planeB + i);
             acc = mma16(ah, bh, acc);
@@ -635,47 +642,54 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
         }
         return acc;
     };
+    const std::integral_constant<int, M> along_m;
+    const std::integral_constant<int, NP> along_n;
     const int ti = wave >> 2 << 4, tj = (wave & 3) << 4;
+    const bool has_s = ti < sm && tj < sm; // a tile of S
+    auto has_x = [&](int j0) { return ti < sm && j0 < sn; };
     uint16_t *const mine = S + (tj + lr) * PM + ti + 4 * lg; // S and B are symmetric: down a column is along a row
-    for (int step = 0; step < steps; ++step) {
-        f32x4 v = product(X, PX, XP, ti, X, PX, XP, tj, NP) * (1.0f / kUnit);
-        store4(mine, SP, v);
-        __syncthreads();
-        v = product(S, PM, SP, ti, S, PM, SP, tj, M) * (1.0f / kUnit);
-        float x[4];
-        load4(mine, SP, x);
+    f32x4 x[T];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            v[e] = kB * x[e] + kC * v[e];
-        __syncthreads(); // S is read
-        store4(mine, SP, v);
+    for (int q = 0; q < T; ++q) {
+        float v[4];
+        load4(Y + (q * 64 + tj + lr) * PM + ti + 4 * lg, YP, v);
+        x[q] = f32x4{v[0], v[1], v[2], v[3]};
+    }
+    for (int step = 0; step < steps; ++step) {
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (has_s) {
+            v = product(X, PX, XP, ti, X, PX, XP, tj, along_n, sn) * (1.0f / kUnit);
+            store4(mine, SP, v);
+        }
         __syncthreads();
-        f32x4 next[T];
+        if (has_s)
+            v = kB * v + product(S, PM, SP, ti, S, PM, SP, tj, along_m, sm) * (kC / kUnit);
+        __syncthreads(); // S is read
+        if (has_s)
+            store4(mine, SP, v);
+        __syncthreads();
 #pragma unroll
         for (int q = 0; q < T; ++q) {
-            const int j0 = (tj >> 4) * (NP / 4) + q * 16;
-            next[q] = product(S, PM, SP, ti, Y, PM, YP, j0, M) * (1.0f / kUnit);
-            load4(Y + (j0 + lr) * PM + ti + 4 * lg, YP, x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                next[q][e] = kA * x[e] + next[q][e];
+            const int j0 = q * 64 + tj;
+            if (has_x(j0))
+                x[q] = kA * x[q] + product(S, PM, SP, ti, Y, PM, YP, j0, along_m, sm) * (1.0f / kUnit);
         }
         if (step + 1 == steps) {
 #pragma unroll
             for (int q = 0; q < T; ++q) {
-                const int i = ti + 4 * lg, j = (tj >> 4) * (NP / 4) + q * 16 + lr, m = tall ? cols : rows, n = tall ? rows : cols;
-                if (i >= m || j >= n)
+                const int i = ti + 4 * lg, j = q * 64 + tj + lr;
+                if (i >= sm || j >= sn)
                     continue;
                 if (tall) {
-                    const size_t at = (size_t)j * m + i;
-                    const int some = m - i < 4 ? m - i : 4;
-                    finish4(s, at, weights4(s, at, some), next[q], some);
+                    const size_t at = (size_t)j * sm + i;
+                    const int some = sm - i < 4 ? sm - i : 4;
+                    finish4(s, at, weights4(s, at, some), x[q], some);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (i + e < m) {
-                            const size_t at = (size_t)(i + e) * n + j;
-                            finish4(s, at, weights4(s, at, 1), f32x4{next[q][e], 0.0f, 0.0f, 0.0f}, 1);
+                        if (i + e < sm) {
+                            const size_t at = (size_t)(i + e) * sn + j;
+                            finish4(s, at, weights4(s, at, 1), f32x4{x[q][e], 0.0f, 0.0f, 0.0f}, 1);
                         }
                 }
             }
@@ -684,15 +698,17 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
         __syncthreads(); // X is read
 #pragma unroll
         for (int q = 0; q < T; ++q) {
-            const int j = (tj >> 4) * (NP / 4) + q * 16 + lr, i = ti + 4 * lg;
+            const int j0 = q * 64 + tj, j = j0 + lr, i = ti + 4 * lg;
+            if (!has_x(j0))
+                continue;
             uint16_t h[4], l[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                pieces(next[q][e], h[e], l[e]);
+                pieces(x[q][e], h[e], l[e]);
                 X[(i + e) * PX + j] = h[e];
                 X[XP + (i + e) * PX + j] = l[e];
             }
-            store4(Y + j * PM + i, YP, next[q]);
+            store4(Y + j * PM + i, YP, x[q]);
         }
         __syncthreads();
     }

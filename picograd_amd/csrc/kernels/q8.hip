@@ -24,18 +24,23 @@ constexpr size_t kMostBlocks = (size_t)1 << 20; // of a grid; kernels loop past 
 
 // ---------------------------------------------------------------- rounding
 
-// A code from 1 / s: fma with 1.5 2^23 rounds v / s to a whole number in the low
-// bits of the sum.  What is left over, v - q s, is exact in f32; where it reaches
-// s / 2 (a tie, or 1 / s on the wrong side of one) or s is next to the subnormals
-// the quotient is taken in 64 bits, which separates every quotient of two f32 from
-// a tie.
+// A code from 1 / s: fma with 1.5 2^23 rounds v / s to a whole number q in the low
+// bits of the sum.  What is left over, v - q s, is exact in f32 (a multiple of half
+// the last place of s, below s / 2 but for some units of it).  Where it reaches s / 2,
+// a tie or 1 / s on the wrong side of one, q moves by one towards v or to the even
+// one.  A scale next to the subnormals is taken with its values times 2^100; one
+// rounded there may leave v / s past 127.
 constexpr float kRound = 12582912.0f;
 constexpr float kLeastScale = 0x1p-120f;
 
-__device__ __forceinline__ uint32_t code_exact(float v, float s)
+// the code from v, s and t, the sum with kRound
+__device__ __forceinline__ uint32_t code_exact(float v, float s, float t)
 {
-    const double q = rint((double)v / (double)s);
-    return (uint32_t)(int)fmin(fmax(q, -127.0), 127.0);
+    float q = t - kRound;
+    const float r = fmaf(-q, s, v), a = fabsf(r), half = 0.5f * s;
+    const bool away = (a > half) | ((a == half) & (bool)(__float_as_uint(t) & 1));
+    q += away ? copysignf(1.0f, r) : 0.0f;
+    return (uint32_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
@@ -56,9 +61,10 @@ __device__ __forceinline__ uint4 codes16(const float (&v)[16], float s, float in
         b[i] = __float_as_uint(t);
     }
     if (!(worst < 0.5f * s) || s < kLeastScale) {
+        const float unit = s < kLeastScale ? 0x1p100f : 1.0f, su = s * unit, iu = s < kLeastScale ? 1.0f / su : inv;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            b[i] = code_exact(v[i], s);
+            b[i] = code_exact(v[i] * unit, su, fmaf(v[i] * unit, iu, kRound));
     }
     return make_uint4(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]), pack4(b[8], b[9], b[10], b[11]),
                       pack4(b[12], b[13], b[14], b[15]));
@@ -205,30 +211,34 @@ __global__ void __launch_bounds__(256) k_q8_tops(pgk_q8 q, const T *__restrict__
     }
 }
 
-// Codes of columns: a thread takes 16 bytes of 16 neighbouring rows of src, so that
-// it has a whole piece of each of its columns' codes; four lanes (two of 16-bit
-// types) side by side, the others down a wave, the waves below each other.  HELD:
-// a block holds its 16 columns whole (kHeld long) and finds their scales by itself,
-// src is read once; else the tops are there.  Bound by the stream of the source: 4096 x
-// 4096 in f32, 84 MB with the codes, 18.6 us; the search and the rounding in passes
-// of their own took 28.
+// Codes of columns: a thread takes C neighbours of 16 neighbouring rows of src, so that
+// it has a whole piece of each of its columns' codes; 16 / C lanes side by side, the
+// others down a wave, the waves below each other.  HELD: a block holds its 16 columns
+// whole (kHeld long) and finds their scales by itself, src is read once; else the
+// tops are there.  C is four, of 16-bit columns past 4096 eight (shorter ones' blocks
+// would have half the waves).  Bound by the stream of the source: 4096 x 4096 in f32, 84
+// MB with the codes, 22 us; the search and the rounding in passes of their own took 28.
 constexpr int kColumns = 16; // of a block
-template <class T>
-constexpr int kHeld = 64 / (kColumns * sizeof(T) / 16) * 16 * 16; // rows of 16 waves
+template <int C>
+constexpr int kHeld = 64 / (kColumns / C) * 16 * 16; // rows of 16 waves
 
-template <class T, bool HELD>
+template <class T, int C, bool HELD>
 __global__ void __launch_bounds__(1024, 1) k_q8_columns(pgk_q8 q, const T *__restrict__ src, const uint32_t *__restrict__ part,
                                                         int slabs, size_t nx, size_t ny)
 {
-    constexpr int C = 16 / sizeof(T), A = kColumns / C; // columns of a thread; lanes side by side
+    constexpr int A = kColumns / C; // lanes side by side
     typedef T tv __attribute__((ext_vector_type(C), aligned(sizeof(T))));
-    __shared__ uint32_t tops[16][kColumns];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
+    __shared__ uint32_t tops[2][kColumns];
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int lc = lane % A * C, lrow = (wave * (64 / A) + lane / A) * 16;
-    for (size_t job = blockIdx.x; job < nx * ny; job += gridDim.x) {
+    if (tid < kColumns)
+        tops[0][tid] = 0;
+    __syncthreads();
+    int turn = 0;
+    for (size_t job = blockIdx.x; job < nx * ny; job += gridDim.x, turn ^= 1) {
         // neighbouring columns share lines: on one XCD
         const size_t at = gridDim.x == nx * ny ? (size_t)xcd_tile((int)job, (int)gridDim.x) : job, x = at % nx;
-        const size_t col = x * kColumns + lc, k0 = at / nx * kHeld<T> + lrow;
+        const size_t col = x * kColumns + lc, k0 = at / nx * kHeld<C> + lrow;
         const int left = col < q.rows ? (int)(q.rows - col < C ? q.rows - col : C) : 0;
         tv raw[16];
 #pragma unroll
@@ -247,22 +257,28 @@ __global__ void __launch_bounds__(1024, 1) k_q8_columns(pgk_q8 q, const T *__res
             }
         }
         if constexpr (HELD) {
+            // magnitudes order as their bits do, in the source's own width
+            using B = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+            typedef B bits __attribute__((ext_vector_type(C)));
+            bits top = {};
 #pragma unroll
-            for (int e = 0; e < C; ++e) {
-                uint32_t top = 0;
+            for (int i = 0; i < 16; ++i)
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(bits, raw[i]) & (B)((B)~0u >> 1));
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t a = magnitude((float)raw[i][e]);
-                    top = a > top ? a : top;
-                }
+            for (int o = A; o < 64; o <<= 1) {
+                typedef int words __attribute__((ext_vector_type(sizeof(bits) / 4)));
+                words w = __builtin_bit_cast(words, top);
 #pragma unroll
-                for (int o = A; o < 64; o <<= 1) {
-                    const uint32_t a = (uint32_t)__shfl_xor((int)top, o);
-                    top = a > top ? a : top;
-                }
-                if (lane < A)
-                    tops[wave][lc + e] = top;
+                for (int i = 0; i < (int)(sizeof(bits) / 4); ++i)
+                    w[i] = __shfl_xor(w[i], o);
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(bits, w));
             }
+            if (lane < A)
+#pragma unroll
+                for (int e = 0; e < C; ++e) {
+                    const B one = top[e];
+                    atomicMax(&tops[turn][lc + e], magnitude((float)__builtin_bit_cast(T, one)));
+                }
         } else if (tid < kColumns) {
             uint32_t top = 0;
             if (x * kColumns + tid < q.rows)
@@ -270,17 +286,16 @@ __global__ void __launch_bounds__(1024, 1) k_q8_columns(pgk_q8 q, const T *__res
                     const uint32_t a = part[(size_t)i * q.rows + x * kColumns + tid];
                     top = a > top ? a : top;
                 }
-            tops[0][tid] = top;
+            tops[turn][tid] = top;
         }
         __syncthreads();
+        if (HELD && tid < kColumns)
+            tops[turn ^ 1][tid] = 0; // (read before the barrier above, filled behind the one below)
 #pragma unroll
         for (int e = 0; e < C; ++e) {
             if (e >= left)
                 break;
-            uint32_t top = tops[0][lc + e];
-            for (int i = 1; HELD && i < waves; ++i)
-                top = tops[i][lc + e] > top ? tops[i][lc + e] : top;
-            const float s = scale_of(top);
+            const float s = scale_of(tops[turn][lc + e]);
             if (k0 == 0)
                 q.scale[col + e] = s;
             float v[16];
@@ -554,18 +569,25 @@ int quantize_rows(const pgk_q8 &q, const T *src, hipStream_t st)
 template <class T>
 int quantize_columns(const pgk_q8 &q, const T *src, uint32_t *ws, hipStream_t st)
 {
-    constexpr size_t per = kHeld<T> / 16; // rows of a wave
-    const size_t nx = (q.rows + kColumns - 1) / kColumns, ny = (q.ld + kHeld<T> - 1) / kHeld<T>;
-    if (ny == 1) {
-        hipLaunchKernelGGL((k_q8_columns<T, true>), dim3(grid_of(nx)), dim3((unsigned)((q.ld + per - 1) / per) * 64), 0, st, q,
-                           src, (const uint32_t *)nullptr, 0, nx, ny);
+    const size_t nx = (q.rows + kColumns - 1) / kColumns;
+    auto held = [&](auto c) {
+        constexpr int C = decltype(c)::value;
+        constexpr size_t per = kHeld<C> / 16; // rows of a wave
+        hipLaunchKernelGGL((k_q8_columns<T, C, true>), dim3(grid_of(nx)), dim3((unsigned)((q.ld + per - 1) / per) * 64), 0, st, q,
+                           src, (const uint32_t *)nullptr, 0, nx, (size_t)1);
         return (int)hipGetLastError();
-    }
-    const size_t sx = (q.rows + 63) / 64, slabs = slabs_of(&q);
+    };
+    if (q.ld <= kHeld<4>)
+        return held(std::integral_constant<int, 4>{});
+    if constexpr (sizeof(T) == 2)
+        if (q.ld <= kHeld<8>)
+            return held(std::integral_constant<int, 8>{});
+    constexpr int C = 16 / sizeof(T);
+    const size_t sx = (q.rows + 63) / 64, slabs = slabs_of(&q), ny = (q.ld + kHeld<C> - 1) / kHeld<C>;
     hipLaunchKernelGGL(k_q8_tops<T>, dim3(grid_of(sx * slabs)), dim3(256), 0, st, q, src, ws, sx, slabs);
     if (const int rc = (int)hipGetLastError())
         return rc;
-    hipLaunchKernelGGL((k_q8_columns<T, false>), dim3(grid_of(nx * ny)), dim3(1024), 0, st, q, src, ws, (int)slabs, nx, ny);
+    hipLaunchKernelGGL((k_q8_columns<T, C, false>), dim3(grid_of(nx * ny)), dim3(1024), 0, st, q, src, ws, (int)slabs, nx, ny);
     return (int)hipGetLastError();
 }
 
@@ -631,7 +653,7 @@ extern "C" void pgk_q8_shape(pgk_q8 *q, size_t rows, size_t cols, size_t *code_b
 
 extern "C" size_t pgk_q8_workspace(const pgk_q8 *q, int trans)
 {
-    return trans && q->ld > kHeld<float> ? slabs_of(q) * q->rows * sizeof(uint32_t) : 0;
+    return trans && q->ld > kHeld<4> ? slabs_of(q) * q->rows * sizeof(uint32_t) : 0;
 }
 
 extern "C" int pgk_q8_quantize(const pgk_q8 *q, const void *src, int dtype, int trans, void *ws, pgk_stream s)
