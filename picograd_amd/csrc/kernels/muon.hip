@@ -320,6 +320,22 @@ __device__ __forceinline__ void finish4(const pgk_muon_seg &s, size_t i, const f
         }
 }
 
+// the same of one
+__device__ __forceinline__ void finish1(const pgk_muon_seg &s, uint32_t i, float x)
+{
+    const float o = s.w ? s.decay * s.w[i] - s.step * (x * (1.0f / kUnit)) : x * (1.0f / kUnit);
+    if (s.w)
+        s.w[i] = o;
+    else if (s.out_dtype == 0)
+        ((float *)s.out)[i] = o;
+    uint16_t *const narrow = s.w ? s.shadow : (uint16_t *)s.out;
+    const int dt = s.w ? s.shadow_dtype : s.out_dtype;
+    if (narrow && dt != 0) {
+        const uint32_t c = (uint32_t)s.shadow_cols;
+        narrow[c ? i / c * s.shadow_ld + i % c : i] = to16(dt, o);
+    }
+}
+
 enum { NS_S = 0, NS_B = 1, NS_X = 2, NS_LAST = 3 };
 
 // row and column of tile i of a lower triangle, row by row
@@ -714,6 +730,250 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
     }
 }
 
+// ---------------------------------------------------------------- thin matrices, a block each
+
+// Short sides of up to 16 MB (MB 1 or 2), long ones of up to 256 SW: X stays in
+// registers.  A wave owns strips of 16 columns; a lane holds column lane % 16 of rows
+// 4 (lane / 16) .. + 3 of each 16 x 16 block, as the 16 x 16 x 16 products give their
+// sums and as they take an operand whose reduction runs along those rows.  So
+//   B X takes X as it lies, and leaves it so;
+//   X X^T takes X turned, which is its pieces' product with the unit matrix (exact);
+//   S, symmetric, serves as either operand as it lies.
+// Only the waves' parts of S pass through LDS, joined in the waves' order; B each wave
+// works out by itself.  Bound by the conversions between f32 and pieces: 16 x 4096
+// with its 16 strips a wave by one CU's vector units, a few strips by the two
+// barriers of a step.
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+struct halves4 {
+    f16x4 h, l;
+    __device__ __forceinline__ halves4() {}
+    __device__ __forceinline__ explicit halves4(const f32x4 &v)
+    {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            h[e] = (_Float16)v[e];
+            l[e] = (_Float16)(v[e] - (float)h[e]);
+        }
+    }
+};
+__device__ __forceinline__ f32x4 mma4(const f16x4 &a, const f16x4 &b, const f32x4 &c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma4(const halves4 &a, const halves4 &b, f32x4 c)
+{
+    c = mma4(a.h, b.h, c);
+    c = mma4(a.h, b.l, c);
+    return mma4(a.l, b.h, c);
+}
+
+template <int MB, int SW>
+__global__ void __launch_bounds__(1024, 1) k_ns_thin(seg_table t, int steps)
+{
+    constexpr int SIZE = MB * MB * 256;
+    __shared__ float parts[16][SIZE], joined[SIZE];
+    __shared__ double sums[16];
+    const pgk_muon_seg s = t.seg[blockIdx.x];
+    const int tid = (int)threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6); // (uniform to the compiler: matrix instructions heed no mask)
+    const int rows = (int)s.rows, cols = (int)s.cols;
+    const bool tall = rows > cols;
+    const int m = tall ? cols : rows, n = tall ? rows : cols, strips = (n + 15) / 16, waves = strips < 16 ? strips : 16;
+    // neighbours of a lane lie `along` apart
+    const uint32_t along = tall ? 1 : n;
+    auto place = [&](int q, int b) { // of the first
+        const uint32_t i = b * 16 + 4 * lg, j = (q * 16 + wave) * 16 + lr;
+        return tall ? j * m + i : i * n + j;
+    };
+    auto some = [&](int q, int b) { // how many there are
+        const int left = m - (b * 16 + 4 * lg);
+        return (q * 16 + wave) * 16 + lr < n && left > 0 ? left < 4 ? left : 4 : 0;
+    };
+    f32x4 x[SW][MB];
+    auto fetch = [&](auto *p) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+        T raw[SW][MB][4];
+#pragma unroll
+        for (int q = 0; q < SW; ++q)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                __builtin_amdgcn_sched_barrier(0); // (all addresses at once would not fit the registers)
+                const uint32_t at = place(q, b);
+                const int k = some(q, b);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    raw[q][b][e] = p[e < k ? at + e * along : 0];
+            }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < SW; ++q)
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[q][b][e] = e < some(q, b) ? (float)raw[q][b][e] : 0.0f;
+    };
+    if (s.g_dtype == 1)
+        fetch((const _Float16 *)s.g);
+    else if (s.g_dtype == 2)
+        fetch((const __bf16 *)s.g);
+    else
+        fetch((const float *)s.g);
+    double sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < SW; ++q)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+            f32x4 &u = x[q][b];
+            if (s.gclip)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    u[e] = u[e] * s.gmul * s.ginv; // as a pending scale is written
+            __builtin_amdgcn_sched_barrier(0);
+            if (s.m) {
+                const uint32_t at = place(q, b);
+                const int k = some(q, b);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = s.m[e < k ? at + e * along : 0];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < k) {
+                        v[e] = t.mu * v[e] + u[e];
+                        s.m[at + e * along] = v[e];
+                        u[e] = t.nesterov ? u[e] + t.mu * v[e] : v[e];
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                sum += (double)u[e] * (double)u[e];
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        sum += __shfl_xor(sum, o);
+    if (lane == 0)
+        sums[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w)
+        sum += sums[w];
+    const double scale = sum == 0.0 ? 0.0 : (double)kUnit / sqrt(sum);
+#pragma unroll
+    for (int q = 0; q < SW; ++q)
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[q][b][e] = (float)((double)x[q][b][e] * scale);
+    f16x4 unit;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        unit[e] = (_Float16)(4 * lg + e == lr ? 1.0f : 0.0f);
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int step = 0; step < steps; ++step) {
+        f32x4 g[MB][MB];
+#pragma unroll
+        for (int r = 0; r < MB; ++r)
+#pragma unroll
+            for (int c = 0; c < MB; ++c)
+                g[r][c] = zero;
+#pragma unroll
+        for (int q = 0; q < SW; ++q) {
+            if (q * 16 + wave >= strips)
+                break;
+            halves4 turned[MB];
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                const halves4 v(x[q][b]);
+                const f32x4 h = mma4(v.h, unit, zero), l = mma4(v.l, unit, zero);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    turned[b].h[e] = (_Float16)h[e];
+                    turned[b].l[e] = (_Float16)l[e];
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < MB; ++r)
+#pragma unroll
+                for (int c = 0; c < MB; ++c)
+                    g[r][c] = mma4(turned[r], turned[c], g[r][c]);
+        }
+        if (wave < waves)
+#pragma unroll
+            for (int r = 0; r < MB; ++r)
+#pragma unroll
+                for (int c = 0; c < MB; ++c)
+                    *(f32x4 *)&parts[wave][(r * MB + c) * 256 + lane * 4] = g[r][c];
+        __syncthreads();
+        if (tid < SIZE) {
+            float v = 0.0f;
+            for (int w = 0; w < waves; ++w)
+                v += parts[w][tid];
+            joined[tid] = v * (1.0f / kUnit);
+        }
+        __syncthreads();
+        if (wave >= waves)
+            continue;
+        // blocks [r][c] of S and B: rows of r, a column of c; by symmetry a row of c along r
+        f32x4 f[MB][MB];
+        halves4 a[MB][MB];
+#pragma unroll
+        for (int r = 0; r < MB; ++r)
+#pragma unroll
+            for (int c = 0; c < MB; ++c) {
+                f[r][c] = *(const f32x4 *)&joined[(r * MB + c) * 256 + lane * 4];
+                a[r][c] = halves4(f[r][c]);
+            }
+#pragma unroll
+        for (int r = 0; r < MB; ++r)
+#pragma unroll
+            for (int c = 0; c < MB; ++c) {
+                f32x4 v = zero;
+#pragma unroll
+                for (int k = 0; k < MB; ++k)
+                    v = mma4(a[k][r], a[k][c], v);
+                f[r][c] = kB * f[r][c] + v * (kC / kUnit);
+            }
+#pragma unroll
+        for (int r = 0; r < MB; ++r)
+#pragma unroll
+            for (int c = 0; c < MB; ++c)
+                a[r][c] = halves4(f[r][c]);
+#pragma unroll
+        for (int q = 0; q < SW; ++q) {
+            if (q * 16 + wave >= strips)
+                break;
+            halves4 v[MB];
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+                v[b] = halves4(x[q][b]);
+#pragma unroll
+            for (int r = 0; r < MB; ++r) {
+                f32x4 y = zero;
+#pragma unroll
+                for (int k = 0; k < MB; ++k)
+                    y = mma4(a[k][r], v[k], y);
+                x[q][r] = kA * x[q][r] + y * (1.0f / kUnit);
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < SW; ++q)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+            __builtin_amdgcn_sched_barrier(0);
+            const uint32_t at = place(q, b);
+            const int k = some(q, b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < k)
+                    finish1(s, at + e * along, x[q][b][e]);
+        }
+}
+
 // ---------------------------------------------------------------- launches
 
 template <bool TB>
@@ -872,11 +1132,16 @@ bool fits(const pgk_muon_seg &s)
 
 } // namespace
 
-// matrices that a block holds
-bool small(const pgk_muon_seg &s)
+// matrices that a block holds, by its kernel
+enum { LARGE = -1, SMALL64, SMALL256, THIN16, THIN16_LONG, THIN32, THIN32_LONG, KINDS };
+int kind_of(const pgk_muon_seg &s)
 {
     const size_t lo = s.rows < s.cols ? s.rows : s.cols, hi = s.rows < s.cols ? s.cols : s.rows;
-    return lo <= kSmallM && hi <= kSmallN;
+    if (lo <= 16)
+        return hi <= 1024 ? THIN16 : hi <= 4096 ? THIN16_LONG : LARGE;
+    if (lo <= 32)
+        return hi <= 512 ? THIN32 : hi <= 2048 ? THIN32_LONG : LARGE;
+    return lo > kSmallM || hi > kSmallN ? LARGE : hi <= 64 ? SMALL64 : SMALL256;
 }
 
 extern "C" size_t pgk_muon_workspace(const pgk_muon_seg *segs, int n)
@@ -884,7 +1149,7 @@ extern "C" size_t pgk_muon_workspace(const pgk_muon_seg *segs, int n)
     ns_prob p[kMost];
     int k = 0;
     for (int i = 0; i < n && i < kMost; ++i)
-        if (!small(segs[i]))
+        if (kind_of(segs[i]) == LARGE)
             shape(segs[i], &p[k++]);
     order(p, NULL, k);
     float *partial;
@@ -900,26 +1165,35 @@ extern "C" int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov,
     seg_table t = {};
     t.mu = mu;
     t.nesterov = nesterov;
-    size_t longest = 0;
-    for (int i = 0; i < n; ++i) {
+    for (int i = 0; i < n; ++i)
         if (!fits(segs[i]))
             return (int)hipErrorInvalidValue;
-        if (small(segs[i])) {
-            t.seg[t.n++] = segs[i];
-            longest = std::max({longest, segs[i].rows, segs[i].cols});
-        }
-    }
-    if (t.n) {
-        if (longest <= 64)
-            hipLaunchKernelGGL(k_ns_small<64>, dim3((unsigned)t.n), dim3(1024), 0, st, t, steps);
+    for (int kind = 0; kind < KINDS; ++kind) {
+        t.n = 0;
+        for (int i = 0; i < n; ++i)
+            if (kind_of(segs[i]) == kind)
+                t.seg[t.n++] = segs[i];
+        if (!t.n)
+            continue;
+        const dim3 grid((unsigned)t.n), block(1024);
+        if (kind == SMALL64)
+            hipLaunchKernelGGL(k_ns_small<64>, grid, block, 0, st, t, steps);
+        else if (kind == SMALL256)
+            hipLaunchKernelGGL(k_ns_small<kSmallN>, grid, block, 0, st, t, steps);
+        else if (kind == THIN16)
+            hipLaunchKernelGGL((k_ns_thin<1, 4>), grid, block, 0, st, t, steps);
+        else if (kind == THIN16_LONG)
+            hipLaunchKernelGGL((k_ns_thin<1, 16>), grid, block, 0, st, t, steps);
+        else if (kind == THIN32)
+            hipLaunchKernelGGL((k_ns_thin<2, 2>), grid, block, 0, st, t, steps);
         else
-            hipLaunchKernelGGL(k_ns_small<kSmallN>, dim3((unsigned)t.n), dim3(1024), 0, st, t, steps);
+            hipLaunchKernelGGL((k_ns_thin<2, 8>), grid, block, 0, st, t, steps);
         if (const int rc = (int)hipGetLastError())
             return rc;
     }
     t.n = 0;
     for (int i = 0; i < n; ++i)
-        if (!small(segs[i])) {
+        if (kind_of(segs[i]) == LARGE) {
             t.seg[t.n] = segs[i];
             shape(segs[i], &t.p[t.n++]);
         }

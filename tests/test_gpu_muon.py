@@ -81,6 +81,17 @@ def test_factor(bench, dtype, k, n):
         near(orth(bench, g, dtype, out), want, tol + (UNIT[out] if out != F32 else 0), NAMES[out])
 
 
+# either side of what a block holds in registers
+THIN = [(16, 16), (16, 17), (1, 4096), (16, 1024), (1025, 15), (4096, 16), (16, 4097), (17, 31), (32, 512), (513, 30),
+        (2047, 32), (18, 2048), (17, 2049)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("k,n", THIN)
+def test_thin_factors(bench, dtype, k, n):
+    test_factor(bench, dtype, k, n)
+
+
 # enough tiles for the larger ones, square, wide and tall
 @pytest.mark.parametrize("k,n", [(2000, 2100), (2950, 2901), (700, 6100), (4500, 1500)])
 def test_large_factors(bench, k, n):
@@ -134,7 +145,7 @@ def test_ranks_zeros_and_what_is_no_number(bench):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
-@pytest.mark.parametrize("k,n", [(33, 70), (70, 33), (200, 200)])
+@pytest.mark.parametrize("k,n", [(5, 90), (33, 70), (70, 33), (30, 700), (200, 200)])
 def test_in_place_strided_and_inside_a_storage(bench, dtype, k, n):
     L = bench.L
     g = rounded(grads(k, n, 6), dtype)
@@ -159,7 +170,7 @@ def test_in_place_strided_and_inside_a_storage(bench, dtype, k, n):
     assert np.array_equal(whole[3:-9].reshape(k, n), want) and (whole[:3] == 5).all() and (whole[-9:] == 6).all()
 
 
-@pytest.mark.parametrize("k,n", [(64, 64), (130, 700), (2000, 2100)])
+@pytest.mark.parametrize("k,n", [(64, 64), (16, 3000), (31, 1500), (130, 700), (2000, 2100)])
 def test_the_same_call_gives_the_same_bits(bench, k, n):
     g = grads(k, n, 7)
     first = orth(bench, g)
