@@ -189,21 +189,25 @@ void pgo_layernorm_backward(pg_node *n)
     pgt_materialize(n->grad);
     pgk_norm_args a = {.x = px->value->dev, .m = m, .d = d, .w = pw ? pw->value->dev : NULL, .stats = cx->stats->dev,
                        .dy = n->grad->dev};
-    /* a node that is two of them takes its parts one after the other: dx lands
-     * before the sums, and one node's two sums are two calls */
     pg_tensor *gx = px->requires_grad ? pga_grad_for_write(px, &a.beta_x) : NULL;
     pg_tensor *gw = pw && pw->requires_grad ? pga_grad_for_write(pw, &a.beta_w) : NULL;
     pg_tensor *gb = pb && pb->requires_grad ? pga_grad_for_write(pb, &a.beta_b) : NULL;
+    /* a node that is two of them takes its parts in calls of their own, one after
+     * the other: within a call dx and the sums may be written at the same time */
+    const bool w_apart = gw && pw == px, b_apart = gb && (pb == px || pb == pw);
     a.dx = gx ? gx->dev : NULL;
-    a.dw = gw ? gw->dev : NULL;
-    a.db = gb && pb != pw ? gb->dev : NULL;
+    a.dw = gw && !w_apart ? gw->dev : NULL;
+    a.db = gb && !b_apart ? gb->dev : NULL;
     if ((a.dx || a.dw || a.db) && !run(what, &a, true))
         return;
-    if (gb && pb == pw) {
-        a.dx = a.dw = NULL;
-        a.db = gb->dev;
+    a.dx = a.db = NULL;
+    a.dw = w_apart ? gw->dev : NULL;
+    if (a.dw && !run(what, &a, true))
+        return;
+    a.dw = NULL;
+    a.db = b_apart ? gb->dev : NULL;
+    if (a.db)
         run(what, &a, true);
-    }
 }
 
 /* a node's value as an operand: f32, contiguous, its elements current */

@@ -305,6 +305,17 @@ def test_node(bench, m, d, weights, jit):
         L.pg_autograd_set_jit(True)
 
 
+def test_a_grad_of_ones(bench):
+    L = bench.L
+    x, w, b, _ = data(33, 70, F32, 13)
+    nx, nw, nb = (bench.var(v) for v in (x, w, b))
+    L.pg_backward(bench.node(L.op("sum_all", bench.node(L.pg_ag_layernorm(nx, nw, nb, EPS)))))
+    want = Model(x, w, b, np.ones((33, 70)))
+    within(L.grad(nx), want.dx, want.edx, "dx")
+    within(L.grad(nw), want.dw, want.edw, "dw")
+    assert (L.grad(nb) == 33).all()
+
+
 def test_grads_add_to_what_is_there(bench):
     """One x under two norms with one weight: the grads are the sums."""
     L = bench.L
@@ -322,11 +333,11 @@ def test_grads_add_to_what_is_there(bench):
     within(L.grad(nb), a.db + c.db, a.edb + c.edb + U * np.abs(a.db + c.db), "db")
 
 
+@pytest.mark.parametrize("d", [40, 20000])
 @pytest.mark.parametrize("same", ["xw", "xb", "wb", "xwb"])
-def test_one_node_as_several_operands(bench, same):
+def test_one_node_as_several_operands(bench, same, d):
     L = bench.L
     g = np.random.default_rng(11)
-    d = 40
     v = {k: rounded(g.standard_normal(d), F32) for k in "xwb"}
     dy = rounded(g.standard_normal((1, d)), F32)
     for k in same[1:]:
