@@ -374,6 +374,22 @@ __device__ __forceinline__ i32x4 mma16(const uint4 &a, const uint4 &b, const i32
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
+// N sums under both scales.  Under a scale of x outside these bounds the first product
+// may leave f32 where the second comes back into it (x of 1e33 under weights of
+// 1e-10): then 64 bits hold all three.
+template <int N, class V>
+__device__ __forceinline__ void scaled(const V &sum, float sx, const float (&sw)[N], float (&y)[N])
+{
+    if (sx < 0x1p90f && sx > 0x1p-90f)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            y[e] = (float)sum[e] * sx * sw[e];
+    else
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            y[e] = (float)((double)sum[e] * (double)sx * (double)sw[e]);
+}
+
 // `n` neighbours of a row of y, at most four
 template <class O>
 __device__ __forceinline__ void put4(O *p, const float (&v)[4], int n)
@@ -487,12 +503,15 @@ __global__ void __launch_bounds__(kFewWaves * 64, 1)
         __syncthreads();
         const int row = tid >> 4, col = tid & 15;
         if (row < m && row < 16 && n0 + col < w.rows) {
-            int sum = 0;
+            int sum[1] = {0};
 #pragma unroll
             for (int i = 0; i < kFewWaves; ++i)
-                sum += part[i][row][col];
+                sum[0] += part[i][row][col];
             const float sx = FUSED ? scale_of(tops[row]) : xq.scale[row];
-            y[(size_t)row * w.rows + n0 + col] = (O)((float)sum * sx * w.scale[n0 + col]);
+            const float sw[1] = {w.scale[n0 + col]};
+            float o[1];
+            scaled(sum, sx, sw, o);
+            y[(size_t)row * w.rows + n0 + col] = (O)o[0];
         }
         __syncthreads();
     }
@@ -529,9 +548,7 @@ __global__ void __launch_bounds__(CF::NT, 1) k_q8_tiles(pgk_q8 x, pgk_q8 w, O *_
             acc[i], i, m0, n0, M, N, lds, false, [&](int row, int) { return x.scale[row]; },
             [&](int row, int col, const i32x4 &v, float sx, bool) {
                 float o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    o[e] = (float)v[e] * sx * sw[e];
+                scaled(v, sx, sw, o);
                 put4(y + (size_t)row * N + col, o, N - col < 4 ? N - col : 4);
             });
 }

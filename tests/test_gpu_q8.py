@@ -174,6 +174,17 @@ def test_wide_ranges_zero_rows_and_strides(bench, m):
     L.pg_amd_q8_free(q)
 
 
+@pytest.mark.parametrize("m", [3, 16, 200, 4000])
+@pytest.mark.parametrize("up", [True, False])
+def test_ranges_that_meet_in_the_middle(bench, m, up):
+    """A sum times x's scale leaves f32 before the weights' scale brings it back."""
+    g = np.random.default_rng(6)
+    k, n = 1000, 70
+    x, w = rounded(np.abs(g.standard_normal((m, k))), F32), rounded(np.abs(g.standard_normal((k, n))), F32)
+    p = 2.0 ** (119 if up else -110)
+    within(product(bench, x * p, w / p, F32, F32), *wanted(x * p, w / p, F32), "y")
+
+
 @pytest.mark.parametrize("m", [1, 17, 300])
 def test_the_longest_reduction_is_exact(bench, m):
     """2^17 products of 127 and 127 or -127: sums of up to 2^17 127^2, next to the ends of 32 bits."""
