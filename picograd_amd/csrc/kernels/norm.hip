@@ -23,27 +23,60 @@ namespace {
 constexpr int kChunks = 2; // of 16 bytes of x, per thread of a slice
 constexpr unsigned kMostBlocks = 1u << 20; // of a grid; kernels loop past it
 
+// Chunk c of E of a row of d: its place, and which of the E there are its own.  The last
+// one of a row lies over its neighbour, so that it is loaded as the others are (its
+// elements one by one held up the row's whole block: 8192 x 4095 in bf16, backward,
+// 96 us against 43 of 4096).  Of a slice of a longer row the neighbour may be the
+// slice before; with SHORT a row of less than a chunk has one of d.
+template <int E, bool SHORT = false>
+struct spot {
+    int at, lo, hi;
+    __device__ __forceinline__ spot(int c, int d)
+    {
+        const int over = (c + 1) * E - d;
+        lo = over > 0 ? over : 0;
+        at = c * E - lo;
+        hi = E;
+        if (SHORT && d < E) {
+            lo = at = 0;
+            hi = d;
+        }
+    }
+    __device__ __forceinline__ bool full() const { return !SHORT || hi == E; }
+    __device__ __forceinline__ bool whole() const { return full() && lo == 0; }
+    __device__ __forceinline__ bool has(int e) const { return e >= lo && (!SHORT || e < hi); }
+};
+
 // as many values of S as 16 bytes hold of T, at any alignment of an element
 template <class T, class S>
 struct piece {
     static constexpr int E = 16 / sizeof(T);
     typedef S sv __attribute__((ext_vector_type(E), aligned(sizeof(S))));
     sv q;
-    // elements c E .. of the row p [d]; past the end: 0
-    __device__ __forceinline__ void load(const S *p, int c, int d)
+    // of the row p; past a short row's end: 0
+    template <bool SHORT>
+    __device__ __forceinline__ void load(const S *p, const spot<E, SHORT> &c)
     {
-        const int at = c * E, left = d - at;
-        if (left >= E) {
-            q = *(const sv *)(p + at);
+        if (c.full()) {
+            q = *(const sv *)(p + c.at);
         } else {
             q = sv{};
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (e < left)
-                    q[e] = p[at + e];
+                if (e < c.hi)
+                    q[e] = p[e];
         }
     }
     __device__ __forceinline__ float operator[](int e) const { return (float)q[e]; }
+    // 0 for the neighbour's
+    template <bool SHORT>
+    __device__ __forceinline__ void own(const spot<E, SHORT> &c)
+    {
+        if (c.lo)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                q[e] = e < c.lo ? (S)0.0f : q[e];
+    }
     // new to the compiler: the values read from here on are converted anew, where
     // those converted before would be kept in twice the registers
     __device__ __forceinline__ void again()
@@ -65,31 +98,31 @@ template <class T>
 struct chunk {
     static constexpr int E = 16 / sizeof(T);
     float v[E];
-    template <class S>
-    __device__ __forceinline__ void load(const S *p, int c, int d)
+    template <bool SHORT, class S>
+    __device__ __forceinline__ void load(const S *p, const spot<E, SHORT> &c)
     {
         piece<T, S> q;
-        q.load(p, c, d);
+        q.load(p, c);
 #pragma unroll
         for (int e = 0; e < E; ++e)
             v[e] = q[e];
     }
-    template <class O>
-    __device__ __forceinline__ void store(O *p, int c, int d) const
+    // (of its own)
+    template <bool SHORT, class O>
+    __device__ __forceinline__ void store(O *p, const spot<E, SHORT> &c) const
     {
         typedef O ov __attribute__((ext_vector_type(E), aligned(sizeof(O))));
-        const int at = c * E, left = d - at;
-        if (left >= E) {
+        if (c.whole()) {
             ov q;
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 q[e] = (O)v[e];
-            *(ov *)(p + at) = q;
+            *(ov *)(p + c.at) = q;
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (e < left)
-                    p[at + e] = (O)v[e];
+                if (c.has(e))
+                    p[c.at + e] = (O)v[e];
         }
     }
     __device__ __forceinline__ void fill(float f)
@@ -138,6 +171,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
                                                                 O *y, float *__restrict__ stats)
 {
     using ch = chunk<T>;
+    using at = spot<ch::E, TPR == 8>;
     constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
     __shared__ float red[4][TPR > 64 ? TPR / 64 : 1][1];
     const int tid = (int)threadIdx.x, lane = tid % TPR;
@@ -147,22 +181,31 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
     auto weights = [&](int i, ch &wi, ch &bi) {
         const int c = lane + i * TPR;
         if (w && c < nc)
-            wi.load(w, c, d);
+            wi.load(w, at(c, d));
         else
             wi.fill(1.0f);
         if (b && c < nc)
-            bi.load(b, c, d);
+            bi.load(b, at(c, d));
         else
             bi.fill(0.0f);
+    };
+    // as if new to the compiler: what follows from it for R chunks is worked out anew,
+    // not kept in registers
+    auto anew = [&] {
+        int l = lane;
+        if constexpr (R > 2)
+            __asm__("" : "+v"(l));
+        return l;
     };
     piece<T, T> cur[R];
     auto ask = [&](size_t row, piece<T, T>(&q)[R]) {
         const T *p = x + row * d;
+        const int l = anew();
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             q[i].q = {};
-            if (row < m && lane + i * TPR < nc)
-                q[i].load(p, lane + i * TPR, d);
+            if (row < m && l + i * TPR < nc)
+                q[i].load(p, at(l + i * TPR, d));
         }
     };
     const size_t step = (size_t)gridDim.x * RPB;
@@ -178,22 +221,28 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
         if (r0 + step < m)
             ask(row + step, next);
         float s[1] = {0.0f};
+        int l = anew();
 #pragma unroll
-        for (int i = 0; i < R; ++i)
+        for (int i = 0; i < R; ++i) {
+            if (l + i * TPR < nc)
+                cur[i].own(at(l + i * TPR, d));
 #pragma unroll
             for (int e = 0; e < ch::E; ++e)
                 s[0] += cur[i][e];
+        }
         row_sum<TPR>(s, red[turn], tid);
         const float mean = s[0] / (float)d;
         s[0] = 0.0f;
+        l = anew();
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             cur[i].again();
-            const bool whole = (lane + i * TPR + 1) * ch::E <= d;
+            const at k(l + i * TPR, d);
+            const bool in = l + i * TPR < nc, whole = k.whole();
 #pragma unroll
             for (int e = 0; e < ch::E; ++e) {
                 const float c = cur[i][e] - mean;
-                s[0] += whole || (lane + i * TPR) * ch::E + e < d ? c * c : 0.0f;
+                s[0] += in && (whole || k.has(e)) ? c * c : 0.0f;
             }
         }
         row_sum<TPR>(s, red[turn + 1], tid);
@@ -203,7 +252,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
                 *(float2 *)(stats + row * 2) = make_float2(mean, rstd);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const int c = lane + i * TPR;
+                const int c = anew() + i * TPR;
                 if (c >= nc)
                     break;
                 if constexpr (!HOLD)
@@ -213,7 +262,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
 #pragma unroll
                 for (int e = 0; e < ch::E; ++e)
                     o.v[e] = (cur[i][e] - mean) * rstd * wv[HOLD ? i : 0].v[e] + bv[HOLD ? i : 0].v[e];
-                o.store(y + row * d, c, d);
+                o.store(y + row * d, at(c, d));
             }
         }
 #pragma unroll
@@ -231,6 +280,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_bwd(const T *__r
                                                      int d, O *__restrict__ dx, int beta, float *__restrict__ part)
 {
     using ch = chunk<T>;
+    using at = spot<ch::E, TPR == 8>;
     constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR, COLS = TPR * R * ch::E;
     __shared__ float red[2][TPR > 64 ? TPR / 64 : 1][2];
     __shared__ float sums[RPB > 1 ? RPB : 1][RPB > 1 ? COLS : 1];
@@ -244,7 +294,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_bwd(const T *__r
         float2 st;
     } cur;
     auto ask = [&](size_t row, rows &q) { // (past the end of a row and of all rows dy is 0)
-        const size_t at = row * d;
+        const size_t first = row * d;
         q.st = row < m ? *(const float2 *)(stats + row * 2) : make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -252,8 +302,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_bwd(const T *__r
             q.x[i].q = {};
             q.dy[i].q = {};
             if (row < m && c < nc) {
-                q.x[i].load(x + at, c, d);
-                q.dy[i].load(dy + at, c, d);
+                q.x[i].load(x + first, at(c, d));
+                q.dy[i].load(dy + first, at(c, d));
             }
         }
     };
@@ -265,7 +315,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_bwd(const T *__r
         gw[i].fill(0.0f);
         gb[i].fill(0.0f);
         if (w && lane + i * TPR < nc)
-            wv[i].load(w, lane + i * TPR, d);
+            wv[i].load(w, at(lane + i * TPR, d));
         else
             wv[i].fill(1.0f);
     }
@@ -277,11 +327,12 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_bwd(const T *__r
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const bool whole = (lane + i * TPR + 1) * ch::E <= d;
+            if (lane + i * TPR < nc)
+                cur.dy[i].own(at(lane + i * TPR, d));
 #pragma unroll
             for (int e = 0; e < ch::E; ++e) {
                 const float g = cur.dy[i][e], h = g * wv[i].v[e];
-                const float n = whole || (lane + i * TPR) * ch::E + e < d ? (cur.x[i][e] - cur.st.x) * cur.st.y : 0.0f;
+                const float n = (cur.x[i][e] - cur.st.x) * cur.st.y; // (beside a g of 0 if not its own)
                 gw[i].v[e] += g * n;
                 gb[i].v[e] += g;
                 s[0] += h;
@@ -300,13 +351,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_bwd(const T *__r
                 cur.dy[i].again();
                 ch o;
                 if (beta)
-                    o.load(dx + row * d, c, d);
+                    o.load(dx + row * d, at(c, d));
                 else
                     o.fill(0.0f);
 #pragma unroll
                 for (int e = 0; e < ch::E; ++e)
                     o.v[e] += cur.st.y * (cur.dy[i][e] * wv[i].v[e] - c1 - (cur.x[i][e] - cur.st.x) * cur.st.y * c2);
-                o.store(dx + row * d, c, d);
+                o.store(dx + row * d, at(c, d));
             }
         }
         cur = next;
@@ -319,14 +370,17 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm_bwd(const T *__r
 #pragma unroll
             for (int i = 0; i < R; ++i)
                 if (lane + i * TPR < nc)
-                    g[i].store(out, lane + i * TPR, d);
+                    g[i].store(out, at(lane + i * TPR, d));
         } else {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < R; ++i)
+            for (int i = 0; i < R; ++i) {
+                const at k(lane + i * TPR, d);
 #pragma unroll
                 for (int e = 0; e < ch::E; ++e)
-                    sums[group][(lane + i * TPR) * ch::E + e] = g[i].v[e];
+                    if (lane + i * TPR < nc && k.has(e))
+                        sums[group][k.at + e] = g[i].v[e];
+            }
             __syncthreads();
             for (int c = tid; c < d; c += NT) {
                 float t = 0.0f;
@@ -419,6 +473,7 @@ __global__ void __launch_bounds__(256) k_norm_slices(const T *__restrict__ x, si
                                                      float2 *__restrict__ part)
 {
     using ch = chunk<T>;
+    using at = spot<ch::E>;
     __shared__ float red[4][4][1];
     const int tid = (int)threadIdx.x;
     int turn = 0;
@@ -432,24 +487,28 @@ __global__ void __launch_bounds__(256) k_norm_slices(const T *__restrict__ x, si
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
             if (tid + i * 256 < nc)
-                v[i].load(p, tid + i * 256, len);
+                v[i].load(p, at(tid + i * 256, len));
             else
                 v[i].fill(0.0f);
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i)
+        for (int i = 0; i < kChunks; ++i) {
+            const at k(tid + i * 256, len);
 #pragma unroll
             for (int e = 0; e < ch::E; ++e)
-                s[0] += v[i].v[e];
+                s[0] += e >= k.lo ? v[i].v[e] : 0.0f; // (0 past a short row)
+        }
         row_sum<256>(s, red[turn], tid);
         const float mean = s[0] / (float)len;
         s[0] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i)
+        for (int i = 0; i < kChunks; ++i) {
+            const at k(tid + i * 256, len);
 #pragma unroll
             for (int e = 0; e < ch::E; ++e) {
                 const float c = v[i].v[e] - mean;
-                s[0] += (tid + i * 256) * ch::E + e < len ? c * c : 0.0f;
+                s[0] += tid + i * 256 < nc && k.has(e) ? c * c : 0.0f;
             }
+        }
         row_sum<256>(s, red[turn + 1], tid);
         if (tid == 0)
             part[job] = make_float2(mean, s[0]);
@@ -462,17 +521,18 @@ __global__ void __launch_bounds__(256) k_norm_long(const T *x, const float *__re
                                                    const float2 *__restrict__ part, O *y, float *__restrict__ stats)
 {
     using ch = chunk<T>;
+    using at = spot<ch::E>;
     const int tid = (int)threadIdx.x, lane = tid & 63;
     for (size_t job = blockIdx.x; job < m * slices; job += gridDim.x) {
         const size_t row = job / slices;
         const int k = (int)(job - row * slices), first = k * kSlice<T>;
         const int len = d - first < kSlice<T> ? d - first : kSlice<T>, nc = (len + ch::E - 1) / ch::E;
-        const size_t at = row * d + first;
+        const size_t from = row * d + first;
         ch v[kChunks];
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
             if (tid + i * 256 < nc)
-                v[i].load(x + at, tid + i * 256, len);
+                v[i].load(x + from, at(tid + i * 256, len));
         // every wave joins the row's slices by itself
         moments a = {0.0f, 0.0f, 0.0f};
         for (int i = lane; i < slices; i += 64) {
@@ -500,17 +560,17 @@ __global__ void __launch_bounds__(256) k_norm_long(const T *x, const float *__re
                 break;
             ch wv, bv;
             if (w)
-                wv.load(w + first, c, len);
+                wv.load(w + first, at(c, len));
             else
                 wv.fill(1.0f);
             if (b)
-                bv.load(b + first, c, len);
+                bv.load(b + first, at(c, len));
             else
                 bv.fill(0.0f);
 #pragma unroll
             for (int e = 0; e < ch::E; ++e)
                 v[i].v[e] = (v[i].v[e] - mean) * rstd * wv.v[e] + bv.v[e];
-            v[i].store(y + at, c, len);
+            v[i].store(y + from, at(c, len));
         }
     }
 }
@@ -525,6 +585,7 @@ __global__ void __launch_bounds__(256) k_norm_sums(const T *__restrict__ x, cons
                                                    float2 *__restrict__ rows, float *__restrict__ part)
 {
     using ch = chunk<T>;
+    using at = spot<ch::E>;
     constexpr int U = 4;
     __shared__ float red[2][4][2 * U];
     const int tid = (int)threadIdx.x, c = (int)blockIdx.x * 256 + tid;
@@ -532,9 +593,10 @@ __global__ void __launch_bounds__(256) k_norm_sums(const T *__restrict__ x, cons
     gw.fill(0.0f);
     gb.fill(0.0f);
     wv.fill(1.0f);
-    const bool in = c * ch::E < d, whole = (c + 1) * ch::E <= d;
+    const at k(c, d);
+    const bool in = c * ch::E < d;
     if (w && in)
-        wv.load(w, c, d);
+        wv.load(w, k);
     int turn = 0;
     for (size_t r0 = blockIdx.y; r0 < m; r0 += (size_t)gridDim.y * U, turn ^= 1) {
         piece<T, T> n[U];
@@ -547,8 +609,8 @@ __global__ void __launch_bounds__(256) k_norm_sums(const T *__restrict__ x, cons
             g[u].q = {};
             st[u] = make_float2(0.0f, 0.0f);
             if (row < m && in) {
-                n[u].load(x + row * d, c, d);
-                g[u].load(dy + row * d, c, d);
+                n[u].load(x + row * d, k);
+                g[u].load(dy + row * d, k);
                 st[u] = *(const float2 *)(stats + row * 2);
             }
         }
@@ -556,9 +618,11 @@ __global__ void __launch_bounds__(256) k_norm_sums(const T *__restrict__ x, cons
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             s[2 * u] = s[2 * u + 1] = 0.0f;
+            if (in)
+                g[u].own(k);
 #pragma unroll
             for (int e = 0; e < ch::E; ++e) {
-                const float f = whole || c * ch::E + e < d ? (n[u][e] - st[u].x) * st[u].y : 0.0f, h = g[u][e] * wv.v[e];
+                const float f = (n[u][e] - st[u].x) * st[u].y, h = g[u][e] * wv.v[e]; // (beside a g of 0 if not its own)
                 gw.v[e] += g[u][e] * f;
                 gb.v[e] += g[u][e];
                 s[2 * u] += h;
@@ -580,8 +644,8 @@ __global__ void __launch_bounds__(256) k_norm_sums(const T *__restrict__ x, cons
     }
     if (part && in) {
         float *out = part + (size_t)blockIdx.y * 2 * d;
-        gw.store(out, c, d);
-        gb.store(out + d, c, d);
+        gw.store(out, k);
+        gb.store(out + d, k);
     }
 }
 
@@ -595,6 +659,7 @@ __global__ void __launch_bounds__(256) k_norm_bwd_long(const T *__restrict__ x, 
                                                        float *db, int beta_b)
 {
     using ch = chunk<T>;
+    using at = spot<ch::E>;
     if ((int)blockIdx.x >= blocks) {
         join_sums<256>(part, parts, d, (int)blockIdx.x - blocks, dw, beta_w, db, beta_b);
         return;
@@ -604,15 +669,15 @@ __global__ void __launch_bounds__(256) k_norm_bwd_long(const T *__restrict__ x, 
     for (size_t job = blockIdx.x; job < m * slices; job += blocks) {
         const size_t row = job / slices;
         const int first = (int)(job - row * slices) * kSlice<T>, len = d - first < kSlice<T> ? d - first : kSlice<T>;
-        const size_t at = row * d + first;
+        const size_t from = row * d + first;
         const int nc = (len + ch::E - 1) / ch::E;
         piece<T, T> n[kChunks];
         piece<T, G> g[kChunks];
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
             if (tid + i * 256 < nc) {
-                n[i].load(x + at, tid + i * 256, len);
-                g[i].load(dy + at, tid + i * 256, len);
+                n[i].load(x + from, at(tid + i * 256, len));
+                g[i].load(dy + from, at(tid + i * 256, len));
             }
         const float2 st = *(const float2 *)(stats + row * 2), s = slice_sums(rows + row * across, across, lane);
         const float c1 = s.x * inv, c2 = s.y * inv;
@@ -623,17 +688,17 @@ __global__ void __launch_bounds__(256) k_norm_bwd_long(const T *__restrict__ x, 
                 break;
             ch wv, o;
             if (w)
-                wv.load(w + first, c, len);
+                wv.load(w + first, at(c, len));
             else
                 wv.fill(1.0f);
             if (beta)
-                o.load(dx + at, c, len);
+                o.load(dx + from, at(c, len));
             else
                 o.fill(0.0f);
 #pragma unroll
             for (int e = 0; e < ch::E; ++e)
                 o.v[e] += st.y * (g[i][e] * wv.v[e] - c1 - (n[i][e] - st.x) * st.y * c2);
-            o.store(dx + at, c, len);
+            o.store(dx + from, at(c, len));
         }
     }
 }
