@@ -231,7 +231,7 @@ def test_steps(bench, cfg):
     L = bench.L
     r = np.random.default_rng(8)
     opt, nodes, models = optimiser(bench, **cfg), [], []
-    for k, n in ((64, 64), (10, 300), (300, 10), (129, 200), (1, 5), (700, 650)):
+    for k, n in ((64, 64), (10, 300), (300, 10), (129, 200), (1, 5), (700, 650), (2000, 10), (30, 600)):
         w = rounded(r.uniform(-1, 1, (k, n)) * k ** -0.5, F32)
         nodes.append(bench.var(w))
         models.append(Model(w, **cfg))
