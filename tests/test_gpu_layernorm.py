@@ -77,7 +77,8 @@ def forward(bench, x, w, b, y, stats=None, eps=EPS):
 # that start anywhere, one row and more rows than blocks, rows in slices
 SHAPES = [(1, 1), (3, 1), (5, 2), (1, 3), (7, 8), (33, 10), (1000, 31), (300, 32), (257, 33), (4, 64), (40, 255), (65, 256),
           (9, 257), (3, 1000), (1030, 1023), (2, 1024), (5, 1025), (17, 2048), (6, 2049), (1, 4096), (2, 4097), (3, 8192),
-          (2, 8200), (1, 16384), (2, 16391), (3, 32768), (2, 32775), (1, 65537), (5, 50001)]
+          (2, 8200), (1, 16384), (2, 16391), (3, 32768), (2, 32775), (1, 65537), (5, 50001), (256, 9001), (257, 17000),
+          (300, 33001)]
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)

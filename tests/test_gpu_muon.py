@@ -278,7 +278,7 @@ def test_more_matrices_than_a_launch_takes(bench):
     assert np.array_equal(L.value(n), L.value(nodes[0]))
 
 
-@pytest.mark.parametrize("k,n", [(48, 64), (50, 33)])
+@pytest.mark.parametrize("k,n", [(48, 64), (50, 33), (16, 700), (301, 9), (24, 37), (1100, 20)])
 def test_kept_copies_follow(bench, k, n):
     """A 16-bit layer before and after a step: its product uses the stepped weights."""
     L = bench.L
@@ -298,11 +298,12 @@ def test_kept_copies_follow(bench, k, n):
         assert np.array_equal(L.value(again), L.value(fresh)) and not np.array_equal(L.value(again), L.value(y))
 
 
-def test_a_clipped_grad(bench):
+@pytest.mark.parametrize("shape", [(40, 60), (9, 130), (300, 30), (100, 110)])
+def test_a_clipped_grad(bench, shape):
     """The direction does not change with the norm, the momentum does."""
     L = bench.L
     r = np.random.default_rng(11)
-    w, g = rounded(r.uniform(-1, 1, (40, 60)), F32), rounded(r.standard_normal((40, 60)), F32)
+    w, g = rounded(r.uniform(-1, 1, shape), F32), rounded(r.standard_normal(shape), F32)
     n, model = bench.var(w), Model(w)
     opt = optimiser(bench)
     assert L.pg_amd_muon_add_param(opt, n) == 0
