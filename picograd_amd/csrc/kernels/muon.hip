@@ -983,6 +983,8 @@ template <bool TB>
 using T128 = pcfg<f32x16, 2, 128, 128, 4, 2, TB, 32, 4>;
 template <bool TB>
 using T64 = pcfg<f32x16, 2, 64, 64, 2, 2, TB, 64, 2>;
+template <bool TB>
+using ONE64 = pcfg<f32x16, 2, 64, 64, 2, 2, TB, 32, 4>; // for one to a CU: more stages on their way
 
 size_t up64(size_t v) { return (v + 63) & ~(size_t)63; }
 
@@ -1022,17 +1024,18 @@ int tiles_of(const ns_prob &p, int what, int side)
 // as they are; what is left, less than a round, is split along the reduction
 // where that is faster.  The time of 32 along the reduction was measured with few
 // blocks and with as many as fit (two on a CU of 64, else one), in us: 1.7 and 2.4
-// for a side of 256, 0.5 and 0.75 for 128, 0.36 and 0.44 for 64; a joining launch
-// takes some 5 us and the partial sums' way at 3.5 TB/s.
+// for a side of 256, 0.5 and 0.75 for 128, 0.36 and 0.44 for 64, 0.25 and 0.29 for 64 one
+// to a CU; a joining launch takes some 5 us and the partial sums' way at 3.5 TB/s.
 struct ns_plan {
-    int side, whole, z, tiles;
+    int side, kind, whole, z, tiles;
 };
+enum { KIND256, KIND128, KIND64, KIND_ONE64 };
 ns_plan plan_of(const ns_prob *p, int n, int what)
 {
     static const struct {
         int side, blocks;
         double alone, full;
-    } kinds[3] = {{256, 1, 1.7, 2.4}, {128, 1, 0.5, 0.75}, {64, 2, 0.36, 0.44}};
+    } kinds[4] = {{256, 1, 1.7, 2.4}, {128, 1, 0.5, 0.75}, {64, 2, 0.36, 0.44}, {64, 1, 0.25, 0.29}};
     ns_plan best = {};
     double least = 0.0;
     for (const auto &c : kinds) {
@@ -1063,7 +1066,7 @@ ns_plan plan_of(const ns_prob *p, int n, int what)
                 time += 5.0 + units * (double)c.side * c.side * 8.0 / 3.5e6;
             if (!best.side || time < least) {
                 least = time;
-                best = {c.side, z == 1 ? tiles : whole, z, tiles};
+                best = {c.side, (int)(&c - kinds), z == 1 ? tiles : whole, z, tiles};
             }
         }
     }
@@ -1089,7 +1092,10 @@ template <int WHAT, class TAB>
 int product(TAB &t, hipStream_t st)
 {
     const ns_plan q = plan_of(t.p, t.n, WHAT);
-    return q.side == 256 ? launch<T256, WHAT>(t, q, st) : q.side == 128 ? launch<T128, WHAT>(t, q, st) : launch<T64, WHAT>(t, q, st);
+    return q.kind == KIND256   ? launch<T256, WHAT>(t, q, st)
+           : q.kind == KIND128 ? launch<T128, WHAT>(t, q, st)
+           : q.kind == KIND64  ? launch<T64, WHAT>(t, q, st)
+                               : launch<ONE64, WHAT>(t, q, st);
 }
 
 // the matrices' own places and the partial sums'
