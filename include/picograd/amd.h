@@ -170,7 +170,9 @@ pg_node *pg_amd_ag_gated16(pg_node *x, pg_node *w, pg_node *b, int act, pg_dtype
  * Statistics and sums are f32; y and dx round once.  A row that holds a NaN or an
  * infinity becomes NaN whole, and so do dw and (where dy is) db.  M is under 2^31, D
  * from 1 to 2^28, eps finite and at least 0 (with 0 a row of equal values is NaN).
- * Differences from the mean past 2^63 / sqrt(D) leave f32 in the variance.
+ * The mean is rounded to f32, n is off by that rounding times rstd (rows of equal
+ * values are not: their n is 0).  Differences from the mean past 2^63 / sqrt(D) leave f32
+ * in the variance, values next to its end in the mean.
  * pg_ag_layernorm is the node of it. */
 /* x of any dtype, w and b f32 [D] or NULL (1 and 0), y of x's shape, of its dtype
  * or f32; y may be x itself.  stats (f32, 2 M elements) receives each row's mean

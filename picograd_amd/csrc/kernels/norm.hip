@@ -4,10 +4,11 @@
 //   y = n w + b
 //   h = dy w: dx = rstd (h - sum h / d - n sum (h n) / d), dw = sum over rows of dy n, db = of dy
 //
-// Statistics and sums are f32 from values held in registers (the variance is of
-// the differences from the mean, not of squares); y and dx round once.  A row
-// that a block holds is read once; longer ones are cut into slices for blocks of
-// their own and read twice.  Bound by the stream of the rows: HBM for large calls
+// Statistics and sums are f32 from values held in registers; y and dx round once.  The
+// variance is of differences, not of squares: those from a first mean, whose own mean
+// then corrects both (settled), so that a row of equal values has its value as mean
+// and no variance.  A row that a block holds is read once; longer ones are cut into
+// slices for blocks of their own and read twice.  Bound by the stream of the rows: HBM for large calls
 // (8192 x 8192 in bf16: forward 54 to 57 us, 4.8 TB/s, backward 92 to 95, 4.3 TB/s, where a
 // copy reaches 5.2), the launches and a row's loads for small ones (1 x 4096: 2.9 us;
 // 33 x 50001 in f16 with its backward, four launches: 20).
@@ -135,17 +136,38 @@ struct chunk {
     }
 };
 
+// s of a lane and of lane ^ O, for O from 32 down one after the other (so that O = 4 finds
+// a period of eight lanes, as a rotation in 16 needs it), without LDS (f32 4096 x 1024,
+// forward: 9.5 us, with shuffles 11.2)
+template <int O>
+__device__ __forceinline__ float with_xor(float s)
+{
+    const uint32_t v = __float_as_uint(s);
+    if constexpr (O >= 16) { // both halves of the wave, or of 32 lanes
+        const auto both = O == 32 ? __builtin_amdgcn_permlane32_swap(v, v, false, false)
+                                  : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    } else { // rotations by 8 and 4 in 16 lanes, exchanges in 4
+        constexpr int how = O == 8 ? 0x128 : O == 4 ? 0x124 : O == 2 ? 0x4e : 0xb1;
+        return s + __uint_as_float(__builtin_amdgcn_update_dpp(0, v, how, 0xf, 0xf, true));
+    }
+}
+
 // sums over the TPR threads that share a row, in a fixed order.  TPR over 64:
 // through `red` [waves of a row], which the caller does not reuse before the
-// next barrier but one
-template <int TPR, int N>
+// next barrier but one; the waves' sums are read ON at a time
+template <int TPR, int ON = TPR / 64, int N>
 __device__ __forceinline__ void row_sum(float (&s)[N], float (*red)[N], int tid)
 {
+    static_assert(TPR == 8 || TPR >= 64, "eight lanes or whole waves");
 #pragma unroll
-    for (int o = TPR < 64 ? TPR / 2 : 32; o > 0; o >>= 1)
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            s[i] += __shfl_xor(s[i], o);
+    for (int i = 0; i < N; ++i) {
+        if constexpr (TPR == 8)
+            s[i] += __shfl_xor(s[i], 4);
+        else
+            s[i] = with_xor<4>(with_xor<8>(with_xor<16>(with_xor<32>(s[i]))));
+        s[i] = with_xor<1>(with_xor<2>(s[i]));
+    }
     if constexpr (TPR > 64) {
         if ((tid & 63) == 0)
 #pragma unroll
@@ -153,13 +175,37 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float (*red)[N], int tid)
                 red[tid >> 6][i] = s[i];
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < N; ++i)
             s[i] = 0.0f;
+#pragma unroll ON
+        for (int w = 0; w < TPR / 64; ++w)
 #pragma unroll
-            for (int w = 0; w < TPR / 64; ++w)
+            for (int i = 0; i < N; ++i)
                 s[i] += red[w][i];
-        }
     }
+}
+
+// The mean and the sum of the squares of what differs from it, from a first mean, which
+// is off by the roundings of its sum (some 80 half units of its last place at most).
+// sums(mean, s, k): those of the differences c = x - mean and of their squares, the k'th
+// time (0, 1).  With D = sum c / d the mean is D further and the squares about it are
+// sum c^2 - D sum c.  Where D is what carries the squares (a row of values that differ by
+// a few of those units, or not at all), the difference would be mostly rounding: both
+// sums are taken once more, about the moved mean.
+template <class FN>
+__device__ __forceinline__ float settled(float &mean, float inv, FN sums)
+{
+    float s[2];
+    sums(mean, s, 0);
+    float off = s[0] * inv;
+    mean += off;
+    if (off != 0.0f && !(s[0] * off < 0.25f * s[1])) { // (also where the squares leave f32)
+        sums(mean, s, 1);
+        off = s[0] * inv;
+        mean += off;
+    }
+    const float squares = s[1] - s[0] * off;
+    return squares < 0.0f ? 0.0f : squares; // (a NaN stays)
 }
 
 // ---------------------------------------------------------------- rows that a block holds
@@ -175,7 +221,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
     using ch = chunk<T>;
     using at = spot<ch::E, TPR == 8>;
     constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
-    __shared__ float red[4][TPR > 64 ? TPR / 64 : 1][1];
+    constexpr int W = TPR > 64 ? TPR / 64 : 1;
+    __shared__ float first[2][W][1], about[3][W][2];
     const int tid = (int)threadIdx.x, lane = tid % TPR;
     const int nc = (d + ch::E - 1) / ch::E;
     const float inv = 1.0f / (float)d;
@@ -218,11 +265,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
         for (int i = 0; i < R; ++i)
             weights(i, wv[i], bv[i]);
     int turn = 0;
-    for (size_t r0 = (size_t)blockIdx.x * RPB; r0 < m; r0 += step, row += step, turn ^= 2) {
+    for (size_t r0 = (size_t)blockIdx.x * RPB; r0 < m; r0 += step, row += step, turn ^= 1) {
         piece<T, T> next[R];
         if (r0 + step < m)
             ask(row + step, next);
-        float s[1] = {0.0f};
+        float one[1] = {0.0f};
         int l = anew();
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -230,25 +277,29 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_norm(const T *x, cons
                 cur[i].own(at(l + i * TPR, d));
 #pragma unroll
             for (int e = 0; e < ch::E; ++e)
-                s[0] += cur[i][e];
+                one[0] = fmaf(cur[i][e], inv, one[0]); // (the values' sum may leave f32)
         }
-        row_sum<TPR>(s, red[turn], tid);
-        const float mean = s[0] / (float)d;
-        s[0] = 0.0f;
-        l = anew();
+        row_sum<TPR, 8>(one, first[turn], tid);
+        float mean = one[0];
+        const float sum = settled(mean, inv, [&](float mu, float (&t)[2], int again) {
+            t[0] = t[1] = 0.0f;
+            const int q = anew();
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            cur[i].again();
-            const at k(l + i * TPR, d);
-            const bool in = l + i * TPR < nc, whole = k.whole();
+            for (int i = 0; i < R; ++i) {
+                cur[i].again();
+                const at k(q + i * TPR, d);
+                const bool in = q + i * TPR < nc, whole = k.whole();
 #pragma unroll
-            for (int e = 0; e < ch::E; ++e) {
-                const float c = cur[i][e] - mean;
-                s[0] += in && (whole || k.has(e)) ? c * c : 0.0f;
+                for (int e = 0; e < ch::E; ++e) {
+                    const float c = in && (whole || k.has(e)) ? cur[i][e] - mu : 0.0f;
+                    t[0] += c;
+                    t[1] += c * c;
+                }
             }
-        }
-        row_sum<TPR>(s, red[turn + 1], tid);
-        const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+            // (of more waves two at a time: no more registers are left beside the next row's)
+            row_sum<TPR, (TPR <= 256 ? 4 : 2)>(t, about[again ? 2 : turn], tid);
+        });
+        const float rstd = 1.0f / sqrtf(sum * inv + eps);
         if (row < m) {
             if (stats && lane == 0)
                 *(float2 *)(stats + row * 2) = make_float2(mean, rstd);
@@ -465,7 +516,7 @@ struct moments {
     {
         const float all = n + n2, q = m2 - mean, f = all > 0.0f ? n2 / all : 0.0f;
         mean += q * f;
-        sum += s2 + (q * n) * (q * f);
+        sum += s2 + q * (n * f) * q; // (beside nothing q is a mean, whose square may leave f32)
         n = all;
     }
 };
@@ -476,16 +527,17 @@ __global__ void __launch_bounds__(256) k_norm_slices(const T *__restrict__ x, si
 {
     using ch = chunk<T>;
     using at = spot<ch::E>;
-    __shared__ float red[4][4][1];
+    __shared__ float sums[2][4][1], about[3][4][2];
     const int tid = (int)threadIdx.x;
     int turn = 0;
-    for (size_t job = blockIdx.x; job < m * slices; job += gridDim.x, turn ^= 2) {
+    for (size_t job = blockIdx.x; job < m * slices; job += gridDim.x, turn ^= 1) {
         const size_t row = job / slices;
         const int first = (int)(job - row * slices) * kSlice<T>, len = d - first < kSlice<T> ? d - first : kSlice<T>;
         const T *p = x + row * d + first;
         const int nc = (len + ch::E - 1) / ch::E;
+        const float inv = 1.0f / (float)len;
         ch v[kChunks];
-        float s[1] = {0.0f};
+        float one[1] = {0.0f};
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
             if (tid + i * 256 < nc)
@@ -497,23 +549,26 @@ __global__ void __launch_bounds__(256) k_norm_slices(const T *__restrict__ x, si
             const at k(tid + i * 256, len);
 #pragma unroll
             for (int e = 0; e < ch::E; ++e)
-                s[0] += e >= k.lo ? v[i].v[e] : 0.0f; // (0 past a short row)
+                one[0] = fmaf(e >= k.lo ? v[i].v[e] : 0.0f, inv, one[0]); // (0 past a short row)
         }
-        row_sum<256>(s, red[turn], tid);
-        const float mean = s[0] / (float)len;
-        s[0] = 0.0f;
+        row_sum<256>(one, sums[turn], tid);
+        float mean = one[0];
+        const float sum = settled(mean, inv, [&](float mu, float (&t)[2], int again) {
+            t[0] = t[1] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const at k(tid + i * 256, len);
+            for (int i = 0; i < kChunks; ++i) {
+                const at k(tid + i * 256, len);
 #pragma unroll
-            for (int e = 0; e < ch::E; ++e) {
-                const float c = v[i].v[e] - mean;
-                s[0] += tid + i * 256 < nc && k.has(e) ? c * c : 0.0f;
+                for (int e = 0; e < ch::E; ++e) {
+                    const float c = tid + i * 256 < nc && k.has(e) ? v[i].v[e] - mu : 0.0f;
+                    t[0] += c;
+                    t[1] += c * c;
+                }
             }
-        }
-        row_sum<256>(s, red[turn + 1], tid);
+            row_sum<256>(t, about[again ? 2 : turn], tid);
+        });
         if (tid == 0)
-            part[job] = make_float2(mean, s[0]);
+            part[job] = make_float2(mean, sum);
     }
 }
 
