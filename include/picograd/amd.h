@@ -335,8 +335,9 @@ void pg_amd_muon_zero_grad(pg_amd_muon *opt);
 /* Steps every parameter that has a grad, up to 12 of them in shared launches, and
  * rewrites kept 16-bit copies with them; workspace of some 16 bytes per element
  * comes from the allocator's cache.  Enqueued on the library stream.  false and
- * pg_autograd_last_error() on a grad of another shape (nothing is stepped) or a
- * device error. */
+ * pg_autograd_last_error() on a device error, or, nothing being stepped, on a grad
+ * of another shape or a node whose value was replaced by one of another shape or one
+ * that overlaps another parameter's. */
 bool pg_amd_muon_step(pg_amd_muon *opt);
 /* The momenta as "PGMU", u32 version 1, u64 nparams, per parameter u32 has_buf (0
  * or 1) then the buffer's PGT1 record when has_buf.  load_into is for an optimiser

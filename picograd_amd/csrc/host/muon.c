@@ -134,6 +134,20 @@ static bool value_ok(const pg_tensor *v)
     return v && v->dev && v->dtype == PG_DTYPE_F32 && sides_ok(v) && pgt_is_contiguous(v);
 }
 
+/* whether v shares memory with one of the first n parameters' values (with_grad: of
+ * those that have a grad) */
+static bool taken(const pg_amd_muon *opt, size_t n, const pg_tensor *v, bool with_grad)
+{
+    const char *lo = v->dev, *hi = lo + v->numel * 4;
+    for (size_t i = 0; i < n; i++) {
+        const pg_node *p = opt->st[i].param;
+        const pg_tensor *o = p->value;
+        if ((p->grad || !with_grad) && (const char *)o->dev < hi && lo < (const char *)o->dev + o->numel * 4)
+            return true;
+    }
+    return false;
+}
+
 int pg_amd_muon_add_param(pg_amd_muon *opt, pg_node *param)
 {
     static const char *const what = "pg_amd_muon_add_param";
@@ -141,13 +155,9 @@ int pg_amd_muon_add_param(pg_amd_muon *opt, pg_node *param)
         pga_set_err("%s: needs a contiguous f32 matrix node that requires grads, with sides of 1 to 2^16", what);
         return -1;
     }
-    const char *lo = param->value->dev, *hi = lo + param->value->numel * 4;
-    for (size_t i = 0; i < opt->n; i++) {
-        const pg_tensor *v = opt->st[i].param->value;
-        if ((const char *)v->dev < hi && lo < (const char *)v->dev + v->numel * 4) {
-            pga_set_err("%s: the matrix is a parameter already", what);
-            return -1;
-        }
+    if (taken(opt, opt->n, param->value, false)) {
+        pga_set_err("%s: the matrix is a parameter already", what);
+        return -1;
     }
     if (opt->n == opt->cap) {
         const size_t nc = opt->cap ? opt->cap * 2 : 8;
@@ -201,11 +211,20 @@ bool pg_amd_muon_step(pg_amd_muon *opt)
         return false;
     }
     const pg_amd_muon_cfg c = opt->cfg;
+    /* a node's value may have been replaced since it was added */
     for (size_t i = 0; i < opt->n; i++) {
-        const pg_tensor *v = opt->st[i].param->value, *g = opt->st[i].param->grad;
+        const pg_tensor *v = opt->st[i].param->value, *g = opt->st[i].param->grad, *m = opt->st[i].buf;
         if (g && (!value_ok(v) || g->dtype != PG_DTYPE_F32 || !pgt_is_contiguous(g) ||
                   !pg_shape_equal(g->ndim, g->shape, v->ndim, v->shape))) {
             pga_set_err("%s: parameters and grads must be contiguous f32 of one shape", what);
+            return false;
+        }
+        if (g && m && !pg_shape_equal(m->ndim, m->shape, v->ndim, v->shape)) {
+            pga_set_err("%s: a parameter has another shape than its momentum", what);
+            return false;
+        }
+        if (g && taken(opt, i, v, true)) {
+            pga_set_err("%s: two parameters' matrices overlap", what);
             return false;
         }
     }
