@@ -620,9 +620,9 @@ template <class O>
 int product(const pgk_q8 &x, const pgk_q8 &w, O *y, hipStream_t st)
 {
     auto tiles = [&](size_t bm, size_t bn) { return (x.rows + bm - 1) / bm * ((w.rows + bn - 1) / bn); };
-    if (tiles(64, 64) >> 24) { // a grid holds under 2^32 threads: the rows in two halves
-        if (x.rows <= 256) // over 2^28 columns
-            return (int)hipErrorInvalidValue;
+    // a grid holds under 2^32 threads: the rows in two halves (up to 256 of them by 2^30
+    // columns are 2^23 of the larger tiles at most, 2^31 threads)
+    if (x.rows > 256 && tiles(64, 64) >> 24) {
         pgk_q8 a = x, b = x;
         a.rows = (x.rows / 2 + 255) & ~(size_t)255;
         b.rows -= a.rows;
