@@ -271,7 +271,9 @@ __global__ void __launch_bounds__(kFewWaves * 64, 1)
 {
     constexpr int U = 4; // steps in flight
     __shared__ float part[kFewWaves][16][17];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    // (the wave's number is uniform to the compiler: a matrix instruction heeds no mask)
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
     const int t = t0 + xcd_tile((int)blockIdx.x, (int)gridDim.x), steps = (int)w.steps, k = (int)w.cols;
     // runs of U neighbouring steps, dealt to the waves in turn
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
