@@ -7,19 +7,25 @@
 //   out = X, or W <- decay W - step X
 //
 // The singular values s of X follow s <- a s + b s^3 + c s^5; with (a, b, c) =
-// (3.4445, -4.7750, 2.0315) all but the smallest come to 0.7 .. 1.2 in five steps,
-// and none passes 1.21, so no entry of X, S or B passes 2.9.
+// (3.4445, -4.7750, 2.0315) those over 1/660 come to 0.68 .. 1.203 in five steps, and
+// none passes 1.203 in any, so no entry of X, S or B passes 2.9.
 //
 // An error in an early X grows as the small singular values do, by up to a a
 // step, so f32 is held throughout: X, S and B are kept as two f16 pieces each,
 // high and low (22 to 23 bits), times 4096 to keep the low ones from the f16
 // subnormals, and a product is three on the f16 matrix units, hh + hl + lh, in
 // f32 sums.  Against 64 bits the result is as near as f32 products' (2.8e-6
-// against 2.5e-6 of 512 x 512 with singular values over 3.5 decades).  a X is
-// added apart from B X: a on the diagonal of B would round it with each entry
-// and triples the error.
+// against 2.5e-6 of 512 x 512 with singular values over 3.5 decades; measured to
+// sides of 4500).  Entries under 2^-15, such as X's before the first step past sides of
+// some 2^15, have low pieces among the subnormals and are held to 2^-37 itself.
+// a X is added apart from B X: a on the diagonal of B would round it with each
+// entry and triples the error.
 //
 // S and S S are symmetric: tiles below the diagonal, each written twice.
+//
+// How a product is cut depends on all matrices of a launch, and with it the order of
+// its sums: a matrix's last bits may differ with the others beside it, never from one
+// call to the next.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -733,17 +739,18 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
 // ---------------------------------------------------------------- thin matrices, a block each
 
 // Short sides of up to 16 MB (MB 1 or 2), long ones of up to 256 SW: X stays in
-// registers.  A wave owns strips of 16 columns; a lane holds column lane % 16 of rows
+// registers, of the long kinds (16 and 2 x 8 blocks a wave) but for some 100 of them that
+// the compiler spills (356 and 404 bytes a lane).  A wave owns strips of 16 columns; a lane holds column lane % 16 of rows
 // 4 (lane / 16) .. + 3 of each 16 x 16 block, as the 16 x 16 x 16 products give their
 // sums and as they take an operand whose reduction runs along those rows.  So
 //   B X takes X as it lies, and leaves it so;
 //   X X^T takes X turned, which is its pieces' product with the unit matrix (exact);
 //   S, symmetric, serves as either operand as it lies.
 // Only the waves' parts of S pass through LDS, joined in the waves' order; B each wave
-// works out by itself.  Bound by the conversions between f32 and pieces: 16 x 4096
-// with its 16 strips a wave by one CU's vector units (47 us in five steps, in
-// launches of their own some 140), a few strips by the two barriers of a step (1 x 64:
-// 7.4 us).
+// works out by itself.  Bound by one CU: the conversions between f32 and pieces and, of
+// the long kinds, the spills' way (16 x 4096 with its 16 strips a wave: 47 us in five
+// steps, in launches of their own some 140), of a few strips the two barriers of a step
+// (1 x 64: 7.4 us).
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 struct halves4 {
@@ -1137,8 +1144,6 @@ bool fits(const pgk_muon_seg &s)
     return s.rows && s.cols && s.rows <= PGK_MUON_MAX_SIDE && s.cols <= PGK_MUON_MAX_SIDE;
 }
 
-} // namespace
-
 // matrices that a block holds, by its kernel
 enum { LARGE = -1, SMALL64, SMALL256, THIN16, THIN16_LONG, THIN32, THIN32_LONG, KINDS };
 int kind_of(const pgk_muon_seg &s)
@@ -1164,6 +1169,8 @@ void kinds_of(const pgk_muon_seg *segs, int n, int (&kind)[kMost])
         if (large && (kind[i] == THIN16_LONG || kind[i] == THIN32_LONG))
             kind[i] = LARGE;
 }
+
+} // namespace
 
 extern "C" size_t pgk_muon_workspace(const pgk_muon_seg *segs, int n)
 {
