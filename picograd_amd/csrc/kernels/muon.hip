@@ -748,9 +748,9 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
 //   S, symmetric, serves as either operand as it lies.
 // Only the waves' parts of S pass through LDS, joined in the waves' order; B each wave
 // works out by itself.  Bound by one CU: the conversions between f32 and pieces and, of
-// the long kinds, the spills' way (16 x 4096 with its 16 strips a wave: 47 us in five
-// steps, in launches of their own some 140), of a few strips the two barriers of a step
-// (1 x 64: 7.4 us).
+// the long kinds, the spills' way (five steps of 16 x 4096, 16 strips a wave, 74 us, and of
+// 4096 x 16 113; in launches of their own 137 and 139), of a few strips the two barriers
+// of a step (1 x 64: 6.9 us).
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 struct halves4 {
@@ -1157,7 +1157,7 @@ int kind_of(const pgk_muon_seg &s)
 }
 
 // Long thin ones beside a large one take their tiles in its launches: 4096 x 10 costs
-// 40 us on a CU of its own before them, next to nothing in 7.6 ms of theirs.
+// 81 us on a CU of its own before them, next to nothing in 7.4 ms of theirs.
 void kinds_of(const pgk_muon_seg *segs, int n, int (&kind)[kMost])
 {
     bool large = false;

@@ -11,7 +11,7 @@
 // slices for blocks of their own and read twice.  Bound by the stream of the rows: HBM for large calls
 // (8192 x 8192 in bf16: forward 54 to 57 us, 4.8 TB/s, backward 92 to 95, 4.3 TB/s, where a
 // copy reaches 5.2), the launches and a row's loads for small ones (1 x 4096: 2.9 us;
-// 33 x 50001 in f16 with its backward, four launches: 20).
+// 33 x 50001 in f16 with its backward, four launches: 19).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
