@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(1024, 1) k_ns_small(seg_table t, int steps)
 // works out by itself.  Bound by one CU: the conversions between f32 and pieces and, of
 // the long kinds, the spills' way (five steps of 16 x 4096, 16 strips a wave, 74 us, and of
 // 4096 x 16 113; in launches of their own 137 and 139), of a few strips the two barriers
-// of a step (1 x 64: 6.9 us).
+// of a step (1 x 64: 7.0 us).
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 struct halves4 {
@@ -776,10 +776,40 @@ __device__ __forceinline__ f32x4 mma4(const halves4 &a, const halves4 &b, f32x4 
     return mma4(a.l, b.h, c);
 }
 
+// with what both pieces leave over, all of f32's bits
+struct thirds4 : halves4 {
+    f16x4 r;
+    __device__ __forceinline__ thirds4() {}
+    __device__ __forceinline__ explicit thirds4(const f32x4 &v) : halves4(v)
+    {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            r[e] = (_Float16)(v[e] - (float)h[e] - (float)l[e]);
+    }
+};
+// the products beside that of the high pieces
+__device__ __forceinline__ f32x4 rest4(const thirds4 &a, const halves4 &b)
+{
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    return mma4(a.l, b.h, mma4(a.h, b.l, mma4(a.l, b.l, mma4(a.r, b.h, zero))));
+}
+__device__ __forceinline__ f32x4 rest4(const thirds4 &a, const thirds4 &b)
+{
+    return rest4(a, (const halves4 &)b) + mma4(a.h, b.r, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+}
+
 template <int MB, int SW>
 __global__ void __launch_bounds__(1024, 1) k_ns_thin(seg_table t, int steps)
 {
     constexpr int SIZE = MB * MB * 256;
+    // FINE, one strip a wave: products with B and of S with itself take all of f32's bits, and
+    // what cancels between a X and B X (b S and c S S) does so in the high pieces' products,
+    // before the others are added.  The errors of S and B are shared by whole rows of X
+    // and average out over many rows only: over 64 inputs each of 1 x 7 to 4 x 60 those of two
+    // pieces are 1.6 to 2.4 times f32 products' in the root mean square, these 0.7 to 1.2.
+    constexpr bool FINE = SW == 1;
+    static_assert(!FINE || MB == 1, "one block");
+    using whole4 = std::conditional_t<FINE, thirds4, halves4>;
     __shared__ float parts[16][SIZE], joined[SIZE];
     __shared__ double sums[16];
     const pgk_muon_seg s = t.seg[blockIdx.x];
@@ -903,6 +933,11 @@ __global__ void __launch_bounds__(1024, 1) k_ns_thin(seg_table t, int steps)
                     turned[b].l[e] = (_Float16)l[e];
                 }
             }
+            if constexpr (FINE) {
+                const halves4 &t0 = turned[0];
+                g[0][0] = mma4(t0.l, t0.h, mma4(t0.h, t0.l, mma4(t0.l, t0.l, zero))) + mma4(t0.h, t0.h, zero);
+                break;
+            }
 #pragma unroll
             for (int r = 0; r < MB; ++r)
 #pragma unroll
@@ -927,18 +962,23 @@ __global__ void __launch_bounds__(1024, 1) k_ns_thin(seg_table t, int steps)
             continue;
         // blocks [r][c] of S and B: rows of r, a column of c; by symmetry a row of c along r
         f32x4 f[MB][MB];
-        halves4 a[MB][MB];
+        whole4 a[MB][MB];
 #pragma unroll
         for (int r = 0; r < MB; ++r)
 #pragma unroll
             for (int c = 0; c < MB; ++c) {
                 f[r][c] = *(const f32x4 *)&joined[(r * MB + c) * 256 + lane * 4];
-                a[r][c] = halves4(f[r][c]);
+                a[r][c] = whole4(f[r][c]);
             }
 #pragma unroll
         for (int r = 0; r < MB; ++r)
 #pragma unroll
             for (int c = 0; c < MB; ++c) {
+                if constexpr (FINE) {
+                    f[0][0] = kB * f[0][0] + mma4(a[0][0].h, a[0][0].h, zero) * (kC / kUnit);
+                    f[0][0] += rest4(a[0][0], a[0][0]) * (kC / kUnit);
+                    break;
+                }
                 f32x4 v = zero;
 #pragma unroll
                 for (int k = 0; k < MB; ++k)
@@ -949,17 +989,22 @@ __global__ void __launch_bounds__(1024, 1) k_ns_thin(seg_table t, int steps)
         for (int r = 0; r < MB; ++r)
 #pragma unroll
             for (int c = 0; c < MB; ++c)
-                a[r][c] = halves4(f[r][c]);
+                a[r][c] = whole4(f[r][c]);
 #pragma unroll
         for (int q = 0; q < SW; ++q) {
             if (q * 16 + wave >= strips)
                 break;
-            halves4 v[MB];
+            whole4 v[MB];
 #pragma unroll
             for (int b = 0; b < MB; ++b)
-                v[b] = halves4(x[q][b]);
+                v[b] = whole4(x[q][b]);
 #pragma unroll
             for (int r = 0; r < MB; ++r) {
+                if constexpr (FINE) {
+                    x[q][0] = kA * x[q][0] + mma4(a[0][0].h, v[0].h, zero) * (1.0f / kUnit);
+                    x[q][0] += rest4(a[0][0], v[0]) * (1.0f / kUnit);
+                    break;
+                }
                 f32x4 y = zero;
 #pragma unroll
                 for (int k = 0; k < MB; ++k)
@@ -1144,13 +1189,14 @@ bool fits(const pgk_muon_seg &s)
     return s.rows && s.cols && s.rows <= PGK_MUON_MAX_SIDE && s.cols <= PGK_MUON_MAX_SIDE;
 }
 
-// matrices that a block holds, by its kernel
-enum { LARGE = -1, SMALL64, SMALL256, THIN16, THIN16_LONG, THIN32, THIN32_LONG, KINDS };
+// matrices that a block holds, by its kernel; FINE where it costs nothing (16 x 64: 7.5 us, in
+// two pieces 7.7; 16 x 256 11.3 and 10.2) and for few rows, which need it
+enum { LARGE = -1, SMALL64, SMALL256, THIN16_FINE, THIN16, THIN16_LONG, THIN32, THIN32_LONG, KINDS };
 int kind_of(const pgk_muon_seg &s)
 {
     const size_t lo = s.rows < s.cols ? s.rows : s.cols, hi = s.rows < s.cols ? s.cols : s.rows;
     if (lo <= 16)
-        return hi <= 1024 ? THIN16 : hi <= 4096 ? THIN16_LONG : LARGE;
+        return hi <= (lo <= 4 ? 256 : 64) ? THIN16_FINE : hi <= 1024 ? THIN16 : hi <= 4096 ? THIN16_LONG : LARGE;
     if (lo <= 32)
         return hi <= 512 ? THIN32 : hi <= 2048 ? THIN32_LONG : LARGE;
     return lo > kSmallM || hi > kSmallN ? LARGE : hi <= 64 ? SMALL64 : SMALL256;
@@ -1212,6 +1258,8 @@ extern "C" int pgk_muon(const pgk_muon_seg *segs, int n, float mu, int nesterov,
             hipLaunchKernelGGL(k_ns_small<64>, grid, block, 0, st, t, steps);
         else if (kind == SMALL256)
             hipLaunchKernelGGL(k_ns_small<kSmallN>, grid, block, 0, st, t, steps);
+        else if (kind == THIN16_FINE)
+            hipLaunchKernelGGL((k_ns_thin<1, 1>), grid, block, 0, st, t, steps);
         else if (kind == THIN16)
             hipLaunchKernelGGL((k_ns_thin<1, 4>), grid, block, 0, st, t, steps);
         else if (kind == THIN16_LONG)
